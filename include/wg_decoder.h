@@ -321,6 +321,148 @@ int wg_model_matmul_noalloc(wg_model* m, int replica, int layer, int which,
                             const void* x16, int ldx, int rows, float* out, int ldo,
                             void* stream, int wait);
 
+/* ---- serving operators on the caller's device memory -----------------------
+ * For programs that run their own token loop around the decoder's (streams
+ * admitted and dropped step by step, no reference counterpart): page plans,
+ * a paged K/V cache held in 8 bits, attention over it, and token sampling.
+ * One step is wg_kv_plan -> wg_kv8_append -> wg_kv8_attention -> (logits) ->
+ * wg_sample_rows.
+ *
+ * Conventions of this group
+ *  - Every tensor pointer is DEVICE memory of `device`; the descriptors
+ *    (wg_kv8, wg_kv8_attn, wg_sample) are read on the host before the call
+ *    returns. `device` need not be current; the caller's is put back.
+ *  - Calls enqueue on `stream` (a cudaStream_t of `device`; NULL: its default
+ *    stream) and return without waiting. They allocate nothing, keep nothing
+ *    between calls and hold no workspace, so they may be captured into CUDA
+ *    graphs and run at the same time in several streams as long as no call
+ *    writes what another one reads or writes. Make the first call of each
+ *    operator on a device before a capture.
+ *  - Rows are `ld` ELEMENTS apart, the heads and dims of a row contiguous.
+ *    Any stride and any address that fits the type is accepted; rows that
+ *    start on 16 bytes are moved with wide loads.
+ *  - Lengths, slots and page numbers are checked on the device: what is out
+ *    of range is not read or written (see each call). */
+enum { WG_DT_F32 = 0, WG_DT_F16 = 1, WG_DT_BF16 = 30 }; /* GGUF ids of these types */
+
+/* A paged cache of 8-bit keys and values. Value = code * scale:
+ *   codes  int8 [num_pages][2 (K, V)][n_kv_head][page][head_dim], 16-byte aligned
+ *   scales fp32 [num_pages][2][n_kv_head], one per page, K or V, and head
+ * page: tokens per page, a power of two from 16 to 128; head_dim 64 or 128;
+ * num_pages * page < 2^31. The slot of a token is its page * `page` + its
+ * place in the page. Fresh memory needs no initialisation. */
+typedef struct wg_kv8 {
+  int8_t* codes;
+  float* scales;
+  int32_t num_pages, page, n_kv_head, head_dim;
+} wg_kv8;
+
+/* Block tables and slot maps from the requests' lengths, on the device.
+ *   lens[r], new_tokens[r] : tokens of request r after this step, and how many of them are new
+ *   free_pages[0..n_free)  : page numbers to hand out, from index *cursor on, in request order
+ *   block_table            : [R][ld_table]; the first ceil((lens - new) / page) entries of a row
+ *                            are read, the pages the step adds are written behind them, nothing else
+ *   slots[0..n_slots)      : the new tokens' slots, request by request; -1 behind the last one
+ *                            (so a captured step can run over n_slots rows)
+ *   cu_new[0..R]           : where each request's new tokens begin in `slots`
+ *   *cursor_out            : the advanced cursor (may be `cursor` itself)
+ *   status[0], status[1]   : WG_PLAN_*, and the pages taken
+ * A step that cannot be planned takes no page: status holds the largest code
+ * that applies, slots are all -1, cu_new all 0, the cursor and the table stay. */
+enum {
+  WG_PLAN_OK = 0,
+  WG_PLAN_BAD_LENGTH = 1, /* a length is negative, or new_tokens[r] > lens[r] */
+  WG_PLAN_TABLE_FULL = 2, /* a request needs more than max_pages pages */
+  WG_PLAN_SLOTS_FULL = 3, /* more new tokens than n_slots */
+  WG_PLAN_NO_PAGES = 4    /* the free list has too few pages left */
+};
+int wg_kv_plan(const int32_t* lens, const int32_t* new_tokens, int R, int page, const int32_t* free_pages, int n_free,
+               const int32_t* cursor, int32_t* cursor_out, int32_t* block_table, int64_t ld_table, int max_pages,
+               int32_t* slots, int n_slots, int32_t* cu_new, int32_t* status, int device, void* stream);
+
+/* Writes n tokens' keys and values (rows of k and v, [n][n_kv_head][head_dim],
+ * types WG_DT_*) into their slots; a slot outside the cache (-1) skips its row.
+ * The tokens of a page must be consecutive rows with consecutive slots, once
+ * in a call, as wg_kv_plan lays them out (otherwise the contents of that page
+ * are unspecified). For each page, K or V, and head the scale is the least power of two (>= 2^-126)
+ * that takes the largest finite magnitude to at most 127 steps, 0 if that is
+ * 0. Tokens that do not start their page keep the page's earlier tokens: the
+ * scale only grows, and where it does the earlier codes are rounded to the
+ * new step. Codes are rounded half to even; NaN becomes 0, an infinity +-127
+ * steps. */
+int wg_kv8_append(const wg_kv8* cache, const void* k, const void* v, int dtype, int64_t ldk, int64_t ldv,
+                  const int32_t* slots, int n, int device, void* stream);
+
+/* The values of n cached tokens by slot (code * scale, rounded to `dtype`;
+ * exact in fp32 and, for the scales that wg_kv8_append writes, in bf16), into rows of k and v. Rows
+ * whose slot lies outside the cache are left as they were. */
+int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, void* k, void* v, int dtype, int64_t ldk,
+                int64_t ldv, int device, void* stream);
+
+/* Attention of the query rows of n_requests requests over their cached tokens:
+ *   softmax(scale * q K^T) V, query head j on K/V head j / (n_head / n_kv_head).
+ * Request r's queries are rows cu_q[r] .. cu_q[r+1]-1 of q; they see the
+ * first kv_lens[r] tokens of the pages in row r of block_table; with `causal`
+ * the queries are the last tokens of those: query i of nq sees the first
+ * kv_lens[r] - nq + i + 1. Without it every query sees all of them (cross-
+ * attention: the beams of an utterance are its queries). A query that sees
+ * nothing gives zeros. A page number outside the cache hides its tokens.
+ * Rows of `out` that belong to no request are left as they were; a request
+ * whose cu_q pair is out of range or descending has no rows.
+ * max_q: no request has more query rows (rows past it are not computed);
+ * max_kv: the longest kv_lens, a hint for how to split the work (any value
+ * gives the same sums up to rounding).
+ * q: WG_DT_*; its rows enter the product in f16 after an exact scaling by a power of
+ * two (fp32 is rounded to 11 bits), the weights too; sums and the softmax are
+ * fp32. out: WG_DT_F16 or WG_DT_BF16. */
+typedef struct wg_kv8_attn {
+  const void* q;
+  int64_t ldq;
+  int32_t q_dtype, n_head;
+  const int32_t* cu_q; /* [n_requests + 1] */
+  int32_t n_q, n_requests;
+  const int32_t* kv_lens;     /* [n_requests] */
+  const int32_t* block_table; /* [n_requests][ld_table] */
+  int64_t ld_table;
+  int32_t max_pages, max_q, max_kv, causal;
+  float scale;
+  int32_t out_dtype;
+  void* out;
+  int64_t ldo;
+} wg_kv8_attn;
+int wg_kv8_attention(const wg_kv8* cache, const wg_kv8_attn* p, int device, void* stream);
+
+/* Draws one token for each of R rows of logits (types WG_DT_*, rows ld apart;
+ * not modified). With z = logit / temperature, the row in descending order
+ * (lower index first among equals; NaN counts as -inf) and
+ * w = exp(z - max z), the tokens kept are the shortest prefix of that order in
+ * which every one
+ *   - is among the first top_k (top_k <= 0 or >= V: no limit),
+ *   - has less than top_p of the mass of those top_k before it (top_p >= 1: no limit),
+ *   - has w >= min_p (min_p <= 0: no limit);
+ * the first always stays. The token is the first in index order whose running
+ * mass among the kept ones exceeds u * their mass (u in [0, 1); the last kept
+ * one where none does). temperature <= 0 (or NaN): the first maximum. A row without a
+ * finite or +inf logit gives token -1 and log-prob -inf.
+ * temperature, top_k, top_p, min_p: [R], or NULL for 1, 0, 1 and 0.
+ * tokens [R]; logprobs [R] or NULL: log softmax(z) of the token over the whole
+ * row (z = logit where temperature <= 0). Decisions are made on masses held
+ * in 64 bits (fixed point), so a result does not depend on how a
+ * row was split. */
+typedef struct wg_sample {
+  const void* logits;
+  int64_t ld;
+  int32_t dtype, R, V;
+  const float* u;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int32_t* tokens;
+  float* logprobs;
+} wg_sample;
+int wg_sample_rows(const wg_sample* p, int device, void* stream);
+
 /* ---- measurement hooks used by bench.py ---------------------------------- */
 enum {
   WG_KCLASS_GEMV = 0,        /* the 6 weight matmuls of every layer */

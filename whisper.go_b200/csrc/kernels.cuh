@@ -224,4 +224,12 @@ int sample_test(const float* logits, int R, int V, const int32_t* hist, int n_hi
 // Reset of the per-job state before a decode.
 int launch_sample_reset(const SampleState& s, const int* prompt_dev, cudaStream_t st);
 
+// ---- serving operators (kv8.cu, kv8_attn.cu, sample_rows.cu) ------------------------
+// The launches behind wg_kv8_append, wg_kv8_attention and wg_sample_rows, for
+// the decode jobs: arguments are checked by the caller, `device` is current.
+int launch_kv8_append(const wg_kv8& c, const void* k, const void* v, int dt, int64_t ldk, int64_t ldv, bool veck,
+                      bool vecv, const int32_t* slots, int n, cudaStream_t st);
+int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cudaStream_t st);
+int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st);
+
 }  // namespace wg

@@ -1,0 +1,589 @@
+// kv8_attn.cu — attention over the 8-bit paged K/V cache (wg_kv8_attention).
+//
+// For query row i of a request of nq rows over len cached tokens
+//   s_j = scale * sk_j * (q_i . k_j)     k_j, v_j: int8 codes, sk, sv: the page's scales
+//   p_j = exp(s_j - max_j s_j)           over the visible j (causal: j <= len - nq + i)
+//   o_i = (1 / sum_j p_j) * sum_j p_j * sv_j * v_j,   0 where nothing is visible
+// in one pass over the cache with a running maximum and sum.
+//
+// The codes are exact in f16, so both products run on mma.m16n8k16 (f16 in,
+// fp32 accumulators); scales multiply the fp32 results. What bounds it is the
+// cache's bytes (2 * D bytes per token and head), and next to them the
+// instructions that turn a byte into an f16: per 32 tokens a warp spends ~100
+// on K, ~120 on V and ~32 MMAs. So:
+//  - a tile is the 16 rows of one MMA: (query, grouped head) pairs that share
+//    a K/V head, which covers single tokens, beams and grouped heads in one read;
+//  - every warp streams its own 32-token chunks through its own ring of
+//    cp.async stages (no CTA barrier in the loop, no bounded wait needed: a
+//    cp.async group always completes);
+//  - the MMA's k order is free as long as both operands agree, so a thread
+//    takes 16 consecutive codes of a token for Q.K^T (one 16-byte shared load
+//    per 8 tokens) and 8 or 16 consecutive dims of 4 tokens for P.V;
+//  - tokens are split over the CTAs of a cluster and joined through
+//    distributed shared memory: one launch, no workspace in global memory.
+#include <cooperative_groups.h>
+
+#include <mutex>
+
+#include "kernels.cuh"
+#include "ops.cuh"
+
+namespace wg {
+namespace {
+
+constexpr int AW = 4;        // warps per CTA
+constexpr int CH = 32;       // tokens per chunk
+constexpr int STAGES = 4;
+constexpr int MAX_SPLIT = 16;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnArgs {
+  const int8_t* codes;
+  const float* scales;
+  int num_pages, shift, H, G;
+  const void* q;
+  int64_t ldq;
+  int qdt;
+  const int* cu_q;
+  int n_q;
+  const int* kv_lens;
+  const int* table;
+  int64_t ldt;
+  int max_pages, R;
+  int tiles, splits, causal, max_q;
+  float scale;
+  void* out;
+  int64_t ldo;
+  int odt;
+};
+
+template <int D>
+constexpr int stage_bytes() { return 2 * CH * D + 32; }  // K, V, {sk[2], sv[2], page ok[2]}
+template <int D>
+constexpr int warp_bytes() { return STAGES * stage_bytes<D>(); }
+template <int D>
+constexpr int smem_bytes() { return AW * warp_bytes<D>(); }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Bytes (already offset by 128: code + 128) LO / HI of w as an f16 pair:
+// 0x6400 | u is 1024 + u, exact; minus 1152 gives the code.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
+  const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+// 2^x, x <= 0 (hardware approximation, 2^-22 relative; 0 for -inf)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+// Shared-memory byte offset of the 16-byte piece `part` of token tok in a
+// [32][D] block. Swizzled so that a quarter-warp's 16-byte reads of K (two
+// neighbouring tokens x 4 pieces) and a half-warp's 8-byte (D 64) or
+// quarter-warp's 16-byte (D 128) reads of V (tokens 2t + i of t = 0..3) each
+// touch every bank once.
+template <int D>
+__device__ __forceinline__ uint32_t k_off(int tok, int part) {
+  if constexpr (D == 64) return tok * 64 + part * 16;
+  return tok * 128 + ((part ^ ((tok & 1) << 2)) << 4);
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_off(int tok, int part) {
+  if constexpr (D == 64) {  // 128-byte lines of two tokens
+    const int line = tok >> 1, q = ((tok & 1) << 2) | part;
+    return line * 128 + ((q ^ ((line & 3) << 1)) << 4);
+  }
+  return tok * 128 + ((part ^ (((tok >> 1) & 3) << 1)) << 4);
+}
+
+// HALF: at most 8 rows are live, so the MMA's rows 8..15 are not processed
+// past the products. SMALL: 16-token pages (two pages, and scales, per chunk).
+template <int D, bool HALF, bool SMALL>
+__global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  pdl_trigger();
+  pdl_wait();
+  constexpr int PARTS = D / 16;  // 16-byte pieces of a token
+  constexpr int NT = D / 8;      // n-tiles of P.V
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int rank = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
+  const int tile = unit % p.tiles, h = (unit / p.tiles) % p.H, r = unit / p.tiles / p.H;
+  const int page = 1 << p.shift;
+  int q0 = __ldg(p.cu_q + r);
+  int nq = __ldg(p.cu_q + r + 1) - q0;
+  if (q0 < 0 || nq < 0 || q0 > p.n_q || nq > p.n_q - q0) nq = 0;
+  const int rows = min(16, min(nq, p.max_q) * p.G - tile * 16);
+  if (rows <= 0) return;  // the whole cluster: no row of this tile exists
+  const int len = min(max(__ldg(p.kv_lens + r), 0), (int)min((int64_t)p.max_pages << p.shift, (int64_t)0x7fffff00));
+  const int* table = p.table + (int64_t)r * p.ldt;
+  const int row0 = tile * 16;
+  // tokens [0, lim) are visible to a row
+  const int qa = (row0 + g) / p.G, qb = (row0 + g + 8) / p.G, qlast = (row0 + rows - 1) / p.G;
+  const int lim_a = p.causal ? max(0, len - nq + qa + 1) : len;
+  const int lim_b = p.causal ? max(0, len - nq + qb + 1) : len;
+  const int hi = p.causal ? max(0, len - nq + qlast + 1) : len;
+  const int lo_lim = p.causal ? max(0, len - nq + row0 / p.G + 1) : len;  // every row sees [0, lo_lim)
+  const int nch = (hi + CH - 1) / CH, per = (nch + p.splits - 1) / p.splits;
+  const int c_end = min(nch, (rank + 1) * per);
+  int c = rank * per + warp;
+
+  // ---- the warp's ring
+  uint8_t* ring = smem + warp * warp_bytes<D>();
+  const uint32_t ring_u = (uint32_t)__cvta_generic_to_shared(ring);
+  const int pages = (len + page - 1) >> p.shift;
+  auto page_id = [&](int chunk, int half) -> int {
+    const int col = (chunk * CH + half * 16) >> p.shift;
+    return chunk < c_end && col < pages ? __ldg(table + col) : -1;
+  };
+  auto issue = [&](int chunk, int stage, int id0, int id1) {
+    const uint32_t base = ring_u + stage * stage_bytes<D>();
+    const bool ok0 = (unsigned)id0 < (unsigned)p.num_pages, ok1 = (unsigned)id1 < (unsigned)p.num_pages;
+    const int in_page = (chunk * CH) & (page - 1);  // 0 with 16-token pages
+    const int64_t b0 = ((int64_t)(ok0 ? id0 : 0) * 2 * p.H + h), b1 = ((int64_t)(ok1 ? id1 : 0) * 2 * p.H + h);
+    const int8_t* k0 = p.codes + (b0 * page + in_page) * D;
+    const int8_t* k1 = SMALL ? p.codes + b1 * page * D : k0 + 16 * D;
+    const int64_t kv_step = (int64_t)p.H * page * D;
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) {
+      const int idx = i * 32 + lane, tok = idx / PARTS, part = idx % PARTS;
+      const bool second = tok >= 16;
+      const int8_t* src = (second ? k1 + (tok - 16) * D : k0 + tok * D) + part * 16;
+      const bool on = second && SMALL ? ok1 : ok0;
+      cp16(base + k_off<D>(tok, part), src, on);
+      cp16(base + CH * D + v_off<D>(tok, part), src + kv_step, on);
+    }
+    if (lane < 4) {  // sk[0], sk[1], sv[0], sv[1]
+      const bool second = (lane & 1) != 0;
+      cp4(base + 2 * CH * D + lane * 4, p.scales + (second && SMALL ? b1 : b0) + (lane >> 1) * p.H,
+          second && SMALL ? ok1 : ok0);
+    } else if (lane < 6) {
+      reinterpret_cast<int*>(ring + stage * stage_bytes<D>() + 2 * CH * D)[lane] = (lane == 4 || !SMALL) ? ok0 : ok1;
+    }
+  };
+  int id0[STAGES], id1[STAGES];
+#pragma unroll
+  for (int s = 0; s < STAGES; s++) {
+    id0[s] = page_id(c + s * AW, 0);
+    id1[s] = SMALL ? page_id(c + s * AW, 1) : id0[s];
+  }
+#pragma unroll
+  for (int s = 0; s < STAGES; s++) {
+    if (c + s * AW < c_end) issue(c + s * AW, s, id0[s], id1[s]);
+    cp_commit();
+  }
+  int nid0 = page_id(c + STAGES * AW, 0), nid1 = SMALL ? page_id(c + STAGES * AW, 1) : nid0;
+
+  // ---- Q as A fragments: thread t of row g takes dims 16t..16t+15 of each
+  // 64 (the 16 consecutive codes it reads of a token). Rows of bf16 or fp32
+  // are scaled by a power of two so that they fit f16: bf16 stays exact down
+  // to 2^-23 of the row's largest value, fp32 is rounded to f16's 11 bits.
+  uint32_t qa_f[D / 16][4];
+  float mul_a, mul_b;
+  {
+    float e[2];
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const int row = g + half * 8;
+      const bool live = row < rows && !(HALF && half);
+      const int qi = (row0 + row) / p.G, hg = (row0 + row) % p.G;
+      const int64_t base = (int64_t)(q0 + qi) * p.ldq + ((int64_t)h * p.G + hg) * D + 16 * t;
+      float x[D / 4];
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 4; i++) {
+        x[i] = live ? dt_load(p.q, base + (i / 16) * 64 + (i % 16), p.qdt) : 0.f;
+        mx = fmaxf(mx, fabsf(x[i]));
+      }
+      mx = quad_max(mx);
+      float up = 1.f;
+      e[half] = 1.f;
+      if (p.qdt != WG_DT_F16 && mx > 0.f && mx <= 3.402823466e38f) {
+        // 2^-k and 2^k with 2^k <= mx < 2^(k+1)
+        const int k = min(max((int)(__float_as_uint(mx) >> 23) - 127, -120), 120);
+        up = __uint_as_float((uint32_t)(127 - k) << 23);
+        e[half] = __uint_as_float((uint32_t)(127 + k) << 23);
+      }
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) {  // MMA k step j: dims 16t + 4(j%4) .. +3 of 64-block j/4
+        const int o = (j / 4) * 16 + (j % 4) * 4;
+        qa_f[j][half] = pack_f16(x[o] * up, x[o + 1] * up);
+        qa_f[j][2 + half] = pack_f16(x[o + 2] * up, x[o + 3] * up);
+      }
+    }
+    mul_a = e[0] * p.scale * LOG2E;  // scores in units of log 2
+    mul_b = e[1] * p.scale * LOG2E;
+  }
+
+  float o_acc[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; j++) o_acc[j][0] = o_acc[j][1] = o_acc[j][2] = o_acc[j][3] = 0.f;
+  float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+
+  for (int stage = 0; c < c_end; c += AW, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+    cp_wait<STAGES - 1>();
+    __syncwarp();
+    const uint8_t* st = ring + stage * stage_bytes<D>();
+    const float* sc = reinterpret_cast<const float*>(st + 2 * CH * D);
+    const float sk0 = sc[0], sk1 = sc[1], sv0 = sc[2], sv1 = sc[3];
+    const bool ok0 = reinterpret_cast<const int*>(sc)[4] != 0, ok1 = reinterpret_cast<const int*>(sc)[5] != 0;
+
+    // ---- scores of 4 n-tiles of 8 tokens
+    float s[4][4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int b = 0; b < D / 64; b++) {
+        const uint4 w4 = *reinterpret_cast<const uint4*>(st + k_off<D>(n * 8 + g, b * 4 + t));
+        const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          mma16816(s[n], qa_f[b * 4 + j], codes_f16<0x4140>(w[j]), codes_f16<0x4342>(w[j]));
+      }
+      const float sk = n < 2 ? sk0 : sk1;
+      s[n][0] *= sk * mul_a;
+      s[n][1] *= sk * mul_a;
+      s[n][2] *= sk * mul_b;
+      s[n][3] *= sk * mul_b;
+    }
+    if ((c + 1) * CH > lo_lim || !ok0 || !ok1) {
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        const int j = c * CH + n * 8 + 2 * t;
+        const bool ok = n < 2 ? ok0 : ok1;
+        if (!ok || j >= lim_a) s[n][0] = -INFINITY;
+        if (!ok || j + 1 >= lim_a) s[n][1] = -INFINITY;
+        if (!ok || j >= lim_b) s[n][2] = -INFINITY;
+        if (!ok || j + 1 >= lim_b) s[n][3] = -INFINITY;
+      }
+    }
+    // ---- running maximum and sum
+    float x_a = m_a, x_b = m_b;
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      x_a = fmaxf(x_a, fmaxf(s[n][0], s[n][1]));
+      if (!HALF) x_b = fmaxf(x_b, fmaxf(s[n][2], s[n][3]));
+    }
+    x_a = quad_max(x_a);
+    if (!HALF) x_b = quad_max(x_b);
+    const float ref_a = x_a == -INFINITY ? 0.f : x_a, ref_b = x_b == -INFINITY ? 0.f : x_b;
+    const bool moved = HALF ? x_a != m_a : (x_a != m_a || x_b != m_b);
+    if (__any_sync(0xffffffffu, moved)) {
+      const float al_a = ex2(m_a - ref_a), al_b = HALF ? 1.f : ex2(m_b - ref_b);
+      l_a *= al_a;
+      l_b *= al_b;
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        o_acc[j][0] *= al_a;
+        o_acc[j][1] *= al_a;
+        if (!HALF) {
+          o_acc[j][2] *= al_b;
+          o_acc[j][3] *= al_b;
+        }
+      }
+      m_a = x_a;
+      m_b = x_b;
+    }
+    // weights rounded to f16 for the MMA (2^-12 of a weight that is at most 1); the sum keeps fp32
+    uint32_t pf[2][4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      const float p0 = ex2(s[n][0] - ref_a), p1 = ex2(s[n][1] - ref_a);
+      l_a += p0 + p1;
+      pf[n >> 1][(n & 1) * 2] = pack_f16(p0, p1);
+      if (!HALF) {
+        const float p2 = ex2(s[n][2] - ref_b), p3 = ex2(s[n][3] - ref_b);
+        l_b += p2 + p3;
+        pf[n >> 1][(n & 1) * 2 + 1] = pack_f16(p2, p3);
+      } else {
+        pf[n >> 1][(n & 1) * 2 + 1] = 0u;
+      }
+    }
+    // ---- P.V: n-tile j of lane g is dim g * (D/8) + j; tokens 2t, 2t+1, 2t+8, 2t+9 of each 16
+    const uint8_t* vs = st + CH * D;
+    constexpr int VW = D / 32;  // words of a lane's dims per token
+    uint32_t w[2][4][VW];
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int tok = hf * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+        if constexpr (D == 64) {
+          const uint2 v = *reinterpret_cast<const uint2*>(vs + v_off<D>(tok, g >> 1) + (g & 1) * 8);
+          w[hf][i][0] = v.x ^ 0x80808080u;
+          w[hf][i][1] = v.y ^ 0x80808080u;
+        } else {
+          const uint4 v = *reinterpret_cast<const uint4*>(vs + v_off<D>(tok, g));
+          w[hf][i][0] = v.x ^ 0x80808080u;
+          w[hf][i][1] = v.y ^ 0x80808080u;
+          w[hf][i][2] = v.z ^ 0x80808080u;
+          w[hf][i][3] = v.w ^ 0x80808080u;
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < VW; k++) {
+      uint32_t z[2][4];  // bytes (token 0, token 1) of dims 0,1 | 2,3; the same of tokens 2, 3
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        z[hf][0] = __byte_perm(w[hf][0][k], w[hf][1][k], 0x5140);
+        z[hf][1] = __byte_perm(w[hf][0][k], w[hf][1][k], 0x7362);
+        z[hf][2] = __byte_perm(w[hf][2][k], w[hf][3][k], 0x5140);
+        z[hf][3] = __byte_perm(w[hf][2][k], w[hf][3][k], 0x7362);
+      }
+#pragma unroll
+      for (int dd = 0; dd < 4; dd++) {
+        const int j = k * 4 + dd;
+        float acc[2][4];
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          float(&a)[4] = acc[SMALL ? hf : 0];
+          if (SMALL || hf == 0) a[0] = a[1] = a[2] = a[3] = 0.f;
+          const uint32_t b0 = (dd & 1) ? codes_f16<0x4342>(z[hf][dd >> 1]) : codes_f16<0x4140>(z[hf][dd >> 1]);
+          const uint32_t b1 = (dd & 1) ? codes_f16<0x4342>(z[hf][2 + (dd >> 1)]) : codes_f16<0x4140>(z[hf][2 + (dd >> 1)]);
+          mma16816(a, pf[hf], b0, b1);
+        }
+#pragma unroll
+        for (int x = 0; x < (HALF ? 2 : 4); x++) {
+          o_acc[j][x] = fmaf(sv0, acc[0][x], o_acc[j][x]);
+          if (SMALL) o_acc[j][x] = fmaf(sv1, acc[1][x], o_acc[j][x]);
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the stage
+    if (c + STAGES * AW < c_end) issue(c + STAGES * AW, stage, nid0, nid1);
+    cp_commit();
+    nid0 = page_id(c + (STAGES + 1) * AW, 0);
+    nid1 = SMALL ? page_id(c + (STAGES + 1) * AW, 1) : nid0;
+  }
+  cp_wait<0>();
+
+  // ---- join the warps: (m, l, O) of each in its own ring's memory
+  l_a = quad_sum(l_a);
+  l_b = quad_sum(l_b);
+  __syncwarp();
+  float* wo = reinterpret_cast<float*>(ring);  // [16][D] O, then [16] m, [16] l
+  {
+    // lane (g, t) holds dims 2t * D/8 .. (2t + 2) * D/8 - 1 of rows g, g + 8
+#pragma unroll
+    for (int half = 0; half < (HALF ? 1 : 2); half++)
+#pragma unroll
+      for (int cc = 0; cc < 2; cc++)
+#pragma unroll
+        for (int j = 0; j < NT; j += 4)
+          *reinterpret_cast<float4*>(wo + (g + half * 8) * D + (2 * t + cc) * NT + j) =
+              make_float4(o_acc[j][half * 2 + cc], o_acc[j + 1][half * 2 + cc], o_acc[j + 2][half * 2 + cc],
+                          o_acc[j + 3][half * 2 + cc]);
+    if (t == 0) {
+      wo[16 * D + g] = m_a;
+      wo[16 * D + 16 + g] = l_a;
+      if (!HALF) {
+        wo[16 * D + g + 8] = m_b;
+        wo[16 * D + 24 + g] = l_b;
+      }
+    }
+  }
+  __syncthreads();
+  // CTA total into warp 0's block: each (row, 4 dims) by one thread
+  constexpr int WF = warp_bytes<D>() / 4;  // floats between the warps' blocks
+  float* cta = reinterpret_cast<float*>(smem);
+  float* cta_ml = cta + AW * WF;  // [16] m, [16] l of the CTA, past every ring
+  for (int row = tid; row < rows; row += AW * 32) {
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < AW; k++) m = fmaxf(m, cta[k * WF + 16 * D + row]);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int k = 0; k < AW; k++) l += cta[k * WF + 16 * D + 16 + row] * ex2(cta[k * WF + 16 * D + row] - ref);
+    cta_ml[row] = m;
+    cta_ml[16 + row] = l;
+  }
+  for (int i = tid; i < rows * (D / 4); i += AW * 32) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < AW; k++) m = fmaxf(m, cta[k * WF + 16 * D + row]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < AW; k++) {
+      const float f = ex2(cta[k * WF + 16 * D + row] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(cta + k * WF + row * D + d);
+      a.x = fmaf(v.x, f, a.x);
+      a.y = fmaf(v.y, f, a.y);
+      a.z = fmaf(v.z, f, a.z);
+      a.w = fmaf(v.w, f, a.w);
+    }
+    // in place: this thread alone reads and writes these four floats of every warp's block
+    *reinterpret_cast<float4*>(cta + row * D + d) = a;
+  }
+  // ---- join the cluster's CTAs: rank k finishes every splits-th (row, 4 dims)
+  namespace cg = cooperative_groups;
+  if (p.splits > 1) cg::this_cluster().sync();
+  else __syncthreads();
+  for (int i = tid * p.splits + rank; i < rows * (D / 4); i += AW * 32 * p.splits) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    float m = -INFINITY, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.splits; k++) {
+      const float* peer = p.splits > 1 ? cg::this_cluster().map_shared_rank(cta, k) : cta;
+      const float pm = peer[AW * WF + row], pl = peer[AW * WF + 16 + row];
+      const float4 v = *reinterpret_cast<const float4*>(peer + row * D + d);
+      const float nm = fmaxf(m, pm), ref = nm == -INFINITY ? 0.f : nm;
+      const float fo = ex2(m - ref), fn = ex2(pm - ref);
+      l = l * fo + pl * fn;
+      a.x = a.x * fo + v.x * fn;
+      a.y = a.y * fo + v.y * fn;
+      a.z = a.z * fo + v.z * fn;
+      a.w = a.w * fo + v.w * fn;
+      m = nm;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // nothing visible: zeros; NaN stays
+    const int qi = (row0 + row) / p.G, hg = (row0 + row) % p.G;
+    const int64_t at = (int64_t)(q0 + qi) * p.ldo + ((int64_t)h * p.G + hg) * D + d;
+    dt_store(p.out, at, p.odt, a.x * inv);
+    dt_store(p.out, at + 1, p.odt, a.y * inv);
+    dt_store(p.out, at + 2, p.odt, a.z * inv);
+    dt_store(p.out, at + 3, p.odt, a.w * inv);
+  }
+  if (p.splits > 1) cg::this_cluster().sync();  // peers may still be reading this CTA
+}
+
+typedef void (*AttnKernel)(const AttnArgs);
+template <int D>
+AttnKernel pick(bool half, bool small) {
+  if (half) return small ? decode_attn_kernel<D, true, true> : decode_attn_kernel<D, true, false>;
+  return small ? decode_attn_kernel<D, false, true> : decode_attn_kernel<D, false, false>;
+}
+
+std::mutex g_attr_mu;
+bool g_attr_done[OPS_MAX_DEV];
+
+int set_attributes(int device) {
+  if (device >= OPS_MAX_DEV) {
+    set_error("wg_kv8_attention: device %d out of range", device);
+    return WG_ERR_INVALID;
+  }
+  std::lock_guard<std::mutex> lk(g_attr_mu);
+  if (g_attr_done[device]) return WG_OK;
+  for (int i = 0; i < 4; i++) {
+    AttnKernel k64 = pick<64>(i & 1, i & 2), k128 = pick<128>(i & 1, i & 2);
+    WG_CHECK_CUDA(cudaFuncSetAttribute(k64, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<64>() + 128));
+    WG_CHECK_CUDA(cudaFuncSetAttribute(k128, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<128>() + 128));
+    WG_CHECK_CUDA(cudaFuncSetAttribute(k64, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    WG_CHECK_CUDA(cudaFuncSetAttribute(k128, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  }
+  g_attr_done[device] = true;
+  return WG_OK;
+}
+
+}  // namespace
+
+// The launch behind wg_kv8_attention (arguments checked, device current).
+int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cudaStream_t st) {
+  WG_CHECK(set_attributes(device));
+  const int G = p.n_head / c.n_kv_head;
+  AttnArgs a{};
+  a.codes = c.codes; a.scales = c.scales; a.num_pages = c.num_pages; a.shift = log2_of(c.page);
+  a.H = c.n_kv_head; a.G = G; a.q = p.q; a.ldq = p.ldq; a.qdt = p.q_dtype; a.cu_q = p.cu_q; a.n_q = p.n_q;
+  a.kv_lens = p.kv_lens; a.table = p.block_table; a.ldt = p.ld_table; a.max_pages = p.max_pages; a.R = p.n_requests;
+  a.causal = p.causal; a.max_q = p.max_q; a.scale = p.scale; a.out = p.out; a.ldo = p.ldo; a.odt = p.out_dtype;
+  const int64_t rows = (int64_t)p.max_q * G;
+  const int64_t tiles = (rows + 15) / 16, units = tiles * c.n_kv_head * p.n_requests;
+  const int64_t kv = p.max_kv < ((int64_t)p.max_pages << a.shift) ? p.max_kv : (int64_t)p.max_pages << a.shift;
+  const int64_t chunks = (kv + CH - 1) / CH;
+  // CTAs per tile: enough for two rounds of the SMs' resident CTAs, no less
+  // than two chunks for each warp, and no CTA with more than 64 chunks
+  // (2048 tokens), so that one long request among short ones is spread too
+  int64_t s = (148 * 6 + units - 1) / units;
+  if (s > chunks / (2 * AW)) s = chunks / (2 * AW);
+  if (s < (chunks + 63) / 64) s = (chunks + 63) / 64;
+  a.splits = (int)(s < 1 ? 1 : s > MAX_SPLIT ? MAX_SPLIT : s);
+  a.tiles = (int)tiles;
+  if (units * a.splits > 0x7fffffffLL) {
+    set_error("wg_kv8_attention: %lld CTAs are more than a grid holds", (long long)(units * a.splits));
+    return WG_ERR_INVALID;
+  }
+  const bool d64 = c.head_dim == 64;
+  AttnKernel k = d64 ? pick<64>(rows <= 8, c.page == 16) : pick<128>(rows <= 8, c.page == 16);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * a.splits));
+  cfg.blockDim = dim3(AW * 32);
+  cfg.dynamicSmemBytes = (d64 ? smem_bytes<64>() : smem_bytes<128>()) + 128;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = a.splits;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = pdl_enabled() ? at : at + 1;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return launch_check(cudaLaunchKernelEx(&cfg, k, a), "kv8_attention");
+}
+
+}  // namespace wg
+
+extern "C" int wg_kv8_attention(const wg_kv8* cache, const wg_kv8_attn* p, int device, void* stream) {
+  using namespace wg;
+  const char* what = "wg_kv8_attention";
+  WG_CHECK(kv8_check(what, cache));
+  if (!p || p->n_requests < 0 || p->n_q < 0 || p->max_q < 0 || p->max_kv < 0 || p->max_pages < 0 ||
+      p->ld_table < p->max_pages) {
+    set_error("%s: bad argument", what);
+    return WG_ERR_INVALID;
+  }
+  if (p->n_head <= 0 || p->n_head % cache->n_kv_head) {
+    set_error("%s: %d query heads over %d K/V heads", what, p->n_head, cache->n_kv_head);
+    return WG_ERR_INVALID;
+  }
+  if (!dt_ok(p->q_dtype) || (p->out_dtype != WG_DT_F16 && p->out_dtype != WG_DT_BF16)) {
+    set_error("%s: unsupported types (q %d, out %d: out is f16 or bf16)", what, p->q_dtype, p->out_dtype);
+    return WG_ERR_UNSUPPORTED;
+  }
+  if (!(p->scale == p->scale) || p->scale > 3.4e38f || p->scale < -3.4e38f) {
+    set_error("%s: the scale is not finite", what);
+    return WG_ERR_INVALID;
+  }
+  if (p->n_requests == 0 || p->n_q == 0 || p->max_q == 0) return WG_OK;
+  const int64_t width = (int64_t)p->n_head * cache->head_dim;
+  if (!p->q || !p->out || !p->cu_q || !p->kv_lens || (p->max_pages > 0 && !p->block_table) || p->ldq < width ||
+      p->ldo < width || reinterpret_cast<uintptr_t>(p->q) % dt_bytes(p->q_dtype) ||
+      reinterpret_cast<uintptr_t>(p->out) % 2) {
+    set_error("%s: null or misaligned tensor, or rows closer than %lld elements", what, (long long)width);
+    return WG_ERR_INVALID;
+  }
+  OpDevice dev;
+  WG_CHECK(dev.enter(what, device));
+  return launch_kv8_attention(*cache, *p, device, reinterpret_cast<cudaStream_t>(stream));
+}

@@ -85,6 +85,27 @@ class WgDecodeParams(ctypes.Structure):
     ]
 
 
+class WgKv8(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("num_pages", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("n_kv_head", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class WgKv8Attn(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("q_dtype", ctypes.c_int32),
+                ("n_head", ctypes.c_int32), ("cu_q", ctypes.c_void_p), ("n_q", ctypes.c_int32),
+                ("n_requests", ctypes.c_int32), ("kv_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("ld_table", ctypes.c_int64), ("max_pages", ctypes.c_int32), ("max_q", ctypes.c_int32),
+                ("max_kv", ctypes.c_int32), ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("out_dtype", ctypes.c_int32), ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64)]
+
+
+class WgSample(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_int64), ("dtype", ctypes.c_int32), ("R", ctypes.c_int32),
+                ("V", ctypes.c_int32), ("u", ctypes.c_void_p), ("temperature", ctypes.c_void_p),
+                ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
+                ("tokens", ctypes.c_void_p), ("logprobs", ctypes.c_void_p)]
+
+
 _lib = None
 _gen = None
 _lock = threading.Lock()
@@ -138,6 +159,14 @@ def _declare(lib):
                                           c_float_p]),
         "wg_job_time_kernel": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_double),
                                               ctypes.POINTER(ctypes.c_double)]),
+        "wg_kv_plan": (ctypes.c_int, [P, P, ctypes.c_int, ctypes.c_int, P, ctypes.c_int, P, P, P, ctypes.c_int64,
+                                      ctypes.c_int, P, ctypes.c_int, P, P, ctypes.c_int, P]),
+        "wg_kv8_append": (ctypes.c_int, [ctypes.POINTER(WgKv8), P, P, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, P,
+                                         ctypes.c_int, ctypes.c_int, P]),
+        "wg_kv8_read": (ctypes.c_int, [ctypes.POINTER(WgKv8), P, ctypes.c_int, P, P, ctypes.c_int, ctypes.c_int64,
+                                       ctypes.c_int64, ctypes.c_int, P]),
+        "wg_kv8_attention": (ctypes.c_int, [ctypes.POINTER(WgKv8), ctypes.POINTER(WgKv8Attn), ctypes.c_int, P]),
+        "wg_sample_rows": (ctypes.c_int, [ctypes.POINTER(WgSample), ctypes.c_int, P]),
         "wg_model_matmul_noalloc": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                                    ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                                                    ctypes.c_void_p, ctypes.c_int]),
@@ -818,3 +847,181 @@ def quantize_matrix(qtype, m: np.ndarray) -> bytes:
     if gen().wg_gen_quantize_matrix(qt, m.ctypes.data_as(c_float_p), rows, cols, out.ctypes.data) != 0:
         raise ValueError("unsupported qtype")
     return out.tobytes()
+
+
+# ---- serving operators on device tensors ------------------------------------------
+# Torch CUDA tensors in, torch CUDA tensors out: each call is enqueued on the
+# current torch stream of the tensors' device and returns without waiting.
+def _op_check(rc: int, what: str):
+    if rc != WG_OK:
+        raise DecodeError("%s: %s" % (what, last_error()), rc)
+
+
+_DT_NAMES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
+_dt_of = {}
+
+
+def _dt(t, what: str) -> int:
+    """WG_DT_* of a float tensor."""
+    code = _dt_of.get(t.dtype)
+    if code is None:
+        code = _DT_NAMES.get(str(t.dtype))
+        if code is None:
+            raise DecodeError("%s: unsupported type %s" % (what, t.dtype), 4)
+        _dt_of[t.dtype] = code
+    return code
+
+
+def _place(what: str, *tensors):
+    """(device index, raw stream) of tensors that must share a CUDA device."""
+    import torch
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise DecodeError("%s: tensors must be on a CUDA device" % what)
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise DecodeError("%s: tensors on different devices (%s, %s)" % (what, dev, t.device))
+    return dev.index, torch.cuda.current_stream(dev).cuda_stream
+
+
+def _vec(what: str, name: str, t, dtype: str, n: int):
+    """Address of a contiguous one-dimensional tensor of n values (None: NULL)."""
+    if t is None:
+        return None
+    if str(t.dtype) != dtype or t.ndim != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise DecodeError("%s: %s must be %s [%d], contiguous" % (what, name, dtype, n))
+    return t.data_ptr()
+
+
+def _rows(what: str, name: str, t, heads: int, dim: int):
+    """Distance of the rows of a [n, heads, dim] (or [n, heads * dim]) tensor in elements."""
+    if t.ndim == 3:
+        ok = t.shape[1:] == (heads, dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == dim)
+    else:
+        ok = t.ndim == 2 and t.shape[1] == heads * dim and t.stride(1) == 1
+    if not ok:
+        raise DecodeError("%s: %s must be [n, %d, %d] with contiguous heads and dims, got %s strides %s" %
+                          (what, name, heads, dim, tuple(t.shape), tuple(t.stride())))
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+def kv_plan(lens, new_tokens, page: int, free_pages, cursor, block_table, slots, cu_new, status, cursor_out=None):
+    """Block tables and slot maps from the requests' lengths (wg_kv_plan).
+    All int32 CUDA tensors; lens, new_tokens [R], block_table [R, max_pages]
+    (rows may be strided), slots [any], cu_new [R + 1], status [2], cursor [1]
+    (advanced in place unless cursor_out is given)."""
+    what = "kv_plan"
+    R = lens.shape[0]
+    if cursor_out is None:
+        cursor_out = cursor
+    dev, st = _place(what, lens, new_tokens, free_pages, cursor, cursor_out, block_table, slots, cu_new, status)
+    i32 = "torch.int32"
+    if (str(block_table.dtype) != i32 or block_table.ndim != 2 or block_table.shape[0] != R or
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        raise DecodeError("%s: block_table must be int32 [%d, max_pages]" % (what, R))
+    _op_check(lib().wg_kv_plan(
+        _vec(what, "lens", lens, i32, R), _vec(what, "new_tokens", new_tokens, i32, R), R, page,
+        _vec(what, "free_pages", free_pages, i32, free_pages.shape[0]), free_pages.shape[0],
+        _vec(what, "cursor", cursor, i32, 1), _vec(what, "cursor_out", cursor_out, i32, 1), block_table.data_ptr(),
+        block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1],
+        _vec(what, "slots", slots, i32, slots.shape[0]), slots.shape[0], _vec(what, "cu_new", cu_new, i32, R + 1),
+        _vec(what, "status", status, i32, 2), dev, st), what)
+
+
+class Kv8Cache:
+    """A paged K/V cache of 8-bit codes (wg_kv8) over two CUDA tensors of the
+    caller: codes int8 [num_pages, 2, n_kv_head, page, head_dim], scales fp32
+    [num_pages, 2, n_kv_head]; value = code * scale. alloc() makes both."""
+
+    def __init__(self, codes, scales):
+        what = "Kv8Cache"
+        if (str(codes.dtype) != "torch.int8" or codes.ndim != 5 or codes.shape[1] != 2 or not codes.is_contiguous() or
+                str(scales.dtype) != "torch.float32" or tuple(scales.shape) != tuple(codes.shape[:3]) or
+                not scales.is_contiguous()):
+            raise DecodeError("%s: codes must be int8 [pages, 2, heads, page, dim], scales fp32 [pages, 2, heads], "
+                              "both contiguous" % what)
+        if codes.device.type != "cuda" or scales.device != codes.device:
+            raise DecodeError("%s: tensors must be on one CUDA device" % what)
+        self.codes, self.scales = codes, scales
+        self.num_pages, _, self.n_kv_head, self.page, self.head_dim = codes.shape
+        self._c = WgKv8(codes.data_ptr(), scales.data_ptr(), self.num_pages, self.page, self.n_kv_head, self.head_dim)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def alloc(cls, num_pages: int, page: int, n_kv_head: int, head_dim: int = 64, device="cuda") -> "Kv8Cache":
+        import torch
+        return cls(torch.empty(num_pages, 2, n_kv_head, page, head_dim, dtype=torch.int8, device=device),
+                   torch.empty(num_pages, 2, n_kv_head, dtype=torch.float32, device=device))
+
+    def _kv(self, what, k, v, slots):
+        ldk = _rows(what, "k", k, self.n_kv_head, self.head_dim)
+        ldv = _rows(what, "v", v, self.n_kv_head, self.head_dim)
+        n = k.shape[0]
+        if v.shape[0] != n or v.dtype != k.dtype:
+            raise DecodeError("%s: k and v must have the same rows and type" % what)
+        return _vec(what, "slots", slots, "torch.int32", n), n, _dt(k, what), ldk, ldv
+
+    def append(self, k, v, slots):
+        """Writes the rows of k and v ([n, n_kv_head, head_dim]) into their slots (wg_kv8_append)."""
+        what = "kv8_append"
+        sp, n, dt, ldk, ldv = self._kv(what, k, v, slots)
+        dev, st = _place(what, self.codes, k, v, slots)
+        _op_check(lib().wg_kv8_append(self._ref, k.data_ptr(), v.data_ptr(), dt, ldk, ldv, sp, n, dev, st), what)
+
+    def read(self, slots, k, v):
+        """The values at `slots` into the rows of k and v (wg_kv8_read)."""
+        what = "kv8_read"
+        sp, n, dt, ldk, ldv = self._kv(what, k, v, slots)
+        dev, st = _place(what, self.codes, k, v, slots)
+        _op_check(lib().wg_kv8_read(self._ref, sp, n, k.data_ptr(), v.data_ptr(), dt, ldk, ldv, dev, st), what)
+
+    def attention(self, q, cu_q, kv_lens, block_table, max_q: int, max_kv: int, causal: bool = True,
+                  scale: Optional[float] = None, out=None):
+        """Attention of the rows of q ([n_q, n_head, head_dim]) over the cached
+        tokens of their requests (wg_kv8_attention); returns out, by default a
+        new tensor of q's type (f16 where q is fp32)."""
+        what = "kv8_attention"
+        D = self.head_dim
+        if q.ndim != 3 or q.shape[2] != D:
+            raise DecodeError("%s: q must be [n, heads, %d], got %s" % (what, D, tuple(q.shape)))
+        n_head, R = q.shape[1], kv_lens.shape[0]
+        qdt = _dt(q, what)
+        if out is None:
+            import torch
+            out = torch.zeros(q.shape, dtype=torch.float16 if qdt == 0 else q.dtype, device=q.device)
+        if out.shape != q.shape:
+            raise DecodeError("%s: out must be %s" % (what, tuple(q.shape)))
+        if (str(block_table.dtype) != "torch.int32" or block_table.ndim != 2 or block_table.shape[0] != R or
+                (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+            raise DecodeError("%s: block_table must be int32 [%d, max_pages]" % (what, R))
+        dev, st = _place(what, self.codes, q, cu_q, kv_lens, block_table, out)
+        p = WgKv8Attn(q.data_ptr(), _rows(what, "q", q, n_head, D), qdt, n_head,
+                      _vec(what, "cu_q", cu_q, "torch.int32", R + 1), q.shape[0], R,
+                      _vec(what, "kv_lens", kv_lens, "torch.int32", R), block_table.data_ptr(),
+                      block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1], max_q, max_kv,
+                      1 if causal else 0, D ** -0.5 if scale is None else scale, _dt(out, what), out.data_ptr(),
+                      _rows(what, "out", out, n_head, D))
+        _op_check(lib().wg_kv8_attention(self._ref, ctypes.byref(p), dev, st), what)
+        return out
+
+
+def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None):
+    """One token per row of logits [R, V] from the random numbers u [R]
+    (wg_sample_rows); temperature, top_p, min_p fp32 [R], top_k int32 [R], each
+    optional. Returns (tokens int32 [R], logprobs fp32 [R])."""
+    what = "sample_rows"
+    if logits.ndim != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise DecodeError("%s: logits must be [rows, vocabulary] with contiguous rows" % what)
+    R, V = logits.shape
+    if tokens is None or logprobs is None:
+        import torch
+        tokens = torch.empty(R, dtype=torch.int32, device=logits.device) if tokens is None else tokens
+        logprobs = torch.empty(R, dtype=torch.float32, device=logits.device) if logprobs is None else logprobs
+    dev, st = _place(what, logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
+    f32 = "torch.float32"
+    p = WgSample(logits.data_ptr(), logits.stride(0) if R > 1 else V, _dt(logits, what), R, V, _vec(what, "u", u, f32, R),
+                 _vec(what, "temperature", temperature, f32, R), _vec(what, "top_k", top_k, "torch.int32", R),
+                 _vec(what, "top_p", top_p, f32, R), _vec(what, "min_p", min_p, f32, R),
+                 _vec(what, "tokens", tokens, "torch.int32", R), _vec(what, "logprobs", logprobs, f32, R))
+    _op_check(lib().wg_sample_rows(ctypes.byref(p), dev, st), what)
+    return tokens, logprobs
