@@ -19,10 +19,16 @@ DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 ITEM = {"f32": 4, "f16": 2, "bf16": 2}
 
 
+wgdec = None
+
+
 def _wgdec():
-    if str(ROOT / "whisper.go_b200") not in sys.path:
+    """The framework's module, imported once (its folder's name is no module name)."""
+    global wgdec
+    if wgdec is None:
         sys.path.insert(0, str(ROOT / "whisper.go_b200"))
-    import wgdec
+        import wgdec as module
+        wgdec = module
     return wgdec
 
 
@@ -345,9 +351,9 @@ def run(s):
         _append(s)
         _read(s)
         return {"k": s["k_out"], "v": s["v_out"], "scales": s["scales"]}
-    wgdec = _wgdec()
+    lib = _wgdec()
     if op == "plan":
-        wgdec.kv_plan(s["lens"], s["new"], case["page"], s["free"], s["cursor"], s["table"], s["slots"], s["cu"],
+        lib.kv_plan(s["lens"], s["new"], case["page"], s["free"], s["cursor"], s["table"], s["slots"], s["cu"],
                       s["status"], cursor_out=s["cursor_out"])
         return {"table": s["table"], "slots": s["slots"], "cu": s["cu"], "cursor": s["cursor_out"],
                 "status": s["status"]}
@@ -356,7 +362,7 @@ def run(s):
                              causal=case["causal"], scale=s["scale"], out=s["out"])
         return s["out"]
     if op == "sample":
-        wgdec.sample_rows(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"],
+        lib.sample_rows(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"],
                           min_p=s["min_p"], tokens=s["tokens"], logprobs=s["logprobs"])
         return {"tokens": s["tokens"], "logprobs": s["logprobs"]}
     s["cache"].append(s["k"], s["v"], s["slots"])
