@@ -852,57 +852,84 @@ def quantize_matrix(qtype, m: np.ndarray) -> bytes:
 # ---- serving operators on device tensors ------------------------------------------
 # Torch CUDA tensors in, torch CUDA tensors out: each call is enqueued on the
 # current torch stream of the tensors' device and returns without waiting.
+# The checks use the cheapest tensor queries: a decode step makes these calls
+# for every layer, and the GPU's part of a small one is a few microseconds.
+class _Torch:
+    """torch's names that the operators use, looked up once at the first call
+    (the rest of this module needs no torch)."""
+
+    def __init__(self):
+        import torch
+        self.i32, self.f32, self.i8 = torch.int32, torch.float32, torch.int8
+        self.dt = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # WG_DT_*
+        self.torch = torch
+        self.lib = lib()
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.stream = raw or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+_torch = None
+
+
+def _t() -> _Torch:
+    global _torch
+    if _torch is None:
+        _torch = _Torch()
+    return _torch
+
+
 def _op_check(rc: int, what: str):
     if rc != WG_OK:
         raise DecodeError("%s: %s" % (what, last_error()), rc)
 
 
-_DT_NAMES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
-_dt_of = {}
-
-
-def _dt(t, what: str) -> int:
+def _dt(T, t, what: str) -> int:
     """WG_DT_* of a float tensor."""
-    code = _dt_of.get(t.dtype)
+    code = T.dt.get(t.dtype)
     if code is None:
-        code = _DT_NAMES.get(str(t.dtype))
-        if code is None:
-            raise DecodeError("%s: unsupported type %s" % (what, t.dtype), 4)
-        _dt_of[t.dtype] = code
+        raise DecodeError("%s: unsupported type %s" % (what, t.dtype), 4)
     return code
 
 
-def _place(what: str, *tensors):
-    """(device index, raw stream) of tensors that must share a CUDA device."""
-    import torch
-    dev = tensors[0].device
-    if dev.type != "cuda":
+def _place(what: str, first, *tensors) -> int:
+    """The index of the CUDA device that all tensors share."""
+    dev = first.get_device()
+    if dev < 0:
         raise DecodeError("%s: tensors must be on a CUDA device" % what)
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise DecodeError("%s: tensors on different devices (%s, %s)" % (what, dev, t.device))
-    return dev.index, torch.cuda.current_stream(dev).cuda_stream
+        if t is not None and t.get_device() != dev:
+            raise DecodeError("%s: tensors on different devices (%s, %s)" % (what, first.device, t.device))
+    return dev
 
 
-def _vec(what: str, name: str, t, dtype: str, n: int):
+def _vec(what: str, name: str, t, dtype, n: int):
     """Address of a contiguous one-dimensional tensor of n values (None: NULL)."""
     if t is None:
         return None
-    if str(t.dtype) != dtype or t.ndim != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
         raise DecodeError("%s: %s must be %s [%d], contiguous" % (what, name, dtype, n))
     return t.data_ptr()
 
 
 def _rows(what: str, name: str, t, heads: int, dim: int):
     """Distance of the rows of a [n, heads, dim] (or [n, heads * dim]) tensor in elements."""
-    if t.ndim == 3:
-        ok = t.shape[1:] == (heads, dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == dim)
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        ok = (shape[1] == heads and shape[2] == dim and stride[2] == 1 and (heads == 1 or stride[1] == dim))
     else:
-        ok = t.ndim == 2 and t.shape[1] == heads * dim and t.stride(1) == 1
+        ok = len(shape) == 2 and shape[1] == heads * dim and stride[1] == 1
     if not ok:
         raise DecodeError("%s: %s must be [n, %d, %d] with contiguous heads and dims, got %s strides %s" %
-                          (what, name, heads, dim, tuple(t.shape), tuple(t.stride())))
-    return t.stride(0) if t.shape[0] > 1 else heads * dim
+                          (what, name, heads, dim, tuple(shape), stride))
+    return stride[0] if shape[0] > 1 else heads * dim
+
+
+def _table(what: str, T, t, R: int):
+    """(row distance, columns) of an int32 [R, max_pages] tensor."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not T.i32 or len(shape) != 2 or shape[0] != R or (shape[1] > 1 and stride[1] != 1):
+        raise DecodeError("%s: block_table must be int32 [%d, max_pages]" % (what, R))
+    return (stride[0] if R > 1 else shape[1]), shape[1]
 
 
 def kv_plan(lens, new_tokens, page: int, free_pages, cursor, block_table, slots, cu_new, status, cursor_out=None):
@@ -911,21 +938,18 @@ def kv_plan(lens, new_tokens, page: int, free_pages, cursor, block_table, slots,
     (rows may be strided), slots [any], cu_new [R + 1], status [2], cursor [1]
     (advanced in place unless cursor_out is given)."""
     what = "kv_plan"
-    R = lens.shape[0]
+    T = _t()
+    i32, R, n_free, n_slots = T.i32, lens.numel(), free_pages.numel(), slots.numel()
     if cursor_out is None:
         cursor_out = cursor
-    dev, st = _place(what, lens, new_tokens, free_pages, cursor, cursor_out, block_table, slots, cu_new, status)
-    i32 = "torch.int32"
-    if (str(block_table.dtype) != i32 or block_table.ndim != 2 or block_table.shape[0] != R or
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise DecodeError("%s: block_table must be int32 [%d, max_pages]" % (what, R))
-    _op_check(lib().wg_kv_plan(
+    dev = _place(what, lens, new_tokens, free_pages, cursor, cursor_out, block_table, slots, cu_new, status)
+    ld, cols = _table(what, T, block_table, R)
+    _op_check(T.lib.wg_kv_plan(
         _vec(what, "lens", lens, i32, R), _vec(what, "new_tokens", new_tokens, i32, R), R, page,
-        _vec(what, "free_pages", free_pages, i32, free_pages.shape[0]), free_pages.shape[0],
-        _vec(what, "cursor", cursor, i32, 1), _vec(what, "cursor_out", cursor_out, i32, 1), block_table.data_ptr(),
-        block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1],
-        _vec(what, "slots", slots, i32, slots.shape[0]), slots.shape[0], _vec(what, "cu_new", cu_new, i32, R + 1),
-        _vec(what, "status", status, i32, 2), dev, st), what)
+        _vec(what, "free_pages", free_pages, i32, n_free), n_free, _vec(what, "cursor", cursor, i32, 1),
+        _vec(what, "cursor_out", cursor_out, i32, 1), block_table.data_ptr(), ld, cols,
+        _vec(what, "slots", slots, i32, n_slots), n_slots, _vec(what, "cu_new", cu_new, i32, R + 1),
+        _vec(what, "status", status, i32, 2), dev, T.stream(dev)), what)
 
 
 class Kv8Cache:
@@ -935,8 +959,9 @@ class Kv8Cache:
 
     def __init__(self, codes, scales):
         what = "Kv8Cache"
-        if (str(codes.dtype) != "torch.int8" or codes.ndim != 5 or codes.shape[1] != 2 or not codes.is_contiguous() or
-                str(scales.dtype) != "torch.float32" or tuple(scales.shape) != tuple(codes.shape[:3]) or
+        T = _t()
+        if (codes.dtype is not T.i8 or codes.ndim != 5 or codes.shape[1] != 2 or not codes.is_contiguous() or
+                scales.dtype is not T.f32 or tuple(scales.shape) != tuple(codes.shape[:3]) or
                 not scales.is_contiguous()):
             raise DecodeError("%s: codes must be int8 [pages, 2, heads, page, dim], scales fp32 [pages, 2, heads], "
                               "both contiguous" % what)
@@ -953,27 +978,29 @@ class Kv8Cache:
         return cls(torch.empty(num_pages, 2, n_kv_head, page, head_dim, dtype=torch.int8, device=device),
                    torch.empty(num_pages, 2, n_kv_head, dtype=torch.float32, device=device))
 
-    def _kv(self, what, k, v, slots):
+    def _kv(self, what, T, k, v, slots):
         ldk = _rows(what, "k", k, self.n_kv_head, self.head_dim)
         ldv = _rows(what, "v", v, self.n_kv_head, self.head_dim)
-        n = k.shape[0]
-        if v.shape[0] != n or v.dtype != k.dtype:
-            raise DecodeError("%s: k and v must have the same rows and type" % what)
-        return _vec(what, "slots", slots, "torch.int32", n), n, _dt(k, what), ldk, ldv
+        n = slots.numel()
+        if len(k) != n or len(v) != n or v.dtype is not k.dtype:
+            raise DecodeError("%s: k and v must have a row for each slot and the same type" % what)
+        return _vec(what, "slots", slots, T.i32, n), n, _dt(T, k, what), ldk, ldv, _place(what, self.codes, k, v, slots)
 
     def append(self, k, v, slots):
         """Writes the rows of k and v ([n, n_kv_head, head_dim]) into their slots (wg_kv8_append)."""
         what = "kv8_append"
-        sp, n, dt, ldk, ldv = self._kv(what, k, v, slots)
-        dev, st = _place(what, self.codes, k, v, slots)
-        _op_check(lib().wg_kv8_append(self._ref, k.data_ptr(), v.data_ptr(), dt, ldk, ldv, sp, n, dev, st), what)
+        T = _t()
+        sp, n, dt, ldk, ldv, dev = self._kv(what, T, k, v, slots)
+        _op_check(T.lib.wg_kv8_append(self._ref, k.data_ptr(), v.data_ptr(), dt, ldk, ldv, sp, n, dev, T.stream(dev)),
+                  what)
 
     def read(self, slots, k, v):
         """The values at `slots` into the rows of k and v (wg_kv8_read)."""
         what = "kv8_read"
-        sp, n, dt, ldk, ldv = self._kv(what, k, v, slots)
-        dev, st = _place(what, self.codes, k, v, slots)
-        _op_check(lib().wg_kv8_read(self._ref, sp, n, k.data_ptr(), v.data_ptr(), dt, ldk, ldv, dev, st), what)
+        T = _t()
+        sp, n, dt, ldk, ldv, dev = self._kv(what, T, k, v, slots)
+        _op_check(T.lib.wg_kv8_read(self._ref, sp, n, k.data_ptr(), v.data_ptr(), dt, ldk, ldv, dev, T.stream(dev)),
+                  what)
 
     def attention(self, q, cu_q, kv_lens, block_table, max_q: int, max_kv: int, causal: bool = True,
                   scale: Optional[float] = None, out=None):
@@ -981,27 +1008,22 @@ class Kv8Cache:
         tokens of their requests (wg_kv8_attention); returns out, by default a
         new tensor of q's type (f16 where q is fp32)."""
         what = "kv8_attention"
-        D = self.head_dim
-        if q.ndim != 3 or q.shape[2] != D:
+        T, D, R = _t(), self.head_dim, kv_lens.numel()
+        if q.dim() != 3:
             raise DecodeError("%s: q must be [n, heads, %d], got %s" % (what, D, tuple(q.shape)))
-        n_head, R = q.shape[1], kv_lens.shape[0]
-        qdt = _dt(q, what)
+        n_q, n_head, _ = q.shape
+        qdt = _dt(T, q, what)
         if out is None:
-            import torch
-            out = torch.zeros(q.shape, dtype=torch.float16 if qdt == 0 else q.dtype, device=q.device)
-        if out.shape != q.shape:
+            out = T.torch.zeros(q.shape, dtype=T.torch.float16 if qdt == 0 else q.dtype, device=q.device)
+        if len(out) != n_q:
             raise DecodeError("%s: out must be %s" % (what, tuple(q.shape)))
-        if (str(block_table.dtype) != "torch.int32" or block_table.ndim != 2 or block_table.shape[0] != R or
-                (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-            raise DecodeError("%s: block_table must be int32 [%d, max_pages]" % (what, R))
-        dev, st = _place(what, self.codes, q, cu_q, kv_lens, block_table, out)
-        p = WgKv8Attn(q.data_ptr(), _rows(what, "q", q, n_head, D), qdt, n_head,
-                      _vec(what, "cu_q", cu_q, "torch.int32", R + 1), q.shape[0], R,
-                      _vec(what, "kv_lens", kv_lens, "torch.int32", R), block_table.data_ptr(),
-                      block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1], max_q, max_kv,
-                      1 if causal else 0, D ** -0.5 if scale is None else scale, _dt(out, what), out.data_ptr(),
+        dev = _place(what, self.codes, q, cu_q, kv_lens, block_table, out)
+        ld, cols = _table(what, T, block_table, R)
+        p = WgKv8Attn(q.data_ptr(), _rows(what, "q", q, n_head, D), qdt, n_head, _vec(what, "cu_q", cu_q, T.i32, R + 1),
+                      n_q, R, _vec(what, "kv_lens", kv_lens, T.i32, R), block_table.data_ptr(), ld, cols, max_q, max_kv,
+                      1 if causal else 0, D ** -0.5 if scale is None else scale, _dt(T, out, what), out.data_ptr(),
                       _rows(what, "out", out, n_head, D))
-        _op_check(lib().wg_kv8_attention(self._ref, ctypes.byref(p), dev, st), what)
+        _op_check(T.lib.wg_kv8_attention(self._ref, ctypes.byref(p), dev, T.stream(dev)), what)
         return out
 
 
@@ -1010,18 +1032,20 @@ def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
     (wg_sample_rows); temperature, top_p, min_p fp32 [R], top_k int32 [R], each
     optional. Returns (tokens int32 [R], logprobs fp32 [R])."""
     what = "sample_rows"
-    if logits.ndim != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    T = _t()
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise DecodeError("%s: logits must be [rows, vocabulary] with contiguous rows" % what)
     R, V = logits.shape
-    if tokens is None or logprobs is None:
-        import torch
-        tokens = torch.empty(R, dtype=torch.int32, device=logits.device) if tokens is None else tokens
-        logprobs = torch.empty(R, dtype=torch.float32, device=logits.device) if logprobs is None else logprobs
-    dev, st = _place(what, logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
-    f32 = "torch.float32"
-    p = WgSample(logits.data_ptr(), logits.stride(0) if R > 1 else V, _dt(logits, what), R, V, _vec(what, "u", u, f32, R),
-                 _vec(what, "temperature", temperature, f32, R), _vec(what, "top_k", top_k, "torch.int32", R),
-                 _vec(what, "top_p", top_p, f32, R), _vec(what, "min_p", min_p, f32, R),
-                 _vec(what, "tokens", tokens, "torch.int32", R), _vec(what, "logprobs", logprobs, f32, R))
-    _op_check(lib().wg_sample_rows(ctypes.byref(p), dev, st), what)
+    if tokens is None:
+        tokens = T.torch.empty(R, dtype=T.i32, device=logits.device)
+    if logprobs is None:
+        logprobs = T.torch.empty(R, dtype=T.f32, device=logits.device)
+    dev = _place(what, logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
+    f32, i32 = T.f32, T.i32
+    p = WgSample(logits.data_ptr(), logits.stride(0) if R > 1 else V, _dt(T, logits, what), R, V,
+                 _vec(what, "u", u, f32, R), _vec(what, "temperature", temperature, f32, R),
+                 _vec(what, "top_k", top_k, i32, R), _vec(what, "top_p", top_p, f32, R),
+                 _vec(what, "min_p", min_p, f32, R), _vec(what, "tokens", tokens, i32, R),
+                 _vec(what, "logprobs", logprobs, f32, R))
+    _op_check(T.lib.wg_sample_rows(ctypes.byref(p), dev, T.stream(dev)), what)
     return tokens, logprobs
