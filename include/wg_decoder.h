@@ -408,7 +408,8 @@ int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, void* k, void*
  * attention: the beams of an utterance are its queries). A query that sees
  * nothing gives zeros. A page number outside the cache hides its tokens.
  * Rows of `out` that belong to no request are left as they were; a request
- * whose cu_q pair is out of range or descending has no rows.
+ * whose cu_q pair is out of range or descending has no rows. No row may
+ * belong to two requests.
  * max_q: no request has more query rows (rows past it are not computed);
  * max_kv: the longest kv_lens, a hint for how to split the work (any value
  * gives the same sums up to rounding).

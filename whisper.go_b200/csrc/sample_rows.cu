@@ -3,35 +3,59 @@
 //
 // With w_i = exp((x_i - max x) / T), every filter keeps a prefix of the row in
 // descending order (lower index first among equals), so the kept set is one
-// cut: the elements above a value, and the first J of those equal to it. Cuts
-// are found without sorting, by a radix descent over the order-preserving bit
-// patterns of the logits with a count and a mass for each digit.
+// cut: the elements above a value, and the first J of those equal to it.
 //
 // Which token a random number falls on is decided by sums of up to V weights,
-// so the weights are evaluated in 64-bit floats and summed as integers in
-// units of 2^-45 (at most 2^18 * 2^45 for a row): sums are exact and order
-// free, and off by less than V * 2^-46 of the largest weight from the real
-// ones.
+// so the weights that decide are evaluated in 64-bit floats and summed as
+// integers in units of 2^-45 (at most 2^18 * 2^45 for a row): sums are exact,
+// free of any order, and off by less than V * 2^-46 of the largest weight
+// from the real ones. The sum under the log-prob is fp32.
+//
+// A cluster of C CTAs takes a row; each holds its slice in shared memory as
+// fp32, so the row is read from memory once and every later pass is over
+// shared memory. Cuts are found without sorting:
+//  1. a histogram of counts over SR_BINS equal steps of the logit below the
+//     maximum (one shared atomic an element) gives the exact bin of the
+//     top-k cut, and from count * exp(middle) the likely bin of the top-p cut;
+//  2. one pass sums the exact masses of everything and of what lies above
+//     the likely bins (the only pass that needs an exponential of each
+//     element, and only for rows with top-p and no top-k);
+//  3. the cut is pinned inside the bins by descents over the order-preserving
+//     bit patterns of the logits, 9 bits a pass, with exact counts and masses
+//     (two passes as a rule). Where the likely bins were wrong the exact sums
+//     say so and the descent starts again over the whole row.
+// The draw sums the kept weights of each thread's consecutive elements; rank
+// 0 then walks cluster rank -> thread -> element to where the running mass
+// passes u * mass. Equal logits need no list: their count, their common
+// weight and the running count in index order say which of them are kept.
+#include <cooperative_groups.h>
+
+#include <cstddef>
+#include <mutex>
+
 #include "kernels.cuh"
 #include "ops.cuh"
 
 namespace wg {
 namespace {
 
-constexpr int SR_THREADS = 1024;
+namespace cg = cooperative_groups;
+
+#ifndef SR_MINB
+#define SR_MINB 2
+#endif
+
+constexpr int SR_THREADS = 512;
+constexpr int SR_WARPS = SR_THREADS / 32;
+constexpr int SR_BINS = 4 * SR_THREADS;   // first histogram: four bins a thread
+constexpr int SR_SUB = SR_THREADS;        // bins of a descent: one a thread (9 bits)
+constexpr int SR_MAX_CLUSTER = 8;
+constexpr float SR_SPAN = 40.f;           // logits that far below the maximum share the last bin
 constexpr double SR_ONE = 35184372088832.0;  // 2^45
+constexpr int SR_MAX_V = 1 << 18;
 typedef unsigned long long u64;
 
-struct Row {
-  const void* p;
-  int dt, V;
-  __device__ __forceinline__ float at(int i) const {
-    const float x = dt_load(p, i, dt);
-    return x != x ? -INFINITY : x;
-  }
-};
-
-// Unsigned keys in the order of the values (-0 with +0).
+// Unsigned keys in the order of the values (-0 with +0); 0 is no value's key.
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = x == 0.f ? 0u : __float_as_uint(x);
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
@@ -39,225 +63,613 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-struct Weights {
-  double zmax, t;
-  float mx;
-  __device__ __forceinline__ double operator()(float x) const { return x == mx ? 1.0 : exp((double)x / t - zmax); }
+struct Shared {
+  // what peers read, each written before a cluster barrier
+  float mx[SR_MAX_CLUSTER], mn[SR_MAX_CLUSTER];  // pushed by every rank to every rank
+  float sum;                                     // fp32 sum of the slice's weights
+  int first;                                     // lowest index of the slice that holds the maximum
+  u64 mass[2];                                   // exact sums of the slice (whole / above the bins)
+  u64 kept;                                      // kept mass without ties
+  unsigned ties;                                 // elements equal to the cut
+  unsigned sub_c[2][SR_SUB];
+  u64 sub_m[2][SR_SUB];
+  union alignas(16) {  // read 16 bytes at a time
+    unsigned hist[SR_BINS];
+    struct {
+      u64 mass[SR_THREADS];       // kept mass of each thread's elements
+      unsigned ties[SR_THREADS];  // and how many equal the cut
+    } part;
+  };
+  // this CTA's own
+  double pow2[64];  // 2^(-j / 64)
+  u64 red_m[SR_WARPS];
+  unsigned red_c[SR_WARPS];
+  float red_f[2][SR_WARPS];
+  int found[2];
+  u64 found_m;
+  unsigned found_c;
 };
-__device__ __forceinline__ u64 fixed_of(double w) { return __double2ull_rn(w * SR_ONE); }
 
-__device__ u64 block_sum(u64 v) {
-  __shared__ u64 part[32];
-  __shared__ u64 total;
+// The weight of a logit: the definition's 64-bit value by argument reduction,
+// w = 2^-(y / 64) with y = 64 (max - x) / (T ln 2) = n + r, n the nearest
+// integer: 2^-(n >> 6) from the exponent, 2^-((n & 63) / 64) from a table,
+// 2^(-r / 64) by its Taylor series (|r ln 2 / 64| <= 0.0055: five terms leave
+// 4e-17).
+struct Weigh {
+  double mx, c64;
+  const double* pow2;
+  // the weight; 0 where it is below 2^-46
+  __device__ __forceinline__ double value(float x, float mxf) const {
+    if (x == mxf) return 1.0;
+    const double y = (mx - (double)x) * c64;
+    if (!(y < 46.0 * 64.0)) return 0.0;
+    const double magic = 6755399441055744.0;  // 2^52 + 2^51: the sum's low word is the nearest integer
+    const double shifted = y + magic;
+    const int n = __double2loint(shifted);
+    const double s = (y - (shifted - magic)) * -0.010830424696249145;  // -ln 2 / 64
+    double p = fma(s, 1.0 / 120.0, 1.0 / 24.0);
+    p = fma(p, s, 1.0 / 6.0);
+    p = fma(p, s, 0.5);
+    p = fma(p, s, 1.0);
+    p = fma(p, s, 1.0);
+    return pow2[n & 63] * p * __hiloint2double((1023 - (n >> 6)) << 20, 0);
+  }
+  static __device__ __forceinline__ u64 fixed(double w) {
+    // w * 2^45 + 2^52 leaves the rounded integer in the low 52 bits
+    return (u64)__double_as_longlong(fma(w, SR_ONE, 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+};
+
+__device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    u64 s = 0;
-    for (int w = 0; w < SR_THREADS / 32; w++) s += part[w];
-    total = s;
-  }
-  __syncthreads();
-  return total;
+  return v;
 }
+
+// Inclusive scans over the CTA of a mass and a count; *tm, *tc: the totals.
+__device__ void block_scan(Shared& sh, u64& m, unsigned& c, u64* tm, unsigned* tc) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 a = __shfl_up_sync(0xffffffffu, m, o);
+    const unsigned b = __shfl_up_sync(0xffffffffu, c, o);
+    if (lane >= o) { m += a; c += b; }
+  }
+  __syncthreads();  // earlier readers of red_* are done
+  if (lane == 31) { sh.red_m[warp] = m; sh.red_c[warp] = c; }
+  __syncthreads();
+  u64 am = 0, pm = 0;
+  unsigned ac = 0, pc = 0;
+#pragma unroll
+  for (int w = 0; w < SR_WARPS; w++) {
+    if (w == warp) { pm = am; pc = ac; }
+    am += sh.red_m[w];
+    ac += sh.red_c[w];
+  }
+  m += pm;
+  c += pc;
+  *tm = am;
+  *tc = ac;
+}
+
+static_assert(alignof(Shared) == 16 && offsetof(Shared, hist) % 16 == 0, "the histogram is read as uint4");
 
 struct Cut {
-  uint32_t key;  // elements above it are kept
-  int ties;      // and so many of those equal to it, in index order
-  u64 mass;      // their mass
+  uint32_t key;   // elements above it are kept (0: every element)
+  unsigned ties;  // and so many of those equal to it, in index order
 };
 
-// The shortest prefix of `in` (a cut itself) with at least k elements, or with
-// a mass of at least `target` where by_mass.
-__device__ Cut descend(const Row& row, const Weights& wt, const Cut& in, bool by_mass, u64 target) {
-  __shared__ unsigned hc[256];
-  __shared__ u64 hs[256];
-  __shared__ uint32_t prefix_sh;
-  __shared__ u64 above_sh, cabove_sh;
-  __shared__ unsigned eq_sh;
-  uint32_t prefix = 0, mask = 0;
-  u64 above = 0, cabove = 0;  // mass and count of the elements above the current digits
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += SR_THREADS) { hc[i] = 0; hs[i] = 0; }
-    __syncthreads();
-    for (int i = threadIdx.x; i < row.V; i += SR_THREADS) {
-      const float x = row.at(i);
-      const uint32_t key = key_of(x);
-      if ((key & mask) != prefix || key <= in.key) continue;
-      atomicAdd(&hc[(key >> shift) & 255], 1u);
-      atomicAdd(&hs[(key >> shift) & 255], fixed_of(wt(x)));
-    }
-    if (threadIdx.x == 0 && (in.key & mask) == prefix && in.ties) {
-      atomicAdd(&hc[(in.key >> shift) & 255], (unsigned)in.ties);
-      atomicAdd(&hs[(in.key >> shift) & 255], (u64)in.ties * fixed_of(wt(of_key(in.key))));
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int sel = -1, last = -1;
-      u64 a = above, c = cabove;
-      for (int d = 255; d >= 0; d--) {
-        if (!hc[d]) continue;
-        last = d;
-        if ((by_mass ? a + hs[d] : c + hc[d]) >= target) { sel = d; break; }
-        a += hs[d];
-        c += hc[d];
-      }
-      if (sel < 0) {  // less than the target in all: everything is kept
-        sel = last;
-        a -= hs[sel];
-        c -= hc[sel];
-      }
-      above_sh = a;
-      cabove_sh = c;
-      prefix_sh = prefix | ((uint32_t)sel << shift);
-      eq_sh = hc[sel];
-    }
-    __syncthreads();
-    above = above_sh;
-    cabove = cabove_sh;
-    prefix = prefix_sh;
-    mask |= 255u << shift;
-  }
-  const u64 each = fixed_of(wt(of_key(prefix)));
-  u64 j = by_mass ? (each ? (target > above ? (target - above + each - 1) / each : 1) : eq_sh)
-                  : (target > cabove ? target - cabove : 1);
-  if (j > eq_sh) j = eq_sh;
-  if (j < 1) j = 1;
-  __syncthreads();
-  return Cut{prefix, (int)j, above + j * each};
+template <typename T>
+__device__ __forceinline__ const T* peer(const T* p, int rank, int C) {
+  return C > 1 ? cg::this_cluster().map_shared_rank(p, rank) : p;
+}
+__device__ __forceinline__ void cluster_barrier(int C) {
+  if (C > 1) cg::this_cluster().sync();
+  else __syncthreads();
 }
 
-struct Args {
-  wg_sample s;
-};
-
-__global__ void __launch_bounds__(SR_THREADS) sample_rows_kernel(const Args a) {
+// grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the slice
+__global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const wg_sample s, int C, int per) {
+  extern __shared__ __align__(16) uint8_t dyn[];
+  Shared& sh = *reinterpret_cast<Shared*>(dyn);
   pdl_trigger();
   pdl_wait();
-  const wg_sample& s = a.s;
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Row row{reinterpret_cast<const char*>(s.logits) + (int64_t)r * s.ld * dt_bytes(s.dtype), s.dtype, s.V};
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x % C, r = blockIdx.x / C;
+  const int slice = per * SR_THREADS;
+  const int c0 = min(s.V, rank * slice), n = min(s.V, c0 + slice) - c0;
   const float T = s.temperature ? s.temperature[r] : 1.f;
   const int k = s.top_k ? s.top_k[r] : 0;
   const float top_p = s.top_p ? s.top_p[r] : 1.f, min_p = s.min_p ? s.min_p[r] : 0.f;
-  float u = s.u[r];
-  if (!(u >= 0.f)) u = 0.f;
-  // first maximum
-  __shared__ u64 best_sh[32];
-  u64 best = 0;
-  for (int i = tid; i < s.V; i += SR_THREADS) {
-    const u64 v = ((u64)key_of(row.at(i)) << 32) | (0xffffffffu - (uint32_t)i);
-    best = v > best ? v : best;
-  }
+  const bool by_k = k > 0 && k < s.V, by_p = !(top_p >= 1.f);
+  // rows where only the first maximum can stay
+  const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
+  if (tid < 64) sh.pow2[tid] = exp2(-(double)tid / 64.0);
+  for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.hist[i] = 0;
+  sh.sub_c[0][tid] = 0;
+  sh.sub_m[0][tid] = 0;
+
+  // ---- the slice into shared memory, 16-byte loads between its ragged ends;
+  // xs starts at the address's place in 16 bytes, so both sides are aligned
+  const int es = dt_bytes(s.dtype), vec = 16 / es;
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + c0) * es;
+  const int lead = (int)((reinterpret_cast<uintptr_t>(src) / es) % vec);
+  float* xs = reinterpret_cast<float*>(dyn + ((sizeof(Shared) + 15) / 16) * 16) + lead;
+  float mx = -INFINITY, mn = INFINITY;
+  {
+    auto clean = [&](float x) {
+      x = x != x ? -INFINITY : x;
+      mx = fmaxf(mx, x);
+      mn = fminf(mn, x == -INFINITY ? INFINITY : x);  // the least finite one
+      return x;
+    };
+    const int head = min(n, (vec - lead) % vec), body = (n - head) / vec, tail = n - head - body * vec;
+    if (tid < head) xs[tid] = clean(dt_load(src, tid, s.dtype));
+    if (tid < tail) xs[n - tail + tid] = clean(dt_load(src, n - tail + tid, s.dtype));
+    const uint4* v = reinterpret_cast<const uint4*>(src + head * es);
+    float4* d = reinterpret_cast<float4*>(xs + head);
+    constexpr int U = 4;  // loads in flight per thread
+    for (int i0 = tid; i0 < body; i0 += U * SR_THREADS) {
+      uint4 w[U];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 v = __shfl_xor_sync(0xffffffffu, best, o);
-    best = v > best ? v : best;
+      for (int j = 0; j < U; j++) w[j] = i0 + j * SR_THREADS < body ? __ldg(v + i0 + j * SR_THREADS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < U; j++) {
+        const int i = i0 + j * SR_THREADS;
+        if (i >= body) break;
+        if (s.dtype == WG_DT_F32) {
+          d[i] = make_float4(clean(__uint_as_float(w[j].x)), clean(__uint_as_float(w[j].y)),
+                             clean(__uint_as_float(w[j].z)), clean(__uint_as_float(w[j].w)));
+        } else {
+          const float2 a = dt_unpack2(s.dtype, w[j].x), b = dt_unpack2(s.dtype, w[j].y);
+          const float2 e = dt_unpack2(s.dtype, w[j].z), f = dt_unpack2(s.dtype, w[j].w);
+          d[2 * i] = make_float4(clean(a.x), clean(a.y), clean(b.x), clean(b.y));
+          d[2 * i + 1] = make_float4(clean(e.x), clean(e.y), clean(f.x), clean(f.y));
+        }
+      }
+    }
   }
-  if (lane == 0) best_sh[warp] = best;
+  mx = warp_max(mx);
+  mn = -warp_max(-mn);
+  if (lane == 0) { sh.red_f[0][warp] = mx; sh.red_f[1][warp] = mn; }
   __syncthreads();
-  best = best_sh[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 v = __shfl_xor_sync(0xffffffffu, best, o);
-    best = v > best ? v : best;
+  for (int w = 0; w < SR_WARPS; w++) {
+    mx = fmaxf(mx, sh.red_f[0][w]);
+    mn = fminf(mn, sh.red_f[1][w]);
   }
-  const float mx = of_key((uint32_t)(best >> 32));
-  const int first = (int)(0xffffffffu - (uint32_t)best);
-  if (mx == -INFINITY) {
-    if (tid == 0) {
+  if (C > 1) {
+    cg::this_cluster().sync();  // every rank runs: its shared memory may be written
+    if (tid < C) {
+      cg::this_cluster().map_shared_rank(sh.mx, tid)[rank] = mx;
+      cg::this_cluster().map_shared_rank(sh.mn, tid)[rank] = mn;
+    }
+    cg::this_cluster().sync();
+    for (int q = 0; q < C; q++) {
+      mx = fmaxf(mx, sh.mx[q]);
+      mn = fminf(mn, sh.mn[q]);
+    }
+  }
+  if (mx == -INFINITY) {  // nothing to draw from (the same for every rank)
+    if (rank == 0 && tid == 0) {
       s.tokens[r] = -1;
       if (s.logprobs) s.logprobs[r] = -INFINITY;
     }
     return;
   }
-  const double t = T > 0.f ? (double)T : 1.0;
-  const Weights wt{(double)mx / t, t, mx};
-  u64 all = 0;
-  for (int i = tid; i < s.V; i += SR_THREADS) all += fixed_of(wt(row.at(i)));
-  all = block_sum(all);
-  int token = first;
-  if (T > 0.f) {
-    Cut cut{0u, 0, all};  // everything (key 0 is no value's but -NaN's)
-    if (k > 0 && k < s.V) cut = descend(row, wt, cut, false, (u64)k);
-    if (!(top_p >= 1.f)) {
-      const double goal = ceil((double)top_p * (double)cut.mass);
-      cut = descend(row, wt, cut, true, goal >= 1.0 ? (u64)goal : 1);
-    }
-    // index of the last tie that is kept
-    __shared__ int run_sh[SR_THREADS];
-    __shared__ int last_sh, token_sh;
-    const int per = (s.V + SR_THREADS - 1) / SR_THREADS, beg = min(s.V, tid * per), end = min(s.V, beg + per);
-    int eq = 0;
-    for (int i = beg; i < end; i++) eq += key_of(row.at(i)) == cut.key;
-    run_sh[tid] = eq;
-    if (tid == 0) last_sh = -1;
-    __syncthreads();
-    if (tid == 0) {
-      int acc = 0;
-      for (int w = 0; w < SR_THREADS; w++) { const int v = run_sh[w]; run_sh[w] = acc; acc += v; }
-    }
-    __syncthreads();
-    if (eq && run_sh[tid] < cut.ties && cut.ties <= run_sh[tid] + eq) {
-      int n = run_sh[tid];
-      for (int i = beg; i < end; i++)
-        if (key_of(row.at(i)) == cut.key && ++n == cut.ties) last_sh = i;
-    }
-    __syncthreads();
-    const int last = last_sh;
-    auto kept_mass = [&](int i) -> u64 {
-      const float x = row.at(i);
-      const uint32_t key = key_of(x);
-      if (key < cut.key || (key == cut.key && i > last)) return 0;
-      const double w = wt(x);
-      return w >= (double)min_p || i == first ? fixed_of(w) : 0;
-    };
-    u64 mine = 0;
-    for (int i = beg; i < end; i++) mine += kept_mass(i);
-    const u64 mass = block_sum(mine);
-    __shared__ u64 mass_sh[SR_THREADS];
-    mass_sh[tid] = mine;
-    if (tid == 0) token_sh = first;
-    __syncthreads();
-    if (tid == 0) {
-      u64 acc = 0;
-      for (int w = 0; w < SR_THREADS; w++) { const u64 v = mass_sh[w]; mass_sh[w] = acc; acc += v; }
-    }
-    __syncthreads();
-    u64 goal = (u64)((double)u * (double)mass) + 1;
-    if (goal > mass) goal = mass;
-    u64 run = mass_sh[tid];
-    if (run < goal && goal <= run + mine)
-      for (int i = beg; i < end; i++) {
-        run += kept_mass(i);
-        if (run >= goal) {
-          token_sh = i;
-          break;
-        }
+
+  // ---- fp32 sum of the weights, first maximum, histogram of counts
+  const float t1 = T > 0.f ? T : 1.f;
+  const float c2 = 1.4426950408889634f / t1;
+  const float span = fminf(fmaxf(mx - mn, 1e-30f), SR_SPAN);
+  const float bin_scale = (float)SR_BINS / span;
+  auto below = [&](float x) { return x == mx ? 0.f : mx - x; };
+  auto bin_of = [&](float d) { return min(SR_BINS - 1, __float2int_rd(fminf(d * bin_scale, 1e6f))); };
+  const int beg = min(n, tid * per), end = min(n, beg + per);  // consecutive elements; per is odd: no bank conflicts
+  const bool need_bins = !top1 && (by_k || by_p);
+  {
+    float sum = 0.f;
+    int first = 0x7fffffff;
+    for (int i = beg; i < end; i++) {
+      const float d = below(xs[i]);
+      sum += d == 0.f ? 1.f : d < INFINITY ? ex2f(-d * c2) : 0.f;
+      if (top1 && d == 0.f) first = min(first, i);
+      if (need_bins) {
+        const int b = bin_of(d);
+        if (b < SR_BINS - 1) atomicAdd(&sh.hist[b], 1u);  // the last bin is the rest
       }
+    }
+    sum = warp_sum(sum);
+    first = __reduce_min_sync(0xffffffffu, first);
+    __syncthreads();  // red_f has been read
+    if (lane == 0) { sh.red_f[0][warp] = sum; sh.red_c[warp] = (unsigned)first; }
     __syncthreads();
-    token = token_sh;
+    if (tid == 0) {
+      float a = 0.f;
+      int f = 0x7fffffff;
+      for (int w = 0; w < SR_WARPS; w++) { a += sh.red_f[0][w]; f = min(f, (int)sh.red_c[w]); }
+      sh.sum = a;
+      sh.first = f == 0x7fffffff ? f : c0 + f;
+    }
   }
-  if (tid == 0) {
+  const Weigh wt{(double)mx, 92.332482616893656877 / (double)t1, sh.pow2};  // 64 / ln 2 / T
+  auto finish = [&](int token, float x) {
     s.tokens[r] = token;
     if (s.logprobs) {
-      const float x = row.at(token);
-      const double d = x == mx ? 0.0 : (double)x / t - wt.zmax;
-      s.logprobs[r] = (float)(d - log((double)all / SR_ONE));
+      double z = 0.0;
+      for (int q = 0; q < C; q++) z += (double)peer(&sh, q, C)->sum;
+      const double d = x == mx ? 0.0 : ((double)x - (double)mx) / (double)t1;
+      s.logprobs[r] = (float)(d - log(z));
+    }
+  };
+  if (top1 || need_bins) cluster_barrier(C);
+  if (top1) {
+    if (rank == 0 && tid == 0) {
+      int f = 0x7fffffff;
+      for (int q = 0; q < C; q++) f = min(f, peer(&sh, q, C)->first);
+      finish(f, mx);
+    }
+    cluster_barrier(C);  // rank 0 has read its peers
+    return;
+  }
+
+  int level = 0;  // descents so far: their buffers alternate
+  // The cut where the running count (or mass) in descending order reaches
+  // `target`, known to lie in bins ba..bb, above which there are `above`;
+  // among the elements inside `in`. Returns false, with *total the sum inside
+  // the bins, where it does not lie there.
+  auto descend = [&](const Cut& in, bool mass, u64 target, int ba, int bb, u64 above, Cut* out, u64* total) -> bool {
+    // keys that the bins can hold (a hundredth of a bin and a few ulps around them)
+    const float w = span / (float)SR_BINS, slack = 0.01f * w + 1e-6f * fabsf(mx);
+    uint32_t klo = bb >= SR_BINS - 1 ? 0u : key_of(mx - (float)(bb + 1) * w - slack);
+    uint32_t khi = ba <= 0 ? key_of(mx) : key_of(fminf(mx, mx - (float)ba * w + slack));
+    if (mx == INFINITY) { klo = 0u; khi = key_of(mx); }
+    bool started = false;
+    for (;;) {
+      int shift = 0;
+      while (((khi - klo) >> shift) >= (uint32_t)SR_SUB) shift++;
+      const int buf = level & 1;
+      auto put = [&](float x, uint32_t key, unsigned count) {
+        const int b = bin_of(below(x));
+        if (b < ba || b > bb) return;
+        const uint32_t sub = min((uint32_t)(SR_SUB - 1), (key - klo) >> shift);
+        atomicAdd(&sh.sub_c[buf][sub], count);
+        if (mass) atomicAdd(&sh.sub_m[buf][sub], (u64)count * Weigh::fixed(wt.value(x, mx)));
+      };
+      for (int i = beg; i < end; i++) {
+        const float x = xs[i];
+        const uint32_t key = key_of(x);
+        if (key >= klo && key <= khi && key > in.key) put(x, key, 1u);
+      }
+      if (rank == 0 && tid == 0 && in.ties && in.key >= klo && in.key <= khi) put(of_key(in.key), in.key, in.ties);
+      cluster_barrier(C);
+      // sub-bins in descending order: thread t has SUB - 1 - t
+      const int mine = SR_SUB - 1 - tid;
+      unsigned c = 0;
+      u64 m = 0;
+      for (int q = 0; q < C; q++) {
+        const Shared* o = peer(&sh, q, C);
+        c += o->sub_c[buf][mine];
+        if (mass) m += o->sub_m[buf][mine];
+      }
+      level++;
+      sh.sub_c[level & 1][tid] = 0;  // read last before the barrier above
+      sh.sub_m[level & 1][tid] = 0;
+      const unsigned c1 = c;
+      const u64 m1 = m;
+      u64 tm;
+      unsigned tc;
+      block_scan(sh, m, c, &tm, &tc);
+      const u64 inside = mass ? tm : (u64)tc;
+      if (!started) {
+        *total = inside;
+        if (above >= target || above + inside < target) {
+          __syncthreads();
+          return false;
+        }
+        started = true;
+      }
+      const u64 incl = above + (mass ? m : (u64)c), one = mass ? m1 : (u64)c1;
+      if (tid == 0) sh.found[0] = -1;
+      __syncthreads();
+      if (c1 && incl >= target && incl - one < target) {
+        sh.found[0] = mine;
+        sh.found_m = incl - one;
+        sh.found_c = c1;
+      }
+      __syncthreads();
+      const int sel = sh.found[0];
+      if (sel < 0) return false;  // not reached: the bins' sum passed the target
+      above = sh.found_m;
+      klo += (uint32_t)sel << shift;
+      khi = min(khi, klo + ((1u << shift) - 1u));
+      if (shift == 0) {
+        const u64 each = mass ? Weigh::fixed(wt.value(of_key(klo), mx)) : 1;
+        u64 j = each ? (target - above + each - 1) / each : sh.found_c;
+        if (j > sh.found_c) j = sh.found_c;
+        out->key = klo;
+        out->ties = (unsigned)j;
+        __syncthreads();  // found_* has been read
+        return true;
+      }
+      __syncthreads();
+    }
+  };
+
+  Cut cut{0u, 0u};
+  if (need_bins) {
+    // ---- the first histogram over the cluster: thread t has bins 4t .. 4t + 3
+    unsigned c[4] = {0, 0, 0, 0};
+    for (int q = 0; q < C; q++) {
+      const uint4 v = *reinterpret_cast<const uint4*>(&peer(&sh, q, C)->hist[4 * tid]);
+      c[0] += v.x; c[1] += v.y; c[2] += v.z; c[3] += v.w;
+    }
+    // running counts, and masses estimated at the middle of each bin (2^-20
+    // units: only a guess, checked below)
+    const float w = span / (float)SR_BINS;
+    u64 m4 = 0, mb[4];
+    unsigned c4 = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      mb[j] = (u64)((float)c[j] * ex2f(-((float)(4 * tid + j) + 0.5f) * w * c2) * 1048576.f);
+      m4 += mb[j];
+      c4 += c[j];
+    }
+    u64 mt, m_in = m4;
+    unsigned ct, c_in = c4;
+    block_scan(sh, m_in, c_in, &mt, &ct);
+    if (tid == 0) { sh.found[0] = SR_BINS - 1; sh.found_c = ct; sh.found_m = mt; }
+    __syncthreads();
+    if (by_k) {
+      unsigned run = c_in - c4;
+      u64 mrun = m_in - m4;
+      if (run < (unsigned)k && (unsigned)k <= c_in) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (run < (unsigned)k && (unsigned)k <= run + c[j]) {
+            sh.found[0] = 4 * tid + j;
+            sh.found_c = run;
+            sh.found_m = mrun + (u64)((float)mb[j] * ((float)(k - run) / (float)c[j]));
+          }
+          run += c[j];
+          mrun += mb[j];
+        }
+      }
+      __syncthreads();
+    }
+    const int kbin = sh.found[0];
+    const unsigned kabove = sh.found_c;
+    const u64 guess = sh.found_m;
+    int pbin = 0;
+    if (by_p) {
+      __syncthreads();
+      if (tid == 0) sh.found[1] = by_k ? kbin : SR_BINS - 1;
+      __syncthreads();
+      const u64 goal = max((u64)1, (u64)((float)guess * top_p));
+      if (m_in - m4 < goal && goal <= m_in) {
+        u64 run = m_in - m4;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (run < goal && goal <= run + mb[j]) sh.found[1] = by_k ? min(kbin, 4 * tid + j) : 4 * tid + j;
+          run += mb[j];
+        }
+      }
+      __syncthreads();
+      pbin = sh.found[1];
+    }
+    u64 total;
+    if (by_k) {
+      const Cut every{0u, 0u};
+      if (!descend(every, false, (u64)k, kbin, kbin, kabove, &cut, &total))
+        descend(every, false, (u64)k, 0, SR_BINS - 1, 0, &cut, &total);
+    }
+    if (by_p) {
+      // ---- exact masses: of the top-k, and of what lies above the likely bins
+      const int ba = max(0, pbin - 1), bb = min(SR_BINS - 1, pbin + 1);
+      u64 all = 0, over = 0;
+      for (int i = beg; i < end; i++) {
+        const float x = xs[i];
+        if (key_of(x) <= cut.key) continue;
+        const u64 f = Weigh::fixed(wt.value(x, mx));
+        all += f;
+        if (bin_of(below(x)) < ba) over += f;
+      }
+      all = warp_sum64(all);
+      over = warp_sum64(over);
+      __syncthreads();
+      if (tid == 0) sh.mass[0] = sh.mass[1] = 0;
+      __syncthreads();
+      if (lane == 0) {
+        atomicAdd(&sh.mass[0], all);
+        atomicAdd(&sh.mass[1], over);
+      }
+      cluster_barrier(C);
+      all = over = 0;
+      for (int q = 0; q < C; q++) {
+        all += peer(&sh, q, C)->mass[0];
+        over += peer(&sh, q, C)->mass[1];
+      }
+      if (cut.ties) {
+        const float x = of_key(cut.key);
+        const u64 f = (u64)cut.ties * Weigh::fixed(wt.value(x, mx));
+        all += f;
+        if (bin_of(below(x)) < ba) over += f;
+      }
+      const double want = ceil((double)top_p * (double)all);
+      u64 goal = want >= 1.0 ? (u64)want : 1;
+      if (goal > all) goal = all;
+      const Cut in = cut;
+      if (!descend(in, true, goal, ba, bb, over, &cut, &total))
+        descend(in, true, goal, 0, SR_BINS - 1, 0, &cut, &total);  // the guess was wrong: over the whole row
     }
   }
+
+  // ---- the kept mass of every thread's elements
+  const double least = (double)min_p;
+  {
+    u64 m = 0;
+    unsigned e = 0;
+    for (int i = beg; i < end; i++) {
+      const float x = xs[i];
+      const uint32_t key = key_of(x);
+      if (key < cut.key) continue;
+      if (key == cut.key) {
+        e++;
+        continue;
+      }
+      const double w = wt.value(x, mx);
+      if (w >= least) m += Weigh::fixed(w);
+    }
+    // `part` shares the histogram's memory: that was read last before the latest barrier
+    sh.part.mass[tid] = m;
+    sh.part.ties[tid] = e;
+    m = warp_sum64(m);
+    e = __reduce_add_sync(0xffffffffu, e);
+    __syncthreads();
+    if (lane == 0) { sh.red_m[warp] = m; sh.red_c[warp] = e; }
+    __syncthreads();
+    if (tid == 0) {
+      u64 a = 0;
+      unsigned b = 0;
+      for (int w = 0; w < SR_WARPS; w++) { a += sh.red_m[w]; b += sh.red_c[w]; }
+      sh.kept = a;
+      sh.ties = b;
+    }
+  }
+  cluster_barrier(C);
+  if (rank == 0) {
+    // ties at the cut: their common weight, 0 where min-p drops them
+    double tie_w = 0.0;
+    if (cut.ties) {
+      tie_w = wt.value(of_key(cut.key), mx);
+      if (!(tie_w >= least)) tie_w = 0.0;
+    }
+    const u64 tie = Weigh::fixed(tie_w);
+    u64 mass = 0;
+    unsigned left = cut.ties;
+    for (int q = 0; q < C; q++) {
+      const Shared* o = peer(&sh, q, C);
+      const unsigned e = min(left, o->ties);
+      mass += o->kept + e * tie;
+      left -= e;
+    }
+    float u = s.u[r];
+    if (!(u >= 0.f)) u = 0.f;
+    const double at = (double)u * (double)mass;
+    u64 goal = at < (double)mass ? (u64)at + 1 : mass;  // first running mass above u * mass
+    if (goal > mass) goal = mass;
+    // cluster rank
+    int q = 0;
+    left = cut.ties;
+    for (; q < C - 1; q++) {
+      const Shared* o = peer(&sh, q, C);
+      const unsigned e = min(left, o->ties);
+      const u64 here = o->kept + e * tie;
+      if (goal <= here) break;
+      goal -= here;
+      left -= e;
+    }
+    const Shared* o = peer(&sh, q, C);
+    // thread: the running number of ties first, then the running mass
+    u64 m = o->part.mass[tid], tm;
+    unsigned e = o->part.ties[tid], tc;
+    const unsigned e1 = e;
+    u64 none = 0;
+    block_scan(sh, none, e, &tm, &tc);
+    const unsigned before = e - e1, kept_e = before >= left ? 0u : min(e1, left - before);
+    const u64 m1 = m + kept_e * tie;
+    m = m1;
+    unsigned zero = 0;
+    block_scan(sh, m, zero, &tm, &tc);
+    if (tid == 0) { sh.found[0] = 0; sh.found_m = 0; sh.found_c = 0; }
+    __syncthreads();
+    if (m >= goal && m - m1 < goal) {
+      sh.found[0] = tid;
+      sh.found_m = goal - (m - m1);
+      sh.found_c = before >= left ? 0u : left - before;  // ties still to keep in it
+    }
+    __syncthreads();
+    const int owner = sh.found[0];
+    goal = sh.found_m;
+    left = sh.found_c;
+    // element: the owner's `per` consecutive ones, one a thread at a time
+    const int qc0 = min(s.V, q * slice), qn = min(s.V, qc0 + slice) - qc0;
+    const int ob = min(qn, owner * per), on = min(qn, ob + per) - ob;
+    const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + qc0) * es;
+    const int qlead = (int)((reinterpret_cast<uintptr_t>(qsrc) / es) % vec);
+    const float* qx = peer(reinterpret_cast<const float*>(dyn + ((sizeof(Shared) + 15) / 16) * 16), q, C) + qlead + ob;
+    for (int i0 = 0; i0 < on; i0 += SR_THREADS) {
+      const int i = i0 + tid;
+      const float x = i < on ? qx[i] : -INFINITY;
+      const uint32_t key = key_of(x);
+      const bool is_tie = i < on && key == cut.key;
+      e = is_tie;
+      none = 0;
+      block_scan(sh, none, e, &tm, &tc);
+      const unsigned ties_here = tc;
+      u64 f = 0;
+      if (is_tie) f = e <= left ? tie : 0;
+      else if (i < on && key > cut.key) {
+        const double w = wt.value(x, mx);
+        if (w >= least) f = Weigh::fixed(w);
+      }
+      m = f;
+      zero = 0;
+      block_scan(sh, m, zero, &tm, &tc);
+      if (f && m >= goal && m - f < goal) finish(qc0 + ob + i, x);
+      if (goal <= tm) break;
+      goal -= tm;
+      left = left > ties_here ? left - ties_here : 0;
+    }
+  }
+  cluster_barrier(C);  // rank 0 has read its peers
+}
+
+std::mutex g_attr_mu;
+bool g_attr_done[OPS_MAX_DEV];
+constexpr int SR_SMEM_MAX = 227 * 1024;
+
+int set_attributes(int device) {
+  if (device < 0 || device >= OPS_MAX_DEV) {
+    set_error("wg_sample_rows: device %d out of range", device);
+    return WG_ERR_INVALID;
+  }
+  std::lock_guard<std::mutex> lk(g_attr_mu);
+  if (g_attr_done[device]) return WG_OK;
+  WG_CHECK_CUDA(cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SR_SMEM_MAX));
+  g_attr_done[device] = true;
+  return WG_OK;
 }
 
 }  // namespace
 
 int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
-  (void)device;
-  Args a{p};
-  return launch_check(launch_k(sample_rows_kernel, dim3(p.R), dim3(SR_THREADS), 0, st, a), "sample_rows");
+  WG_CHECK(set_attributes(device));
+  int C = SR_MAX_CLUSTER;
+  if (const char* e = getenv("WG_SR_C")) C = atoi(e);
+  auto per_of = [&](int c) { return ((p.V + c * SR_THREADS - 1) / (c * SR_THREADS)) | 1; };
+  const int per = per_of(C);
+  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)per * SR_THREADS * 4 + 32;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)p.R * C));
+  cfg.blockDim = dim3(SR_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = C;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = pdl_enabled() ? at : at + 1;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return launch_check(cudaLaunchKernelEx(&cfg, sample_rows_kernel, p, C, per), "sample_rows");
 }
 
 }  // namespace wg
@@ -265,8 +677,8 @@ int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
 extern "C" int wg_sample_rows(const wg_sample* p, int device, void* stream) {
   using namespace wg;
   const char* what = "wg_sample_rows";
-  if (!p || p->R < 0 || p->V <= 0 || p->V > (1 << 18) || p->ld < p->V) {
-    set_error("%s: bad argument (V from 1 to %d, rows at least V apart)", what, 1 << 18);
+  if (!p || p->R < 0 || p->R > (1 << 24) || p->V <= 0 || p->V > SR_MAX_V || p->ld < p->V) {
+    set_error("%s: bad argument (V from 1 to %d, rows at least V apart)", what, SR_MAX_V);
     return WG_ERR_INVALID;
   }
   if (!dt_ok(p->dtype)) {
