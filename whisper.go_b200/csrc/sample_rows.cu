@@ -45,12 +45,17 @@ namespace cg = cooperative_groups;
 #define SR_MINB 2
 #endif
 
-constexpr int SR_THREADS = 512;
+#ifndef SR_T
+#define SR_T 512
+#endif
+constexpr int SR_THREADS = SR_T;
 constexpr int SR_WARPS = SR_THREADS / 32;
-constexpr int SR_BINS = 4 * SR_THREADS;   // first histogram: four bins a thread
+constexpr int SR_BINS = SR_THREADS;       // first histogram: one bin a thread
+constexpr int SR_UNROLL = 4;              // elements a thread works on at once
 constexpr int SR_SUB = SR_THREADS;        // bins of a descent: one a thread (9 bits)
 constexpr int SR_MAX_CLUSTER = 8;
 constexpr float SR_SPAN = 40.f;           // logits that far below the maximum share the last bin
+constexpr float SR_HEAVY = 1.f / 1024.f;   // weights above it are summed in the first histogram
 constexpr double SR_ONE = 35184372088832.0;  // 2^45
 constexpr int SR_MAX_V = 1 << 18;
 typedef unsigned long long u64;
@@ -70,17 +75,18 @@ __device__ __forceinline__ float ex2f(float x) {
 }
 
 struct Shared {
-  // what peers read, each written before a cluster barrier
-  float mx[SR_MAX_CLUSTER], mn[SR_MAX_CLUSTER];  // pushed by every rank to every rank
-  float sum;                                     // fp32 sum of the slice's weights
-  int first;                                     // lowest index of the slice that holds the maximum
-  u64 mass[2];                                   // exact sums of the slice (whole / above the bins)
-  u64 kept;                                      // kept mass without ties
-  unsigned ties;                                 // elements equal to the cut
-  unsigned sub_c[2][SR_SUB];
-  u64 sub_m[2][SR_SUB];
-  union alignas(16) {  // read 16 bytes at a time
-    unsigned hist[SR_BINS];
+  // per rank, pushed by every rank to every rank before a cluster barrier (a
+  // remote store costs its sender nothing, a remote load is ~0.3 us of waiting)
+  float mx[SR_MAX_CLUSTER], mn[SR_MAX_CLUSTER];
+  float sum[SR_MAX_CLUSTER];                       // fp32 sum of the slice's weights
+  int first[SR_MAX_CLUSTER];                       // lowest index of the slice that holds the maximum
+  u64 all[SR_MAX_CLUSTER], over[SR_MAX_CLUSTER];   // exact sums of the slice: whole, and above the likely bins
+  u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
+  unsigned ties[SR_MAX_CLUSTER];                   // elements equal to the cut
+  // read by peers after a cluster barrier
+  uint4 sub[2][SR_SUB];  // count, mass in three 15-bit digits (summed in 32 bits: for < 2^17 elements)
+  union {
+    uint2 hist[SR_BINS];            // count, mass of the heavy ones (2^-16 units)
     struct {
       u64 mass[SR_THREADS];       // kept mass of each thread's elements
       unsigned ties[SR_THREADS];  // and how many equal the cut
@@ -88,7 +94,7 @@ struct Shared {
   };
   // this CTA's own
   double pow2[64];  // 2^(-j / 64)
-  u64 red_m[SR_WARPS];
+  u64 red_m[SR_WARPS], red_o[SR_WARPS];
   unsigned red_c[SR_WARPS];
   float red_f[2][SR_WARPS];
   int found[2];
@@ -158,7 +164,7 @@ __device__ void block_scan(Shared& sh, u64& m, unsigned& c, u64* tm, unsigned* t
   *tc = ac;
 }
 
-static_assert(alignof(Shared) == 16 && offsetof(Shared, hist) % 16 == 0, "the histogram is read as uint4");
+static_assert(alignof(Shared) == 16 && offsetof(Shared, sub) % 16 == 0, "descent bins are read as uint4");
 
 struct Cut {
   uint32_t key;   // elements above it are kept (0: every element)
@@ -169,6 +175,12 @@ template <typename T>
 __device__ __forceinline__ const T* peer(const T* p, int rank, int C) {
   return C > 1 ? cg::this_cluster().map_shared_rank(p, rank) : p;
 }
+template <typename T>
+__device__ __forceinline__ T* to_peer(T* p, int rank, int C) {
+  return C > 1 ? cg::this_cluster().map_shared_rank(p, rank) : p;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier(int C) {
   if (C > 1) cg::this_cluster().sync();
   else __syncthreads();
@@ -179,6 +191,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
   extern __shared__ __align__(16) uint8_t dyn[];
   Shared& sh = *reinterpret_cast<Shared*>(dyn);
   pdl_trigger();
+  if (C > 1) cluster_arrive();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x % C, r = blockIdx.x / C;
@@ -190,10 +203,8 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
   const bool by_k = k > 0 && k < s.V, by_p = !(top_p >= 1.f);
   // rows where only the first maximum can stay
   const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
-  if (tid < 64) sh.pow2[tid] = exp2(-(double)tid / 64.0);
-  for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.hist[i] = 0;
-  sh.sub_c[0][tid] = 0;
-  sh.sub_m[0][tid] = 0;
+  sh.hist[tid] = make_uint2(0u, 0u);
+  sh.sub[0][tid] = make_uint4(0u, 0u, 0u, 0u);
 
   // ---- the slice into shared memory, 16-byte loads between its ragged ends;
   // xs starts at the address's place in 16 bytes, so both sides are aligned
@@ -235,25 +246,26 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       }
     }
   }
+  if (tid < 64) sh.pow2[tid] = exp2(-(double)tid / 64.0);
   mx = warp_max(mx);
   mn = -warp_max(-mn);
   if (lane == 0) { sh.red_f[0][warp] = mx; sh.red_f[1][warp] = mn; }
   __syncthreads();
-  for (int w = 0; w < SR_WARPS; w++) {
-    mx = fmaxf(mx, sh.red_f[0][w]);
-    mn = fminf(mn, sh.red_f[1][w]);
+  if (C > 1) cluster_wait();  // every rank runs: its shared memory may be written
+  if (warp == 0) {
+    mx = warp_max(sh.red_f[0][lane % SR_WARPS]);
+    mn = -warp_max(-sh.red_f[1][lane % SR_WARPS]);
+    if (lane < C) {
+      to_peer(sh.mx, lane, C)[rank] = mx;
+      to_peer(sh.mn, lane, C)[rank] = mn;
+    }
   }
-  if (C > 1) {
-    cg::this_cluster().sync();  // every rank runs: its shared memory may be written
-    if (tid < C) {
-      cg::this_cluster().map_shared_rank(sh.mx, tid)[rank] = mx;
-      cg::this_cluster().map_shared_rank(sh.mn, tid)[rank] = mn;
-    }
-    cg::this_cluster().sync();
-    for (int q = 0; q < C; q++) {
-      mx = fmaxf(mx, sh.mx[q]);
-      mn = fminf(mn, sh.mn[q]);
-    }
+  cluster_barrier(C);
+  mx = sh.mx[0];
+  mn = sh.mn[0];
+  for (int q = 1; q < C; q++) {
+    mx = fmaxf(mx, sh.mx[q]);
+    mn = fminf(mn, sh.mn[q]);
   }
   if (mx == -INFINITY) {  // nothing to draw from (the same for every rank)
     if (rank == 0 && tid == 0) {
@@ -272,111 +284,131 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
   auto bin_of = [&](float d) { return min(SR_BINS - 1, __float2int_rd(fminf(d * bin_scale, 1e6f))); };
   const int beg = min(n, tid * per), end = min(n, beg + per);  // consecutive elements; per is odd: no bank conflicts
   const bool need_bins = !top1 && (by_k || by_p);
+  // f(x[4], index of the first) over the thread's elements; -inf past the end
+  // (no weight, no bin). The loads of a group come before any atomic.
+  auto each = [&](auto&& f) {
+    for (int i = beg; i < end; i += SR_UNROLL) {
+      float x[SR_UNROLL];
+#pragma unroll
+      for (int j = 0; j < SR_UNROLL; j++) x[j] = i + j < end ? xs[i + j] : -INFINITY;
+      f(x, i);
+    }
+  };
   {
     float sum = 0.f;
     int first = 0x7fffffff;
-    for (int i = beg; i < end; i++) {
-      const float d = below(xs[i]);
-      sum += d == 0.f ? 1.f : d < INFINITY ? ex2f(-d * c2) : 0.f;
-      if (top1 && d == 0.f) first = min(first, i);
-      if (need_bins) {
-        const int b = bin_of(d);
-        if (b < SR_BINS - 1) atomicAdd(&sh.hist[b], 1u);  // the last bin is the rest
+    each([&](const float (&x)[SR_UNROLL], int i) {
+      float d[SR_UNROLL], e[SR_UNROLL];
+#pragma unroll
+      for (int j = 0; j < SR_UNROLL; j++) {
+        d[j] = below(x[j]);
+        e[j] = d[j] == 0.f ? 1.f : d[j] < INFINITY ? ex2f(-d[j] * c2) : 0.f;
+        sum += e[j];
+        if (top1 && d[j] == 0.f && i + j < end) first = min(first, i + j);
       }
-    }
+      if (need_bins) {
+#pragma unroll
+        for (int j = 0; j < SR_UNROLL; j++) {
+          const int b = bin_of(d[j]);
+          if (b < SR_BINS - 1) {  // the last bin is the rest
+            atomicAdd(&sh.hist[b].x, 1u);
+            if (e[j] > SR_HEAVY) atomicAdd(&sh.hist[b].y, __float2uint_rn(e[j] * 65536.f));
+          }
+        }
+      }
+    });
     sum = warp_sum(sum);
     first = __reduce_min_sync(0xffffffffu, first);
-    __syncthreads();  // red_f has been read
     if (lane == 0) { sh.red_f[0][warp] = sum; sh.red_c[warp] = (unsigned)first; }
     __syncthreads();
-    if (tid == 0) {
-      float a = 0.f;
-      int f = 0x7fffffff;
-      for (int w = 0; w < SR_WARPS; w++) { a += sh.red_f[0][w]; f = min(f, (int)sh.red_c[w]); }
-      sh.sum = a;
-      sh.first = f == 0x7fffffff ? f : c0 + f;
+    if (warp == 0) {
+      sum = warp_sum(lane < SR_WARPS ? sh.red_f[0][lane] : 0.f);
+      first = __reduce_min_sync(0xffffffffu, (int)sh.red_c[lane % SR_WARPS]);
+      if (lane < C) {
+        to_peer(sh.sum, lane, C)[rank] = sum;
+        to_peer(sh.first, lane, C)[rank] = first == 0x7fffffff ? first : c0 + first;
+      }
     }
   }
   const Weigh wt{(double)mx, 92.332482616893656877 / (double)t1, sh.pow2};  // 64 / ln 2 / T
   auto finish = [&](int token, float x) {
     s.tokens[r] = token;
     if (s.logprobs) {
-      double z = 0.0;
-      for (int q = 0; q < C; q++) z += (double)peer(&sh, q, C)->sum;
-      const double d = x == mx ? 0.0 : ((double)x - (double)mx) / (double)t1;
-      s.logprobs[r] = (float)(d - log(z));
+      float z = 0.f;
+      for (int q = 0; q < C; q++) z += sh.sum[q];
+      s.logprobs[r] = -(below(x) / t1) - logf(z);
     }
   };
   if (top1 || need_bins) cluster_barrier(C);
   if (top1) {
     if (rank == 0 && tid == 0) {
       int f = 0x7fffffff;
-      for (int q = 0; q < C; q++) f = min(f, peer(&sh, q, C)->first);
+      for (int q = 0; q < C; q++) f = min(f, sh.first[q]);
       finish(f, mx);
     }
-    cluster_barrier(C);  // rank 0 has read its peers
     return;
   }
 
   int level = 0;  // descents so far: their buffers alternate
   // The cut where the running count (or mass) in descending order reaches
   // `target`, known to lie in bins ba..bb, above which there are `above`;
-  // among the elements inside `in`. Returns false, with *total the sum inside
-  // the bins, where it does not lie there.
-  auto descend = [&](const Cut& in, bool mass, u64 target, int ba, int bb, u64 above, Cut* out, u64* total) -> bool {
+  // among the elements inside `in`. False where it does not lie there.
+  auto descend = [&](const Cut& in, bool mass, u64 target, int ba, int bb, u64 above, Cut* out) -> bool {
     // keys that the bins can hold (a hundredth of a bin and a few ulps around them)
     const float w = span / (float)SR_BINS, slack = 0.01f * w + 1e-6f * fabsf(mx);
     uint32_t klo = bb >= SR_BINS - 1 ? 0u : key_of(mx - (float)(bb + 1) * w - slack);
     uint32_t khi = ba <= 0 ? key_of(mx) : key_of(fminf(mx, mx - (float)ba * w + slack));
     if (mx == INFINITY) { klo = 0u; khi = key_of(mx); }
-    bool started = false;
     for (;;) {
       int shift = 0;
       while (((khi - klo) >> shift) >= (uint32_t)SR_SUB) shift++;
-      const int buf = level & 1;
+      uint4* sub = sh.sub[level & 1];
       auto put = [&](float x, uint32_t key, unsigned count) {
         const int b = bin_of(below(x));
         if (b < ba || b > bb) return;
-        const uint32_t sub = min((uint32_t)(SR_SUB - 1), (key - klo) >> shift);
-        atomicAdd(&sh.sub_c[buf][sub], count);
-        if (mass) atomicAdd(&sh.sub_m[buf][sub], (u64)count * Weigh::fixed(wt.value(x, mx)));
+        unsigned* to = &sub[(key - klo) >> shift].x;
+        atomicAdd(to, count);
+        if (mass) {
+          const u64 f = Weigh::fixed(wt.value(x, mx));
+          atomicAdd(to + 1, (unsigned)(f & 0x7fffu) * count);
+          atomicAdd(to + 2, (unsigned)(f >> 15 & 0x7fffu) * count);
+          atomicAdd(to + 3, (unsigned)(f >> 30) * count);
+        }
       };
-      for (int i = beg; i < end; i++) {
-        const float x = xs[i];
-        const uint32_t key = key_of(x);
-        if (key >= klo && key <= khi && key > in.key) put(x, key, 1u);
+      each([&](const float (&x)[SR_UNROLL], int) {
+#pragma unroll
+        for (int j = 0; j < SR_UNROLL; j++) {
+          const uint32_t key = key_of(x[j]);
+          if (key >= klo && key <= khi && key > in.key) put(x[j], key, 1u);
+        }
+      });
+      // the ties of `in`, dealt over the ranks: a digit's sum holds a slice's elements and as many ties
+      if (in.ties && tid == 0 && in.key >= klo && in.key <= khi) {
+        const unsigned share = (in.ties + C - 1) / C, from = min(in.ties, share * rank);
+        put(of_key(in.key), in.key, min(in.ties, from + share) - from);
       }
-      if (rank == 0 && tid == 0 && in.ties && in.key >= klo && in.key <= khi) put(of_key(in.key), in.key, in.ties);
       cluster_barrier(C);
       // sub-bins in descending order: thread t has SUB - 1 - t
       const int mine = SR_SUB - 1 - tid;
       unsigned c = 0;
       u64 m = 0;
-      for (int q = 0; q < C; q++) {
-        const Shared* o = peer(&sh, q, C);
-        c += o->sub_c[buf][mine];
-        if (mass) m += o->sub_m[buf][mine];
-      }
+#pragma unroll
+      for (int q = 0; q < SR_MAX_CLUSTER; q++)
+        if (q < C) {
+          const uint4 v = peer(sub, q, C)[mine];
+          c += v.x;
+          m += (u64)v.y + ((u64)v.z << 15) + ((u64)v.w << 30);
+        }
       level++;
-      sh.sub_c[level & 1][tid] = 0;  // read last before the barrier above
-      sh.sub_m[level & 1][tid] = 0;
+      sh.sub[level & 1][tid] = make_uint4(0u, 0u, 0u, 0u);  // read last before the barrier above
       const unsigned c1 = c;
       const u64 m1 = m;
       u64 tm;
       unsigned tc;
       block_scan(sh, m, c, &tm, &tc);
-      const u64 inside = mass ? tm : (u64)tc;
-      if (!started) {
-        *total = inside;
-        if (above >= target || above + inside < target) {
-          __syncthreads();
-          return false;
-        }
-        started = true;
-      }
-      const u64 incl = above + (mass ? m : (u64)c), one = mass ? m1 : (u64)c1;
       if (tid == 0) sh.found[0] = -1;
       __syncthreads();
+      const u64 incl = above + (mass ? m : (u64)c), one = mass ? m1 : (u64)c1;
       if (c1 && incl >= target && incl - one < target) {
         sh.found[0] = mine;
         sh.found_m = incl - one;
@@ -384,64 +416,48 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       }
       __syncthreads();
       const int sel = sh.found[0];
-      if (sel < 0) return false;  // not reached: the bins' sum passed the target
+      if (sel < 0) return false;
       above = sh.found_m;
       klo += (uint32_t)sel << shift;
       khi = min(khi, klo + ((1u << shift) - 1u));
       if (shift == 0) {
-        const u64 each = mass ? Weigh::fixed(wt.value(of_key(klo), mx)) : 1;
-        u64 j = each ? (target - above + each - 1) / each : sh.found_c;
+        const u64 each_w = mass ? Weigh::fixed(wt.value(of_key(klo), mx)) : 1;
+        u64 j = each_w ? (target - above + each_w - 1) / each_w : sh.found_c;
         if (j > sh.found_c) j = sh.found_c;
         out->key = klo;
         out->ties = (unsigned)j;
-        __syncthreads();  // found_* has been read
         return true;
       }
-      __syncthreads();
     }
   };
 
   Cut cut{0u, 0u};
   if (need_bins) {
-    // ---- the first histogram over the cluster: thread t has bins 4t .. 4t + 3
-    unsigned c[4] = {0, 0, 0, 0};
-    for (int q = 0; q < C; q++) {
-      const uint4 v = *reinterpret_cast<const uint4*>(&peer(&sh, q, C)->hist[4 * tid]);
-      c[0] += v.x; c[1] += v.y; c[2] += v.z; c[3] += v.w;
-    }
-    // running counts, and masses estimated at the middle of each bin (2^-20
-    // units: only a guess, checked below)
-    const float w = span / (float)SR_BINS;
-    u64 m4 = 0, mb[4];
-    unsigned c4 = 0;
+    // ---- the first histogram over the cluster: thread t has bin t. Masses
+    // are a guess, checked below: sums of 2^-16 units where the bin's weights
+    // are heavy, count * weight at the middle of the bin where they are light
+    unsigned c1 = 0;
+    u64 heavy = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      mb[j] = (u64)((float)c[j] * ex2f(-((float)(4 * tid + j) + 0.5f) * w * c2) * 1048576.f);
-      m4 += mb[j];
-      c4 += c[j];
-    }
-    u64 mt, m_in = m4;
-    unsigned ct, c_in = c4;
+    for (int q = 0; q < SR_MAX_CLUSTER; q++)
+      if (q < C) {
+        const uint2 v = peer(sh.hist, q, C)[tid];
+        c1 += v.x;
+        heavy += v.y;
+      }
+    const float mid = ex2f(-((float)tid + 0.5f) * (span / (float)SR_BINS) * c2);
+    const u64 m1 = mid > SR_HEAVY ? heavy << 16 : (u64)((float)c1 * mid * 4294967296.f);
+    u64 mt, m_in = m1;
+    unsigned ct, c_in = c1;
     block_scan(sh, m_in, c_in, &mt, &ct);
     if (tid == 0) { sh.found[0] = SR_BINS - 1; sh.found_c = ct; sh.found_m = mt; }
     __syncthreads();
-    if (by_k) {
-      unsigned run = c_in - c4;
-      u64 mrun = m_in - m4;
-      if (run < (unsigned)k && (unsigned)k <= c_in) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (run < (unsigned)k && (unsigned)k <= run + c[j]) {
-            sh.found[0] = 4 * tid + j;
-            sh.found_c = run;
-            sh.found_m = mrun + (u64)((float)mb[j] * ((float)(k - run) / (float)c[j]));
-          }
-          run += c[j];
-          mrun += mb[j];
-        }
-      }
-      __syncthreads();
+    if (by_k && c_in - c1 < (unsigned)k && (unsigned)k <= c_in) {
+      sh.found[0] = tid;
+      sh.found_c = c_in - c1;
+      sh.found_m = m_in - m1 + (u64)((float)m1 * ((float)(k - (int)(c_in - c1)) / (float)c1));
     }
+    __syncthreads();
     const int kbin = sh.found[0];
     const unsigned kabove = sh.found_c;
     const u64 guess = sh.found_m;
@@ -450,49 +466,50 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       __syncthreads();
       if (tid == 0) sh.found[1] = by_k ? kbin : SR_BINS - 1;
       __syncthreads();
-      const u64 goal = max((u64)1, (u64)((float)guess * top_p));
-      if (m_in - m4 < goal && goal <= m_in) {
-        u64 run = m_in - m4;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (run < goal && goal <= run + mb[j]) sh.found[1] = by_k ? min(kbin, 4 * tid + j) : 4 * tid + j;
-          run += mb[j];
-        }
-      }
+      const u64 goal = max((u64)1, (u64)((double)guess * (double)top_p));
+      if (m_in - m1 < goal && goal <= m_in) sh.found[1] = by_k ? min(kbin, tid) : tid;
       __syncthreads();
       pbin = sh.found[1];
     }
-    u64 total;
     if (by_k) {
       const Cut every{0u, 0u};
-      if (!descend(every, false, (u64)k, kbin, kbin, kabove, &cut, &total))
-        descend(every, false, (u64)k, 0, SR_BINS - 1, 0, &cut, &total);
+      if (!descend(every, false, (u64)k, kbin, kbin, kabove, &cut))
+        descend(every, false, (u64)k, 0, SR_BINS - 1, 0, &cut);
     }
     if (by_p) {
       // ---- exact masses: of the top-k, and of what lies above the likely bins
-      const int ba = max(0, pbin - 1), bb = min(SR_BINS - 1, pbin + 1);
+      const int ba = max(0, pbin - 1), bb = min(SR_BINS - 1, pbin + 1);  // and one bin either side
       u64 all = 0, over = 0;
-      for (int i = beg; i < end; i++) {
-        const float x = xs[i];
-        if (key_of(x) <= cut.key) continue;
-        const u64 f = Weigh::fixed(wt.value(x, mx));
-        all += f;
-        if (bin_of(below(x)) < ba) over += f;
-      }
+      each([&](const float (&x)[SR_UNROLL], int) {
+        bool in[SR_UNROLL], any = false;
+#pragma unroll
+        for (int j = 0; j < SR_UNROLL; j++) any |= in[j] = key_of(x[j]) > cut.key;
+        if (!any) return;
+#pragma unroll
+        for (int j = 0; j < SR_UNROLL; j++) {
+          const u64 f = in[j] ? Weigh::fixed(wt.value(x[j], mx)) : 0;
+          all += f;
+          over += bin_of(below(x[j])) < ba ? f : 0;
+        }
+      });
       all = warp_sum64(all);
       over = warp_sum64(over);
+      __syncthreads();  // red_m has been read
+      if (lane == 0) { sh.red_m[warp] = all; sh.red_o[warp] = over; }
       __syncthreads();
-      if (tid == 0) sh.mass[0] = sh.mass[1] = 0;
-      __syncthreads();
-      if (lane == 0) {
-        atomicAdd(&sh.mass[0], all);
-        atomicAdd(&sh.mass[1], over);
+      if (warp == 0) {
+        all = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
+        over = warp_sum64(lane < SR_WARPS ? sh.red_o[lane] : 0);
+        if (lane < C) {
+          to_peer(sh.all, lane, C)[rank] = all;
+          to_peer(sh.over, lane, C)[rank] = over;
+        }
       }
       cluster_barrier(C);
       all = over = 0;
       for (int q = 0; q < C; q++) {
-        all += peer(&sh, q, C)->mass[0];
-        over += peer(&sh, q, C)->mass[1];
+        all += sh.all[q];
+        over += sh.over[q];
       }
       if (cut.ties) {
         const float x = of_key(cut.key);
@@ -504,8 +521,8 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       u64 goal = want >= 1.0 ? (u64)want : 1;
       if (goal > all) goal = all;
       const Cut in = cut;
-      if (!descend(in, true, goal, ba, bb, over, &cut, &total))
-        descend(in, true, goal, 0, SR_BINS - 1, 0, &cut, &total);  // the guess was wrong: over the whole row
+      if (over >= goal || !descend(in, true, goal, ba, bb, over, &cut))
+        descend(in, true, goal, 0, SR_BINS - 1, 0, &cut);  // the guess was wrong: over the whole row
     }
   }
 
@@ -514,17 +531,21 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
   {
     u64 m = 0;
     unsigned e = 0;
-    for (int i = beg; i < end; i++) {
-      const float x = xs[i];
-      const uint32_t key = key_of(x);
-      if (key < cut.key) continue;
-      if (key == cut.key) {
-        e++;
-        continue;
+    each([&](const float (&x)[SR_UNROLL], int) {
+      bool in[SR_UNROLL], any = false;
+#pragma unroll
+      for (int j = 0; j < SR_UNROLL; j++) {
+        const uint32_t key = key_of(x[j]);
+        any |= in[j] = key > cut.key;
+        e += key == cut.key;
       }
-      const double w = wt.value(x, mx);
-      if (w >= least) m += Weigh::fixed(w);
-    }
+      if (!any) return;
+#pragma unroll
+      for (int j = 0; j < SR_UNROLL; j++) {
+        const double w = in[j] ? wt.value(x[j], mx) : 0.0;
+        if (w >= least) m += Weigh::fixed(w);
+      }
+    });
     // `part` shares the histogram's memory: that was read last before the latest barrier
     sh.part.mass[tid] = m;
     sh.part.ties[tid] = e;
@@ -533,12 +554,13 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
     __syncthreads();
     if (lane == 0) { sh.red_m[warp] = m; sh.red_c[warp] = e; }
     __syncthreads();
-    if (tid == 0) {
-      u64 a = 0;
-      unsigned b = 0;
-      for (int w = 0; w < SR_WARPS; w++) { a += sh.red_m[w]; b += sh.red_c[w]; }
-      sh.kept = a;
-      sh.ties = b;
+    if (warp == 0) {
+      m = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
+      e = __reduce_add_sync(0xffffffffu, lane < SR_WARPS ? sh.red_c[lane] : 0u);
+      if (lane == 0) {
+        to_peer(sh.kept, 0, C)[rank] = m;
+        to_peer(sh.ties, 0, C)[rank] = e;
+      }
     }
   }
   cluster_barrier(C);
@@ -553,9 +575,8 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
     u64 mass = 0;
     unsigned left = cut.ties;
     for (int q = 0; q < C; q++) {
-      const Shared* o = peer(&sh, q, C);
-      const unsigned e = min(left, o->ties);
-      mass += o->kept + e * tie;
+      const unsigned e = min(left, sh.ties[q]);
+      mass += sh.kept[q] + e * tie;
       left -= e;
     }
     float u = s.u[r];
@@ -567,64 +588,62 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
     int q = 0;
     left = cut.ties;
     for (; q < C - 1; q++) {
-      const Shared* o = peer(&sh, q, C);
-      const unsigned e = min(left, o->ties);
-      const u64 here = o->kept + e * tie;
+      const unsigned e = min(left, sh.ties[q]);
+      const u64 here = sh.kept[q] + e * tie;
       if (goal <= here) break;
       goal -= here;
       left -= e;
     }
     const Shared* o = peer(&sh, q, C);
-    // thread: the running number of ties first, then the running mass
-    u64 m = o->part.mass[tid], tm;
-    unsigned e = o->part.ties[tid], tc;
-    const unsigned e1 = e;
-    u64 none = 0;
-    block_scan(sh, none, e, &tm, &tc);
-    const unsigned before = e - e1, kept_e = before >= left ? 0u : min(e1, left - before);
-    const u64 m1 = m + kept_e * tie;
-    m = m1;
-    unsigned zero = 0;
-    block_scan(sh, m, zero, &tm, &tc);
-    if (tid == 0) { sh.found[0] = 0; sh.found_m = 0; sh.found_c = 0; }
-    __syncthreads();
-    if (m >= goal && m - m1 < goal) {
+    // thread: running mass with the running number of ties, of which `left` stay
+    const u64 m1 = o->part.mass[tid];
+    const unsigned e1 = o->part.ties[tid];
+    u64 m = m1, tm;
+    unsigned e = e1, tc;
+    if (tid == 0) { sh.found[0] = 0; sh.found_m = 1; sh.found_c = 0; }
+    block_scan(sh, m, e, &tm, &tc);
+    const u64 upto = m + min(e, left) * tie, before = m - m1 + min(e - e1, left) * tie;
+    if (upto >= goal && before < goal) {
       sh.found[0] = tid;
-      sh.found_m = goal - (m - m1);
-      sh.found_c = before >= left ? 0u : left - before;  // ties still to keep in it
+      sh.found_m = goal - before;
+      sh.found_c = left - min(e - e1, left);  // ties still to keep in it
     }
     __syncthreads();
-    const int owner = sh.found[0];
-    goal = sh.found_m;
-    left = sh.found_c;
-    // element: the owner's `per` consecutive ones, one a thread at a time
-    const int qc0 = min(s.V, q * slice), qn = min(s.V, qc0 + slice) - qc0;
-    const int ob = min(qn, owner * per), on = min(qn, ob + per) - ob;
-    const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + qc0) * es;
-    const int qlead = (int)((reinterpret_cast<uintptr_t>(qsrc) / es) % vec);
-    const float* qx = peer(reinterpret_cast<const float*>(dyn + ((sizeof(Shared) + 15) / 16) * 16), q, C) + qlead + ob;
-    for (int i0 = 0; i0 < on; i0 += SR_THREADS) {
-      const int i = i0 + tid;
-      const float x = i < on ? qx[i] : -INFINITY;
-      const uint32_t key = key_of(x);
-      const bool is_tie = i < on && key == cut.key;
-      e = is_tie;
-      none = 0;
-      block_scan(sh, none, e, &tm, &tc);
-      const unsigned ties_here = tc;
-      u64 f = 0;
-      if (is_tie) f = e <= left ? tie : 0;
-      else if (i < on && key > cut.key) {
-        const double w = wt.value(x, mx);
-        if (w >= least) f = Weigh::fixed(w);
+    if (warp == 0) {
+      const int owner = sh.found[0];
+      goal = sh.found_m;
+      left = sh.found_c;
+      // element: the owner's consecutive ones, 32 at a time
+      const int qc0 = min(s.V, q * slice), qn = min(s.V, qc0 + slice) - qc0;
+      const int ob = min(qn, owner * per), on = min(qn, ob + per) - ob;
+      const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + qc0) * es;
+      const int qlead = (int)((reinterpret_cast<uintptr_t>(qsrc) / es) % vec);
+      const float* qx = peer(reinterpret_cast<const float*>(dyn + ((sizeof(Shared) + 15) / 16) * 16), q, C) + qlead + ob;
+      for (int i0 = 0; i0 < on; i0 += 32) {
+        const int i = i0 + lane;
+        const float x = i < on ? qx[i] : -INFINITY;
+        const uint32_t key = key_of(x);
+        const bool is_tie = i < on && key == cut.key;
+        const unsigned ties = __ballot_sync(0xffffffffu, is_tie);
+        u64 f = 0;
+        if (is_tie) {
+          f = (unsigned)__popc(ties & ((1u << lane) - 1u)) < left ? tie : 0;
+        } else if (i < on && key > cut.key) {
+          const double w = wt.value(x, mx);
+          if (w >= least) f = Weigh::fixed(w);
+        }
+        u64 run = f;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const u64 v = __shfl_up_sync(0xffffffffu, run, d);
+          if (lane >= d) run += v;
+        }
+        if (f && run >= goal && run - f < goal) finish(qc0 + ob + i, x);
+        const u64 here = __shfl_sync(0xffffffffu, run, 31);
+        if (goal <= here) break;
+        goal -= here;
+        left -= min(left, (unsigned)__popc(ties));
       }
-      m = f;
-      zero = 0;
-      block_scan(sh, m, zero, &tm, &tc);
-      if (f && m >= goal && m - f < goal) finish(qc0 + ob + i, x);
-      if (goal <= tm) break;
-      goal -= tm;
-      left = left > ties_here ? left - ties_here : 0;
     }
   }
   cluster_barrier(C);  // rank 0 has read its peers
