@@ -13,21 +13,25 @@
 //
 // A cluster of C CTAs takes a row; each holds its slice in shared memory as
 // fp32, so the row is read from memory once and every later pass is over
-// shared memory. Cuts are found without sorting:
+// shared memory. Nothing is sorted but a short list:
 //  1. a histogram of counts over SR_BINS equal steps of the logit below the
-//     maximum (one shared atomic an element) gives the exact bin of the
-//     top-k cut, and from count * exp(middle) the likely bin of the top-p cut;
-//  2. one pass sums the exact masses of everything and of what lies above
-//     the likely bins (the only pass that needs an exponential of each
-//     element, and only for rows with top-p and no top-k);
-//  3. the cut is pinned inside the bins by descents over the order-preserving
-//     bit patterns of the logits, 9 bits a pass, with exact counts and masses
-//     (two passes as a rule). Where the likely bins were wrong the exact sums
-//     say so and the descent starts again over the whole row.
-// The draw sums the kept weights of each thread's consecutive elements; rank
-// 0 then walks cluster rank -> thread -> element to where the running mass
-// passes u * mass. Equal logits need no list: their count, their common
-// weight and the running count in index order say which of them are kept.
+//     maximum (one shared atomic an element) gives the bin of the top-k cut,
+//     and with the masses of the heavy elements and count * exp(middle) for
+//     the light bins the likely bin of the top-p cut;
+//  2. where the bins that can be kept hold at most SR_LIST elements (as a
+//     rule: a nucleus, a top-k, a min-p set), those go to rank 0 in index
+//     order, which sorts them and finishes alone. Of the rest of the row only
+//     the exact mass is needed, and only by top-p without top-k;
+//  3. else the cut is pinned by descents over the order-preserving bit
+//     patterns of the logits, 9 bits a pass, with exact counts and masses, and
+//     the draw walks cluster rank -> thread -> element over the kept masses of
+//     each thread's consecutive elements. Rows without filters go straight to
+//     that walk. Where the likely bin of a top-p cut was wrong the exact sums
+//     say so and the descent covers the whole row.
+//
+// What bounds it: 64-bit floats run at a sixteenth of the fp32 rate here, so
+// a weight takes 11 of them; the rest is the latency of the cluster's
+// exchanges (a barrier ~1 us with its skew), which rows in flight hide.
 #include <cooperative_groups.h>
 
 #include <cstddef>
@@ -44,20 +48,19 @@ namespace cg = cooperative_groups;
 #ifndef SR_MINB
 #define SR_MINB 2
 #endif
-
-#ifndef SR_T
-#define SR_T 512
-#endif
-constexpr int SR_THREADS = SR_T;
+constexpr int SR_THREADS = 512;
 constexpr int SR_WARPS = SR_THREADS / 32;
 constexpr int SR_BINS = SR_THREADS;       // first histogram: one bin a thread
-constexpr int SR_UNROLL = 4;              // elements a thread works on at once
 constexpr int SR_SUB = SR_THREADS;        // bins of a descent: one a thread (9 bits)
+constexpr int SR_LIST = 2 * SR_THREADS;   // candidates that rank 0 can finish alone
 constexpr int SR_MAX_CLUSTER = 8;
+constexpr int SR_TABLE = 256;
 constexpr float SR_SPAN = 40.f;           // logits that far below the maximum share the last bin
-constexpr float SR_HEAVY = 1.f / 1024.f;   // weights above it are summed in the first histogram
-constexpr double SR_ONE = 35184372088832.0;  // 2^45
+constexpr float SR_HEAVY = 1.f / 1024.f;  // weights above it are summed in the first histogram
+constexpr double SR_STEP = -0.69314718055994530942 / SR_TABLE;  // ln of a table step
+constexpr float SR_OCTAVES = 46.5f;       // weights below 2^-46.5 are 0 in those units
 constexpr int SR_MAX_V = 1 << 18;
+constexpr int SR_PAD = 8;                 // a slice may start up to 7 elements into its 16 bytes
 typedef unsigned long long u64;
 
 // Unsigned keys in the order of the values (-0 with +0); 0 is no value's key.
@@ -83,17 +86,25 @@ struct Shared {
   u64 all[SR_MAX_CLUSTER], over[SR_MAX_CLUSTER];   // exact sums of the slice: whole, and above the likely bins
   u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
   unsigned ties[SR_MAX_CLUSTER];                   // elements equal to the cut
+  unsigned listed[SR_MAX_CLUSTER];                 // candidates of the slice
+  int again;                                       // rank 0: the list did not reach the top-p cut
   // read by peers after a cluster barrier
-  uint4 sub[2][SR_SUB];  // count, mass in three 15-bit digits (summed in 32 bits: for < 2^17 elements)
-  union {
-    uint2 hist[SR_BINS];            // count, mass of the heavy ones (2^-16 units)
+  uint2 hist[SR_BINS];                             // count, mass of the heavy ones (2^-16 units)
+  union alignas(16) {
+    uint4 sub[2][SR_SUB];  // descents: count, mass in three 15-bit digits (summed in 32 bits: for < 2^17 elements)
+    struct {
+      float x[SR_LIST];    // candidates of the slice in index order
+      int i[SR_LIST];
+    } list;
     struct {
       u64 mass[SR_THREADS];       // kept mass of each thread's elements
       unsigned ties[SR_THREADS];  // and how many equal the cut
     } part;
   };
   // this CTA's own
-  double pow2[64];  // 2^(-j / 64)
+  double pow2[SR_TABLE];  // 2^(-j / 256)
+  u64 order[SR_LIST];     // rank 0: candidates to sort, then their kept masses in index order
+  int index[SR_LIST];
   u64 red_m[SR_WARPS], red_o[SR_WARPS];
   unsigned red_c[SR_WARPS];
   float red_f[2][SR_WARPS];
@@ -101,34 +112,45 @@ struct Shared {
   u64 found_m;
   unsigned found_c;
 };
+static_assert(offsetof(Shared, sub) % 16 == 0, "descent bins are read as uint4");
+constexpr int SR_HEAD = (int)((sizeof(Shared) + 15) / 16 * 16);  // the slice begins here
 
-// The weight of a logit: the definition's 64-bit value by argument reduction,
-// w = 2^-(y / 64) with y = 64 (max - x) / (T ln 2) = n + r, n the nearest
-// integer: 2^-(n >> 6) from the exponent, 2^-((n & 63) / 64) from a table,
-// 2^(-r / 64) by its Taylor series (|r ln 2 / 64| <= 0.0055: five terms leave
-// 4e-17).
+// The weight of a logit: the definition's 64-bit value by argument reduction.
+// With y = 256 (max - x) / (T ln 2) = n + r, n the nearest integer,
+// w = 2^-(n >> 8) * 2^-((n & 255) / 256) * exp(-r ln 2 / 256): the exponent, a
+// table, and a Taylor series (|r ln 2 / 256| <= 0.00136: four terms leave 4e-17).
 struct Weigh {
-  double mx, c64;
+  double mx, c;  // c = 256 / (T ln 2)
   const double* pow2;
-  // the weight; 0 where it is below 2^-46
-  __device__ __forceinline__ double value(float x, float mxf) const {
-    if (x == mxf) return 1.0;
-    const double y = (mx - (double)x) * c64;
-    if (!(y < 46.0 * 64.0)) return 0.0;
-    const double magic = 6755399441055744.0;  // 2^52 + 2^51: the sum's low word is the nearest integer
-    const double shifted = y + magic;
+  // w = v * 2^-oct
+  __device__ __forceinline__ double value(float x, int* oct) const {
+    const double magic = 6755399441055744.0;  // 2^52 + 2^51: a sum's low word is the nearest integer
+    const double d = mx - (double)x, shifted = fma(d, c, magic);
     const int n = __double2loint(shifted);
-    const double s = (y - (shifted - magic)) * -0.010830424696249145;  // -ln 2 / 64
-    double p = fma(s, 1.0 / 120.0, 1.0 / 24.0);
-    p = fma(p, s, 1.0 / 6.0);
-    p = fma(p, s, 0.5);
-    p = fma(p, s, 1.0);
-    p = fma(p, s, 1.0);
-    return pow2[n & 63] * p * __hiloint2double((1023 - (n >> 6)) << 20, 0);
+    const double r = fma(d, c, magic - shifted);
+    constexpr double a1 = SR_STEP, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4;
+    double p = fma(r, a4, a3);
+    p = fma(p, r, a2);
+    p = fma(p, r, a1);
+    p = fma(p, r, 1.0);
+    *oct = n >> 8;
+    return pow2[n & (SR_TABLE - 1)] * p;
   }
-  static __device__ __forceinline__ u64 fixed(double w) {
-    // w * 2^45 + 2^52 leaves the rounded integer in the low 52 bits
-    return (u64)__double_as_longlong(fma(w, SR_ONE, 4503599627370496.0)) & 0xfffffffffffffull;
+  // w in units of 2^-45: v * 2^(45 - oct) + 2^52 leaves the rounded integer in the low 52 bits
+  static __device__ __forceinline__ u64 fixed(double v, int oct) {
+    const double scale = __hiloint2double((1023 + 45 - oct) << 20, 0);
+    return (u64)__double_as_longlong(fma(v, scale, 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ u64 fixed_of(float x) const {
+    int oct;
+    const double v = value(x, &oct);
+    return fixed(v, oct);
+  }
+  // the same, 0 where w < least
+  __device__ __forceinline__ u64 fixed_from(float x, double least) const {
+    int oct;
+    const double v = value(x, &oct);
+    return v * __hiloint2double((1023 - oct) << 20, 0) >= least ? fixed(v, oct) : 0;
   }
 };
 
@@ -139,7 +161,7 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
 }
 
 // Inclusive scans over the CTA of a mass and a count; *tm, *tc: the totals.
-__device__ void block_scan(Shared& sh, u64& m, unsigned& c, u64* tm, unsigned* tc) {
+__device__ __forceinline__ void block_scan(Shared& sh, u64& m, unsigned& c, u64* tm, unsigned* tc) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -164,19 +186,13 @@ __device__ void block_scan(Shared& sh, u64& m, unsigned& c, u64* tm, unsigned* t
   *tc = ac;
 }
 
-static_assert(alignof(Shared) == 16 && offsetof(Shared, sub) % 16 == 0, "descent bins are read as uint4");
-
 struct Cut {
   uint32_t key;   // elements above it are kept (0: every element)
   unsigned ties;  // and so many of those equal to it, in index order
 };
 
 template <typename T>
-__device__ __forceinline__ const T* peer(const T* p, int rank, int C) {
-  return C > 1 ? cg::this_cluster().map_shared_rank(p, rank) : p;
-}
-template <typename T>
-__device__ __forceinline__ T* to_peer(T* p, int rank, int C) {
+__device__ __forceinline__ T* peer(T* p, int rank, int C) {
   return C > 1 ? cg::this_cluster().map_shared_rank(p, rank) : p;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
@@ -186,32 +202,57 @@ __device__ __forceinline__ void cluster_barrier(int C) {
   else __syncthreads();
 }
 
-// grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the slice
+// Descending bitonic sort of n2 (a power of two, at most SR_LIST) values.
+// Strides up to 32 stay inside the 64 values of a warp's pairs.
+__device__ void sort_desc(u64* v, int n2) {
+  const int t = threadIdx.x;
+  __syncthreads();  // the values are in place
+  for (int size = 2; size <= n2; size <<= 1) {
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      if (stride >= 32) __syncthreads();
+      else __syncwarp();
+      const int i = 2 * t - (t & (stride - 1)), j = i + stride;
+      if (j < n2) {
+        const u64 a = v[i], b = v[j];
+        if ((a < b) == ((i & size) == 0)) {
+          v[i] = b;
+          v[j] = a;
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the
+// slice: `per` (4 times an odd number: no bank conflicts) consecutive elements
+// for each thread, padded with -inf
 __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const wg_sample s, int C, int per) {
   extern __shared__ __align__(16) uint8_t dyn[];
   Shared& sh = *reinterpret_cast<Shared*>(dyn);
+  float* xs = reinterpret_cast<float*>(dyn + SR_HEAD);
   pdl_trigger();
   if (C > 1) cluster_arrive();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x % C, r = blockIdx.x / C;
-  const int slice = per * SR_THREADS;
+  const int slice = per * SR_THREADS - SR_PAD;
   const int c0 = min(s.V, rank * slice), n = min(s.V, c0 + slice) - c0;
   const float T = s.temperature ? s.temperature[r] : 1.f;
   const int k = s.top_k ? s.top_k[r] : 0;
   const float top_p = s.top_p ? s.top_p[r] : 1.f, min_p = s.min_p ? s.min_p[r] : 0.f;
-  const bool by_k = k > 0 && k < s.V, by_p = !(top_p >= 1.f);
+  const bool by_k = k > 0 && k < s.V, by_p = !(top_p >= 1.f), by_m = min_p > 0.f;
   // rows where only the first maximum can stay
   const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
+  const bool need_bins = !top1 && (by_k || by_p || by_m);
   sh.hist[tid] = make_uint2(0u, 0u);
-  sh.sub[0][tid] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid == 0) sh.again = 0;
 
   // ---- the slice into shared memory, 16-byte loads between its ragged ends;
-  // xs starts at the address's place in 16 bytes, so both sides are aligned
+  // it starts at the address's place in 16 bytes, so both sides are aligned
   const int es = dt_bytes(s.dtype), vec = 16 / es;
   const uint8_t* src = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + c0) * es;
   const int lead = (int)((reinterpret_cast<uintptr_t>(src) / es) % vec);
-  float* xs = reinterpret_cast<float*>(dyn + ((sizeof(Shared) + 15) / 16) * 16) + lead;
   float mx = -INFINITY, mn = INFINITY;
   {
     auto clean = [&](float x) {
@@ -221,10 +262,12 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       return x;
     };
     const int head = min(n, (vec - lead) % vec), body = (n - head) / vec, tail = n - head - body * vec;
-    if (tid < head) xs[tid] = clean(dt_load(src, tid, s.dtype));
-    if (tid < tail) xs[n - tail + tid] = clean(dt_load(src, n - tail + tid, s.dtype));
+    if (tid < lead) xs[tid] = -INFINITY;
+    for (int i = lead + n + tid; i < per * SR_THREADS; i += SR_THREADS) xs[i] = -INFINITY;
+    if (tid < head) xs[lead + tid] = clean(dt_load(src, tid, s.dtype));
+    if (tid < tail) xs[lead + n - tail + tid] = clean(dt_load(src, n - tail + tid, s.dtype));
     const uint4* v = reinterpret_cast<const uint4*>(src + head * es);
-    float4* d = reinterpret_cast<float4*>(xs + head);
+    float4* d = reinterpret_cast<float4*>(xs + lead + head);
     constexpr int U = 4;  // loads in flight per thread
     for (int i0 = tid; i0 < body; i0 += U * SR_THREADS) {
       uint4 w[U];
@@ -246,7 +289,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       }
     }
   }
-  if (tid < 64) sh.pow2[tid] = exp2(-(double)tid / 64.0);
+  if (tid < SR_TABLE) sh.pow2[tid] = exp2(-(double)tid / SR_TABLE);
   mx = warp_max(mx);
   mn = -warp_max(-mn);
   if (lane == 0) { sh.red_f[0][warp] = mx; sh.red_f[1][warp] = mn; }
@@ -256,8 +299,8 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
     mx = warp_max(sh.red_f[0][lane % SR_WARPS]);
     mn = -warp_max(-sh.red_f[1][lane % SR_WARPS]);
     if (lane < C) {
-      to_peer(sh.mx, lane, C)[rank] = mx;
-      to_peer(sh.mn, lane, C)[rank] = mn;
+      peer(sh.mx, lane, C)[rank] = mx;
+      peer(sh.mn, lane, C)[rank] = mn;
     }
   }
   cluster_barrier(C);
@@ -274,49 +317,60 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
     }
     return;
   }
-
-  // ---- fp32 sum of the weights, first maximum, histogram of counts
-  const float t1 = T > 0.f ? T : 1.f;
-  const float c2 = 1.4426950408889634f / t1;
-  const float span = fminf(fmaxf(mx - mn, 1e-30f), SR_SPAN);
-  const float bin_scale = (float)SR_BINS / span;
-  auto below = [&](float x) { return x == mx ? 0.f : mx - x; };
-  auto bin_of = [&](float d) { return min(SR_BINS - 1, __float2int_rd(fminf(d * bin_scale, 1e6f))); };
-  const int beg = min(n, tid * per), end = min(n, beg + per);  // consecutive elements; per is odd: no bank conflicts
-  const bool need_bins = !top1 && (by_k || by_p);
-  // f(x[4], index of the first) over the thread's elements; -inf past the end
-  // (no weight, no bin). The loads of a group come before any atomic.
+  float4* mine = reinterpret_cast<float4*>(xs + tid * per);  // this thread's consecutive elements
+  const int first_i = c0 - lead + tid * per;                 // index of the first (below 0 only in padding)
+  if (mx == INFINITY) {  // the infinite ones share the mass: a row of 0 and -inf
+    auto flat = [](float x) { return x == INFINITY ? 0.f : -INFINITY; };
+    for (int i = 0; i < per / 4; i++) mine[i] = make_float4(flat(mine[i].x), flat(mine[i].y), flat(mine[i].z), flat(mine[i].w));
+    mx = mn = 0.f;
+    __syncthreads();
+  }
+  // f(x[4], i) over the thread's elements, i the place of the first of the four
   auto each = [&](auto&& f) {
-    for (int i = beg; i < end; i += SR_UNROLL) {
-      float x[SR_UNROLL];
-#pragma unroll
-      for (int j = 0; j < SR_UNROLL; j++) x[j] = i + j < end ? xs[i + j] : -INFINITY;
+#pragma unroll 1
+    for (int i = 0; i < per; i += 4) {
+      const float4 v = mine[i / 4];
+      const float x[4] = {v.x, v.y, v.z, v.w};
       f(x, i);
     }
   };
+
+  // ---- fp32 sum of the weights, first maximum, histogram of counts
+  const float t1 = fminf(fmaxf(T > 0.f ? T : 1.f, 1e-30f), 1e30f);
+  const float c2 = 1.4426950408889634f / t1;
+  const float span = fminf(fmaxf(mx - mn, 1e-30f), SR_SPAN);
+  const float bin_scale = (float)(SR_BINS - 1) / span;
+  // nearest bin, the last one for everything further down (2^23 + b holds b in its low bits)
+  auto bin_bits = [&](float x) { return fminf((mx - x) * bin_scale, (float)(SR_BINS - 1)) + 8388608.f; };
+  auto bin_of = [&](float x) { return __float_as_int(bin_bits(x)) & (SR_BINS - 1); };
   {
     float sum = 0.f;
     int first = 0x7fffffff;
-    each([&](const float (&x)[SR_UNROLL], int i) {
-      float d[SR_UNROLL], e[SR_UNROLL];
+    if (need_bins) {
+      each([&](const float (&x)[4], int) {
+        float e[4];
+        int b[4];
 #pragma unroll
-      for (int j = 0; j < SR_UNROLL; j++) {
-        d[j] = below(x[j]);
-        e[j] = d[j] == 0.f ? 1.f : d[j] < INFINITY ? ex2f(-d[j] * c2) : 0.f;
-        sum += e[j];
-        if (top1 && d[j] == 0.f && i + j < end) first = min(first, i + j);
-      }
-      if (need_bins) {
-#pragma unroll
-        for (int j = 0; j < SR_UNROLL; j++) {
-          const int b = bin_of(d[j]);
-          if (b < SR_BINS - 1) {  // the last bin is the rest
-            atomicAdd(&sh.hist[b].x, 1u);
-            if (e[j] > SR_HEAVY) atomicAdd(&sh.hist[b].y, __float2uint_rn(e[j] * 65536.f));
-          }
+        for (int j = 0; j < 4; j++) {
+          e[j] = ex2f((x[j] - mx) * c2);
+          b[j] = bin_of(x[j]);
+          sum += e[j];
         }
-      }
-    });
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (b[j] < SR_BINS - 1) atomicAdd(&sh.hist[b[j]].x, 1u);  // the last bin is the rest
+          if (e[j] > SR_HEAVY) atomicAdd(&sh.hist[b[j]].y, (unsigned)(__float_as_int(e[j] + 128.f) - 0x43000000));
+        }
+      });
+    } else {
+      each([&](const float (&x)[4], int i) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          sum += ex2f((x[j] - mx) * c2);
+          if (top1 && x[j] == mx) first = min(first, first_i + i + j);
+        }
+      });
+    }
     sum = warp_sum(sum);
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) { sh.red_f[0][warp] = sum; sh.red_c[warp] = (unsigned)first; }
@@ -325,19 +379,37 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       sum = warp_sum(lane < SR_WARPS ? sh.red_f[0][lane] : 0.f);
       first = __reduce_min_sync(0xffffffffu, (int)sh.red_c[lane % SR_WARPS]);
       if (lane < C) {
-        to_peer(sh.sum, lane, C)[rank] = sum;
-        to_peer(sh.first, lane, C)[rank] = first == 0x7fffffff ? first : c0 + first;
+        peer(sh.sum, lane, C)[rank] = sum;
+        peer(sh.first, lane, C)[rank] = first;
       }
     }
   }
-  const Weigh wt{(double)mx, 92.332482616893656877 / (double)t1, sh.pow2};  // 64 / ln 2 / T
+  const Weigh wt{(double)mx, -1.0 / (SR_STEP * (double)t1), sh.pow2};
+  auto light = [&](float x) { return !((mx - x) * c2 < SR_OCTAVES); };
+  auto weight = [&](float x) { return light(x) ? (u64)0 : wt.fixed_of(x); };
+  const double least = (double)min_p;
+  auto weight_kept = [&](float x) { return light(x) ? (u64)0 : by_m ? wt.fixed_from(x, least) : wt.fixed_of(x); };
   auto finish = [&](int token, float x) {
     s.tokens[r] = token;
     if (s.logprobs) {
       float z = 0.f;
       for (int q = 0; q < C; q++) z += sh.sum[q];
-      s.logprobs[r] = -(below(x) / t1) - logf(z);
+      s.logprobs[r] = (x - mx) / t1 - logf(z);
     }
+  };
+  // first running mass above u * mass
+  auto draw = [&](u64 mass) {
+    float u = s.u[r];
+    if (!(u >= 0.f)) u = 0.f;
+    const double at = (double)u * (double)mass;
+    const u64 goal = at < (double)mass ? (u64)at + 1 : mass;
+    return goal > mass ? mass : goal;
+  };
+  // the running mass that top-p asks for
+  auto share = [&](u64 mass) {
+    const double want = ceil((double)top_p * (double)mass);
+    const u64 goal = want >= 1.0 ? (u64)want : 1;
+    return goal > mass ? mass : goal;
   };
   if (top1 || need_bins) cluster_barrier(C);
   if (top1) {
@@ -349,53 +421,216 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
     return;
   }
 
+  int kbin = SR_BINS - 1, pbin = 0;
+  unsigned kabove = 0;
+  u64 all = 0;
+  if (need_bins) {
+    // ---- the first histogram over the cluster: thread t has bin t. Masses
+    // are a guess, checked below: sums of 2^-16 units where the bin's weights
+    // are heavy, count * weight at the middle of the bin where they are light
+    unsigned c1 = 0;
+    u64 heavy = 0;
+#pragma unroll
+    for (int q = 0; q < SR_MAX_CLUSTER; q++)
+      if (q < C) {
+        const uint2 v = peer(sh.hist, q, C)[tid];
+        c1 += v.x;
+        heavy += v.y;
+      }
+    const float mid = ex2f(-(float)tid * (span / (float)(SR_BINS - 1)) * c2);
+    const u64 m1 = mid > SR_HEAVY ? heavy << 16 : (u64)((float)c1 * mid * 4294967296.f);
+    u64 mt, m_in = m1;
+    unsigned ct, c_in = c1;
+    block_scan(sh, m_in, c_in, &mt, &ct);
+    if (tid == 0) { sh.found[0] = sh.found[1] = SR_BINS - 1; sh.found_c = ct; sh.found_m = mt; }
+    __syncthreads();
+    if (by_k && c_in - c1 < (unsigned)k && (unsigned)k <= c_in) {
+      sh.found[0] = tid;
+      sh.found_c = c_in - c1;
+      sh.found_m = m_in - m1 + (u64)((float)m1 * ((float)(k - (int)(c_in - c1)) / (float)c1));
+    }
+    __syncthreads();
+    kbin = sh.found[0];
+    kabove = sh.found_c;
+    if (by_p) {
+      const u64 goal = max((u64)1, (u64)((double)sh.found_m * (double)top_p));
+      if (m_in - m1 < goal && goal <= m_in) sh.found[1] = tid;
+      __syncthreads();
+      pbin = min(kbin, sh.found[1]);
+    }
+    // ---- the bins that can be kept, and how many elements they hold
+    int last = kbin;
+    bool covers = by_k;  // the bins hold all that can stay, whatever the guess is worth
+    if (!by_k) {
+      if (by_p) last = min(SR_BINS - 1, pbin + 1);
+      if (by_m) {  // min-p keeps max - x <= T ln(1 / min_p); two bins on the safe side
+        const float reach = -log2f(min_p) / c2 * bin_scale;
+        const int down = reach < (float)(SR_BINS - 4) ? (int)reach + 3 : SR_BINS - 1;
+        covers = down <= last;
+        last = min(last, down);
+      }
+    }
+    __syncthreads();
+    if (tid == last) sh.found_c = last == SR_BINS - 1 ? (unsigned)s.V : c_in;
+    __syncthreads();
+    if (sh.found_c <= SR_LIST) {
+      // ---- candidates in index order; with top-p alone also the row's exact mass
+      const float edge = 8388608.f + (float)last;
+      unsigned hits = 0;
+      each([&](const float (&x)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) hits += bin_bits(x[j]) <= edge && x[j] > -INFINITY;
+      });
+      if (by_p && !by_k) each([&](const float (&x)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) all += weight(x[j]);
+      });
+      const unsigned own = hits;
+      u64 all_t = all;
+      unsigned hits_t;
+      block_scan(sh, all, hits, &all_t, &hits_t);
+      unsigned at = hits - own;
+      if (own) each([&](const float (&x)[4], int i) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (bin_bits(x[j]) <= edge && x[j] > -INFINITY) {
+            sh.list.x[at] = x[j];
+            sh.list.i[at++] = first_i + i + j;
+          }
+      });
+      if (tid == 0) {
+        peer(sh.all, 0, C)[rank] = all_t;
+        peer(sh.listed, 0, C)[rank] = hits_t;
+      }
+      cluster_barrier(C);
+      if (rank == 0) {
+        int total = 0;
+        all = 0;
+        for (int q = 0; q < C; q++) {
+          const int cnt = (int)sh.listed[q];
+          Shared* o = peer(&sh, q, C);
+          for (int i = tid; i < cnt; i += SR_THREADS) {
+            const float x = o->list.x[i];
+            sh.index[total + i] = o->list.i[i];
+            sh.order[total + i] = ((u64)key_of(x) << 32) | (0xffffffffu - (unsigned)(total + i));
+          }
+          total += cnt;
+          all += sh.all[q];
+        }
+        int n2 = 32;
+        while (n2 < total) n2 <<= 1;
+        for (int i = total + tid; i < n2; i += SR_THREADS) sh.order[i] = 0;
+        sort_desc(sh.order, n2);
+        // thread t has places 2t and 2t + 1 of the order
+        const int e0 = 2 * tid;
+        u64 f[2] = {0, 0}, o2[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          if (e0 + j < total) {
+            o2[j] = sh.order[e0 + j];
+            f[j] = weight(of_key((uint32_t)(o2[j] >> 32)));
+          }
+        u64 m = f[0] + f[1], mt2;
+        unsigned none = 0, nt;
+        block_scan(sh, m, none, &mt2, &nt);
+        const u64 before[2] = {m - f[0] - f[1], m - f[1]};
+        const int nk = by_k ? min(k, total) : total;
+        if (tid == 0) { sh.found_m = by_k ? mt2 : all; }
+        __syncthreads();
+        if (by_k) {
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            if (e0 + j == nk - 1) sh.found_m = before[j] + f[j];
+          __syncthreads();
+        }
+        const u64 goal = by_p ? share(sh.found_m) : 0;
+        // a list that ends before the top-p cut (a wrong guess) decides nothing
+        const bool wrong = by_p && !covers && mt2 < goal;
+        // kept masses back in index order
+        u64 kept[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          if (e0 + j < nk && (!by_p || before[j] < goal))
+            kept[j] = by_m ? weight_kept(of_key((uint32_t)(o2[j] >> 32))) : f[j];
+        __syncthreads();  // the order has been read
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          if (e0 + j < total) sh.order[0xffffffffu - (uint32_t)o2[j]] = kept[j];
+        if (wrong && tid < C) peer(&sh, tid, C)->again = 1;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; j++) f[j] = e0 + j < total ? sh.order[e0 + j] : 0;
+        m = f[0] + f[1];
+        block_scan(sh, m, none, &mt2, &nt);
+        if (!wrong) {
+          const u64 to = draw(mt2);
+          const u64 b0 = m - f[0] - f[1], b1 = m - f[1];
+          int win = -1;
+          if (f[0] && b0 < to && to <= b1) win = e0;
+          if (f[1] && b1 < to && to <= m) win = e0 + 1;
+          if (win >= 0) {
+            const int i = sh.index[win];
+            float x = dt_load(s.logits, (int64_t)r * s.ld + i, s.dtype);
+            finish(i, x == INFINITY ? mx : x);
+          }
+        }
+      }
+      cluster_barrier(C);  // rank 0 has read its peers, and told them whether that was all
+      if (!sh.again) return;
+    }
+  }
+
+  // ---- the cut by descents
   int level = 0;  // descents so far: their buffers alternate
+  if (need_bins) {
+    sh.sub[0][tid] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+  }
   // The cut where the running count (or mass) in descending order reaches
   // `target`, known to lie in bins ba..bb, above which there are `above`;
   // among the elements inside `in`. False where it does not lie there.
   auto descend = [&](const Cut& in, bool mass, u64 target, int ba, int bb, u64 above, Cut* out) -> bool {
     // keys that the bins can hold (a hundredth of a bin and a few ulps around them)
-    const float w = span / (float)SR_BINS, slack = 0.01f * w + 1e-6f * fabsf(mx);
-    uint32_t klo = bb >= SR_BINS - 1 ? 0u : key_of(mx - (float)(bb + 1) * w - slack);
-    uint32_t khi = ba <= 0 ? key_of(mx) : key_of(fminf(mx, mx - (float)ba * w + slack));
-    if (mx == INFINITY) { klo = 0u; khi = key_of(mx); }
+    const float w = span / (float)(SR_BINS - 1), slack = 0.01f * w + 1e-6f * fabsf(mx);
+    uint32_t klo = bb >= SR_BINS - 1 ? 0u : key_of(mx - ((float)bb + 0.5f) * w - slack);
+    uint32_t khi = ba <= 0 ? key_of(mx) : key_of(fminf(mx, mx - ((float)ba - 0.5f) * w + slack));
     for (;;) {
       int shift = 0;
       while (((khi - klo) >> shift) >= (uint32_t)SR_SUB) shift++;
       uint4* sub = sh.sub[level & 1];
       auto put = [&](float x, uint32_t key, unsigned count) {
-        const int b = bin_of(below(x));
+        const int b = bin_of(x);
         if (b < ba || b > bb) return;
         unsigned* to = &sub[(key - klo) >> shift].x;
         atomicAdd(to, count);
         if (mass) {
-          const u64 f = Weigh::fixed(wt.value(x, mx));
+          const u64 f = weight(x);
           atomicAdd(to + 1, (unsigned)(f & 0x7fffu) * count);
           atomicAdd(to + 2, (unsigned)(f >> 15 & 0x7fffu) * count);
           atomicAdd(to + 3, (unsigned)(f >> 30) * count);
         }
       };
-      each([&](const float (&x)[SR_UNROLL], int) {
+      each([&](const float (&x)[4], int) {
 #pragma unroll
-        for (int j = 0; j < SR_UNROLL; j++) {
+        for (int j = 0; j < 4; j++) {
           const uint32_t key = key_of(x[j]);
           if (key >= klo && key <= khi && key > in.key) put(x[j], key, 1u);
         }
       });
       // the ties of `in`, dealt over the ranks: a digit's sum holds a slice's elements and as many ties
       if (in.ties && tid == 0 && in.key >= klo && in.key <= khi) {
-        const unsigned share = (in.ties + C - 1) / C, from = min(in.ties, share * rank);
-        put(of_key(in.key), in.key, min(in.ties, from + share) - from);
+        const unsigned part = (in.ties + C - 1) / C, from = min(in.ties, part * rank);
+        put(of_key(in.key), in.key, min(in.ties, from + part) - from);
       }
       cluster_barrier(C);
       // sub-bins in descending order: thread t has SUB - 1 - t
-      const int mine = SR_SUB - 1 - tid;
+      const int sb = SR_SUB - 1 - tid;
       unsigned c = 0;
       u64 m = 0;
 #pragma unroll
       for (int q = 0; q < SR_MAX_CLUSTER; q++)
         if (q < C) {
-          const uint4 v = peer(sub, q, C)[mine];
+          const uint4 v = peer(sub, q, C)[sb];
           c += v.x;
           m += (u64)v.y + ((u64)v.z << 15) + ((u64)v.w << 30);
         }
@@ -410,7 +645,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       __syncthreads();
       const u64 incl = above + (mass ? m : (u64)c), one = mass ? m1 : (u64)c1;
       if (c1 && incl >= target && incl - one < target) {
-        sh.found[0] = mine;
+        sh.found[0] = sb;
         sh.found_m = incl - one;
         sh.found_c = c1;
       }
@@ -421,7 +656,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       klo += (uint32_t)sel << shift;
       khi = min(khi, klo + ((1u << shift) - 1u));
       if (shift == 0) {
-        const u64 each_w = mass ? Weigh::fixed(wt.value(of_key(klo), mx)) : 1;
+        const u64 each_w = mass ? weight(of_key(klo)) : 1;
         u64 j = each_w ? (target - above + each_w - 1) / each_w : sh.found_c;
         if (j > sh.found_c) j = sh.found_c;
         out->key = klo;
@@ -432,121 +667,70 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
   };
 
   Cut cut{0u, 0u};
-  if (need_bins) {
-    // ---- the first histogram over the cluster: thread t has bin t. Masses
-    // are a guess, checked below: sums of 2^-16 units where the bin's weights
-    // are heavy, count * weight at the middle of the bin where they are light
-    unsigned c1 = 0;
-    u64 heavy = 0;
+  if (by_k) {
+    const Cut every{0u, 0u};
+    if (!descend(every, false, (u64)k, kbin, kbin, kabove, &cut))
+      descend(every, false, (u64)k, 0, SR_BINS - 1, 0, &cut);
+  }
+  if (by_p) {
+    // exact masses: of the top-k, and of what lies above the likely bins
+    const int ba = max(0, pbin - 1), bb = min(SR_BINS - 1, pbin + 1);
+    u64 over = 0;
+    all = 0;
+    each([&](const float (&x)[4], int) {
 #pragma unroll
-    for (int q = 0; q < SR_MAX_CLUSTER; q++)
-      if (q < C) {
-        const uint2 v = peer(sh.hist, q, C)[tid];
-        c1 += v.x;
-        heavy += v.y;
-      }
-    const float mid = ex2f(-((float)tid + 0.5f) * (span / (float)SR_BINS) * c2);
-    const u64 m1 = mid > SR_HEAVY ? heavy << 16 : (u64)((float)c1 * mid * 4294967296.f);
-    u64 mt, m_in = m1;
-    unsigned ct, c_in = c1;
-    block_scan(sh, m_in, c_in, &mt, &ct);
-    if (tid == 0) { sh.found[0] = SR_BINS - 1; sh.found_c = ct; sh.found_m = mt; }
-    __syncthreads();
-    if (by_k && c_in - c1 < (unsigned)k && (unsigned)k <= c_in) {
-      sh.found[0] = tid;
-      sh.found_c = c_in - c1;
-      sh.found_m = m_in - m1 + (u64)((float)m1 * ((float)(k - (int)(c_in - c1)) / (float)c1));
-    }
-    __syncthreads();
-    const int kbin = sh.found[0];
-    const unsigned kabove = sh.found_c;
-    const u64 guess = sh.found_m;
-    int pbin = 0;
-    if (by_p) {
-      __syncthreads();
-      if (tid == 0) sh.found[1] = by_k ? kbin : SR_BINS - 1;
-      __syncthreads();
-      const u64 goal = max((u64)1, (u64)((double)guess * (double)top_p));
-      if (m_in - m1 < goal && goal <= m_in) sh.found[1] = by_k ? min(kbin, tid) : tid;
-      __syncthreads();
-      pbin = sh.found[1];
-    }
-    if (by_k) {
-      const Cut every{0u, 0u};
-      if (!descend(every, false, (u64)k, kbin, kbin, kabove, &cut))
-        descend(every, false, (u64)k, 0, SR_BINS - 1, 0, &cut);
-    }
-    if (by_p) {
-      // ---- exact masses: of the top-k, and of what lies above the likely bins
-      const int ba = max(0, pbin - 1), bb = min(SR_BINS - 1, pbin + 1);  // and one bin either side
-      u64 all = 0, over = 0;
-      each([&](const float (&x)[SR_UNROLL], int) {
-        bool in[SR_UNROLL], any = false;
-#pragma unroll
-        for (int j = 0; j < SR_UNROLL; j++) any |= in[j] = key_of(x[j]) > cut.key;
-        if (!any) return;
-#pragma unroll
-        for (int j = 0; j < SR_UNROLL; j++) {
-          const u64 f = in[j] ? Weigh::fixed(wt.value(x[j], mx)) : 0;
-          all += f;
-          over += bin_of(below(x[j])) < ba ? f : 0;
-        }
-      });
-      all = warp_sum64(all);
-      over = warp_sum64(over);
-      __syncthreads();  // red_m has been read
-      if (lane == 0) { sh.red_m[warp] = all; sh.red_o[warp] = over; }
-      __syncthreads();
-      if (warp == 0) {
-        all = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
-        over = warp_sum64(lane < SR_WARPS ? sh.red_o[lane] : 0);
-        if (lane < C) {
-          to_peer(sh.all, lane, C)[rank] = all;
-          to_peer(sh.over, lane, C)[rank] = over;
-        }
-      }
-      cluster_barrier(C);
-      all = over = 0;
-      for (int q = 0; q < C; q++) {
-        all += sh.all[q];
-        over += sh.over[q];
-      }
-      if (cut.ties) {
-        const float x = of_key(cut.key);
-        const u64 f = (u64)cut.ties * Weigh::fixed(wt.value(x, mx));
+      for (int j = 0; j < 4; j++) {
+        const u64 f = key_of(x[j]) > cut.key ? weight(x[j]) : 0;
         all += f;
-        if (bin_of(below(x)) < ba) over += f;
+        over += bin_of(x[j]) < ba ? f : 0;
       }
-      const double want = ceil((double)top_p * (double)all);
-      u64 goal = want >= 1.0 ? (u64)want : 1;
-      if (goal > all) goal = all;
-      const Cut in = cut;
-      if (over >= goal || !descend(in, true, goal, ba, bb, over, &cut))
-        descend(in, true, goal, 0, SR_BINS - 1, 0, &cut);  // the guess was wrong: over the whole row
+    });
+    all = warp_sum64(all);
+    over = warp_sum64(over);
+    __syncthreads();  // red_m has been read
+    if (lane == 0) { sh.red_m[warp] = all; sh.red_o[warp] = over; }
+    __syncthreads();
+    if (warp == 0) {
+      all = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
+      over = warp_sum64(lane < SR_WARPS ? sh.red_o[lane] : 0);
+      if (lane < C) {
+        peer(sh.all, lane, C)[rank] = all;
+        peer(sh.over, lane, C)[rank] = over;
+      }
     }
+    cluster_barrier(C);
+    all = over = 0;
+    for (int q = 0; q < C; q++) {
+      all += sh.all[q];
+      over += sh.over[q];
+    }
+    if (cut.ties) {
+      const float x = of_key(cut.key);
+      const u64 f = (u64)cut.ties * weight(x);
+      all += f;
+      if (bin_of(x) < ba) over += f;
+    }
+    const u64 goal = share(all);
+    const Cut in = cut;
+    if (over >= goal || !descend(in, true, goal, ba, bb, over, &cut))
+      descend(in, true, goal, 0, SR_BINS - 1, 0, &cut);  // the guess was wrong: over the whole row
   }
 
   // ---- the kept mass of every thread's elements
-  const double least = (double)min_p;
   {
     u64 m = 0;
     unsigned e = 0;
-    each([&](const float (&x)[SR_UNROLL], int) {
-      bool in[SR_UNROLL], any = false;
+    each([&](const float (&x)[4], int) {
 #pragma unroll
-      for (int j = 0; j < SR_UNROLL; j++) {
+      for (int j = 0; j < 4; j++) {
         const uint32_t key = key_of(x[j]);
-        any |= in[j] = key > cut.key;
         e += key == cut.key;
-      }
-      if (!any) return;
-#pragma unroll
-      for (int j = 0; j < SR_UNROLL; j++) {
-        const double w = in[j] ? wt.value(x[j], mx) : 0.0;
-        if (w >= least) m += Weigh::fixed(w);
+        if (key > cut.key) m += weight_kept(x[j]);
       }
     });
-    // `part` shares the histogram's memory: that was read last before the latest barrier
+    // `part` shares the descents' memory: that was read last before a cluster barrier only
+    // where a rank waits for its peers once more
+    if (by_k || by_p) cluster_barrier(C);
     sh.part.mass[tid] = m;
     sh.part.ties[tid] = e;
     m = warp_sum64(m);
@@ -558,20 +742,15 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       m = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
       e = __reduce_add_sync(0xffffffffu, lane < SR_WARPS ? sh.red_c[lane] : 0u);
       if (lane == 0) {
-        to_peer(sh.kept, 0, C)[rank] = m;
-        to_peer(sh.ties, 0, C)[rank] = e;
+        peer(sh.kept, 0, C)[rank] = m;
+        peer(sh.ties, 0, C)[rank] = e;
       }
     }
   }
   cluster_barrier(C);
   if (rank == 0) {
     // ties at the cut: their common weight, 0 where min-p drops them
-    double tie_w = 0.0;
-    if (cut.ties) {
-      tie_w = wt.value(of_key(cut.key), mx);
-      if (!(tie_w >= least)) tie_w = 0.0;
-    }
-    const u64 tie = Weigh::fixed(tie_w);
+    const u64 tie = cut.ties ? weight_kept(of_key(cut.key)) : 0;
     u64 mass = 0;
     unsigned left = cut.ties;
     for (int q = 0; q < C; q++) {
@@ -579,11 +758,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       mass += sh.kept[q] + e * tie;
       left -= e;
     }
-    float u = s.u[r];
-    if (!(u >= 0.f)) u = 0.f;
-    const double at = (double)u * (double)mass;
-    u64 goal = at < (double)mass ? (u64)at + 1 : mass;  // first running mass above u * mass
-    if (goal > mass) goal = mass;
+    u64 goal = draw(mass);
     // cluster rank
     int q = 0;
     left = cut.ties;
@@ -594,7 +769,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       goal -= here;
       left -= e;
     }
-    const Shared* o = peer(&sh, q, C);
+    Shared* o = peer(&sh, q, C);
     // thread: running mass with the running number of ties, of which `left` stay
     const u64 m1 = o->part.mass[tid];
     const unsigned e1 = o->part.ties[tid];
@@ -614,31 +789,26 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       goal = sh.found_m;
       left = sh.found_c;
       // element: the owner's consecutive ones, 32 at a time
-      const int qc0 = min(s.V, q * slice), qn = min(s.V, qc0 + slice) - qc0;
-      const int ob = min(qn, owner * per), on = min(qn, ob + per) - ob;
+      const int qc0 = min(s.V, q * slice);
       const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + qc0) * es;
-      const int qlead = (int)((reinterpret_cast<uintptr_t>(qsrc) / es) % vec);
-      const float* qx = peer(reinterpret_cast<const float*>(dyn + ((sizeof(Shared) + 15) / 16) * 16), q, C) + qlead + ob;
-      for (int i0 = 0; i0 < on; i0 += 32) {
+      const int qi = qc0 - (int)((reinterpret_cast<uintptr_t>(qsrc) / es) % vec) + owner * per;
+      const float* qx = peer(xs, q, C) + owner * per;
+      for (int i0 = 0; i0 < per; i0 += 32) {
         const int i = i0 + lane;
-        const float x = i < on ? qx[i] : -INFINITY;
+        const float x = i < per ? qx[i] : -INFINITY;
         const uint32_t key = key_of(x);
-        const bool is_tie = i < on && key == cut.key;
+        const bool is_tie = key == cut.key;
         const unsigned ties = __ballot_sync(0xffffffffu, is_tie);
         u64 f = 0;
-        if (is_tie) {
-          f = (unsigned)__popc(ties & ((1u << lane) - 1u)) < left ? tie : 0;
-        } else if (i < on && key > cut.key) {
-          const double w = wt.value(x, mx);
-          if (w >= least) f = Weigh::fixed(w);
-        }
+        if (is_tie) f = (unsigned)__popc(ties & ((1u << lane) - 1u)) < left ? tie : 0;
+        else if (key > cut.key) f = weight_kept(x);
         u64 run = f;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const u64 v = __shfl_up_sync(0xffffffffu, run, d);
           if (lane >= d) run += v;
         }
-        if (f && run >= goal && run - f < goal) finish(qc0 + ob + i, x);
+        if (f && run >= goal && run - f < goal) finish(qi + i, x);
         const u64 here = __shfl_sync(0xffffffffu, run, 31);
         if (goal <= here) break;
         goal -= here;
@@ -671,9 +841,13 @@ int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));
   int C = SR_MAX_CLUSTER;
   if (const char* e = getenv("WG_SR_C")) C = atoi(e);
-  auto per_of = [&](int c) { return ((p.V + c * SR_THREADS - 1) / (c * SR_THREADS)) | 1; };
+  // elements a thread: 4 times an odd number that covers the slice and its padding
+  auto per_of = [&](int c) {
+    const int each = (p.V + c - 1) / c + SR_PAD;
+    return 4 * (((each + 4 * SR_THREADS - 1) / (4 * SR_THREADS)) | 1);
+  };
   const int per = per_of(C);
-  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)per * SR_THREADS * 4 + 32;
+  const size_t smem = SR_HEAD + (size_t)per * SR_THREADS * 4;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)p.R * C));
   cfg.blockDim = dim3(SR_THREADS);
