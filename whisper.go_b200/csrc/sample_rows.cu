@@ -45,14 +45,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-#ifndef SR_MINB
-#define SR_MINB 2
-#endif
 constexpr int SR_THREADS = 512;
 constexpr int SR_WARPS = SR_THREADS / 32;
 constexpr int SR_BINS = SR_THREADS;       // first histogram: one bin a thread
 constexpr int SR_SUB = SR_THREADS;        // bins of a descent: one a thread (9 bits)
 constexpr int SR_LIST = 2 * SR_THREADS;   // candidates that rank 0 can finish alone
+constexpr int SR_COUNT = 256;             // so many or fewer are ordered by counting instead of sorting
 constexpr int SR_MAX_CLUSTER = 8;
 constexpr int SR_TABLE = 256;
 constexpr float SR_SPAN = 40.f;           // logits that far below the maximum share the last bin
@@ -61,6 +59,12 @@ constexpr double SR_STEP = -0.69314718055994530942 / SR_TABLE;  // ln of a table
 constexpr float SR_OCTAVES = 46.5f;       // weights below 2^-46.5 are 0 in those units
 constexpr int SR_MAX_V = 1 << 18;
 constexpr int SR_PAD = 8;                 // a slice may start up to 7 elements into its 16 bytes
+// Bound on the relative error of a row's fp32 sum: ex2.approx 2^-22, three
+// roundings of its argument (3 * 2^-24 ln 2 of it, whose mean over the mass is
+// at most log2 V = 18: 2^-18.8), partial sums of at most 32 weights and the
+// adds that join them (2^-18.5).
+constexpr double SR_SUM_ERR = 1.0 / 131072;
+enum { SR_DONE = 0, SR_EXACT = 1, SR_WHOLE = 2 };  // what rank 0 still needs: nothing, the exact mass, the whole row
 typedef unsigned long long u64;
 
 // Unsigned keys in the order of the values (-0 with +0); 0 is no value's key.
@@ -87,7 +91,7 @@ struct Shared {
   u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
   unsigned ties[SR_MAX_CLUSTER];                   // elements equal to the cut
   unsigned listed[SR_MAX_CLUSTER];                 // candidates of the slice
-  int again;                                       // rank 0: the list did not reach the top-p cut
+  int again;                                       // from rank 0: SR_DONE, SR_EXACT or SR_WHOLE
   // read by peers after a cluster barrier
   uint2 hist[SR_BINS];                             // count, mass of the heavy ones (2^-16 units)
   union alignas(16) {
@@ -95,6 +99,7 @@ struct Shared {
     struct {
       float x[SR_LIST];    // candidates of the slice in index order
       int i[SR_LIST];
+      u64 order[SR_LIST];  // rank 0: all candidates to order, then their kept masses in index order
     } list;
     struct {
       u64 mass[SR_THREADS];       // kept mass of each thread's elements
@@ -103,8 +108,6 @@ struct Shared {
   };
   // this CTA's own
   double pow2[SR_TABLE];  // 2^(-j / 256)
-  u64 order[SR_LIST];     // rank 0: candidates to sort, then their kept masses in index order
-  int index[SR_LIST];
   u64 red_m[SR_WARPS], red_o[SR_WARPS];
   unsigned red_c[SR_WARPS];
   float red_f[2][SR_WARPS];
@@ -227,7 +230,7 @@ __device__ void sort_desc(u64* v, int n2) {
 // grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the
 // slice: `per` (4 times an odd number: no bank conflicts) consecutive elements
 // for each thread, padded with -inf
-__global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const wg_sample s, int C, int per) {
+__global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sample s, int C, int per) {
   extern __shared__ __align__(16) uint8_t dyn[];
   Shared& sh = *reinterpret_cast<Shared*>(dyn);
   float* xs = reinterpret_cast<float*>(dyn + SR_HEAD);
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
   auto bin_bits = [&](float x) { return fminf((mx - x) * bin_scale, (float)(SR_BINS - 1)) + 8388608.f; };
   auto bin_of = [&](float x) { return __float_as_int(bin_bits(x)) & (SR_BINS - 1); };
   {
-    float sum = 0.f;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
     int first = 0x7fffffff;
     if (need_bins) {
       each([&](const float (&x)[4], int) {
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
         for (int j = 0; j < 4; j++) {
           e[j] = ex2f((x[j] - mx) * c2);
           b[j] = bin_of(x[j]);
-          sum += e[j];
+          part[j] += e[j];
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -366,12 +369,12 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
       each([&](const float (&x)[4], int i) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          sum += ex2f((x[j] - mx) * c2);
+          part[j] += ex2f((x[j] - mx) * c2);
           if (top1 && x[j] == mx) first = min(first, first_i + i + j);
         }
       });
     }
-    sum = warp_sum(sum);
+    float sum = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) { sh.red_f[0][warp] = sum; sh.red_c[warp] = (unsigned)first; }
     __syncthreads();
@@ -474,109 +477,166 @@ __global__ void __launch_bounds__(SR_THREADS, SR_MINB) sample_rows_kernel(const 
     if (tid == last) sh.found_c = last == SR_BINS - 1 ? (unsigned)s.V : c_in;
     __syncthreads();
     if (sh.found_c <= SR_LIST) {
-      // ---- candidates in index order; with top-p alone also the row's exact mass
+      // ---- candidates in index order
       const float edge = 8388608.f + (float)last;
-      unsigned hits = 0;
+      auto candidate = [&](float x) { return bin_bits(x) <= edge && x > -INFINITY; };
+      unsigned hits = 0, hits_t;
+      u64 none = 0, none_t;
       each([&](const float (&x)[4], int) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) hits += bin_bits(x[j]) <= edge && x[j] > -INFINITY;
-      });
-      if (by_p && !by_k) each([&](const float (&x)[4], int) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) all += weight(x[j]);
+        for (int j = 0; j < 4; j++) hits += candidate(x[j]);
       });
       const unsigned own = hits;
-      u64 all_t = all;
-      unsigned hits_t;
-      block_scan(sh, all, hits, &all_t, &hits_t);
+      block_scan(sh, none, hits, &none_t, &hits_t);
       unsigned at = hits - own;
       if (own) each([&](const float (&x)[4], int i) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          if (bin_bits(x[j]) <= edge && x[j] > -INFINITY) {
+          if (candidate(x[j])) {
             sh.list.x[at] = x[j];
             sh.list.i[at++] = first_i + i + j;
           }
       });
-      if (tid == 0) {
-        peer(sh.all, 0, C)[rank] = all_t;
-        peer(sh.listed, 0, C)[rank] = hits_t;
-      }
+      if (tid == 0) peer(sh.listed, 0, C)[rank] = hits_t;
       cluster_barrier(C);
+      // ---- rank 0 orders them: a thread gets up to two, with their place in
+      // the order and the exact mass before them
+      u64 f[2] = {0, 0}, o[2] = {0, 0}, before[2] = {0, 0}, inside = 0;
+      int place[2] = {SR_LIST, SR_LIST}, total = 0;
       if (rank == 0) {
-        int total = 0;
-        all = 0;
         for (int q = 0; q < C; q++) {
           const int cnt = (int)sh.listed[q];
-          Shared* o = peer(&sh, q, C);
-          for (int i = tid; i < cnt; i += SR_THREADS) {
-            const float x = o->list.x[i];
-            sh.index[total + i] = o->list.i[i];
-            sh.order[total + i] = ((u64)key_of(x) << 32) | (0xffffffffu - (unsigned)(total + i));
-          }
+          const float* from = peer(sh.list.x, q, C);
+          for (int i = tid; i < cnt; i += SR_THREADS)
+            sh.list.order[total + i] = ((u64)key_of(from[i]) << 32) | (0xffffffffu - (unsigned)(total + i));
           total += cnt;
-          all += sh.all[q];
         }
-        int n2 = 32;
-        while (n2 < total) n2 <<= 1;
-        for (int i = total + tid; i < n2; i += SR_THREADS) sh.order[i] = 0;
-        sort_desc(sh.order, n2);
-        // thread t has places 2t and 2t + 1 of the order
-        const int e0 = 2 * tid;
-        u64 f[2] = {0, 0}, o2[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          if (e0 + j < total) {
-            o2[j] = sh.order[e0 + j];
-            f[j] = weight(of_key((uint32_t)(o2[j] >> 32)));
+        if (total <= SR_COUNT) {
+          __syncthreads();
+          ulonglong2* both = reinterpret_cast<ulonglong2*>(sh.list.order);  // (order, mass)
+          u64 v = 0, fv = 0;
+          if (tid < total) {
+            v = sh.list.order[tid];
+            fv = weight(of_key((uint32_t)(v >> 32)));
           }
-        u64 m = f[0] + f[1], mt2;
-        unsigned none = 0, nt;
-        block_scan(sh, m, none, &mt2, &nt);
-        const u64 before[2] = {m - f[0] - f[1], m - f[1]};
-        const int nk = by_k ? min(k, total) : total;
-        if (tid == 0) { sh.found_m = by_k ? mt2 : all; }
-        __syncthreads();
-        if (by_k) {
+          __syncthreads();
+          if (tid < total) both[tid] = make_ulonglong2(v, fv);
+          __syncthreads();
+          if (tid < total) {
+            int ahead = 0;
+            u64 mass = 0;
+#pragma unroll 4
+            for (int j = 0; j < total; j++) {
+              const ulonglong2 w = both[j];
+              if (w.x > v) { ahead++; mass += w.y; }
+            }
+            o[0] = v;
+            f[0] = fv;
+            before[0] = mass;
+            place[0] = ahead;
+          }
+        } else {
+          int n2 = 2 * SR_COUNT;
+          while (n2 < total) n2 <<= 1;
+          for (int i = total + tid; i < n2; i += SR_THREADS) sh.list.order[i] = 0;
+          sort_desc(sh.list.order, n2);
 #pragma unroll
           for (int j = 0; j < 2; j++)
-            if (e0 + j == nk - 1) sh.found_m = before[j] + f[j];
-          __syncthreads();
-        }
-        const u64 goal = by_p ? share(sh.found_m) : 0;
-        // a list that ends before the top-p cut (a wrong guess) decides nothing
-        const bool wrong = by_p && !covers && mt2 < goal;
-        // kept masses back in index order
-        u64 kept[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          if (e0 + j < nk && (!by_p || before[j] < goal))
-            kept[j] = by_m ? weight_kept(of_key((uint32_t)(o2[j] >> 32))) : f[j];
-        __syncthreads();  // the order has been read
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          if (e0 + j < total) sh.order[0xffffffffu - (uint32_t)o2[j]] = kept[j];
-        if (wrong && tid < C) peer(&sh, tid, C)->again = 1;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 2; j++) f[j] = e0 + j < total ? sh.order[e0 + j] : 0;
-        m = f[0] + f[1];
-        block_scan(sh, m, none, &mt2, &nt);
-        if (!wrong) {
-          const u64 to = draw(mt2);
-          const u64 b0 = m - f[0] - f[1], b1 = m - f[1];
-          int win = -1;
-          if (f[0] && b0 < to && to <= b1) win = e0;
-          if (f[1] && b1 < to && to <= m) win = e0 + 1;
-          if (win >= 0) {
-            const int i = sh.index[win];
-            float x = dt_load(s.logits, (int64_t)r * s.ld + i, s.dtype);
-            finish(i, x == INFINITY ? mx : x);
-          }
+            if (2 * tid + j < total) {
+              place[j] = 2 * tid + j;
+              o[j] = sh.list.order[2 * tid + j];
+              f[j] = weight(of_key((uint32_t)(o[j] >> 32)));
+            }
+          u64 m = f[0] + f[1];
+          unsigned zero = 0, zero_t;
+          block_scan(sh, m, zero, &inside, &zero_t);
+          before[0] = m - f[0] - f[1];
+          before[1] = m - f[1];
         }
       }
-      cluster_barrier(C);  // rank 0 has read its peers, and told them whether that was all
-      if (!sh.again) return;
+      const int nk = by_k ? min(k, total) : total;
+      for (int pass = 0;; pass++) {  // at most two: the second with the row's exact mass
+        if (rank == 0) {
+          u64 lo = 0, hi = 0;  // the running mass that top-p asks for, as far as it is known
+          if (by_p) {
+            if (by_k) {
+              if (tid == 0) sh.found_m = 0;
+              __syncthreads();
+#pragma unroll
+              for (int j = 0; j < 2; j++)
+                if (place[j] == nk - 1) sh.found_m = before[j] + f[j];
+              __syncthreads();
+              lo = hi = share(sh.found_m);
+            } else if (pass) {
+              all = 0;
+              for (int q = 0; q < C; q++) all += sh.all[q];
+              lo = hi = share(all);
+            } else {
+              double z = 0.0;
+              for (int q = 0; q < C; q++) z += (double)sh.sum[q];
+              lo = share((u64)(z * (1.0 - SR_SUM_ERR) * 35184372088832.0));  // 2^45
+              hi = share((u64)(z * (1.0 + SR_SUM_ERR) * 35184372088832.0) + 1);
+            }
+          }
+          // kept masses in index order; two ends of the top-p mass must keep the same ones,
+          // and a list that ends before them decides nothing
+          bool unsure = false, past = false, ended = false;
+          u64 kept[2] = {0, 0};
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            if (place[j] < nk && (!by_p || before[j] < lo)) kept[j] = by_m ? weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
+            unsure |= by_p && place[j] < nk && before[j] >= lo && before[j] < hi;
+            if (by_p && !covers && place[j] == total - 1) {
+              ended = before[j] + f[j] < hi;
+              past = before[j] + f[j] < lo;
+            }
+          }
+          const int doubt = __syncthreads_or(unsure || ended), whole = __syncthreads_or(past);
+          const int todo = whole ? SR_WHOLE : doubt ? SR_EXACT : SR_DONE;
+          if (todo == SR_DONE) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+              if (place[j] < total) sh.list.order[0xffffffffu - (uint32_t)o[j]] = kept[j];
+            __syncthreads();
+            const u64 f0 = 2 * tid < total ? sh.list.order[2 * tid] : 0;
+            const u64 f1 = 2 * tid + 1 < total ? sh.list.order[2 * tid + 1] : 0;
+            u64 m = f0 + f1, mass;
+            unsigned zero = 0, zero_t;
+            block_scan(sh, m, zero, &mass, &zero_t);
+            const u64 to = draw(mass), b0 = m - f0 - f1, b1 = m - f1;
+            int win = -1;
+            if (f0 && b0 < to && to <= b1) win = 2 * tid;
+            if (f1 && b1 < to && to <= m) win = 2 * tid + 1;
+            if (win >= 0) {
+              int q = 0;
+              while (win >= (int)sh.listed[q]) win -= (int)sh.listed[q++];
+              finish(peer(sh.list.i, q, C)[win], peer(sh.list.x, q, C)[win]);
+            }
+          } else if (tid < C) {
+            peer(&sh, tid, C)->again = todo;
+          }
+        }
+        cluster_barrier(C);  // rank 0 has read its peers, and told them what it needs
+        const int todo = sh.again;
+        if (todo == SR_DONE) return;
+        if (todo == SR_WHOLE) break;
+        // the exact mass of the row
+        all = 0;
+        each([&](const float (&x)[4], int) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) all += weight(x[j]);
+        });
+        all = warp_sum64(all);
+        __syncthreads();  // `again` and red_m have been read
+        if (lane == 0) sh.red_m[warp] = all;
+        if (tid == 0) sh.again = SR_DONE;
+        __syncthreads();
+        if (warp == 0) {
+          all = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
+          if (lane == 0) peer(sh.all, 0, C)[rank] = all;
+        }
+        cluster_barrier(C);
+      }
     }
   }
 
@@ -839,15 +899,22 @@ int set_attributes(int device) {
 
 int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));
-  int C = SR_MAX_CLUSTER;
-  if (const char* e = getenv("WG_SR_C")) C = atoi(e);
+  // CTAs a row: as many as the SMs take in one round (two CTAs each from 4 a
+  // row on), at least two (a row of 51866 fp32 fits no SM), none with less
+  // than 2048 elements (their exchanges cost more than such slices). Measured
+  // at 51866 fp32: one row 25 / 21 / 17 us with 2 / 4 / 8 CTAs, 320 rows 99 /
+  // 106 / 187; 48 rows of f16 34 / 29 / 38.
+  int C = p.R * 8 <= 148 ? 8 : p.R * 4 <= 296 ? 4 : 2;
+  while (C > 1 && p.V <= 2048 * (C / 2)) C /= 2;
   // elements a thread: 4 times an odd number that covers the slice and its padding
   auto per_of = [&](int c) {
     const int each = (p.V + c - 1) / c + SR_PAD;
     return 4 * (((each + 4 * SR_THREADS - 1) / (4 * SR_THREADS)) | 1);
   };
+  auto smem_of = [&](int c) { return SR_HEAD + (size_t)per_of(c) * SR_THREADS * 4; };
+  while (C < SR_MAX_CLUSTER && smem_of(C) > SR_SMEM_MAX) C *= 2;
   const int per = per_of(C);
-  const size_t smem = SR_HEAD + (size_t)per * SR_THREADS * 4;
+  const size_t smem = smem_of(C);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)p.R * C));
   cfg.blockDim = dim3(SR_THREADS);
