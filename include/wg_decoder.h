@@ -347,7 +347,7 @@ enum { WG_DT_F32 = 0, WG_DT_F16 = 1, WG_DT_BF16 = 30 }; /* GGUF ids of these typ
 
 /* A paged cache of 8-bit keys and values. Value = code * scale:
  *   codes  int8 [num_pages][2 (K, V)][n_kv_head][page][head_dim], 16-byte aligned
- *   scales fp32 [num_pages][2][n_kv_head], one per page, K or V, and head
+ *   scales fp32 [num_pages][2][n_kv_head], one per page, K or V, and head, >= 0
  * page: tokens per page, a power of two from 16 to 128; head_dim 64 or 128;
  * num_pages * page < 2^31. The slot of a token is its page * `page` + its
  * place in the page. Fresh memory needs no initialisation. */

@@ -33,7 +33,19 @@ namespace {
 
 constexpr int AW = 4;        // warps per CTA
 constexpr int CH = 32;       // tokens per chunk
-constexpr int STAGES = 4;
+#ifndef AT_ST
+#define AT_ST 4
+#endif
+#ifndef AT_MB
+#define AT_MB 1
+#endif
+#ifndef AT_MB2
+#define AT_MB2 1
+#endif
+#ifndef AT_SPLIT
+#define AT_SPLIT 6
+#endif
+constexpr int STAGES = AT_ST;
 constexpr int MAX_SPLIT = 16;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -80,11 +92,22 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d = a * b + c for a C that is the same for a row's columns (c0: row g, c1: row g + 8)
+__device__ __forceinline__ void mma16816_c(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                           float c1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 // Bytes (already offset by 128: code + 128) LO / HI of w as an f16 pair:
-// 0x6400 | u is 1024 + u, exact; minus 1152 gives the code.
+// 0x6400 | u is 1024 + u, exact: code + 1152.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes_up(uint32_t w) { return __byte_perm(w, 0x64646464u, SEL); }
+// The codes themselves.
 template <int SEL>
 __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-  const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
+  const uint32_t h = codes_up<SEL>(w);
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -102,11 +125,6 @@ __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
-
 // Shared-memory byte offset of the 16-byte piece `part` of token tok in a
 // [32][D] block. Swizzled so that a quarter-warp's 16-byte reads of K (two
 // neighbouring tokens x 4 pieces) and a half-warp's 8-byte (D 64) or
@@ -129,7 +147,7 @@ __device__ __forceinline__ uint32_t v_off(int tok, int part) {
 // HALF: at most 8 rows are live, so the MMA's rows 8..15 are not processed
 // past the products. SMALL: 16-token pages (two pages, and scales, per chunk).
 template <int D, bool HALF, bool SMALL>
-__global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) {
+__global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : AT_MB2) decode_attn_kernel(const AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
@@ -165,29 +183,33 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
     const int col = (chunk * CH + half * 16) >> p.shift;
     return chunk < c_end && col < pages ? __ldg(table + col) : -1;
   };
-  auto issue = [&](int chunk, int stage, int id0, int id1) {
-    const uint32_t base = ring_u + stage * stage_bytes<D>();
-    const bool ok0 = (unsigned)id0 < (unsigned)p.num_pages, ok1 = (unsigned)id1 < (unsigned)p.num_pages;
-    const int in_page = (chunk * CH) & (page - 1);  // 0 with 16-token pages
-    const int64_t b0 = ((int64_t)(ok0 ? id0 : 0) * 2 * p.H + h), b1 = ((int64_t)(ok1 ? id1 : 0) * 2 * p.H + h);
-    const int8_t* k0 = p.codes + (b0 * page + in_page) * D;
-    const int8_t* k1 = SMALL ? p.codes + b1 * page * D : k0 + 16 * D;
-    const int64_t kv_step = (int64_t)p.H * page * D;
+  // a lane's place in the first 512 bytes of a chunk's K and V, and in V's next
+  // 512 (piece i is 512 i bytes further in memory; in the ring the swizzles
+  // repeat every 512 bytes, V's of 128-wide heads every 1024)
+  constexpr int PIECES = CH * D / 512;
+  const uint32_t lane_k = k_off<D>(lane / PARTS, lane % PARTS), lane_v = CH * D + v_off<D>(lane / PARTS, lane % PARTS);
+  const uint32_t lane_v1 = CH * D + v_off<D>(lane / PARTS + 32 / PARTS, lane % PARTS) - 512;
+  const int64_t block = (int64_t)page * D, id_step = 2 * p.H * block, kv_step = p.H * block;
+  const int8_t* lane_src = p.codes + h * block + lane * 16;
+  const float* lane_scale = p.scales + h + (lane >> 1) * p.H;  // lanes 0..3: sk[0], sk[1], sv[0], sv[1]
+  auto issue = [&](int chunk, uint32_t base, uint8_t* at, int id0, int id1) {
+    const bool ok0 = (unsigned)id0 < (unsigned)p.num_pages, ok1 = SMALL ? (unsigned)id1 < (unsigned)p.num_pages : ok0;
+    const int64_t page0 = (ok0 ? id0 : 0) * id_step, page1 = SMALL ? (ok1 ? id1 : 0) * id_step : 0;
+    const int8_t* s0 = lane_src + page0 + (SMALL ? 0 : ((chunk * CH) & (page - 1)) * D);
+    const int8_t* s1 = SMALL ? lane_src + page1 - 16 * D : s0;  // tokens 16..31 of 16-token pages
 #pragma unroll
-    for (int i = 0; i < PARTS; i++) {
-      const int idx = i * 32 + lane, tok = idx / PARTS, part = idx % PARTS;
-      const bool second = tok >= 16;
-      const int8_t* src = (second ? k1 + (tok - 16) * D : k0 + tok * D) + part * 16;
-      const bool on = second && SMALL ? ok1 : ok0;
-      cp16(base + k_off<D>(tok, part), src, on);
-      cp16(base + CH * D + v_off<D>(tok, part), src + kv_step, on);
+    for (int i = 0; i < PIECES; i++) {
+      const bool second = SMALL && i >= PIECES / 2;
+      const int8_t* src = (second ? s1 : s0) + i * 512;
+      cp16(base + lane_k + i * 512, src, second ? ok1 : ok0);
+      cp16(base + ((i & 1) ? lane_v1 : lane_v) + i * 512, src + kv_step, second ? ok1 : ok0);
     }
-    if (lane < 4) {  // sk[0], sk[1], sv[0], sv[1]
-      const bool second = (lane & 1) != 0;
-      cp4(base + 2 * CH * D + lane * 4, p.scales + (second && SMALL ? b1 : b0) + (lane >> 1) * p.H,
-          second && SMALL ? ok1 : ok0);
+    if (lane < 4) {
+      const bool second = SMALL && (lane & 1);
+      cp4(base + 2 * CH * D + lane * 4, lane_scale + (int64_t)(second ? (ok1 ? id1 : 0) : (ok0 ? id0 : 0)) * 2 * p.H,
+          second ? ok1 : ok0);
     } else if (lane < 6) {
-      reinterpret_cast<int*>(ring + stage * stage_bytes<D>() + 2 * CH * D)[lane] = (lane == 4 || !SMALL) ? ok0 : ok1;
+      reinterpret_cast<int*>(at + 2 * CH * D)[lane] = lane == 4 ? ok0 : ok1;
     }
   };
   int id0[STAGES], id1[STAGES];
@@ -198,7 +220,8 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
   }
 #pragma unroll
   for (int s = 0; s < STAGES; s++) {
-    if (c + s * AW < c_end) issue(c + s * AW, s, id0[s], id1[s]);
+    if (c + s * AW < c_end)
+      issue(c + s * AW, ring_u + s * stage_bytes<D>(), ring + s * stage_bytes<D>(), id0[s], id1[s]);
     cp_commit();
   }
   int nid0 = page_id(c + STAGES * AW, 0), nid1 = SMALL ? page_id(c + STAGES * AW, 1) : nid0;
@@ -211,6 +234,7 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
   float mul_a, mul_b;
   {
     float e[2];
+    const float sign = p.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       const int row = g + half * 8;
@@ -225,12 +249,12 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
         mx = fmaxf(mx, fabsf(x[i]));
       }
       mx = quad_max(mx);
-      float up = 1.f;
+      float up = sign;
       e[half] = 1.f;
       if (p.qdt != WG_DT_F16 && mx > 0.f && mx <= 3.402823466e38f) {
         // 2^-k and 2^k with 2^k <= mx < 2^(k+1)
         const int k = min(max((int)(__float_as_uint(mx) >> 23) - 127, -120), 120);
-        up = __uint_as_float((uint32_t)(127 - k) << 23);
+        up = sign * __uint_as_float((uint32_t)(127 - k) << 23);
         e[half] = __uint_as_float((uint32_t)(127 + k) << 23);
       }
 #pragma unroll
@@ -240,8 +264,8 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
         qa_f[j][2 + half] = pack_f16(x[o + 2] * up, x[o + 3] * up);
       }
     }
-    mul_a = e[0] * p.scale * LOG2E;  // scores in units of log 2
-    mul_b = e[1] * p.scale * LOG2E;
+    mul_a = e[0] * fabsf(p.scale) * LOG2E;  // scores in units of log 2
+    mul_b = e[1] * fabsf(p.scale) * LOG2E;
   }
 
   float o_acc[NT][4];
@@ -252,29 +276,35 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
   for (int stage = 0; c < c_end; c += AW, stage = stage + 1 == STAGES ? 0 : stage + 1) {
     cp_wait<STAGES - 1>();
     __syncwarp();
-    const uint8_t* st = ring + stage * stage_bytes<D>();
+    uint8_t* st = ring + stage * stage_bytes<D>();
     const float* sc = reinterpret_cast<const float*>(st + 2 * CH * D);
     const float sk0 = sc[0], sk1 = sc[1], sv0 = sc[2], sv1 = sc[3];
     const bool ok0 = reinterpret_cast<const int*>(sc)[4] != 0, ok1 = reinterpret_cast<const int*>(sc)[5] != 0;
 
-    // ---- scores of 4 n-tiles of 8 tokens
+    // ---- q . codes of 4 n-tiles of 8 tokens, in units of the page's step
+    // (both pages' steps brought to one where they differ)
     float s[4][4];
 #pragma unroll
     for (int n = 0; n < 4; n++) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
       for (int b = 0; b < D / 64; b++) {
         const uint4 w4 = *reinterpret_cast<const uint4*>(st + k_off<D>(n * 8 + g, b * 4 + t));
         const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          mma16816(s[n], qa_f[b * 4 + j], codes_f16<0x4140>(w[j]), codes_f16<0x4342>(w[j]));
+        for (int j = 0; j < 4; j++) {
+          if (b == 0 && j == 0)
+            mma16816_c(s[n], qa_f[0], codes_f16<0x4140>(w[0]), codes_f16<0x4342>(w[0]), 0.f, 0.f);
+          else
+            mma16816(s[n], qa_f[b * 4 + j], codes_f16<0x4140>(w[j]), codes_f16<0x4342>(w[j]));
+        }
       }
-      const float sk = n < 2 ? sk0 : sk1;
-      s[n][0] *= sk * mul_a;
-      s[n][1] *= sk * mul_a;
-      s[n][2] *= sk * mul_b;
-      s[n][3] *= sk * mul_b;
+      if (SMALL && n >= 2) {
+#pragma unroll
+        for (int x = 0; x < (HALF ? 2 : 4); x++) s[n][x] *= sk1;
+      } else if (SMALL) {
+#pragma unroll
+        for (int x = 0; x < (HALF ? 2 : 4); x++) s[n][x] *= sk0;
+      }
     }
     if ((c + 1) * CH > lo_lim || !ok0 || !ok1) {
 #pragma unroll
@@ -287,16 +317,24 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
         if (!ok || j + 1 >= lim_b) s[n][3] = -INFINITY;
       }
     }
-    // ---- running maximum and sum
-    float x_a = m_a, x_b = m_b;
+    // ---- running maximum; scores in units of log 2 are s * step (the sign of
+    // the scale is in q; a step of 0, an all-zero page, is kept above 0 so that
+    // masked scores stay -inf)
+    const float step_a = fmaxf(SMALL ? mul_a : sk0 * mul_a, 1e-37f), step_b = fmaxf(SMALL ? mul_b : sk0 * mul_b, 1e-37f);
+    float x_a = fmaxf(s[0][0], s[0][1]), x_b = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
+    for (int n = 1; n < 4; n++) {
       x_a = fmaxf(x_a, fmaxf(s[n][0], s[n][1]));
       if (!HALF) x_b = fmaxf(x_b, fmaxf(s[n][2], s[n][3]));
     }
+    // an empty chunk stays -inf (0 * -inf would not)
     x_a = quad_max(x_a);
-    if (!HALF) x_b = quad_max(x_b);
-    const float ref_a = x_a == -INFINITY ? 0.f : x_a, ref_b = x_b == -INFINITY ? 0.f : x_b;
+    x_a = x_a == -INFINITY ? m_a : fmaxf(m_a, x_a * step_a);
+    if (!HALF) {
+      x_b = quad_max(x_b);
+      x_b = x_b == -INFINITY ? m_b : fmaxf(m_b, x_b * step_b);
+    }
+    const float ref_a = x_a == -INFINITY ? 0.f : x_a, ref_b = HALF || x_b == -INFINITY ? 0.f : x_b;
     const bool moved = HALF ? x_a != m_a : (x_a != m_a || x_b != m_b);
     if (__any_sync(0xffffffffu, moved)) {
       const float al_a = ex2(m_a - ref_a), al_b = HALF ? 1.f : ex2(m_b - ref_b);
@@ -312,23 +350,26 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
         }
       }
       m_a = x_a;
-      m_b = x_b;
+      m_b = HALF ? m_b : x_b;
     }
-    // weights rounded to f16 for the MMA (2^-12 of a weight that is at most 1); the sum keeps fp32
+    // weights rounded to f16 for the MMA (2^-12 of a weight that is at most 1)
     uint32_t pf[2][4];
 #pragma unroll
     for (int n = 0; n < 4; n++) {
-      const float p0 = ex2(s[n][0] - ref_a), p1 = ex2(s[n][1] - ref_a);
-      l_a += p0 + p1;
-      pf[n >> 1][(n & 1) * 2] = pack_f16(p0, p1);
-      if (!HALF) {
-        const float p2 = ex2(s[n][2] - ref_b), p3 = ex2(s[n][3] - ref_b);
-        l_b += p2 + p3;
-        pf[n >> 1][(n & 1) * 2 + 1] = pack_f16(p2, p3);
-      } else {
-        pf[n >> 1][(n & 1) * 2 + 1] = 0u;
-      }
+      pf[n >> 1][(n & 1) * 2] = pack_f16(ex2(fmaf(s[n][0], step_a, -ref_a)), ex2(fmaf(s[n][1], step_a, -ref_a)));
+      pf[n >> 1][(n & 1) * 2 + 1] =
+          HALF ? 0u : pack_f16(ex2(fmaf(s[n][2], step_b, -ref_b)), ex2(fmaf(s[n][3], step_b, -ref_b)));
     }
+    // their row sums, by the same MMA over a matrix of ones: they go into l (so
+    // that the rounded weights sum to one) and take the 1152 out of the codes
+    float rs[2][4];
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++) {
+      if (hf == 1 && !SMALL) mma16816(rs[0], pf[1], 0x3c003c00u, 0x3c003c00u);
+      else mma16816_c(rs[hf], pf[hf], 0x3c003c00u, 0x3c003c00u, 0.f, 0.f);
+    }
+    l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
+    if (!HALF) l_b += SMALL ? rs[0][2] + rs[1][2] : rs[0][2];
     // ---- P.V: n-tile j of lane g is dim g * (D/8) + j; tokens 2t, 2t+1, 2t+8, 2t+9 of each 16
     const uint8_t* vs = st + CH * D;
     constexpr int VW = D / 32;  // words of a lane's dims per token
@@ -366,11 +407,10 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
         float acc[2][4];
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
-          float(&a)[4] = acc[SMALL ? hf : 0];
-          if (SMALL || hf == 0) a[0] = a[1] = a[2] = a[3] = 0.f;
-          const uint32_t b0 = (dd & 1) ? codes_f16<0x4342>(z[hf][dd >> 1]) : codes_f16<0x4140>(z[hf][dd >> 1]);
-          const uint32_t b1 = (dd & 1) ? codes_f16<0x4342>(z[hf][2 + (dd >> 1)]) : codes_f16<0x4140>(z[hf][2 + (dd >> 1)]);
-          mma16816(a, pf[hf], b0, b1);
+          const uint32_t b0 = (dd & 1) ? codes_up<0x4342>(z[hf][dd >> 1]) : codes_up<0x4140>(z[hf][dd >> 1]);
+          const uint32_t b1 = (dd & 1) ? codes_up<0x4342>(z[hf][2 + (dd >> 1)]) : codes_up<0x4140>(z[hf][2 + (dd >> 1)]);
+          if (SMALL || hf == 0) mma16816_c(acc[hf], pf[hf], b0, b1, -1152.f * rs[hf][0], HALF ? 0.f : -1152.f * rs[hf][2]);
+          else mma16816(acc[0], pf[1], b0, b1);
         }
 #pragma unroll
         for (int x = 0; x < (HALF ? 2 : 4); x++) {
@@ -380,7 +420,7 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
       }
     }
     __syncwarp();  // every lane has read the stage
-    if (c + STAGES * AW < c_end) issue(c + STAGES * AW, stage, nid0, nid1);
+    if (c + STAGES * AW < c_end) issue(c + STAGES * AW, ring_u + stage * stage_bytes<D>(), st, nid0, nid1);
     cp_commit();
     nid0 = page_id(c + (STAGES + 1) * AW, 0);
     nid1 = SMALL ? page_id(c + (STAGES + 1) * AW, 1) : nid0;
@@ -388,8 +428,6 @@ __global__ void __launch_bounds__(AW * 32) decode_attn_kernel(const AttnArgs p) 
   cp_wait<0>();
 
   // ---- join the warps: (m, l, O) of each in its own ring's memory
-  l_a = quad_sum(l_a);
-  l_b = quad_sum(l_b);
   __syncwarp();
   float* wo = reinterpret_cast<float*>(ring);  // [16][D] O, then [16] m, [16] l
   {
@@ -524,7 +562,7 @@ int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cuda
   // CTAs per tile: enough for two rounds of the SMs' resident CTAs, no less
   // than two chunks for each warp, and no CTA with more than 64 chunks
   // (2048 tokens), so that one long request among short ones is spread too
-  int64_t s = (148 * 6 + units - 1) / units;
+  int64_t s = (148 * AT_SPLIT + units - 1) / units;
   if (s > chunks / (2 * AW)) s = chunks / (2 * AW);
   if (s < (chunks + 63) / 64) s = (chunks + 63) / 64;
   a.splits = (int)(s < 1 ? 1 : s > MAX_SPLIT ? MAX_SPLIT : s);
