@@ -34,13 +34,10 @@ namespace {
 constexpr int AW = 4;        // warps per CTA
 constexpr int CH = 32;       // tokens per chunk
 #ifndef AT_ST
-#define AT_ST 4
+#define AT_ST 2
 #endif
 #ifndef AT_MB
-#define AT_MB 1
-#endif
-#ifndef AT_MB2
-#define AT_MB2 1
+#define AT_MB 5
 #endif
 #ifndef AT_SPLIT
 #define AT_SPLIT 6
@@ -67,6 +64,7 @@ struct AttnArgs {
   void* out;
   int64_t ldo;
   int odt;
+  bool q_vec, o_vec;  // rows that start on 16 bytes
 };
 
 template <int D>
@@ -100,6 +98,25 @@ __device__ __forceinline__ void mma16816_c(float (&d)[4], const uint32_t (&a)[4]
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
+// d = a * b + c for a C that is the same for a column's rows (c0: column 2t, c1: column 2t + 1)
+__device__ __forceinline__ void mma16816_cols(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  const uint32_t a[4] = {a0, a1, a2, a3};
+  mma16816(c, a, b0, b1);
+}
+// Transposes an 8 x 8 matrix of 16-bit values held as row g, columns 2t and 2t + 1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // Bytes (already offset by 128: code + 128) LO / HI of w as an f16 pair:
 // 0x6400 | u is 1024 + u, exact: code + 1152.
 template <int SEL>
@@ -115,11 +132,20 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+__device__ __forceinline__ float sum_f16(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f.x + f.y;
+}
 // 2^x, x <= 0 (hardware approximation, 2^-22 relative; 0 for -inf)
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float column_max(float v) {  // over the lanes of one t
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
@@ -144,10 +170,33 @@ __device__ __forceinline__ uint32_t v_off(int tok, int part) {
   return tok * 128 + ((part ^ (((tok >> 1) & 3) << 1)) << 4);
 }
 
+// A lane's share of 32 tokens of V: D/8 dims (from g) of tokens 2t, 2t + 1,
+// 2t + 8 and 2t + 9 of either 16, offset by 128.
+template <int D>
+__device__ __forceinline__ void load_v(const uint8_t* vs, int g, int t, uint32_t (&w)[2][4][D / 32]) {
+#pragma unroll
+  for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int tok = hf * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+      if constexpr (D == 64) {
+        const uint2 v = *reinterpret_cast<const uint2*>(vs + v_off<D>(tok, g >> 1) + (g & 1) * 8);
+        w[hf][i][0] = v.x ^ 0x80808080u;
+        w[hf][i][1] = v.y ^ 0x80808080u;
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(vs + v_off<D>(tok, g));
+        w[hf][i][0] = v.x ^ 0x80808080u;
+        w[hf][i][1] = v.y ^ 0x80808080u;
+        w[hf][i][2] = v.z ^ 0x80808080u;
+        w[hf][i][3] = v.w ^ 0x80808080u;
+      }
+    }
+}
+
 // HALF: at most 8 rows are live, so the MMA's rows 8..15 are not processed
 // past the products. SMALL: 16-token pages (two pages, and scales, per chunk).
 template <int D, bool HALF, bool SMALL>
-__global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : AT_MB2) decode_attn_kernel(const AttnArgs p) {
+__global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : 2) decode_attn_kernel(const AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
@@ -231,23 +280,36 @@ __global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : AT_MB2) decode_attn
   // are scaled by a power of two so that they fit f16: bf16 stays exact down
   // to 2^-23 of the row's largest value, fp32 is rounded to f16's 11 bits.
   uint32_t qa_f[D / 16][4];
-  float mul_a, mul_b;
+  float mul_a, mul_b, q_sum = 0.f;
   {
     float e[2];
     const float sign = p.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
+    for (int half = 0; half < (HALF ? 1 : 2); half++) {
       const int row = g + half * 8;
-      const bool live = row < rows && !(HALF && half);
+      const bool live = row < rows;
       const int qi = (row0 + row) / p.G, hg = (row0 + row) % p.G;
       const int64_t base = (int64_t)(q0 + qi) * p.ldq + ((int64_t)h * p.G + hg) * D + 16 * t;
       float x[D / 4];
       float mx = 0.f;
+      if (live && p.q_vec) {  // 16-bit types, 16-byte rows
 #pragma unroll
-      for (int i = 0; i < D / 4; i++) {
-        x[i] = live ? dt_load(p.q, base + (i / 16) * 64 + (i % 16), p.qdt) : 0.f;
-        mx = fmaxf(mx, fabsf(x[i]));
+        for (int i = 0; i < D / 4; i += 8) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + base + (i / 16) * 64 + i % 16));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float2 f = dt_unpack2(p.qdt, w[j]);
+            x[i + 2 * j] = f.x;
+            x[i + 2 * j + 1] = f.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 4; i++) x[i] = live ? dt_load(p.q, base + (i / 16) * 64 + (i % 16), p.qdt) : 0.f;
       }
+#pragma unroll
+      for (int i = 0; i < D / 4; i++) mx = fmaxf(mx, fabsf(x[i]));
       mx = quad_max(mx);
       float up = sign;
       e[half] = 1.f;
@@ -262,16 +324,31 @@ __global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : AT_MB2) decode_attn
         const int o = (j / 4) * 16 + (j % 4) * 4;
         qa_f[j][half] = pack_f16(x[o] * up, x[o + 1] * up);
         qa_f[j][2 + half] = pack_f16(x[o + 2] * up, x[o + 3] * up);
+        if (HALF) q_sum += sum_f16(qa_f[j][0]) + sum_f16(qa_f[j][2]);  // of the row's f16 values
       }
     }
     mul_a = e[0] * fabsf(p.scale) * LOG2E;  // scores in units of log 2
-    mul_b = e[1] * fabsf(p.scale) * LOG2E;
+    mul_b = HALF ? 0.f : e[1] * fabsf(p.scale) * LOG2E;
   }
 
-  float o_acc[NT][4];
+  constexpr int OT = HALF ? D / 16 : NT;  // accumulator tiles
+  float o_acc[OT][4];
 #pragma unroll
-  for (int j = 0; j < NT; j++) o_acc[j][0] = o_acc[j][1] = o_acc[j][2] = o_acc[j][3] = 0.f;
+  for (int j = 0; j < OT; j++) o_acc[j][0] = o_acc[j][1] = o_acc[j][2] = o_acc[j][3] = 0.f;
+  // of rows g and g + 8, or with few rows of queries 2t and 2t + 1
   float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+  float mul0 = 0.f, mul1 = 0.f, bias0 = 0.f, bias1 = 0.f;
+  int lim0 = 0, lim1 = 0;
+  if (HALF) {  // lane 4r + t holds row r's factors
+    q_sum += __shfl_xor_sync(0xffffffffu, q_sum, 1);
+    q_sum += __shfl_xor_sync(0xffffffffu, q_sum, 2);
+    mul0 = __shfl_sync(0xffffffffu, mul_a, 8 * t);
+    mul1 = __shfl_sync(0xffffffffu, mul_a, 8 * t + 4);
+    bias0 = -1152.f * __shfl_sync(0xffffffffu, q_sum, 8 * t);
+    bias1 = -1152.f * __shfl_sync(0xffffffffu, q_sum, 8 * t + 4);
+    lim0 = __shfl_sync(0xffffffffu, lim_a, 8 * t);
+    lim1 = __shfl_sync(0xffffffffu, lim_a, 8 * t + 4);
+  }
 
   for (int stage = 0; c < c_end; c += AW, stage = stage + 1 == STAGES ? 0 : stage + 1) {
     cp_wait<STAGES - 1>();
@@ -281,141 +358,228 @@ __global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : AT_MB2) decode_attn
     const float sk0 = sc[0], sk1 = sc[1], sv0 = sc[2], sv1 = sc[3];
     const bool ok0 = reinterpret_cast<const int*>(sc)[4] != 0, ok1 = reinterpret_cast<const int*>(sc)[5] != 0;
 
-    // ---- q . codes of 4 n-tiles of 8 tokens, in units of the page's step
-    // (both pages' steps brought to one where they differ)
-    float s[4][4];
+    if constexpr (HALF) {
+      // ---- at most 8 rows: tokens (then dims) are the MMA's 16 rows, queries
+      // its 8 columns. q . (codes + 1152), the 1152 taken out through C
+      float s[2][4];
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
+      for (int i = 0; i < 2; i++) {
 #pragma unroll
-      for (int b = 0; b < D / 64; b++) {
-        const uint4 w4 = *reinterpret_cast<const uint4*>(st + k_off<D>(n * 8 + g, b * 4 + t));
-        const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
+        for (int b = 0; b < D / 64; b++) {
+          const uint4 u4 = *reinterpret_cast<const uint4*>(st + k_off<D>(i * 16 + g, b * 4 + t));
+          const uint4 v4 = *reinterpret_cast<const uint4*>(st + k_off<D>(i * 16 + 8 + g, b * 4 + t));
+          const uint32_t u[4] = {u4.x ^ 0x80808080u, u4.y ^ 0x80808080u, u4.z ^ 0x80808080u, u4.w ^ 0x80808080u};
+          const uint32_t v[4] = {v4.x ^ 0x80808080u, v4.y ^ 0x80808080u, v4.z ^ 0x80808080u, v4.w ^ 0x80808080u};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (b == 0 && j == 0)
-            mma16816_c(s[n], qa_f[0], codes_f16<0x4140>(w[0]), codes_f16<0x4342>(w[0]), 0.f, 0.f);
-          else
-            mma16816(s[n], qa_f[b * 4 + j], codes_f16<0x4140>(w[j]), codes_f16<0x4342>(w[j]));
+          for (int j = 0; j < 4; j++) {
+            const int ks = b * 4 + j;
+            const uint32_t a0 = codes_up<0x4140>(u[j]), a1 = codes_up<0x4140>(v[j]);
+            const uint32_t a2 = codes_up<0x4342>(u[j]), a3 = codes_up<0x4342>(v[j]);
+            if (ks == 0) mma16816_cols(s[i], a0, a1, a2, a3, qa_f[0][0], qa_f[0][2], bias0, bias1);
+            else mma16816(s[i], a0, a1, a2, a3, qa_f[ks][0], qa_f[ks][2]);
+          }
+        }
+        if (SMALL) {
+#pragma unroll
+          for (int x = 0; x < 4; x++) s[i][x] *= i ? sk1 : sk0;
         }
       }
-      if (SMALL && n >= 2) {
+      if ((c + 1) * CH > lo_lim || !ok0 || !ok1) {
 #pragma unroll
-        for (int x = 0; x < (HALF ? 2 : 4); x++) s[n][x] *= sk1;
-      } else if (SMALL) {
-#pragma unroll
-        for (int x = 0; x < (HALF ? 2 : 4); x++) s[n][x] *= sk0;
+        for (int i = 0; i < 2; i++) {
+          const int j = c * CH + i * 16 + g;
+          const bool ok = i ? ok1 : ok0;
+          if (!ok || j >= lim0) s[i][0] = -INFINITY;
+          if (!ok || j >= lim1) s[i][1] = -INFINITY;
+          if (!ok || j + 8 >= lim0) s[i][2] = -INFINITY;
+          if (!ok || j + 8 >= lim1) s[i][3] = -INFINITY;
+        }
       }
-    }
-    if ((c + 1) * CH > lo_lim || !ok0 || !ok1) {
+      // running maximum; scores in units of log 2 are s * step (the sign of the
+      // scale is in q; a step of 0, an all-zero page, is kept above 0 so that
+      // masked scores stay -inf)
+      const float step0 = fmaxf(SMALL ? mul0 : sk0 * mul0, 1e-37f), step1 = fmaxf(SMALL ? mul1 : sk0 * mul1, 1e-37f);
+      float x0 = column_max(fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])));
+      float x1 = column_max(fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])));
+      x0 = fmaxf(m_a, x0 * step0);
+      x1 = fmaxf(m_b, x1 * step1);
+      const float ref0 = x0 == -INFINITY ? 0.f : x0, ref1 = x1 == -INFINITY ? 0.f : x1;
+      if (__any_sync(0xffffffffu, x0 != m_a || x1 != m_b)) {
+        const float al0 = ex2(m_a - ref0), al1 = ex2(m_b - ref1);
+        l_a *= al0;
+        l_b *= al1;
+#pragma unroll
+        for (int j = 0; j < D / 16; j++) {
+          o_acc[j][0] *= al0;
+          o_acc[j][1] *= al1;
+          o_acc[j][2] *= al0;
+          o_acc[j][3] *= al1;
+        }
+        m_a = x0;
+        m_b = x1;
+      }
+      // weights rounded to f16 (2^-12 of a weight that is at most 1), queries in
+      // rows: the other operand of P.V
+      uint32_t pb[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        pb[i][0] = transpose8(pack_f16(ex2(fmaf(s[i][0], step0, -ref0)), ex2(fmaf(s[i][1], step1, -ref1))));
+        pb[i][1] = transpose8(pack_f16(ex2(fmaf(s[i][2], step0, -ref0)), ex2(fmaf(s[i][3], step1, -ref1))));
+      }
+      // their sums, by the same MMA over a matrix of ones: they go into l (so
+      // that the rounded weights sum to one) and take the 1152 out of V's codes
+      constexpr uint32_t ONES = 0x3c003c00u;
+      float rs[2][4];
+      mma16816_cols(rs[0], ONES, ONES, ONES, ONES, pb[0][0], pb[0][1], 0.f, 0.f);
+      if (SMALL) mma16816_cols(rs[1], ONES, ONES, ONES, ONES, pb[1][0], pb[1][1], 0.f, 0.f);
+      else mma16816(rs[0], ONES, ONES, ONES, ONES, pb[1][0], pb[1][1]);
+      l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
+      l_b += SMALL ? rs[0][1] + rs[1][1] : rs[0][1];
+      // ---- V^T.P^T: rows g and g + 8 of m-tile j are dims 2j and 2j + 1 of lane g's D/8
+      const uint8_t* vs = st + CH * D;
+      constexpr int VW = D / 32;  // words of a lane's dims per token
+      uint32_t w[2][4][VW];
+      load_v<D>(vs, g, t, w);
+#pragma unroll
+      for (int k = 0; k < VW; k++) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {  // dims 4k + 2e and 4k + 2e + 1
+          const int j = 2 * k + e;
+          float acc[2][4];
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            const uint32_t z0 = __byte_perm(w[hf][0][k], w[hf][1][k], e ? 0x7362 : 0x5140);
+            const uint32_t z1 = __byte_perm(w[hf][2][k], w[hf][3][k], e ? 0x7362 : 0x5140);
+            const uint32_t a0 = codes_up<0x4140>(z0), a1 = codes_up<0x4342>(z0);
+            const uint32_t a2 = codes_up<0x4140>(z1), a3 = codes_up<0x4342>(z1);
+            if (SMALL || hf == 0)
+              mma16816_cols(acc[hf], a0, a1, a2, a3, pb[hf][0], pb[hf][1], -1152.f * rs[hf][0], -1152.f * rs[hf][1]);
+            else mma16816(acc[0], a0, a1, a2, a3, pb[1][0], pb[1][1]);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            o_acc[j][x] = fmaf(sv0, acc[0][x], o_acc[j][x]);
+            if (SMALL) o_acc[j][x] = fmaf(sv1, acc[1][x], o_acc[j][x]);
+          }
+        }
+      }
+    } else {
+      // ---- q . codes of 4 n-tiles of 8 tokens, in units of the page's step
+      // (both pages' steps brought to one where they differ)
+      float s[4][4];
 #pragma unroll
       for (int n = 0; n < 4; n++) {
-        const int j = c * CH + n * 8 + 2 * t;
-        const bool ok = n < 2 ? ok0 : ok1;
-        if (!ok || j >= lim_a) s[n][0] = -INFINITY;
-        if (!ok || j + 1 >= lim_a) s[n][1] = -INFINITY;
-        if (!ok || j >= lim_b) s[n][2] = -INFINITY;
-        if (!ok || j + 1 >= lim_b) s[n][3] = -INFINITY;
-      }
-    }
-    // ---- running maximum; scores in units of log 2 are s * step (the sign of
-    // the scale is in q; a step of 0, an all-zero page, is kept above 0 so that
-    // masked scores stay -inf)
-    const float step_a = fmaxf(SMALL ? mul_a : sk0 * mul_a, 1e-37f), step_b = fmaxf(SMALL ? mul_b : sk0 * mul_b, 1e-37f);
-    float x_a = fmaxf(s[0][0], s[0][1]), x_b = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
-    for (int n = 1; n < 4; n++) {
-      x_a = fmaxf(x_a, fmaxf(s[n][0], s[n][1]));
-      if (!HALF) x_b = fmaxf(x_b, fmaxf(s[n][2], s[n][3]));
-    }
-    // an empty chunk stays -inf (0 * -inf would not)
-    x_a = quad_max(x_a);
-    x_a = x_a == -INFINITY ? m_a : fmaxf(m_a, x_a * step_a);
-    if (!HALF) {
+        for (int b = 0; b < D / 64; b++) {
+          const uint4 w4 = *reinterpret_cast<const uint4*>(st + k_off<D>(n * 8 + g, b * 4 + t));
+          const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            if (b == 0 && j == 0)
+              mma16816_c(s[n], qa_f[0], codes_f16<0x4140>(w[0]), codes_f16<0x4342>(w[0]), 0.f, 0.f);
+            else
+              mma16816(s[n], qa_f[b * 4 + j], codes_f16<0x4140>(w[j]), codes_f16<0x4342>(w[j]));
+          }
+        }
+        if (SMALL && n >= 2) {
+#pragma unroll
+          for (int x = 0; x < 4; x++) s[n][x] *= sk1;
+        } else if (SMALL) {
+#pragma unroll
+          for (int x = 0; x < 4; x++) s[n][x] *= sk0;
+        }
+      }
+      if ((c + 1) * CH > lo_lim || !ok0 || !ok1) {
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          const int j = c * CH + n * 8 + 2 * t;
+          const bool ok = n < 2 ? ok0 : ok1;
+          if (!ok || j >= lim_a) s[n][0] = -INFINITY;
+          if (!ok || j + 1 >= lim_a) s[n][1] = -INFINITY;
+          if (!ok || j >= lim_b) s[n][2] = -INFINITY;
+          if (!ok || j + 1 >= lim_b) s[n][3] = -INFINITY;
+        }
+      }
+      // ---- running maximum; scores in units of log 2 are s * step (the sign of
+      // the scale is in q; a step of 0, an all-zero page, is kept above 0 so that
+      // masked scores stay -inf)
+      const float step_a = fmaxf(SMALL ? mul_a : sk0 * mul_a, 1e-37f), step_b = fmaxf(SMALL ? mul_b : sk0 * mul_b, 1e-37f);
+      float x_a = fmaxf(s[0][0], s[0][1]), x_b = fmaxf(s[0][2], s[0][3]);
+#pragma unroll
+      for (int n = 1; n < 4; n++) {
+        x_a = fmaxf(x_a, fmaxf(s[n][0], s[n][1]));
+        x_b = fmaxf(x_b, fmaxf(s[n][2], s[n][3]));
+      }
+      // an empty chunk stays -inf (0 * -inf would not)
+      x_a = quad_max(x_a);
+      x_a = x_a == -INFINITY ? m_a : fmaxf(m_a, x_a * step_a);
       x_b = quad_max(x_b);
       x_b = x_b == -INFINITY ? m_b : fmaxf(m_b, x_b * step_b);
-    }
-    const float ref_a = x_a == -INFINITY ? 0.f : x_a, ref_b = HALF || x_b == -INFINITY ? 0.f : x_b;
-    const bool moved = HALF ? x_a != m_a : (x_a != m_a || x_b != m_b);
-    if (__any_sync(0xffffffffu, moved)) {
-      const float al_a = ex2(m_a - ref_a), al_b = HALF ? 1.f : ex2(m_b - ref_b);
-      l_a *= al_a;
-      l_b *= al_b;
+      const float ref_a = x_a == -INFINITY ? 0.f : x_a, ref_b = x_b == -INFINITY ? 0.f : x_b;
+      const bool moved = x_a != m_a || x_b != m_b;
+      if (__any_sync(0xffffffffu, moved)) {
+        const float al_a = ex2(m_a - ref_a), al_b = ex2(m_b - ref_b);
+        l_a *= al_a;
+        l_b *= al_b;
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        o_acc[j][0] *= al_a;
-        o_acc[j][1] *= al_a;
-        if (!HALF) {
+        for (int j = 0; j < NT; j++) {
+          o_acc[j][0] *= al_a;
+          o_acc[j][1] *= al_a;
           o_acc[j][2] *= al_b;
           o_acc[j][3] *= al_b;
         }
+        m_a = x_a;
+        m_b = x_b;
       }
-      m_a = x_a;
-      m_b = HALF ? m_b : x_b;
-    }
-    // weights rounded to f16 for the MMA (2^-12 of a weight that is at most 1)
-    uint32_t pf[2][4];
+      // weights rounded to f16 for the MMA (2^-12 of a weight that is at most 1)
+      uint32_t pf[2][4];
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-      pf[n >> 1][(n & 1) * 2] = pack_f16(ex2(fmaf(s[n][0], step_a, -ref_a)), ex2(fmaf(s[n][1], step_a, -ref_a)));
-      pf[n >> 1][(n & 1) * 2 + 1] =
-          HALF ? 0u : pack_f16(ex2(fmaf(s[n][2], step_b, -ref_b)), ex2(fmaf(s[n][3], step_b, -ref_b)));
-    }
-    // their row sums, by the same MMA over a matrix of ones: they go into l (so
-    // that the rounded weights sum to one) and take the 1152 out of the codes
-    float rs[2][4];
-#pragma unroll
-    for (int hf = 0; hf < 2; hf++) {
-      if (hf == 1 && !SMALL) mma16816(rs[0], pf[1], 0x3c003c00u, 0x3c003c00u);
-      else mma16816_c(rs[hf], pf[hf], 0x3c003c00u, 0x3c003c00u, 0.f, 0.f);
-    }
-    l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
-    if (!HALF) l_b += SMALL ? rs[0][2] + rs[1][2] : rs[0][2];
-    // ---- P.V: n-tile j of lane g is dim g * (D/8) + j; tokens 2t, 2t+1, 2t+8, 2t+9 of each 16
-    const uint8_t* vs = st + CH * D;
-    constexpr int VW = D / 32;  // words of a lane's dims per token
-    uint32_t w[2][4][VW];
-#pragma unroll
-    for (int hf = 0; hf < 2; hf++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int tok = hf * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
-        if constexpr (D == 64) {
-          const uint2 v = *reinterpret_cast<const uint2*>(vs + v_off<D>(tok, g >> 1) + (g & 1) * 8);
-          w[hf][i][0] = v.x ^ 0x80808080u;
-          w[hf][i][1] = v.y ^ 0x80808080u;
-        } else {
-          const uint4 v = *reinterpret_cast<const uint4*>(vs + v_off<D>(tok, g));
-          w[hf][i][0] = v.x ^ 0x80808080u;
-          w[hf][i][1] = v.y ^ 0x80808080u;
-          w[hf][i][2] = v.z ^ 0x80808080u;
-          w[hf][i][3] = v.w ^ 0x80808080u;
-        }
+      for (int n = 0; n < 4; n++) {
+        pf[n >> 1][(n & 1) * 2] = pack_f16(ex2(fmaf(s[n][0], step_a, -ref_a)), ex2(fmaf(s[n][1], step_a, -ref_a)));
+        pf[n >> 1][(n & 1) * 2 + 1] =
+            pack_f16(ex2(fmaf(s[n][2], step_b, -ref_b)), ex2(fmaf(s[n][3], step_b, -ref_b)));
       }
-#pragma unroll
-    for (int k = 0; k < VW; k++) {
-      uint32_t z[2][4];  // bytes (token 0, token 1) of dims 0,1 | 2,3; the same of tokens 2, 3
+      // their row sums, by the same MMA over a matrix of ones: they go into l (so
+      // that the rounded weights sum to one) and take the 1152 out of the codes
+      float rs[2][4];
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
-        z[hf][0] = __byte_perm(w[hf][0][k], w[hf][1][k], 0x5140);
-        z[hf][1] = __byte_perm(w[hf][0][k], w[hf][1][k], 0x7362);
-        z[hf][2] = __byte_perm(w[hf][2][k], w[hf][3][k], 0x5140);
-        z[hf][3] = __byte_perm(w[hf][2][k], w[hf][3][k], 0x7362);
+        if (hf == 1 && !SMALL) mma16816(rs[0], pf[1], 0x3c003c00u, 0x3c003c00u);
+        else mma16816_c(rs[hf], pf[hf], 0x3c003c00u, 0x3c003c00u, 0.f, 0.f);
       }
+      l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
+      l_b += SMALL ? rs[0][2] + rs[1][2] : rs[0][2];
+      // ---- P.V: n-tile j of lane g is dim g * (D/8) + j; tokens 2t, 2t+1, 2t+8, 2t+9 of each 16
+      const uint8_t* vs = st + CH * D;
+      constexpr int VW = D / 32;  // words of a lane's dims per token
+      uint32_t w[2][4][VW];
+      load_v<D>(vs, g, t, w);
 #pragma unroll
-      for (int dd = 0; dd < 4; dd++) {
-        const int j = k * 4 + dd;
-        float acc[2][4];
+      for (int k = 0; k < VW; k++) {
+        uint32_t z[2][4];  // bytes (token 0, token 1) of dims 0,1 | 2,3; the same of tokens 2, 3
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
-          const uint32_t b0 = (dd & 1) ? codes_up<0x4342>(z[hf][dd >> 1]) : codes_up<0x4140>(z[hf][dd >> 1]);
-          const uint32_t b1 = (dd & 1) ? codes_up<0x4342>(z[hf][2 + (dd >> 1)]) : codes_up<0x4140>(z[hf][2 + (dd >> 1)]);
-          if (SMALL || hf == 0) mma16816_c(acc[hf], pf[hf], b0, b1, -1152.f * rs[hf][0], HALF ? 0.f : -1152.f * rs[hf][2]);
-          else mma16816(acc[0], pf[1], b0, b1);
+          z[hf][0] = __byte_perm(w[hf][0][k], w[hf][1][k], 0x5140);
+          z[hf][1] = __byte_perm(w[hf][0][k], w[hf][1][k], 0x7362);
+          z[hf][2] = __byte_perm(w[hf][2][k], w[hf][3][k], 0x5140);
+          z[hf][3] = __byte_perm(w[hf][2][k], w[hf][3][k], 0x7362);
         }
 #pragma unroll
-        for (int x = 0; x < (HALF ? 2 : 4); x++) {
-          o_acc[j][x] = fmaf(sv0, acc[0][x], o_acc[j][x]);
-          if (SMALL) o_acc[j][x] = fmaf(sv1, acc[1][x], o_acc[j][x]);
+        for (int dd = 0; dd < 4; dd++) {
+          const int j = k * 4 + dd;
+          float acc[2][4];
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            const uint32_t b0 = (dd & 1) ? codes_up<0x4342>(z[hf][dd >> 1]) : codes_up<0x4140>(z[hf][dd >> 1]);
+            const uint32_t b1 = (dd & 1) ? codes_up<0x4342>(z[hf][2 + (dd >> 1)]) : codes_up<0x4140>(z[hf][2 + (dd >> 1)]);
+            if (SMALL || hf == 0) mma16816_c(acc[hf], pf[hf], b0, b1, -1152.f * rs[hf][0], -1152.f * rs[hf][2]);
+            else mma16816(acc[0], pf[1], b0, b1);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            o_acc[j][x] = fmaf(sv0, acc[0][x], o_acc[j][x]);
+            if (SMALL) o_acc[j][x] = fmaf(sv1, acc[1][x], o_acc[j][x]);
+          }
         }
       }
     }
@@ -431,20 +595,34 @@ __global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : AT_MB2) decode_attn
   __syncwarp();
   float* wo = reinterpret_cast<float*>(ring);  // [16][D] O, then [16] m, [16] l
   {
-    // lane (g, t) holds dims 2t * D/8 .. (2t + 2) * D/8 - 1 of rows g, g + 8
-#pragma unroll
-    for (int half = 0; half < (HALF ? 1 : 2); half++)
+    if constexpr (HALF) {
+      // lane (g, t) holds dims g * D/8 .. of queries 2t and 2t + 1
 #pragma unroll
       for (int cc = 0; cc < 2; cc++)
 #pragma unroll
-        for (int j = 0; j < NT; j += 4)
-          *reinterpret_cast<float4*>(wo + (g + half * 8) * D + (2 * t + cc) * NT + j) =
-              make_float4(o_acc[j][half * 2 + cc], o_acc[j + 1][half * 2 + cc], o_acc[j + 2][half * 2 + cc],
-                          o_acc[j + 3][half * 2 + cc]);
-    if (t == 0) {
-      wo[16 * D + g] = m_a;
-      wo[16 * D + 16 + g] = l_a;
-      if (!HALF) {
+        for (int j = 0; j < D / 16; j += 2)
+          *reinterpret_cast<float4*>(wo + (2 * t + cc) * D + g * NT + 2 * j) =
+              make_float4(o_acc[j][cc], o_acc[j][2 + cc], o_acc[j + 1][cc], o_acc[j + 1][2 + cc]);
+      if (g == 0) {
+        wo[16 * D + 2 * t] = m_a;
+        wo[16 * D + 2 * t + 1] = m_b;
+        wo[16 * D + 16 + 2 * t] = l_a;
+        wo[16 * D + 17 + 2 * t] = l_b;
+      }
+    } else {
+      // lane (g, t) holds dims 2t * D/8 .. (2t + 2) * D/8 - 1 of rows g, g + 8
+#pragma unroll
+      for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int cc = 0; cc < 2; cc++)
+#pragma unroll
+          for (int j = 0; j < NT; j += 4)
+            *reinterpret_cast<float4*>(wo + (g + half * 8) * D + (2 * t + cc) * NT + j) =
+                make_float4(o_acc[j][half * 2 + cc], o_acc[j + 1][half * 2 + cc], o_acc[j + 2][half * 2 + cc],
+                            o_acc[j + 3][half * 2 + cc]);
+      if (t == 0) {
+        wo[16 * D + g] = m_a;
+        wo[16 * D + 16 + g] = l_a;
         wo[16 * D + g + 8] = m_b;
         wo[16 * D + 24 + g] = l_b;
       }
@@ -508,10 +686,15 @@ __global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : AT_MB2) decode_attn
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // nothing visible: zeros; NaN stays
     const int qi = (row0 + row) / p.G, hg = (row0 + row) % p.G;
     const int64_t at = (int64_t)(q0 + qi) * p.ldo + ((int64_t)h * p.G + hg) * D + d;
-    dt_store(p.out, at, p.odt, a.x * inv);
-    dt_store(p.out, at + 1, p.odt, a.y * inv);
-    dt_store(p.out, at + 2, p.odt, a.z * inv);
-    dt_store(p.out, at + 3, p.odt, a.w * inv);
+    if (p.o_vec) {
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) =
+          make_uint2(dt_pack2(p.odt, a.x * inv, a.y * inv), dt_pack2(p.odt, a.z * inv, a.w * inv));
+    } else {
+      dt_store(p.out, at, p.odt, a.x * inv);
+      dt_store(p.out, at + 1, p.odt, a.y * inv);
+      dt_store(p.out, at + 2, p.odt, a.z * inv);
+      dt_store(p.out, at + 3, p.odt, a.w * inv);
+    }
   }
   if (p.splits > 1) cg::this_cluster().sync();  // peers may still be reading this CTA
 }
@@ -555,6 +738,8 @@ int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cuda
   a.H = c.n_kv_head; a.G = G; a.q = p.q; a.ldq = p.ldq; a.qdt = p.q_dtype; a.cu_q = p.cu_q; a.n_q = p.n_q;
   a.kv_lens = p.kv_lens; a.table = p.block_table; a.ldt = p.ld_table; a.max_pages = p.max_pages; a.R = p.n_requests;
   a.causal = p.causal; a.max_q = p.max_q; a.scale = p.scale; a.out = p.out; a.ldo = p.ldo; a.odt = p.out_dtype;
+  a.q_vec = p.q_dtype != WG_DT_F32 && aligned16(p.q) && p.ldq % 8 == 0;
+  a.o_vec = aligned16(p.out) && p.ldo % 8 == 0;
   const int64_t rows = (int64_t)p.max_q * G;
   const int64_t tiles = (rows + 15) / 16, units = tiles * c.n_kv_head * p.n_requests;
   const int64_t kv = p.max_kv < ((int64_t)p.max_pages << a.shift) ? p.max_kv : (int64_t)p.max_pages << a.shift;
