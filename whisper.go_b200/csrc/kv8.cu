@@ -52,33 +52,59 @@ __device__ __forceinline__ float needed_scale(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// 8 consecutive elements as fp32.
-__device__ __forceinline__ void load8(const void* p, int64_t i, int dt, bool vec, float (&x)[8]) {
-  if (vec && dt == WG_DT_F32) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else if (vec) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 16 bytes of a row: 8 elements of 16 bits or 4 of 32.
+template <int ES>
+__device__ __forceinline__ uint4 load16(const void* p, int64_t i, bool vec) {
+  const uint8_t* at = reinterpret_cast<const uint8_t*>(p) + i * ES;
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(at));
+  uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+  for (int k = 0; k < 4; k++) {
+    if (ES == 4) w[k] = __ldg(reinterpret_cast<const uint32_t*>(at) + k);
+    else
+      w[k] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + 2 * k) |
+             (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + 2 * k + 1) << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Their values.
+template <int ES>
+__device__ __forceinline__ void values16(uint4 v, int dt, float (&x)[16 / ES]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    if constexpr (ES == 4) {
+      x[k] = __uint_as_float(w[k]);
+    } else {
       const float2 f = dt_unpack2(dt, w[k]);
       x[2 * k] = f.x;
       x[2 * k + 1] = f.y;
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; k++) x[k] = dt_load(p, i + k, dt);
   }
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-  // NaN -> 0; an infinity (and what an infinity's neighbours cannot reach) -> +-127
-  const float y = x * inv;
-  const int c = y != y ? 0 : __float2int_rn(fminf(fmaxf(y, -127.f), 127.f));
-  return (uint32_t)c & 255u;
+// Codes of 4 values as bytes. x / scale is exact (a power of two), so the one
+// rounding is that of the sum with 1.5 * 2^23, whose low byte is the nearest
+// integer, half to even. Finite values need no clamp: |x| <= 127 * scale.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+  const float magic = 12582912.f;
+  const uint32_t lo = __byte_perm(__float_as_uint(fmaf(a, inv, magic)), __float_as_uint(fmaf(b, inv, magic)), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(fmaf(c, inv, magic)), __float_as_uint(fmaf(d, inv, magic)), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+// NaN as 0, an infinity as 127 steps.
+__device__ __forceinline__ float tame(float x, float scale) {
+  const float most = 127.f * scale;
+  return x != x ? 0.f : fminf(fmaxf(x, -most), most);
+}
+// Largest magnitude in 16 bytes, as the bits of its type (what is not finite is
+// larger than anything finite), joined into m: two 16-bit maxima, or one of 32.
+template <int ES>
+__device__ __forceinline__ uint32_t join_max(uint32_t m, uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; k++) m = ES == 2 ? __vmaxu2(m, w[k] & 0x7fff7fffu) : max(m, w[k] & 0x7fffffffu);
+  return m;
 }
 
 struct AppendArgs {
@@ -95,60 +121,113 @@ struct AppendArgs {
 
 constexpr int APPEND_WARPS = 8;
 constexpr int APPEND_CHUNK = 64;  // most tokens a CTA looks for runs in
+constexpr int APPEND_HOLD = 16;   // 16-byte pieces a lane holds between the two passes over a run
+constexpr int PAGE_MAX = 128;
 
 // One warp per (run of consecutive slots in a page, K or V, head). A CTA
 // finds the runs that begin among its `chunk` tokens (grid x) and its warps
-// deal the (run, unit) pairs of its 8 units (grid y).
+// deal the (run, unit) pairs of its 8 units (grid y). The run's values stay in
+// registers between finding the largest magnitude and coding (8 KB a warp: a
+// page of 64 tokens of 64 16-bit values), so they are read once; what is
+// longer is read again from its second block on.
+template <int ES>
 __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(AppendArgs p) {
   pdl_trigger();
   pdl_wait();
-  __shared__ int start_sh[APPEND_CHUNK], len_sh[APPEND_CHUNK];
+  constexpr int EPL = 16 / ES;  // elements a lane takes at once
+  __shared__ int slot_sh[APPEND_CHUNK + PAGE_MAX + 1];
+  __shared__ uint32_t begin_sh[(APPEND_CHUNK + PAGE_MAX) / 32 + 1];  // bit i: a run begins at token t0 + i, or none goes on
+  __shared__ short start_sh[APPEND_CHUNK], len_sh[APPEND_CHUNK];
   __shared__ int runs_sh;
-  const int t0 = blockIdx.x * p.chunk, tid = threadIdx.x;
-  const int page = 1 << p.shift;
+  const int t0 = blockIdx.x * p.chunk, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int page = 1 << p.shift, look = p.chunk + page;  // a run that begins in the chunk ends within `look`
+  // tokens before and after the rows count as outside
+  if (tid <= look) {
+    const int t = t0 + tid - 1;
+    slot_sh[tid] = t >= 0 && t < p.n ? p.slots[t] : -1;
+  }
   if (tid == 0) runs_sh = 0;
   __syncthreads();
-  if (tid < p.chunk && t0 + tid < p.n) {
-    const int t = t0 + tid, s = p.slots[t];
-    const int before = t ? p.slots[t - 1] : -1;
-    if (s >= 0 && s < p.num_slots && (t == 0 || before != s - 1 || (s & (page - 1)) == 0)) {
-      const int most = min(page - (s & (page - 1)), p.n - t);
-      int len = 1;
-      while (len < most && p.slots[t + len] == s + len) len++;
+  {
+    bool begins = true;
+    if (tid < look) {
+      const int s = slot_sh[tid + 1];
+      begins = s < 0 || s >= p.num_slots || slot_sh[tid] != s - 1 || (s & (page - 1)) == 0;
+    }
+    const uint32_t bits = __ballot_sync(0xffffffffu, begins);
+    if (lane == 0 && warp <= look / 32) begin_sh[warp] = bits;
+  }
+  __syncthreads();
+  if (tid < p.chunk) {
+    const int s = slot_sh[tid + 1];
+    if ((begin_sh[tid >> 5] >> (tid & 31) & 1) && s >= 0 && s < p.num_slots) {
+      int w = (tid + 1) >> 5;  // the next beginning is the end
+      uint32_t rest = begin_sh[w] >> ((tid + 1) & 31) << ((tid + 1) & 31);
+      while (!rest && (w + 1) * 32 <= look) rest = begin_sh[++w];
+      const int end = rest ? min(look, w * 32 + __ffs(rest) - 1) : look;
       const int k = atomicAdd(&runs_sh, 1);  // the order of the runs does not matter: each is written alone
-      start_sh[k] = t;
-      len_sh[k] = len;
+      start_sh[k] = (short)tid;
+      len_sh[k] = (short)min(end - tid, page - (s & (page - 1)));
     }
   }
   __syncthreads();
-  const int runs = runs_sh, warp = tid >> 5, lane = tid & 31;
+  const int runs = runs_sh;
   const int u0 = blockIdx.y * APPEND_WARPS, nu = min(APPEND_WARPS, p.units - u0);
-  const int per_tok = p.D >> 3;                 // lanes of 8 elements a token takes
-  const int tok_step = 32 / per_tok;            // tokens a warp takes at once
-  const int d = (lane % per_tok) * 8;
+  const int per_tok = p.D / EPL;         // lanes that a token takes
+  const int tok_step = 32 / per_tok;     // tokens a warp takes at once
+  const int sub = lane / per_tok, d = (lane % per_tok) * EPL;
+  const int block_len = APPEND_HOLD * tok_step;
   for (int w = warp; w < runs * nu; w += APPEND_WARPS) {
     const int run = w / nu, unit = u0 + w % nu;  // unit = kv * H + head
     const int kv = unit >= p.H, head = unit - kv * p.H;
-    const int t = start_sh[run], len = len_sh[run];
-    const int slot = p.slots[t], id = slot >> p.shift, first = slot & (page - 1);
+    const int len = len_sh[run], slot = slot_sh[start_sh[run] + 1];
+    const int id = slot >> p.shift, first = slot & (page - 1);
     const int64_t block = ((int64_t)id * 2 + kv) * p.H + head;
     int8_t* codes = p.codes + block * page * p.D;
     const float old = first ? p.scales[block] : 0.f;
     const void* src = kv ? p.v : p.k;
     const int64_t ld = kv ? p.ldv : p.ldk;
     const bool vec = kv ? p.vecv : p.veck;
-    const int64_t col = (int64_t)head * p.D + d;
-    float amax = 0.f;
-    for (int i = lane / per_tok; i < len; i += tok_step) {
-      float x[8];
-      load8(src, (int64_t)(t + i) * ld + col, p.dt, vec, x);
+    const int64_t from = (int64_t)(t0 + start_sh[run] + sub) * ld + (int64_t)head * p.D + d;
+    uint4 raw[APPEND_HOLD];
+    auto load = [&](int b0) {
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const float a = fabsf(x[k]);
-        if (a <= 3.402823466e38f) amax = fmaxf(amax, a);  // finite values only
+      for (int i = 0; i < APPEND_HOLD; i++) {
+        const int tok = b0 + i * tok_step;
+        raw[i] = tok + sub < len ? load16<ES>(src, from + tok * ld, vec) : make_uint4(0, 0, 0, 0);
       }
+    };
+    uint32_t bits = 0;
+    int held = 0;
+    for (int b0 = 0; b0 < len; b0 += block_len) {
+      load(b0);
+      held = b0;
+#pragma unroll
+      for (int i = 0; i < APPEND_HOLD; i++) bits = join_max<ES>(bits, raw[i]);
     }
-    amax = warp_max(amax);
+    if (ES == 2) bits = max(bits & 0xffffu, bits >> 16);
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    const bool wild = bits >= (ES == 4 ? 0x7f800000u : p.dt == WG_DT_F16 ? 0x7c00u : 0x7f80u);
+    float amax = ES == 4 ? __uint_as_float(bits) : dt_unpack2(p.dt, bits).x;
+    if (wild) {  // something is not finite: the largest of the rest
+      amax = 0.f;
+      for (int b0 = held;;) {
+#pragma unroll 1
+        for (int i = 0; i < APPEND_HOLD; i++) {
+          const int tok = b0 + i * tok_step;
+          float x[EPL];
+          values16<ES>(tok + sub < len ? load16<ES>(src, from + tok * ld, vec) : make_uint4(0, 0, 0, 0), p.dt, x);
+#pragma unroll
+          for (int k = 0; k < EPL; k++) {
+            const float a = fabsf(x[k]);
+            if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
+          }
+        }
+        if (b0 == 0) break;
+        b0 -= block_len;
+      }
+      amax = warp_max(amax);
+    }
     const float scale = fmaxf(old, needed_scale(amax));
     if (first && scale > old && old > 0.f) {
       // the page's earlier tokens in the new step: their codes are the only
@@ -166,13 +245,28 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(AppendArgs p)
       }
     }
     const float inv = scale > 0.f ? 1.f / scale : 0.f;
-    for (int i = lane / per_tok; i < len; i += tok_step) {
-      float x[8];
-      load8(src, (int64_t)(t + i) * ld + col, p.dt, vec, x);
-      uint32_t out[2] = {0, 0};
+    for (int b0 = held;;) {  // the block that is held, then the earlier ones
 #pragma unroll
-      for (int k = 0; k < 8; k++) out[k >> 2] |= code_of(x[k], inv) << (8 * (k & 3));
-      *reinterpret_cast<uint2*>(codes + (int64_t)(first + i) * p.D + d) = make_uint2(out[0], out[1]);
+      for (int i = 0; i < APPEND_HOLD; i++) {
+        const int tok = b0 + i * tok_step + sub;
+        if (tok < len) {
+          float x[EPL];
+          values16<ES>(raw[i], p.dt, x);
+          if (wild) {
+#pragma unroll
+            for (int k = 0; k < EPL; k++) x[k] = tame(x[k], scale);
+          }
+          uint32_t out[EPL / 4];
+#pragma unroll
+          for (int k = 0; k < EPL / 4; k++) out[k] = codes4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3], inv);
+          int8_t* to = codes + (int64_t)(first + tok) * p.D + d;
+          if constexpr (EPL == 8) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
+          else *reinterpret_cast<uint32_t*>(to) = out[0];
+        }
+      }
+      if (b0 == 0) break;
+      b0 -= block_len;
+      load(b0);
     }
     if (lane == 0) p.scales[block] = scale;
   }
@@ -187,42 +281,68 @@ struct ReadArgs {
   int dt;
   bool veck, vecv;
   const int* slots;
-  int64_t total;  // n * 2 * H * D / 16
+  int n, per_cta, units;  // tokens, tokens a CTA takes, (K|V, head) pairs
 };
+constexpr int READ_WARPS = 8;
 
-// One thread per 16 codes of (token, K or V, head).
-__global__ void __launch_bounds__(256) read_kernel(ReadArgs p) {
+// One warp per (K or V, head) and a CTA's tokens, 16 output bytes a lane: the
+// codes of consecutive slots are contiguous, and so are a head's values in a row.
+template <int ES>
+__global__ void __launch_bounds__(READ_WARPS * 32) read_kernel(ReadArgs p) {
   pdl_trigger();
   pdl_wait();
-  const int per_head = p.D >> 4, per_tok = 2 * p.H * per_head;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int t = (int)(i / per_tok), rest = (int)(i - (int64_t)t * per_tok);
-    const int slot = p.slots[t];
-    if (slot < 0 || slot >= p.num_slots) continue;  // no token: the row stays as it was
-    const int unit = rest / per_head, d = (rest - unit * per_head) * 16;
-    const int kv = unit >= p.H, head = unit - kv * p.H, page = 1 << p.shift;
-    const int64_t block = ((int64_t)(slot >> p.shift) * 2 + kv) * p.H + head;
-    const float scale = __ldg(p.scales + block);
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(p.codes + (block * page + (slot & (page - 1))) * p.D + d));
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    float x[16];
+  constexpr int EPL = 16 / ES;
+  const int per_tok = p.D / EPL, tok_step = 32 / per_tok, page = 1 << p.shift;
+  const int lane = threadIdx.x & 31, unit = blockIdx.y * READ_WARPS + (threadIdx.x >> 5);
+  if (unit >= p.units) return;
+  const int sub = lane / per_tok, d = (lane % per_tok) * EPL;
+  const int kv = unit >= p.H, head = unit - kv * p.H;
+  void* dst = kv ? p.v : p.k;
+  const int64_t ld = kv ? p.ldv : p.ldk, col = (int64_t)head * p.D + d;
+  const bool vec = kv ? p.vecv : p.veck;
+  const int t0 = blockIdx.x * p.per_cta, t1 = min(p.n, t0 + p.per_cta);
+  constexpr int U = 4;  // tokens in flight: their slots, then their codes and scales, then the stores
+  for (int tb = t0 + sub; tb < t1; tb += U * tok_step) {
+    int slot[U];
 #pragma unroll
-    for (int k = 0; k < 16; k++) x[k] = (float)(int)(int8_t)(w[k >> 2] >> (8 * (k & 3))) * scale;
-    const int64_t at = (int64_t)t * (kv ? p.ldv : p.ldk) + (int64_t)head * p.D + d;
-    void* dst = kv ? p.v : p.k;
-    if (!(kv ? p.vecv : p.veck)) {
+    for (int i = 0; i < U; i++) slot[i] = tb + i * tok_step < t1 ? __ldg(p.slots + tb + i * tok_step) : -1;
+    uint32_t c[U][EPL / 4];
+    float scale[U];
 #pragma unroll
-      for (int k = 0; k < 16; k++) dt_store(dst, at + k, p.dt, x[k]);
-    } else if (p.dt == WG_DT_F32) {
-      float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + at);
+    for (int i = 0; i < U; i++) {
+      if (slot[i] >= p.num_slots) slot[i] = -1;
+      const int at = max(slot[i], 0);  // no token: a page that exists is read and nothing is written
+      const int64_t block = ((int64_t)(at >> p.shift) * 2 + kv) * p.H + head;
+      scale[i] = __ldg(p.scales + block);
+      const int8_t* src = p.codes + (block * page + (at & (page - 1))) * p.D + d;
+      if constexpr (EPL == 8) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+        c[i][0] = v.x;
+        c[i][1] = v.y;
+      } else {
+        c[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+      }
+    }
 #pragma unroll
-      for (int k = 0; k < 4; k++) o[k] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-    } else {
-      uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dst) + at);
+    for (int i = 0; i < U; i++) {
+      if (slot[i] < 0) continue;  // the row stays as it was
+      // code + 128 in the low byte of 2^23: exact
+      float x[EPL];
 #pragma unroll
-      for (int k = 0; k < 2; k++)
-        o[k] = make_uint4(dt_pack2(p.dt, x[8 * k], x[8 * k + 1]), dt_pack2(p.dt, x[8 * k + 2], x[8 * k + 3]),
-                          dt_pack2(p.dt, x[8 * k + 4], x[8 * k + 5]), dt_pack2(p.dt, x[8 * k + 6], x[8 * k + 7]));
+      for (int k = 0; k < EPL; k++)
+        x[k] = (__uint_as_float(__byte_perm(c[i][k >> 2] ^ 0x80808080u, 0x4b000000u, 0x7540 + (k & 3))) - 8388736.f) *
+               scale[i];
+      const int64_t at = (int64_t)(tb + i * tok_step) * ld + col;
+      if (!vec) {
+#pragma unroll
+        for (int k = 0; k < EPL; k++) dt_store(dst, at + k, p.dt, x[k]);
+      } else if constexpr (ES == 4) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + at) = make_float4(x[0], x[1], x[2], x[3]);
+      } else {
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dst) + at) =
+            make_uint4(dt_pack2(p.dt, x[0], x[1]), dt_pack2(p.dt, x[2], x[3]), dt_pack2(p.dt, x[4], x[5]),
+                       dt_pack2(p.dt, x[6], x[7]));
+      }
     }
   }
 }
@@ -258,7 +378,9 @@ int launch_kv8_append(const wg_kv8& c, const void* k, const void* v, int dt, int
   // enough CTAs
   const int gy = (a.units + APPEND_WARPS - 1) / APPEND_WARPS;
   while (a.chunk < APPEND_CHUNK && (int64_t)(n / (2 * a.chunk)) * gy >= 148 * 4) a.chunk *= 2;
-  return launch_check(launch_k(append_kernel, dim3((n + a.chunk - 1) / a.chunk, gy), dim3(APPEND_WARPS * 32), 0, st, a),
+  const dim3 grid((n + a.chunk - 1) / a.chunk, gy), block(APPEND_WARPS * 32);
+  return launch_check(dt == WG_DT_F32 ? launch_k(append_kernel<4>, grid, block, 0, st, a)
+                                      : launch_k(append_kernel<2>, grid, block, 0, st, a),
                       "kv8_append");
 }
 
@@ -304,9 +426,14 @@ extern "C" int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, voi
   OpDevice dev;
   WG_CHECK(dev.enter(what, device));
   ReadArgs a{cache->codes, cache->scales, cache->num_pages * cache->page, log2_of(cache->page), cache->n_kv_head,
-             cache->head_dim, k, v, ldk, ldv, dtype, vk, vv, slots, (int64_t)n * 2 * width / 16};
-  const int64_t blocks = (a.total + 255) / 256;
-  return launch_check(launch_k(read_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20))), dim3(256), 0,
-                               reinterpret_cast<cudaStream_t>(stream), a),
+             cache->head_dim, k, v, ldk, ldv, dtype, vk, vv, slots, n, 4,
+               2 * cache->n_kv_head};
+  // tokens a CTA: few where calls are short, up to 32 where there are CTAs enough
+  const int gy = (a.units + READ_WARPS - 1) / READ_WARPS;
+  while (a.per_cta < 32 && (int64_t)(n / (2 * a.per_cta)) * gy >= 148 * 8) a.per_cta *= 2;
+  const dim3 grid((n + a.per_cta - 1) / a.per_cta, gy);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return launch_check(dtype == WG_DT_F32 ? launch_k(read_kernel<4>, grid, dim3(256), 0, st, a)
+                                         : launch_k(read_kernel<2>, grid, dim3(256), 0, st, a),
                       "kv8_read");
 }

@@ -31,18 +31,10 @@
 namespace wg {
 namespace {
 
-constexpr int AW = 4;        // warps per CTA
+template <int D>
+constexpr int warps_of() { return 4; }  // warps per CTA (6 and 8 were slower at 128-wide heads: 52 -> 56, 67 us)
 constexpr int CH = 32;       // tokens per chunk
-#ifndef AT_ST
-#define AT_ST 2
-#endif
-#ifndef AT_MB
-#define AT_MB 5
-#endif
-#ifndef AT_SPLIT
-#define AT_SPLIT 6
-#endif
-constexpr int STAGES = AT_ST;
+constexpr int STAGES = 2;    // more hide no more: 3 and 4 stages left 64 x 1500 tokens at 52 us
 constexpr int MAX_SPLIT = 16;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -72,7 +64,7 @@ constexpr int stage_bytes() { return 2 * CH * D + 32; }  // K, V, {sk[2], sv[2],
 template <int D>
 constexpr int warp_bytes() { return STAGES * stage_bytes<D>(); }
 template <int D>
-constexpr int smem_bytes() { return AW * warp_bytes<D>(); }
+constexpr int smem_bytes() { return warps_of<D>() * warp_bytes<D>(); }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -196,10 +188,11 @@ __device__ __forceinline__ void load_v(const uint8_t* vs, int g, int t, uint32_t
 // HALF: at most 8 rows are live, so the MMA's rows 8..15 are not processed
 // past the products. SMALL: 16-token pages (two pages, and scales, per chunk).
 template <int D, bool HALF, bool SMALL>
-__global__ void __launch_bounds__(AW * 32, D == 64 ? AT_MB : 2) decode_attn_kernel(const AttnArgs p) {
+__global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_attn_kernel(const AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
+  constexpr int AW = warps_of<D>();
   constexpr int PARTS = D / 16;  // 16-byte pieces of a token
   constexpr int NT = D / 8;      // n-tiles of P.V
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -747,7 +740,8 @@ int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cuda
   // CTAs per tile: enough for two rounds of the SMs' resident CTAs, no less
   // than two chunks for each warp, and no CTA with more than 64 chunks
   // (2048 tokens), so that one long request among short ones is spread too
-  int64_t s = (148 * AT_SPLIT + units - 1) / units;
+  const int AW = c.head_dim == 64 ? warps_of<64>() : warps_of<128>();
+  int64_t s = (148 * 6 + units - 1) / units;
   if (s > chunks / (2 * AW)) s = chunks / (2 * AW);
   if (s < (chunks + 63) / 64) s = (chunks + 63) / 64;
   a.splits = (int)(s < 1 ? 1 : s > MAX_SPLIT ? MAX_SPLIT : s);
