@@ -25,8 +25,7 @@
 
 #include <mutex>
 
-#include "kernels.cuh"
-#include "ops.cuh"
+#include "kv8_attn.cuh"
 
 namespace wg {
 namespace {
@@ -35,30 +34,6 @@ template <int D>
 constexpr int warps_of() { return 4; }  // warps per CTA (6 and 8 were slower at 128-wide heads: 52 -> 56, 67 us)
 constexpr int CH = 32;       // tokens per chunk
 constexpr int STAGES = 2;    // more hide no more: 3 and 4 stages left 64 x 1500 tokens at 52 us
-constexpr int MAX_SPLIT = 16;
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct AttnArgs {
-  const int8_t* codes;
-  const float* scales;
-  int num_pages, shift, H, G;
-  const void* q;
-  int64_t ldq;
-  int qdt;
-  const int* cu_q;
-  int n_q;
-  const int* kv_lens;
-  const int* table;
-  int64_t ldt;
-  int max_pages, R;
-  int tiles, splits, causal, max_q;
-  float scale;
-  void* out;
-  int64_t ldo;
-  int odt;
-  bool q_vec, o_vec;  // rows that start on 16 bytes
-};
-
 template <int D>
 constexpr int stage_bytes() { return 2 * CH * D + 32; }  // K, V, {sk[2], sv[2], page ok[2]}
 template <int D>
@@ -76,72 +51,10 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// d = a * b + c for a C that is the same for a row's columns (c0: row g, c1: row g + 8)
-__device__ __forceinline__ void mma16816_c(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
-                                           float c1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
-}
-// d = a * b + c for a C that is the same for a column's rows (c0: column 2t, c1: column 2t + 1)
-__device__ __forceinline__ void mma16816_cols(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1, float c0, float c1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  const uint32_t a[4] = {a0, a1, a2, a3};
-  mma16816(c, a, b0, b1);
-}
-// Transposes an 8 x 8 matrix of 16-bit values held as row g, columns 2t and 2t + 1.
-__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-// Bytes (already offset by 128: code + 128) LO / HI of w as an f16 pair:
-// 0x6400 | u is 1024 + u, exact: code + 1152.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes_up(uint32_t w) { return __byte_perm(w, 0x64646464u, SEL); }
-// The codes themselves.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-  const uint32_t h = codes_up<SEL>(w);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ float sum_f16(uint32_t w) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return f.x + f.y;
-}
-// 2^x, x <= 0 (hardware approximation, 2^-22 relative; 0 for -inf)
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float column_max(float v) {  // over the lanes of one t
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-}
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 // Shared-memory byte offset of the 16-byte piece `part` of token tok in a
 // [32][D] block. Swizzled so that a quarter-warp's 16-byte reads of K (two
@@ -188,7 +101,7 @@ __device__ __forceinline__ void load_v(const uint8_t* vs, int g, int t, uint32_t
 // HALF: at most 8 rows are live, so the MMA's rows 8..15 are not processed
 // past the products. SMALL: 16-token pages (two pages, and scales, per chunk).
 template <int D, bool HALF, bool SMALL>
-__global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_attn_kernel(const AttnArgs p) {
+__global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_attn_kernel(const Kv8AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
@@ -320,8 +233,8 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
         if (HALF) q_sum += sum_f16(qa_f[j][0]) + sum_f16(qa_f[j][2]);  // of the row's f16 values
       }
     }
-    mul_a = e[0] * fabsf(p.scale) * LOG2E;  // scores in units of log 2
-    mul_b = HALF ? 0.f : e[1] * fabsf(p.scale) * LOG2E;
+    mul_a = e[0] * fabsf(p.scale) * KV8_LOG2E;  // scores in units of log 2
+    mul_b = HALF ? 0.f : e[1] * fabsf(p.scale) * KV8_LOG2E;
   }
 
   constexpr int OT = HALF ? D / 16 : NT;  // accumulator tiles
@@ -692,7 +605,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
   if (p.splits > 1) cg::this_cluster().sync();  // peers may still be reading this CTA
 }
 
-typedef void (*AttnKernel)(const AttnArgs);
+typedef void (*AttnKernel)(const Kv8AttnArgs);
 template <int D>
 AttnKernel pick(bool half, bool small) {
   if (half) return small ? decode_attn_kernel<D, true, true> : decode_attn_kernel<D, true, false>;
@@ -716,6 +629,7 @@ int set_attributes(int device) {
     WG_CHECK_CUDA(cudaFuncSetAttribute(k64, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     WG_CHECK_CUDA(cudaFuncSetAttribute(k128, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   }
+  WG_CHECK(kv8_prompt_attributes());
   g_attr_done[device] = true;
   return WG_OK;
 }
@@ -726,7 +640,7 @@ int set_attributes(int device) {
 int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));
   const int G = p.n_head / c.n_kv_head;
-  AttnArgs a{};
+  Kv8AttnArgs a{};
   a.codes = c.codes; a.scales = c.scales; a.num_pages = c.num_pages; a.shift = log2_of(c.page);
   a.H = c.n_kv_head; a.G = G; a.q = p.q; a.ldq = p.ldq; a.qdt = p.q_dtype; a.cu_q = p.cu_q; a.n_q = p.n_q;
   a.kv_lens = p.kv_lens; a.table = p.block_table; a.ldt = p.ld_table; a.max_pages = p.max_pages; a.R = p.n_requests;
@@ -734,8 +648,9 @@ int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cuda
   a.q_vec = p.q_dtype != WG_DT_F32 && aligned16(p.q) && p.ldq % 8 == 0;
   a.o_vec = aligned16(p.out) && p.ldo % 8 == 0;
   const int64_t rows = (int64_t)p.max_q * G;
-  const int64_t tiles = (rows + 15) / 16, units = tiles * c.n_kv_head * p.n_requests;
   const int64_t kv = p.max_kv < ((int64_t)p.max_pages << a.shift) ? p.max_kv : (int64_t)p.max_pages << a.shift;
+  if (rows > 16) return launch_kv8_prompt(a, c.head_dim, kv, st);  // more than one MMA's rows
+  const int64_t tiles = 1, units = (int64_t)c.n_kv_head * p.n_requests;
   const int64_t chunks = (kv + CH - 1) / CH;
   // CTAs per tile: enough for two rounds of the SMs' resident CTAs, no less
   // than two chunks for each warp, and no CTA with more than 64 chunks
@@ -744,7 +659,7 @@ int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cuda
   int64_t s = (148 * 6 + units - 1) / units;
   if (s > chunks / (2 * AW)) s = chunks / (2 * AW);
   if (s < (chunks + 63) / 64) s = (chunks + 63) / 64;
-  a.splits = (int)(s < 1 ? 1 : s > MAX_SPLIT ? MAX_SPLIT : s);
+  a.splits = (int)(s < 1 ? 1 : s > KV8_MAX_SPLIT ? KV8_MAX_SPLIT : s);
   a.tiles = (int)tiles;
   if (units * a.splits > 0x7fffffffLL) {
     set_error("wg_kv8_attention: %lld CTAs are more than a grid holds", (long long)(units * a.splits));
