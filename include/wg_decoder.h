@@ -179,6 +179,23 @@ int wg_model_weight_bytes(const wg_model* m, int64_t* bytes);
  * round-robin over the model's devices. */
 int wg_job_create(wg_model* m, int U, int T_enc, const int32_t* prompt, int P,
                   const wg_decode_params* params, wg_job** out);
+/* What a job can do beyond the reference's decoder (no reference counterpart);
+ * zero means off. */
+typedef struct wg_job_options {
+  int32_t cross_cache8; /* the cross K/V cache in 8 bits (wg_kv8_append / wg_kv8_attention over pages of
+                           64 frames): half the memory and half the bytes a token step reads of it;
+                           64-wide heads only; the step kernel is not used */
+  int32_t sample;       /* draw every token with wg_sample_rows instead of the greedy pick and its top-p
+                           fallback, after the repetition penalty, at wg_decode_params' temperature
+                           (0 means 1.0) and attempt; the random number of utterance u's step t is
+                           wg_uniform(seed, u, t). Not with beams or suppress_nst */
+  int32_t top_k;        /* filters of wg_sample_rows: top_k <= 0, */
+  float top_p;          /* top_p >= 1 and */
+  float min_p;          /* min_p <= 0 are no limit */
+} wg_job_options;
+/* wg_job_create with options (NULL: none). */
+int wg_job_create_with(wg_model* m, int U, int T_enc, const int32_t* prompt, int P,
+                       const wg_decode_params* params, const wg_job_options* options, wg_job** out);
 /* Host -> device copy of U encoder outputs, each [T_enc, d] fp32 row-major
  * (enc[u] points at utterance u). */
 int wg_job_upload_encoder(wg_job* j, const float* const* enc);
@@ -238,6 +255,10 @@ int wg_teacher_forced_logits(wg_model* m, const float* const* enc, int U, int T_
                              const int32_t* prompt, int P,
                              const int32_t* forced, int n_forced, int mode,
                              float* logits);
+/* The same for a job with options (cross_cache8 counts; NULL: none). */
+int wg_teacher_forced_logits_with(wg_model* m, const float* const* enc, int U, int T_enc,
+                                  const int32_t* prompt, int P, const int32_t* forced, int n_forced,
+                                  int mode, const wg_job_options* options, float* logits);
 
 /* ---- pipeline batching (internal/model/pipeline.go:90-193) --------------
  * The reference decodes one 30-s chunk per Decode call: the chunks of a file

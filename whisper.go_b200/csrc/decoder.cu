@@ -89,7 +89,15 @@ struct DevJob {
   std::vector<int> utt;  // global utterance ids
   float* enc32 = nullptr;
   __half* enc16 = nullptr;
-  __half* cross = nullptr;
+  __half* cross = nullptr;  // f16 cross K/V of all layers, or of one at a time where the cache is 8 bits
+  // 8-bit cross cache (wg_job_options.cross_cache8): per layer U * pages of
+  // CROSS8_PAGE frames, each utterance's in order
+  bool cross8 = false;
+  int8_t* x8_codes = nullptr;
+  float* x8_scales = nullptr;
+  int* x8_ints = nullptr;  // slots [U * T], table [U][pages], lens [U], cu_q [U + 1]
+  float* samp = nullptr;   // drawn steps: temperature, top_p, min_p [R]
+  int* samp_k = nullptr;   // top_k [R]
   __half* selfkv = nullptr;
   float *x = nullptr, *q = nullptr, *logits = nullptr;
   __half *xln16 = nullptr, *attn16 = nullptr, *h16 = nullptr;
@@ -112,6 +120,8 @@ struct DevJob {
   cudaEvent_t ev[2] = {nullptr, nullptr};
 };
 
+constexpr int CROSS8_PAGE = 64;
+
 // An epilogue descriptor carrying the job's split-K workspace.
 inline Epi job_epi(const DevJob& j) {
   Epi e;
@@ -129,6 +139,7 @@ struct wg_job {
   int U = 0, B = 1, T = 0, P = 0, max_tokens = 0, mode = 0;
   std::vector<int32_t> prompt;
   wg_decode_params params{};
+  wg_job_options options{};
   int steps_done = 0;
   bool all_done = false;
   std::atomic<int> cancel{0};
@@ -324,6 +335,78 @@ int launch_step_job(wg_model* m, DevJob& j, int mode) {
   return launch_step(a, w0, j.st);
 }
 
+// ---- the 8-bit cross cache of a job (wg_job_options.cross_cache8) ----
+int cross8_pages(const DevJob& j) { return (j.T + CROSS8_PAGE - 1) / CROSS8_PAGE; }
+wg_kv8 cross8_cache(const wg_model* m, const DevJob& j, int layer) {
+  const int64_t blocks = (int64_t)j.U * cross8_pages(j) * 2 * m->H;
+  wg_kv8 c{};
+  c.codes = j.x8_codes + layer * blocks * CROSS8_PAGE * m->hd;
+  c.scales = j.x8_scales + layer * blocks;
+  c.num_pages = j.U * cross8_pages(j);
+  c.page = CROSS8_PAGE;
+  c.n_kv_head = m->H;
+  c.head_dim = m->hd;
+  return c;
+}
+
+// Cross-attention of layer l: q (j.q) -> attn16, over the f16 or the 8-bit cache.
+int cross_attention(wg_model* m, DevJob& j, int l) {
+  if (j.cross8) {
+    const int pages = cross8_pages(j);
+    wg_kv8_attn a{};
+    a.q = j.q; a.ldq = m->d; a.q_dtype = WG_DT_F32; a.n_head = m->H;
+    a.n_q = j.R; a.n_requests = j.U;
+    const int* ints = j.x8_ints + (int64_t)j.U * j.T;
+    a.block_table = ints; a.ld_table = pages; a.max_pages = pages;
+    a.kv_lens = ints + (int64_t)j.U * pages; a.cu_q = a.kv_lens + j.U;
+    a.max_q = j.B; a.max_kv = j.T; a.causal = 0; a.scale = 1.0f / sqrtf((float)m->hd);
+    a.out = j.attn16; a.ldo = j.ldd; a.out_dtype = WG_DT_F16;
+    return launch_kv8_attention(cross8_cache(m, j, l), a, j.dev, j.st);
+  }
+  CrossAttnArgs ca{};
+  ca.q = j.q; ca.kv = j.cross + l * ((int64_t)j.U * 2 * m->H * j.T * m->hd);
+  ca.U = j.U; ca.B = j.B; ca.H = m->H; ca.hd = m->hd; ca.T = j.T;
+  ca.out16 = j.attn16;
+  return launch_cross_attn(ca, j.st);
+}
+
+// Layer l's K and V rows of the stacked cross K/V weights (2d rows: a multiple
+// of 128 with 64-wide heads, so the layout's groups stay whole).
+DMat cross_weights(const wg_model* m, const DMat& all, int l) {
+  DMat w = all;
+  const int64_t row = (int64_t)l * 2 * m->d;
+  w.rows = 2 * m->d;
+  if (!qtype_is_quant(w.qtype)) {
+    w.qs += row * w.cols * (w.qtype == WG_QTYPE_F32 ? 4 : 2);
+    return w;
+  }
+  w.ntiles = w.rows / 16;
+  const int64_t slot = slot_of(all, (int)(row / 16), 0);
+  w.qs += slot * 32 * qtype_payload_bytes(w.qtype);
+  w.dsc += slot * 8;
+  if (w.msc) w.msc += slot * 8;
+  if (w.hb) w.hb += slot * 32;
+  return w;
+}
+
+// K_c = E Wk^T, V_c = E Wv^T + vB (decoder.go:923-940): all layers at once, or
+// with the 8-bit cache layer by layer through one f16 buffer.
+int precompute_cross(wg_model* m, DevJob& j) {
+  Epi e = job_epi(j);
+  e.mode = EPI_CROSS_KV; e.kv = j.cross; e.d = m->d; e.H = m->H; e.hd = m->hd; e.T = j.T; e.U = j.U;
+  e.bias_v = j.dm->cross_vb; e.N = 2 * m->L * m->d;
+  if (!j.cross8) return launch_matmul(j.dm->cross_kv, j.enc16, j.ldd, j.U * j.T, e, j.st);
+  e.N = 2 * m->d;
+  const int64_t head = (int64_t)j.T * m->hd, half = m->H * head;
+  const Kv8Rows rows{j.cross, j.cross + half, m->hd, m->hd, head, 2 * half, j.T, WG_DT_F16, true, true};
+  for (int l = 0; l < m->L; l++) {
+    e.bias_v = j.dm->cross_vb + (int64_t)l * m->d;
+    WG_CHECK(launch_matmul(cross_weights(m, j.dm->cross_kv, l), j.enc16, j.ldd, j.U * j.T, e, j.st));
+    WG_CHECK(launch_kv8_append(cross8_cache(m, j, l), rows, j.x8_ints, j.U * j.T, j.st));
+  }
+  return WG_OK;
+}
+
 // ---- one forward pass over all rows of a device job (decoder.go:745-833) ----
 int forward_step(wg_model* m, DevJob& j, const int* tokens, bool want_logits, int mode) {
   DevModel& dm = *j.dm;
@@ -344,7 +427,6 @@ int forward_step(wg_model* m, DevJob& j, const int* tokens, bool want_logits, in
     return launch_matmul(dm.tok, j.xln16, j.ldd, R, e, st);
   }
   const int64_t layer_kv = (int64_t)R * 2 * H * j.Tmax * hd;
-  const int64_t layer_cross = (int64_t)j.U * 2 * H * j.T * hd;
   const bool ref = mode == WG_MODE_REF_COMPAT;
   // LayerNorm of x feeding matmul W: left to the small-batch GEMV where it
   // can take it (no separate kernel), else a LayerNorm kernel into xln16
@@ -380,10 +462,7 @@ int forward_step(wg_model* m, DevJob& j, const int* tokens, bool want_logits, in
     WG_CHECK(norm_for(ly.cq, ly.cln_w, ly.cln_b, e));
     e.mode = EPI_F32; e.out = j.q; e.ldo = d; e.bias = ly.cq_b; e.N = d;
     WG_CHECK(launch_matmul(ly.cq, j.xln16, j.ldd, R, e, st));
-    CrossAttnArgs ca{};
-    ca.q = j.q; ca.kv = j.cross + l * layer_cross; ca.U = j.U; ca.B = j.B; ca.H = H; ca.hd = hd; ca.T = j.T;
-    ca.out16 = j.attn16;
-    WG_CHECK(launch_cross_attn(ca, st));
+    WG_CHECK(cross_attention(m, j, l));
     e = job_epi(j); e.mode = EPI_RESID; e.out = j.x; e.ldo = d; e.bias = ly.co_b; e.N = d;
     WG_CHECK(launch_matmul(ly.co, j.attn16, j.ldd, R, e, st));
     // MLP (decoder.go:974-993)
@@ -417,6 +496,7 @@ void free_devjob(DevJob* j) {
   cudaFree(j->x); cudaFree(j->q); cudaFree(j->logits); cudaFree(j->xln16); cudaFree(j->attn16); cudaFree(j->h16);
   cudaFree(j->ptok); cudaFree(j->prompt_dev); cudaFree(j->forced_dev); cudaFree(j->ints); cudaFree(j->floats);
   cudaFree(j->split_ws);
+  cudaFree(j->x8_codes); cudaFree(j->x8_scales); cudaFree(j->x8_ints); cudaFree(j->samp); cudaFree(j->samp_k);
   cudaFree(j->st_att); cudaFree(j->st_h); cudaFree(j->st_part); cudaFree(j->st_xpart); cudaFree(j->st_xmax);
   cudaFree(j->st_sync);
   if (j->host_done) cudaFreeHost(j->host_done);
@@ -454,13 +534,14 @@ int build_devjob(wg_job* J, DevModel* dm, const std::vector<int>& utt, DevJob** 
   j->Tcap = J->P + J->max_tokens + 1;
   j->ldd = round8(m->d);
   j->ld4 = round8(4 * m->d);
+  j->cross8 = J->options.cross_cache8 != 0;
   int rc = WG_OK;
   auto fail = [&](int r) { free_devjob(j); return r; };
   if (cudaStreamCreateWithFlags(&j->st, cudaStreamNonBlocking) != cudaSuccess) return fail(WG_ERR_CUDA);
   const int d = m->d, H = m->H, hd = m->hd, L = m->L, R = j->R, U = j->U, T = j->T;
   if ((rc = dalloc(&j->enc32, (size_t)U * T * d)) ||
       (rc = dalloc(&j->enc16, (size_t)U * T * j->ldd)) ||
-      (rc = dalloc(&j->cross, (size_t)L * U * 2 * H * T * hd)) ||
+      (rc = dalloc(&j->cross, (size_t)(j->cross8 ? 1 : L) * U * 2 * H * T * hd)) ||
       (rc = dalloc(&j->selfkv, (size_t)L * R * 2 * H * j->Tmax * hd)) ||
       (rc = dalloc(&j->x, (size_t)R * d)) || (rc = dalloc(&j->q, (size_t)R * d)) ||
       (rc = dalloc(&j->logits, (size_t)R * m->V)) ||
@@ -483,7 +564,7 @@ int build_devjob(wg_job* J, DevModel* dm, const std::vector<int>& utt, DevJob** 
   {
     const DevLayer& l0 = dm->layers[0];
     const DMat* w0[6] = {&l0.qkv, &l0.so, &l0.cq, &l0.co, &l0.m0, &l0.m2};
-    if (step_supported(w0, R, hd, d, T, j->Tmax)) {
+    if (!j->cross8 && step_supported(w0, R, hd, d, T, j->Tmax)) {
       int64_t np = 0, nx = 0, nm = 0, ns = 0;
       step_scratch_sizes(w0, R, U, H, T, &np, &nx, &nm, &ns);
       if ((rc = dalloc(&j->st_att, (size_t)R * d)) || (rc = dalloc(&j->st_h, (size_t)R * 4 * d)) ||
@@ -518,6 +599,43 @@ int build_devjob(wg_job* J, DevModel* dm, const std::vector<int>& utt, DevJob** 
     s.seed = p.seed;
   }
   s.correct_mode = J->mode == WG_MODE_CORRECT;
+  s.device = j->dev;
+  if (J->options.sample) {
+    std::vector<float> f(3 * (size_t)R);
+    std::vector<int> kk(R, J->options.top_k);
+    const wg_decode_params& p = J->params;
+    const float temp = (p.temperature == 0.f ? 1.0f : p.temperature) + (float)p.attempt * 0.2f;
+    for (int r = 0; r < R; r++) {
+      f[r] = temp;
+      f[R + r] = J->options.top_p;
+      f[2 * R + r] = J->options.min_p;
+    }
+    if ((rc = init_sample_rows(j->dev)) || (rc = dalloc(&j->samp, f.size())) || (rc = dalloc(&j->samp_k, (size_t)R))) return fail(rc);
+    if (cudaMemcpy(j->samp, f.data(), f.size() * 4, cudaMemcpyHostToDevice) != cudaSuccess ||
+        cudaMemcpy(j->samp_k, kk.data(), kk.size() * 4, cudaMemcpyHostToDevice) != cudaSuccess) {
+      set_error("job setup: sampling settings copy failed");
+      return fail(WG_ERR_CUDA);
+    }
+    s.temperature = j->samp; s.top_p = j->samp + R; s.min_p = j->samp + 2 * R; s.top_k = j->samp_k;
+    s.topp = 0;
+  }
+  if (j->cross8) {
+    const int pages = cross8_pages(*j);
+    const size_t blocks = (size_t)L * U * pages * 2 * H;
+    std::vector<int> v;
+    for (int u = 0; u < U; u++)
+      for (int t = 0; t < T; t++) v.push_back(u * pages * CROSS8_PAGE + t);
+    for (int i = 0; i < U * pages; i++) v.push_back(i);
+    for (int u = 0; u < U; u++) v.push_back(T);
+    for (int u = 0; u <= U; u++) v.push_back(u * j->B);
+    if ((rc = init_kv8_attention(j->dev)) || (rc = dalloc(&j->x8_codes, blocks * CROSS8_PAGE * hd)) || (rc = dalloc(&j->x8_scales, blocks)) ||
+        (rc = dalloc(&j->x8_ints, v.size())))
+      return fail(rc);
+    if (cudaMemcpy(j->x8_ints, v.data(), v.size() * 4, cudaMemcpyHostToDevice) != cudaSuccess) {
+      set_error("job setup: 8-bit cache tables copy failed");
+      return fail(WG_ERR_CUDA);
+    }
+  }
   s.hist = take((size_t)R * j->Tcap);
   s.hist_tmp = take((size_t)R * j->Tcap);
   s.tbl = take((size_t)R * j->Tmax);
@@ -539,6 +657,7 @@ int build_devjob(wg_job* J, DevModel* dm, const std::vector<int>& utt, DevJob** 
   s.score = j->floats;
   s.new_score = j->floats + R;
   s.topk_lp = j->floats + 2 * R;
+  s.u = j->floats + 7 * R;
   s.logits = j->logits;
   s.forced = j->forced_dev;
   std::vector<int> pt((size_t)J->P * R);
@@ -575,11 +694,7 @@ int start_devjob(wg_job* J, DevJob& j) {
     for (int64_t r = 0; r < (int64_t)j.U * j.T; r++)  // test-sized models (d % 8 != 0) only
       WG_CHECK(launch_f32_to_f16(j.enc32 + r * d, j.enc16 + r * j.ldd, d, j.st));
   }
-  // K_c = E Wk^T, V_c = E Wv^T + vB for all layers at once (decoder.go:923-940)
-  Epi e = job_epi(j);
-  e.mode = EPI_CROSS_KV; e.kv = j.cross; e.d = d; e.H = m->H; e.hd = m->hd; e.T = j.T; e.U = j.U;
-  e.bias_v = j.dm->cross_vb; e.N = 2 * m->L * d;
-  WG_CHECK(launch_matmul(j.dm->cross_kv, j.enc16, j.ldd, j.U * j.T, e, j.st));
+  WG_CHECK(precompute_cross(m, j));
   WG_CHECK(launch_sample_reset(j.ss, j.prompt_dev, j.st));
   if (J->mode == WG_MODE_REF_COMPAT) {
     // slot 0 of every (layer, row, k/v, head) starts at zero (decoder.go:346)
@@ -771,6 +886,11 @@ int wg_model_weight_bytes(const wg_model* m, int64_t* bytes) {
 
 int wg_job_create(wg_model* m, int U, int T_enc, const int32_t* prompt, int P, const wg_decode_params* params,
                   wg_job** out) {
+  return wg_job_create_with(m, U, T_enc, prompt, P, params, nullptr, out);
+}
+
+int wg_job_create_with(wg_model* m, int U, int T_enc, const int32_t* prompt, int P, const wg_decode_params* params,
+                       const wg_job_options* options, wg_job** out) {
   if (!m || !out || !params || !prompt) { set_error("wg_job_create: null argument"); return WG_ERR_INVALID; }
   *out = nullptr;
   if (U <= 0 || T_enc <= 0) { set_error("model: decoder: encoder output must be [T, %d]", m->d); return WG_ERR_INVALID; }
@@ -787,6 +907,30 @@ int wg_job_create(wg_model* m, int U, int T_enc, const int32_t* prompt, int P, c
   }
   int B = params->beam_size > 1 ? params->beam_size : 1;
   if (B > 16) { set_error("model: decode: beam size %d > 16 is not supported", B); return WG_ERR_UNSUPPORTED; }
+  if (options) {
+    if (options->cross_cache8 && m->hd != 64) {
+      set_error("wg_job_create_with: the 8-bit cross cache needs 64-wide heads, not %d", m->hd);
+      return WG_ERR_UNSUPPORTED;
+    }
+    if (options->cross_cache8 && (int64_t)U * ((T_enc + 63) / 64) * 64 > 0x7fffffffLL) {
+      set_error("wg_job_create_with: %d utterances of %d frames are too many for the 8-bit cross cache", U, T_enc);
+      return WG_ERR_INVALID;
+    }
+    if (options->sample) {
+      if (B > 1 || params->suppress_nst) {
+        set_error("wg_job_create_with: drawn tokens go with neither beams nor suppress_nst");
+        return WG_ERR_UNSUPPORTED;
+      }
+      if (m->V > (1 << 18)) {
+        set_error("wg_job_create_with: tokens are drawn from at most %d", 1 << 18);
+        return WG_ERR_UNSUPPORTED;
+      }
+      if (!(options->top_p == options->top_p) || !(options->min_p == options->min_p)) {
+        set_error("wg_job_create_with: top_p or min_p is not a number");
+        return WG_ERR_INVALID;
+      }
+    }
+  }
   int mt = params->max_tokens;  // decoder.go:421-430
   if (mt <= 0) mt = m->ctx;
   if (m->ctx - P < mt) mt = m->ctx - P;
@@ -795,6 +939,7 @@ int wg_job_create(wg_model* m, int U, int T_enc, const int32_t* prompt, int P, c
   J->m = m; J->U = U; J->B = B; J->T = T_enc; J->P = P; J->max_tokens = mt; J->mode = params->mode;
   J->prompt.assign(prompt, prompt + P);
   J->params = *params;
+  if (options) J->options = *options;
   J->fault_step = parse_fault("step");
   J->fault_device = parse_fault("device");
   const int nd = (int)m->devs.size();
@@ -1089,6 +1234,12 @@ int wg_decode(wg_model* m, const float* const* enc, int U, int T_enc, const int3
 
 int wg_teacher_forced_logits(wg_model* m, const float* const* enc, int U, int T_enc, const int32_t* prompt, int P,
                              const int32_t* forced, int n_forced, int mode, float* logits) {
+  return wg_teacher_forced_logits_with(m, enc, U, T_enc, prompt, P, forced, n_forced, mode, nullptr, logits);
+}
+
+int wg_teacher_forced_logits_with(wg_model* m, const float* const* enc, int U, int T_enc, const int32_t* prompt, int P,
+                                  const int32_t* forced, int n_forced, int mode, const wg_job_options* options,
+                                  float* logits) {
   if (!m || !enc || !prompt || !logits || U <= 0 || (n_forced > 0 && !forced)) {
     set_error("wg_teacher_forced_logits: bad argument");
     return WG_ERR_INVALID;
@@ -1112,7 +1263,7 @@ int wg_teacher_forced_logits(wg_model* m, const float* const* enc, int U, int T_
   // a single-device job on the model's first device
   std::vector<DevModel*> saved = m->devs;
   m->devs.resize(1);
-  int rc = wg_job_create(m, U, T_enc, prompt, P, &p, &J);
+  int rc = wg_job_create_with(m, U, T_enc, prompt, P, &p, options, &J);
   m->devs = saved;
   if (rc != WG_OK) return rc;
   J->max_tokens = n_forced;
@@ -1276,7 +1427,6 @@ int wg_job_time_kernel(wg_job* J, int kclass, int iters, double* ms, double* byt
   const int d = m->d, H = m->H, hd = m->hd, R = j.R, L = m->L;
   const bool ref = J->mode == WG_MODE_REF_COMPAT;
   const int64_t layer_kv = (int64_t)R * 2 * H * j.Tmax * hd;
-  const int64_t layer_cross = (int64_t)j.U * 2 * H * j.T * hd;
   double b = 0;
   int launches = 0;
   auto run = [&](bool count) -> int {
@@ -1310,22 +1460,18 @@ int wg_job_time_kernel(wg_job* J, int kclass, int iters, double* ms, double* byt
           launches++;
         }
       } else if (kclass == WG_KCLASS_CROSS_ATTN) {
-        CrossAttnArgs ca{};
-        ca.q = j.q; ca.kv = j.cross + l * layer_cross; ca.U = j.U; ca.B = j.B; ca.H = H; ca.hd = hd; ca.T = j.T;
-        ca.out16 = j.attn16;
-        WG_CHECK(launch_cross_attn(ca, j.st));
+        WG_CHECK(cross_attention(m, j, l));
         if (count) {
-          b += (double)j.U * 2 * j.T * d * 2 + (double)R * d * 4 + (double)R * d * 2;
+          b += (double)j.U * 2 * j.T * d * (j.cross8 ? 1 : 2) + (double)R * d * 4 + (double)R * d * 2;
+          if (j.cross8) b += (double)j.U * cross8_pages(j) * 2 * H * 4;
           launches++;
         }
       } else if (kclass == WG_KCLASS_PRECOMPUTE) {
         if (l > 0) break;
-        Epi e = job_epi(j);
-        e.mode = EPI_CROSS_KV; e.kv = j.cross; e.d = d; e.H = H; e.hd = hd; e.T = j.T; e.U = j.U;
-        e.bias_v = dm.cross_vb; e.N = 2 * L * d;
-        WG_CHECK(launch_matmul(dm.cross_kv, j.enc16, j.ldd, j.U * j.T, e, j.st));
+        WG_CHECK(precompute_cross(m, j));
         if (count) {
-          b += (double)dmat_device_bytes(dm.cross_kv) + (double)j.U * j.T * d * 2 + (double)j.U * j.T * 2 * L * d * 2;
+          b += (double)dmat_device_bytes(dm.cross_kv) + (double)j.U * j.T * d * 2 +
+               (double)j.U * j.T * 2 * L * d * (j.cross8 ? 1 : 2);
           launches++;
         }
       } else if (kclass == WG_KCLASS_STEP) {

@@ -210,6 +210,14 @@ struct SampleState {
   float logprob_thold;
   uint64_t seed;           // draws wg_uniform(seed, utt_id[u], utt_steps[u])
   const int* utt_id;       // [U] the job's utterance index of each local utterance
+  // greedy jobs that draw every token (wg_job_options.sample): the filters of
+  // each row and its random number, device arrays [R]; temperature == nullptr: off
+  int device;
+  float* u;
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
 };
 // One token step of sampling: penalty, greedy argmax or beam top-5 + merge,
 // history/KV-table reorder, pos += 1.
@@ -227,9 +235,19 @@ int launch_sample_reset(const SampleState& s, const int* prompt_dev, cudaStream_
 // ---- serving operators (kv8.cu, kv8_attn.cu, sample_rows.cu) ------------------------
 // The launches behind wg_kv8_append, wg_kv8_attention and wg_sample_rows, for
 // the decode jobs: arguments are checked by the caller, `device` is current.
-int launch_kv8_append(const wg_kv8& c, const void* k, const void* v, int dt, int64_t ldk, int64_t ldv, bool veck,
-                      bool vecv, const int32_t* slots, int n, cudaStream_t st);
+struct Kv8Rows {
+  const void *k, *v;
+  int64_t ldk, ldv;          // elements between tokens
+  int64_t head_step;         // between heads
+  int64_t batch_step;        // between batches of `batch` tokens (a batch begins pages of its own)
+  int batch, dtype;
+  bool veck, vecv;           // every head of every token starts on 16 bytes
+};
+int launch_kv8_append(const wg_kv8& c, const Kv8Rows& rows, const int32_t* slots, int n, cudaStream_t st);
 int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cudaStream_t st);
 int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st);
+// Kernel attributes on `device` (current), before a stream capture begins.
+int init_kv8_attention(int device);
+int init_sample_rows(int device);
 
 }  // namespace wg

@@ -113,6 +113,8 @@ struct AppendArgs {
   int num_slots, shift, H, D;
   const void *k, *v;
   int64_t ldk, ldv;
+  int64_t head_step, batch_step;  // elements between heads, and between batches of `batch` tokens
+  int batch;
   int dt;
   bool veck, vecv;
   const int* slots;
@@ -188,7 +190,9 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(AppendArgs p)
     const void* src = kv ? p.v : p.k;
     const int64_t ld = kv ? p.ldv : p.ldk;
     const bool vec = kv ? p.vecv : p.veck;
-    const int64_t from = (int64_t)(t0 + start_sh[run] + sub) * ld + (int64_t)head * p.D + d;
+    // a run lies in one batch: batches begin pages of their own
+    const int t_run = t0 + start_sh[run], in_batch = t_run / p.batch;
+    const int64_t from = in_batch * p.batch_step + (int64_t)(t_run - in_batch * p.batch + sub) * ld + head * p.head_step + d;
     uint4 raw[APPEND_HOLD];
     auto load = [&](int b0) {
 #pragma unroll
@@ -369,10 +373,10 @@ int rows_check(const char* what, const char* name, const void* p, int dt, int64_
 
 }  // namespace
 
-int launch_kv8_append(const wg_kv8& c, const void* k, const void* v, int dt, int64_t ldk, int64_t ldv, bool veck,
-                      bool vecv, const int32_t* slots, int n, cudaStream_t st) {
-  AppendArgs a{c.codes, c.scales, c.num_pages * c.page, log2_of(c.page), c.n_kv_head, c.head_dim, k, v, ldk, ldv,
-               dt, veck, vecv, slots, n, 1, 2 * c.n_kv_head};
+int launch_kv8_append(const wg_kv8& c, const Kv8Rows& r, const int32_t* slots, int n, cudaStream_t st) {
+  const int dt = r.dtype;
+  AppendArgs a{c.codes, c.scales, c.num_pages * c.page, log2_of(c.page), c.n_kv_head, c.head_dim, r.k, r.v, r.ldk, r.ldv,
+               r.head_step, r.batch_step, r.batch, dt, r.veck, r.vecv, slots, n, 1, 2 * c.n_kv_head};
   // tokens a CTA looks through: few, so that short calls spread over the SMs
   // (every token may begin a run of its own), up to 64 where that leaves
   // enough CTAs
@@ -406,7 +410,8 @@ extern "C" int wg_kv8_append(const wg_kv8* cache, const void* k, const void* v, 
   }
   OpDevice dev;
   WG_CHECK(dev.enter(what, device));
-  return launch_kv8_append(*cache, k, v, dtype, ldk, ldv, vk, vv, slots, n, reinterpret_cast<cudaStream_t>(stream));
+  const Kv8Rows rows{k, v, ldk, ldv, cache->head_dim, 0, n, dtype, vk, vv};
+  return launch_kv8_append(*cache, rows, slots, n, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, void* k, void* v, int dtype, int64_t ldk,

@@ -636,6 +636,8 @@ int set_attributes(int device) {
 
 }  // namespace
 
+int init_kv8_attention(int device) { return set_attributes(device); }
+
 // The launch behind wg_kv8_attention (arguments checked, device current).
 int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));

@@ -342,6 +342,27 @@ __global__ void __launch_bounds__(TOPP_THREADS) topp_kernel(SampleState s) {
   if (threadIdx.x == 0) greedy_commit(s, r, u, tok_sh);
 }
 
+// ---- drawn steps (wg_job_options.sample) ------------------------------------------
+// draw_prepare_kernel applies the repetition penalty and the EOT mask to the
+// rows that still run and draws their random numbers, wg_sample_rows' kernel
+// picks from the rows, draw_commit_kernel appends the picks.
+__global__ void __launch_bounds__(128) draw_prepare_kernel(SampleState s) {
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x, u = r;  // B == 1
+  if (s.utt_done[u]) return;
+  penalty_row(s, r);
+  if (threadIdx.x == 0) s.u[r] = uniform_dev(s.seed, (uint32_t)s.utt_id[u], (uint32_t)s.utt_steps[u]);
+}
+__global__ void draw_commit_kernel(SampleState s) {
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x * blockDim.x + threadIdx.x;
+  if (r >= s.R || s.utt_done[r]) return;
+  const int tok = s.new_tok[r];
+  greedy_commit(s, r, r, tok < 0 ? 0 : tok);  // a row of nothing but -inf or NaN: token 0, as the greedy pick
+}
+
 // ---- beam: per-row top-5 of log_softmax(logits / T) ----------------------------
 constexpr int TOPK = 5;
 __device__ void topk_finish(const SampleState& s, int r, const float* lg, float (&fv)[TOPK], int (&fi)[TOPK],
@@ -937,7 +958,14 @@ int sample_split_rows() {
 
 int launch_sample_step(const SampleState& s, cudaStream_t st) {
   const bool split = s.R <= sample_split_rows();
-  if (s.B <= 1) {
+  if (s.temperature) {
+    WG_CHECK(launch_check(launch_k(draw_prepare_kernel, dim3(s.R), dim3(128), 0, st, s), "draw_prepare"));
+    wg_sample p{};
+    p.logits = s.logits; p.ld = s.V; p.dtype = WG_DT_F32; p.R = s.R; p.V = s.V; p.u = s.u;
+    p.temperature = s.temperature; p.top_k = s.top_k; p.top_p = s.top_p; p.min_p = s.min_p; p.tokens = s.new_tok;
+    WG_CHECK(launch_sample_rows(p, s.device, st));
+    WG_CHECK(launch_check(launch_k(draw_commit_kernel, dim3((s.R + 127) / 128), dim3(128), 0, st, s), "draw_commit"));
+  } else if (s.B <= 1) {
     if (split) WG_CHECK(launch_check(launch_split(greedy_split_kernel, s.R, st, s), "greedy_split"));
     else WG_CHECK(launch_check(launch_k(greedy_kernel, dim3(s.R), dim3(1024), 0, st, s), "greedy"));
     if (s.topp) WG_CHECK(launch_check(launch_k(topp_kernel, dim3(s.R), dim3(TOPP_THREADS), 0, st, s), "topp"));

@@ -897,6 +897,8 @@ int set_attributes(int device) {
 
 }  // namespace
 
+int init_sample_rows(int device) { return set_attributes(device); }
+
 int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));
   // CTAs a row: as many as the SMs take in one round (two CTAs each from 4 a

@@ -85,6 +85,11 @@ class WgDecodeParams(ctypes.Structure):
     ]
 
 
+class WgJobOptions(ctypes.Structure):
+    _fields_ = [("cross_cache8", ctypes.c_int32), ("sample", ctypes.c_int32), ("top_k", ctypes.c_int32),
+                ("top_p", ctypes.c_float), ("min_p", ctypes.c_float)]
+
+
 class WgKv8(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("num_pages", ctypes.c_int32),
                 ("page", ctypes.c_int32), ("n_kv_head", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
@@ -127,6 +132,9 @@ def _declare(lib):
         "wg_model_info": (ctypes.c_int, [P] + [ctypes.POINTER(ctypes.c_int)] * 5),
         "wg_job_create": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, c_int32_p, ctypes.c_int,
                                          ctypes.POINTER(WgDecodeParams), ctypes.POINTER(P)]),
+        "wg_job_create_with": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, c_int32_p, ctypes.c_int,
+                                              ctypes.POINTER(WgDecodeParams), ctypes.POINTER(WgJobOptions),
+                                              ctypes.POINTER(P)]),
         "wg_job_upload_encoder": (ctypes.c_int, [P, ctypes.POINTER(c_float_p)]),
         "wg_job_upload_encoder_device": (ctypes.c_int, [P, ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p]),
         "wg_job_utterance_device": (ctypes.c_int, [P, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]),
@@ -145,6 +153,9 @@ def _declare(lib):
         "wg_teacher_forced_logits": (ctypes.c_int, [P, ctypes.POINTER(c_float_p), ctypes.c_int, ctypes.c_int,
                                                     c_int32_p, ctypes.c_int, c_int32_p, ctypes.c_int, ctypes.c_int,
                                                     c_float_p]),
+        "wg_teacher_forced_logits_with": (ctypes.c_int, [P, ctypes.POINTER(c_float_p), ctypes.c_int, ctypes.c_int,
+                                                         c_int32_p, ctypes.c_int, c_int32_p, ctypes.c_int,
+                                                         ctypes.c_int, ctypes.POINTER(WgJobOptions), c_float_p]),
         "wg_batcher_create": (ctypes.c_int, [P, ctypes.c_int, ctypes.c_int, ctypes.POINTER(P)]),
         "wg_batcher_decode": (ctypes.c_int, [P, c_float_p, ctypes.c_int, c_int32_p, ctypes.c_int,
                                              ctypes.POINTER(WgDecodeParams), ctypes.POINTER(ctypes.c_int), c_int32_p,
@@ -302,6 +313,16 @@ class DecoderParams:
     suppress_eot: bool = False
     attempt: int = 0
     seed: int = 0                 # top-p draws: wg_uniform(seed, utterance, step)
+    # job options (wg_job_options; not in the reference)
+    cross_cache8: bool = False    # cross K/V cache in 8 bits
+    sample: bool = False          # draw every token: temperature, then top_k / top_p / min_p
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+    def options(self) -> WgJobOptions:
+        return WgJobOptions(int(bool(self.cross_cache8)), int(bool(self.sample)), int(self.top_k), float(self.top_p),
+                            float(self.min_p))
 
     def to_c(self) -> WgDecodeParams:
         return WgDecodeParams(beam_size=int(self.beam_size), temperature=float(self.temperature),
@@ -621,8 +642,8 @@ class WhisperDecoder:
         finally:
             job.close()
 
-    def teacher_forced_logits(self, encoder_outs, prompt: Sequence[int], forced, mode: int = MODE_CORRECT
-                              ) -> np.ndarray:
+    def teacher_forced_logits(self, encoder_outs, prompt: Sequence[int], forced, mode: int = MODE_CORRECT,
+                              cross_cache8: bool = False) -> np.ndarray:
         """Logits [n_forced, U, V] along forced token sequences (forced: [U, n] or [n])."""
         if isinstance(encoder_outs, np.ndarray) and encoder_outs.ndim == 2:
             encoder_outs = [encoder_outs]
@@ -632,9 +653,10 @@ class WhisperDecoder:
         fo = np.ascontiguousarray(np.asarray(forced, dtype=np.int32).reshape(U, -1))
         n = fo.shape[1]
         out = np.empty((n, U, self.n_vocab), dtype=np.float32)
-        check(lib().wg_teacher_forced_logits(self.h, ptrs, U, arrs[0].shape[0], pr.ctypes.data_as(c_int32_p),
-                                             len(pr), fo.ctypes.data_as(c_int32_p), n, mode,
-                                             out.ctypes.data_as(c_float_p)), "teacher forcing")
+        opts = WgJobOptions(cross_cache8=int(bool(cross_cache8)))
+        check(lib().wg_teacher_forced_logits_with(self.h, ptrs, U, arrs[0].shape[0], pr.ctypes.data_as(c_int32_p),
+                                                  len(pr), fo.ctypes.data_as(c_int32_p), n, mode, ctypes.byref(opts),
+                                                  out.ctypes.data_as(c_float_p)), "teacher forcing")
         return out
 
 
@@ -651,6 +673,8 @@ class Batcher:
 
     def decode_tokens(self, encoder_out: np.ndarray, params: DecoderParams, ctx: Optional[Context] = None):
         """(tokens, score) of one utterance, prompt included."""
+        if params.sample or params.cross_cache8:  # the shared jobs have no options
+            raise DecodeError("model: decode: batcher: sample and cross_cache8 need a job of their own", 4)
         enc = np.ascontiguousarray(encoder_out, dtype=np.float32)
         pr = np.asarray(params.prompt, dtype=np.int32)
         cap = len(pr) + max_tokens_for(params, self.dec.n_text_ctx)
@@ -694,8 +718,9 @@ class Job:
         self.prompt = np.asarray(params.prompt, dtype=np.int32)
         self._cp = params.to_c()
         h = ctypes.c_void_p()
-        check(lib().wg_job_create(dec.h, U, T, self.prompt.ctypes.data_as(c_int32_p), len(self.prompt),
-                                  ctypes.byref(self._cp), ctypes.byref(h)), "job create")
+        check(lib().wg_job_create_with(dec.h, U, T, self.prompt.ctypes.data_as(c_int32_p), len(self.prompt),
+                                       ctypes.byref(self._cp), ctypes.byref(params.options()), ctypes.byref(h)),
+              "job create")
         self.h = h
         self.max_tokens = max_tokens_for(params, dec.n_text_ctx)
         self._keep = None
