@@ -7,12 +7,14 @@
 // = its page * page size + its place in the page.
 //
 // Latency is what bounds it (a decode step plans a few hundred bytes), so the
-// whole plan is one launch: one cluster of up to PLAN_CLUSTER CTAs, each of
-// which scans all requests itself (two integers a request) instead of waiting
-// for another CTA's sums; the cluster barrier only keeps the cursor from
-// being advanced before every CTA has read it. Slots, the only output that
-// can be long, are dealt over the cluster's threads, four to a store, each
-// found by a binary search in the tile's prefix sums.
+// plan is one launch, and every CTA scans all requests itself (two integers a
+// request) instead of waiting for another CTA's sums. Slots, the only output
+// that can be long, are dealt over the CTAs' threads, four to a store, each
+// found by a binary search in the tile's prefix sums. A cursor that is
+// advanced in place must not be written before every CTA has read it: up to
+// PLAN_CLUSTER CTAs are a cluster with a barrier for that, more leave the
+// cursor to a second launch of one thread (1500 prompts of up to 448 tokens:
+// 31 us with 8 CTAs, 17 with 64).
 #include "ops.cuh"
 
 namespace wg {
@@ -20,6 +22,7 @@ namespace {
 
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_CLUSTER = 8;
+constexpr int PLAN_CTAS = 64;
 
 struct PlanArgs {
   const int* lens;
@@ -36,6 +39,7 @@ struct PlanArgs {
   int n_slots;
   int* cu;
   int* status;
+  bool barrier, advance;  // the CTAs are a cluster; this kernel writes the cursor
 };
 
 struct Two {
@@ -71,7 +75,14 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// grid = cluster = (C, 1, 1)
+// The cursor behind a plan whose CTAs could not be sure that all had read it.
+__global__ void plan_cursor_kernel(const int* cursor, int* cursor_out, const int* status) {
+  pdl_trigger();
+  pdl_wait();
+  *cursor_out = *cursor + status[1];
+}
+
+// grid (C, 1, 1), one cluster where p.barrier
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p) {
   pdl_trigger();
   pdl_wait();
@@ -102,11 +113,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p) {
   if (code) atomicMax(&code_sh, code);
   __syncthreads();
   code = code_sh;
-  cluster_sync();  // every CTA has read the cursor: it may be advanced in place
+  if (p.barrier) cluster_sync();  // every CTA has read the cursor: it may be advanced in place
   if (rank == 0 && tid == 0) {
     p.status[0] = code;
     p.status[1] = code ? 0 : (int)total.b;
-    *p.cursor_out = (int)(code ? cursor : cursor + total.b);
+    if (p.advance) *p.cursor_out = (int)(code ? cursor : cursor + total.b);
     p.cu[0] = 0;
   }
   const int live = code ? 0 : (int)total.a;
@@ -206,22 +217,29 @@ extern "C" int wg_kv_plan(const int32_t* lens, const int32_t* new_tokens, int R,
   }
   OpDevice dev;
   WG_CHECK(dev.enter("wg_kv_plan", device));
-  PlanArgs a{lens, new_tokens, R, log2_of(page), free_pages, n_free, cursor, cursor_out, block_table, ld_table,
-             max_pages, slots, n_slots, cu_new, status};
+  // CTAs: four slots a thread, in a cluster while that suffices
+  const int64_t work = (int64_t)n_slots + R;
   int C = 1;
-  while (C < PLAN_CLUSTER && (int64_t)C * PLAN_THREADS * 4 < (int64_t)n_slots + R) C *= 2;
+  while (C < PLAN_CTAS && (int64_t)C * PLAN_THREADS * 4 < work) C *= 2;
+  const bool cluster = C <= PLAN_CLUSTER, apart = cursor_out != cursor;
+  PlanArgs a{lens, new_tokens, R, log2_of(page), free_pages, n_free, cursor, cursor_out, block_table, ld_table,
+             max_pages, slots, n_slots, cu_new, status, cluster, cluster || apart};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C);
   cfg.blockDim = dim3(PLAN_THREADS);
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.x = cluster ? C : 1;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return launch_check(cudaLaunchKernelEx(&cfg, plan_kernel, a), "kv_plan");
+  WG_CHECK(launch_check(cudaLaunchKernelEx(&cfg, plan_kernel, a), "kv_plan"));
+  if (a.advance) return WG_OK;
+  return launch_check(launch_k(plan_cursor_kernel, dim3(1), dim3(1), 0, st, cursor, cursor_out, (const int*)status),
+                      "kv_plan_cursor");
 }
