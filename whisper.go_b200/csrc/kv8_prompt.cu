@@ -24,9 +24,6 @@ namespace cg = cooperative_groups;
 constexpr int PW = 4;        // warps
 constexpr int PR = PW * 16;  // rows of a tile
 constexpr int PT = 64;       // tokens of a chunk
-#ifndef PB64
-#define PB64 3
-#endif
 
 // Byte offset of the 16-byte piece c of token tok in a [PT][D] f16 tile:
 // eight tokens' pieces of one c fall into different banks.
@@ -56,7 +53,7 @@ __device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t at) {
 
 // GT: tokens of a chunk that share a page, and so scales (16, 32 or 64)
 template <int D, int GT>
-__global__ void __launch_bounds__(PW * 32, D == 64 ? PB64 : 2) prompt_attn_kernel(const Kv8AttnArgs p) {
+__global__ void __launch_bounds__(PW * 32, D == 64 ? 4 : 2) prompt_attn_kernel(const Kv8AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
@@ -65,7 +62,8 @@ __global__ void __launch_bounds__(PW * 32, D == 64 ? PB64 : 2) prompt_attn_kerne
   constexpr int NT = D / 8, KS = D / 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-  const int tile = unit % p.tiles, h = (unit / p.tiles) % p.H, r = unit / p.tiles / p.H;
+  // the last rows of a causal prompt see the most tokens: their tiles start first
+  const int tile = p.tiles - 1 - unit / (p.H * p.R), h = unit % p.H, r = unit / p.H % p.R;
   const int page = 1 << p.shift;
   int q0 = __ldg(p.cu_q + r);
   int nq = __ldg(p.cu_q + r + 1) - q0;

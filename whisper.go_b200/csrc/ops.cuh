@@ -43,11 +43,15 @@ __device__ __forceinline__ float2 dt_unpack2(int dt, uint32_t w) {
 class OpDevice {
  public:
   int enter(const char* what, int device) {
-    int n = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
-      cudaGetLastError();
-      set_error("no CUDA device is available");
-      return WG_ERR_NO_DEVICE;
+    static std::atomic<int> known{0};  // devices do not come and go in a process's life
+    int n = known.load(std::memory_order_relaxed);
+    if (n == 0) {
+      if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+        cudaGetLastError();
+        set_error("no CUDA device is available");
+        return WG_ERR_NO_DEVICE;
+      }
+      known.store(n, std::memory_order_relaxed);
     }
     if (device < 0 || device >= n) {
       set_error("%s: device %d does not exist (%d visible)", what, device, n);

@@ -45,11 +45,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int SR_THREADS = 512;
+constexpr int SR_THREADS = 256;
 constexpr int SR_WARPS = SR_THREADS / 32;
-constexpr int SR_BINS = SR_THREADS;       // first histogram: one bin a thread
-constexpr int SR_SUB = SR_THREADS;        // bins of a descent: one a thread (9 bits)
-constexpr int SR_LIST = 2 * SR_THREADS;   // candidates that rank 0 can finish alone
+constexpr int SR_BPT = 2;                 // bins a thread
+constexpr int SR_BINS = SR_BPT * SR_THREADS;  // of the first histogram
+constexpr int SR_SUB = SR_BPT * SR_THREADS;   // of a descent (9 bits)
+constexpr int SR_EPT = 4;                 // candidates a thread
+constexpr int SR_LIST = SR_EPT * SR_THREADS;  // that rank 0 can finish alone
 constexpr int SR_COUNT = 256;             // so many or fewer are ordered by counting instead of sorting
 constexpr int SR_MAX_CLUSTER = 8;
 constexpr int SR_TABLE = 256;
@@ -93,7 +95,7 @@ struct Shared {
   unsigned listed[SR_MAX_CLUSTER];                 // candidates of the slice
   int again;                                       // from rank 0: SR_DONE, SR_EXACT or SR_WHOLE
   // read by peers after a cluster barrier
-  uint2 hist[SR_BINS];                             // count, mass of the heavy ones (2^-16 units)
+  alignas(16) uint2 hist[SR_BINS];                 // count, mass of the heavy ones (2^-16 units)
   union alignas(16) {
     uint4 sub[2][SR_SUB];  // descents: count, mass in three 15-bit digits (summed in 32 bits: for < 2^17 elements)
     struct {
@@ -115,6 +117,8 @@ struct Shared {
   u64 found_m;
   unsigned found_c;
 };
+static_assert(SR_BPT == 2 && offsetof(Shared, hist) % 16 == 0, "a thread's bins are one uint4");
+static_assert(SR_COUNT <= SR_THREADS, "one candidate a thread");
 static_assert(offsetof(Shared, sub) % 16 == 0, "descent bins are read as uint4");
 constexpr int SR_HEAD = (int)((sizeof(Shared) + 15) / 16 * 16);  // the slice begins here
 
@@ -214,8 +218,8 @@ __device__ void sort_desc(u64* v, int n2) {
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
       if (stride >= 32) __syncthreads();
       else __syncwarp();
-      const int i = 2 * t - (t & (stride - 1)), j = i + stride;
-      if (j < n2) {
+      for (int p = t; p < n2 / 2; p += SR_THREADS) {
+        const int i = 2 * p - (p & (stride - 1)), j = i + stride;
         const u64 a = v[i], b = v[j];
         if ((a < b) == ((i & size) == 0)) {
           v[i] = b;
@@ -230,7 +234,7 @@ __device__ void sort_desc(u64* v, int n2) {
 // grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the
 // slice: `per` (4 times an odd number: no bank conflicts) consecutive elements
 // for each thread, padded with -inf
-__global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sample s, int C, int per) {
+__global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sample s, int C, int per) {
   extern __shared__ __align__(16) uint8_t dyn[];
   Shared& sh = *reinterpret_cast<Shared*>(dyn);
   float* xs = reinterpret_cast<float*>(dyn + SR_HEAD);
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
   // rows where only the first maximum can stay
   const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
   const bool need_bins = !top1 && (by_k || by_p || by_m);
-  sh.hist[tid] = make_uint2(0u, 0u);
+  for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.hist[i] = make_uint2(0u, 0u);
   if (tid == 0) sh.again = 0;
 
   // ---- the slice into shared memory, 16-byte loads between its ragged ends;
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
       }
     }
   }
-  if (tid < SR_TABLE) sh.pow2[tid] = exp2(-(double)tid / SR_TABLE);
+  for (int i = tid; i < SR_TABLE; i += SR_THREADS) sh.pow2[i] = exp2(-(double)i / SR_TABLE);
   mx = warp_max(mx);
   mn = -warp_max(-mn);
   if (lane == 0) { sh.red_f[0][warp] = mx; sh.red_f[1][warp] = mn; }
@@ -428,36 +432,57 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
   unsigned kabove = 0;
   u64 all = 0;
   if (need_bins) {
-    // ---- the first histogram over the cluster: thread t has bin t. Masses
-    // are a guess, checked below: sums of 2^-16 units where the bin's weights
-    // are heavy, count * weight at the middle of the bin where they are light
-    unsigned c1 = 0;
-    u64 heavy = 0;
+    // ---- the first histogram over the cluster: a thread has SR_BPT neighbours.
+    // Masses are a guess, checked below: sums of 2^-16 units where the bin's
+    // weights are heavy, count * weight at the middle of the bin where they are light
+    unsigned c1[SR_BPT] = {}, ct, c_in = 0;
+    u64 m1[SR_BPT] = {}, mt, m_in = 0;
 #pragma unroll
     for (int q = 0; q < SR_MAX_CLUSTER; q++)
       if (q < C) {
-        const uint2 v = peer(sh.hist, q, C)[tid];
-        c1 += v.x;
-        heavy += v.y;
+        const uint4 v = *reinterpret_cast<const uint4*>(peer(sh.hist, q, C) + SR_BPT * tid);
+        c1[0] += v.x;
+        m1[0] += v.y;
+        c1[1] += v.z;
+        m1[1] += v.w;
       }
-    const float mid = ex2f(-(float)tid * (span / (float)(SR_BINS - 1)) * c2);
-    const u64 m1 = mid > SR_HEAVY ? heavy << 16 : (u64)((float)c1 * mid * 4294967296.f);
-    u64 mt, m_in = m1;
-    unsigned ct, c_in = c1;
+#pragma unroll
+    for (int b = 0; b < SR_BPT; b++) {
+      const float mid = ex2f(-(float)(SR_BPT * tid + b) * (span / (float)(SR_BINS - 1)) * c2);
+      m1[b] = mid > SR_HEAVY ? m1[b] << 16 : (u64)((float)c1[b] * mid * 4294967296.f);
+      c_in += c1[b];
+      m_in += m1[b];
+    }
     block_scan(sh, m_in, c_in, &mt, &ct);
+    c_in -= c1[0] + c1[1];  // what is above this thread's bins
+    m_in -= m1[0] + m1[1];
     if (tid == 0) { sh.found[0] = sh.found[1] = SR_BINS - 1; sh.found_c = ct; sh.found_m = mt; }
     __syncthreads();
-    if (by_k && c_in - c1 < (unsigned)k && (unsigned)k <= c_in) {
-      sh.found[0] = tid;
-      sh.found_c = c_in - c1;
-      sh.found_m = m_in - m1 + (u64)((float)m1 * ((float)(k - (int)(c_in - c1)) / (float)c1));
+    if (by_k) {
+      unsigned c = c_in;
+      u64 m = m_in;
+#pragma unroll
+      for (int b = 0; b < SR_BPT; b++) {
+        if (c < (unsigned)k && (unsigned)k <= c + c1[b]) {
+          sh.found[0] = SR_BPT * tid + b;
+          sh.found_c = c;
+          sh.found_m = m + (u64)((float)m1[b] * ((float)(k - (int)c) / (float)c1[b]));
+        }
+        c += c1[b];
+        m += m1[b];
+      }
     }
     __syncthreads();
     kbin = sh.found[0];
     kabove = sh.found_c;
     if (by_p) {
       const u64 goal = max((u64)1, (u64)((double)sh.found_m * (double)top_p));
-      if (m_in - m1 < goal && goal <= m_in) sh.found[1] = tid;
+      u64 m = m_in;
+#pragma unroll
+      for (int b = 0; b < SR_BPT; b++) {
+        if (m < goal && goal <= m + m1[b]) sh.found[1] = SR_BPT * tid + b;
+        m += m1[b];
+      }
       __syncthreads();
       pbin = min(kbin, sh.found[1]);
     }
@@ -474,7 +499,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
       }
     }
     __syncthreads();
-    if (tid == last) sh.found_c = last == SR_BINS - 1 ? (unsigned)s.V : c_in;
+    if (tid == last / SR_BPT) sh.found_c = last == SR_BINS - 1 ? (unsigned)s.V : c_in + c1[0] + (last % SR_BPT ? c1[1] : 0u);
     __syncthreads();
     if (sh.found_c <= SR_LIST) {
       // ---- candidates in index order
@@ -499,10 +524,12 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
       });
       if (tid == 0) peer(sh.listed, 0, C)[rank] = hits_t;
       cluster_barrier(C);
-      // ---- rank 0 orders them: a thread gets up to two, with their place in
+      // ---- rank 0 orders them: a thread gets up to SR_EPT, with their place in
       // the order and the exact mass before them
-      u64 f[2] = {0, 0}, o[2] = {0, 0}, before[2] = {0, 0}, inside = 0;
-      int place[2] = {SR_LIST, SR_LIST}, total = 0;
+      u64 f[SR_EPT] = {}, o[SR_EPT] = {}, before[SR_EPT] = {}, inside = 0;
+      int place[SR_EPT], total = 0;
+#pragma unroll
+      for (int j = 0; j < SR_EPT; j++) place[j] = SR_LIST;
       if (rank == 0) {
         for (int q = 0; q < C; q++) {
           const int cnt = (int)sh.listed[q];
@@ -540,18 +567,23 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
           while (n2 < total) n2 <<= 1;
           for (int i = total + tid; i < n2; i += SR_THREADS) sh.list.order[i] = 0;
           sort_desc(sh.list.order, n2);
+          u64 m = 0;
 #pragma unroll
-          for (int j = 0; j < 2; j++)
-            if (2 * tid + j < total) {
-              place[j] = 2 * tid + j;
-              o[j] = sh.list.order[2 * tid + j];
+          for (int j = 0; j < SR_EPT; j++) {
+            const int e = SR_EPT * tid + j;
+            if (e < total) {
+              place[j] = e;
+              o[j] = sh.list.order[e];
               f[j] = weight(of_key((uint32_t)(o[j] >> 32)));
             }
-          u64 m = f[0] + f[1];
+            before[j] = m;
+            m += f[j];
+          }
+          const u64 own_mass = m;
           unsigned zero = 0, zero_t;
           block_scan(sh, m, zero, &inside, &zero_t);
-          before[0] = m - f[0] - f[1];
-          before[1] = m - f[1];
+#pragma unroll
+          for (int j = 0; j < SR_EPT; j++) before[j] += m - own_mass;
         }
       }
       const int nk = by_k ? min(k, total) : total;
@@ -563,7 +595,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
               if (tid == 0) sh.found_m = 0;
               __syncthreads();
 #pragma unroll
-              for (int j = 0; j < 2; j++)
+              for (int j = 0; j < SR_EPT; j++)
                 if (place[j] == nk - 1) sh.found_m = before[j] + f[j];
               __syncthreads();
               lo = hi = share(sh.found_m);
@@ -581,9 +613,9 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
           // kept masses in index order; two ends of the top-p mass must keep the same ones,
           // and a list that ends before them decides nothing
           bool unsure = false, past = false, ended = false;
-          u64 kept[2] = {0, 0};
+          u64 kept[SR_EPT] = {};
 #pragma unroll
-          for (int j = 0; j < 2; j++) {
+          for (int j = 0; j < SR_EPT; j++) {
             if (place[j] < nk && (!by_p || before[j] < lo)) kept[j] = by_m ? weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
             unsure |= by_p && place[j] < nk && before[j] >= lo && before[j] < hi;
             if (by_p && !covers && place[j] == total - 1) {
@@ -595,18 +627,27 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
           const int todo = whole ? SR_WHOLE : doubt ? SR_EXACT : SR_DONE;
           if (todo == SR_DONE) {
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < SR_EPT; j++)
               if (place[j] < total) sh.list.order[0xffffffffu - (uint32_t)o[j]] = kept[j];
             __syncthreads();
-            const u64 f0 = 2 * tid < total ? sh.list.order[2 * tid] : 0;
-            const u64 f1 = 2 * tid + 1 < total ? sh.list.order[2 * tid + 1] : 0;
-            u64 m = f0 + f1, mass;
+            u64 m = 0, mass, fk[SR_EPT];
+#pragma unroll
+            for (int j = 0; j < SR_EPT; j++) {
+              const int e = SR_EPT * tid + j;
+              fk[j] = e < total ? sh.list.order[e] : 0;
+              m += fk[j];
+            }
+            const u64 own_mass = m;
             unsigned zero = 0, zero_t;
             block_scan(sh, m, zero, &mass, &zero_t);
-            const u64 to = draw(mass), b0 = m - f0 - f1, b1 = m - f1;
+            const u64 to = draw(mass);
+            u64 run = m - own_mass;
             int win = -1;
-            if (f0 && b0 < to && to <= b1) win = 2 * tid;
-            if (f1 && b1 < to && to <= m) win = 2 * tid + 1;
+#pragma unroll
+            for (int j = 0; j < SR_EPT; j++) {
+              if (fk[j] && run < to && to <= run + fk[j]) win = SR_EPT * tid + j;
+              run += fk[j];
+            }
             if (win >= 0) {
               int q = 0;
               while (win >= (int)sh.listed[q]) win -= (int)sh.listed[q++];
@@ -643,7 +684,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
   // ---- the cut by descents
   int level = 0;  // descents so far: their buffers alternate
   if (need_bins) {
-    sh.sub[0][tid] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < SR_SUB; i += SR_THREADS) sh.sub[0][i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
   }
   // The cut where the running count (or mass) in descending order reaches
@@ -683,31 +724,41 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const wg_sam
         put(of_key(in.key), in.key, min(in.ties, from + part) - from);
       }
       cluster_barrier(C);
-      // sub-bins in descending order: thread t has SUB - 1 - t
-      const int sb = SR_SUB - 1 - tid;
-      unsigned c = 0;
-      u64 m = 0;
+      // sub-bins in descending order: thread t has SUB - 1 - BPT * t and the next below
+      unsigned c1[SR_BPT] = {}, c = 0, tc;
+      u64 m1[SR_BPT] = {}, m = 0, tm;
 #pragma unroll
       for (int q = 0; q < SR_MAX_CLUSTER; q++)
         if (q < C) {
-          const uint4 v = peer(sub, q, C)[sb];
-          c += v.x;
-          m += (u64)v.y + ((u64)v.z << 15) + ((u64)v.w << 30);
+#pragma unroll
+          for (int b = 0; b < SR_BPT; b++) {
+            const uint4 v = peer(sub, q, C)[SR_SUB - 1 - SR_BPT * tid - b];
+            c1[b] += v.x;
+            m1[b] += (u64)v.y + ((u64)v.z << 15) + ((u64)v.w << 30);
+          }
         }
       level++;
-      sh.sub[level & 1][tid] = make_uint4(0u, 0u, 0u, 0u);  // read last before the barrier above
-      const unsigned c1 = c;
-      const u64 m1 = m;
-      u64 tm;
-      unsigned tc;
+      for (int i = tid; i < SR_SUB; i += SR_THREADS) sh.sub[level & 1][i] = make_uint4(0u, 0u, 0u, 0u);  // read last before the barrier above
+#pragma unroll
+      for (int b = 0; b < SR_BPT; b++) {
+        c += c1[b];
+        m += m1[b];
+      }
+      const unsigned c_own = c;
+      const u64 m_own = m;
       block_scan(sh, m, c, &tm, &tc);
       if (tid == 0) sh.found[0] = -1;
       __syncthreads();
-      const u64 incl = above + (mass ? m : (u64)c), one = mass ? m1 : (u64)c1;
-      if (c1 && incl >= target && incl - one < target) {
-        sh.found[0] = sb;
-        sh.found_m = incl - one;
-        sh.found_c = c1;
+      u64 run = above + (mass ? m - m_own : (u64)(c - c_own));
+#pragma unroll
+      for (int b = 0; b < SR_BPT; b++) {
+        const u64 one = mass ? m1[b] : (u64)c1[b];
+        if (c1[b] && run < target && run + one >= target) {
+          sh.found[0] = SR_SUB - 1 - SR_BPT * tid - b;
+          sh.found_m = run;
+          sh.found_c = c1[b];
+        }
+        run += one;
       }
       __syncthreads();
       const int sel = sh.found[0];
@@ -901,12 +952,11 @@ int init_sample_rows(int device) { return set_attributes(device); }
 
 int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));
-  // CTAs a row: as many as the SMs take in one round (two CTAs each from 4 a
-  // row on), at least two (a row of 51866 fp32 fits no SM), none with less
-  // than 2048 elements (their exchanges cost more than such slices). Measured
-  // at 51866 fp32: one row 25 / 21 / 17 us with 2 / 4 / 8 CTAs, 320 rows 99 /
-  // 106 / 187; 48 rows of f16 34 / 29 / 38.
-  int C = p.R * 8 <= 148 ? 8 : p.R * 4 <= 296 ? 4 : 2;
+  // CTAs a row: 8 while they all fit the SMs, else 4 (two halves of a row of
+  // 51866 fp32 leave one CTA to an SM), none with less than 2048 elements
+  // (their exchanges cost more than such slices). Measured at 51866 fp32: one
+  // row 21 / 16 / 13 us with 2 / 4 / 8 CTAs; 320 rows with a top-k 108 / 74 / 91.
+  int C = p.R * 8 <= 148 ? 8 : 4;
   while (C > 1 && p.V <= 2048 * (C / 2)) C /= 2;
   // elements a thread: 4 times an odd number that covers the slice and its padding
   auto per_of = [&](int c) {

@@ -916,14 +916,13 @@ def _dt(T, t, what: str) -> int:
     return code
 
 
-def _place(what: str, first, *tensors) -> int:
-    """The index of the CUDA device that all tensors share."""
-    dev = first.get_device()
+def _place(what: str, dev: int, *tensors) -> int:
+    """The index `dev` of the CUDA device that all tensors share."""
     if dev < 0:
         raise DecodeError("%s: tensors must be on a CUDA device" % what)
     for t in tensors:
         if t is not None and t.get_device() != dev:
-            raise DecodeError("%s: tensors on different devices (%s, %s)" % (what, first.device, t.device))
+            raise DecodeError("%s: tensors on different devices (cuda:%d, %s)" % (what, dev, t.device))
     return dev
 
 
@@ -938,7 +937,10 @@ def _vec(what: str, name: str, t, dtype, n: int):
 
 def _rows(what: str, name: str, t, heads: int, dim: int):
     """Distance of the rows of a [n, heads, dim] (or [n, heads * dim]) tensor in elements."""
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
+    if t.is_contiguous() and shape[1:] == (heads, dim):
+        return heads * dim
+    stride = t.stride()
     if len(shape) == 3:
         ok = (shape[1] == heads and shape[2] == dim and stride[2] == 1 and (heads == 1 or stride[1] == dim))
     else:
@@ -967,7 +969,7 @@ def kv_plan(lens, new_tokens, page: int, free_pages, cursor, block_table, slots,
     i32, R, n_free, n_slots = T.i32, lens.numel(), free_pages.numel(), slots.numel()
     if cursor_out is None:
         cursor_out = cursor
-    dev = _place(what, lens, new_tokens, free_pages, cursor, cursor_out, block_table, slots, cu_new, status)
+    dev = _place(what, lens.get_device(), new_tokens, free_pages, cursor, cursor_out, block_table, slots, cu_new, status)
     ld, cols = _table(what, T, block_table, R)
     _op_check(T.lib.wg_kv_plan(
         _vec(what, "lens", lens, i32, R), _vec(what, "new_tokens", new_tokens, i32, R), R, page,
@@ -996,6 +998,7 @@ class Kv8Cache:
         self.num_pages, _, self.n_kv_head, self.page, self.head_dim = codes.shape
         self._c = WgKv8(codes.data_ptr(), scales.data_ptr(), self.num_pages, self.page, self.n_kv_head, self.head_dim)
         self._ref = ctypes.byref(self._c)
+        self._dev = codes.get_device()
 
     @classmethod
     def alloc(cls, num_pages: int, page: int, n_kv_head: int, head_dim: int = 64, device="cuda") -> "Kv8Cache":
@@ -1009,7 +1012,7 @@ class Kv8Cache:
         n = slots.numel()
         if len(k) != n or len(v) != n or v.dtype is not k.dtype:
             raise DecodeError("%s: k and v must have a row for each slot and the same type" % what)
-        return _vec(what, "slots", slots, T.i32, n), n, _dt(T, k, what), ldk, ldv, _place(what, self.codes, k, v, slots)
+        return _vec(what, "slots", slots, T.i32, n), n, _dt(T, k, what), ldk, ldv, _place(what, self._dev, k, v, slots)
 
     def append(self, k, v, slots):
         """Writes the rows of k and v ([n, n_kv_head, head_dim]) into their slots (wg_kv8_append)."""
@@ -1042,7 +1045,7 @@ class Kv8Cache:
             out = T.torch.zeros(q.shape, dtype=T.torch.float16 if qdt == 0 else q.dtype, device=q.device)
         if len(out) != n_q:
             raise DecodeError("%s: out must be %s" % (what, tuple(q.shape)))
-        dev = _place(what, self.codes, q, cu_q, kv_lens, block_table, out)
+        dev = _place(what, self._dev, q, cu_q, kv_lens, block_table, out)
         ld, cols = _table(what, T, block_table, R)
         p = WgKv8Attn(q.data_ptr(), _rows(what, "q", q, n_head, D), qdt, n_head, _vec(what, "cu_q", cu_q, T.i32, R + 1),
                       n_q, R, _vec(what, "kv_lens", kv_lens, T.i32, R), block_table.data_ptr(), ld, cols, max_q, max_kv,
@@ -1065,7 +1068,7 @@ def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
         tokens = T.torch.empty(R, dtype=T.i32, device=logits.device)
     if logprobs is None:
         logprobs = T.torch.empty(R, dtype=T.f32, device=logits.device)
-    dev = _place(what, logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
+    dev = _place(what, logits.get_device(), u, temperature, top_k, top_p, min_p, tokens, logprobs)
     f32, i32 = T.f32, T.i32
     p = WgSample(logits.data_ptr(), logits.stride(0) if R > 1 else V, _dt(T, logits, what), R, V,
                  _vec(what, "u", u, f32, R), _vec(what, "temperature", temperature, f32, R),
