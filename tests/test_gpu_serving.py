@@ -86,6 +86,18 @@ def test_plan_that_cannot_be_made(change):
         assert (code > 0) == (change != "pages")
 
 
+def test_plan_page_numbers_without_slots():
+    """A page number that is negative, or whose slots are past 32 bits, goes into the table and gives -1 for its slots."""
+    free = np.array([5, 2 ** 31 - 1, -7, 2 ** 27 - 1, 2 ** 27, 9])
+    st, t, slots, cu, c = run_plan([16 * 6], [16 * 6], 16, free, 0, np.zeros((1, 6), int), 100)
+    assert list(st) == [0, 6] and t[0].tolist() == free.tolist()
+    want = -np.ones(100, np.int64)
+    for i, pg in enumerate(free):
+        if 0 <= pg < 2 ** 27:
+            want[16 * i:16 * i + 16] = pg * 16 + np.arange(16)
+    np.testing.assert_array_equal(slots, want)
+
+
 def test_plan_exactly_full():
     """The last free page, the last slot and the last table column are usable."""
     assert check_plan(np.array([48, 16]), np.array([48, 16]), 16, np.arange(7, 11), 0, np.zeros((2, 3), int), 64) == 0
@@ -394,6 +406,38 @@ def test_sample(V, dt):
     get = lambda n, d: np.array([s.get(n, d) for s in SETTINGS])  # noqa: E731
     for j in range(2):
         check_sample(x, rng.random(R), get("T", 1.0), get("k", 0), get("p", 1.0), get("m", 0.0), dt, ld_pad=3 * j)
+
+
+WIDE = [dict(k=1000), dict(k=1500), dict(k=30000, T=2.0), dict(k=5000, p=0.999, T=1.5), dict(p=0.99, T=2.5),
+        dict(p=0.9, T=5.0, m=1e-4), dict(m=1e-6), dict(m=1e-3, T=4.0), dict(k=1024, m=0.3, T=3.0), dict(p=0.9999999)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", ["normal", "flat", "steps", "far"])
+def test_sample_keeps_many(dt, shape):
+    """Kept sets of thousands: no short list, cuts by descents; flat rows, rows
+    of few distinct values, and rows whose tail lies far below the rest."""
+    V, R = 51865, len(WIDE)
+    rng = np.random.default_rng(len(shape))
+    x = rng.standard_normal((R, V)) * {"normal": 2.5, "flat": 0.05, "steps": 2.0, "far": 1.0}[shape]
+    if shape == "steps":
+        x = np.round(x)
+    if shape == "far":
+        x[:, ::2] -= 200.0
+    get = lambda n, d: np.array([s.get(n, d) for s in WIDE])  # noqa: E731
+    check_sample(x, rng.random(R), get("T", 1.0), get("k", 0), get("p", 1.0), get("m", 0.0), dt)
+
+
+@pytest.mark.parametrize("n", [256, 257, 1023, 1024, 1025])
+def test_sample_lists_of_every_length(n):
+    """Exactly n candidates: ordered by counting, by sorting, and too many for either."""
+    V = 20000
+    rng = np.random.default_rng(n)
+    x = np.full((6, V), -90.0)
+    for r in range(6):
+        x[r, rng.permutation(V)[:n]] = rng.standard_normal(n)
+    check_sample(x, rng.random(6), [1.0] * 6, [0, n, n - 1, 0, 0, 100], [0.95, 1.0, 0.9, 1.0, 0.9999, 0.5],
+                 [0, 0, 0, 1e-9, 1e-9, 0])
 
 
 def test_sample_defaults_and_many_rows():

@@ -22,7 +22,7 @@ int kv8_check(const char* what, const wg_kv8* c) {
     set_error("%s: null cache", what);
     return WG_ERR_INVALID;
   }
-  if (c->num_pages <= 0 || c->n_kv_head <= 0 || !kv_page_ok(c->page) || (c->head_dim != 64 && c->head_dim != 128)) {
+  if (c->num_pages <= 0 || c->n_kv_head <= 0 || c->n_kv_head > 65536 || !kv_page_ok(c->page) || (c->head_dim != 64 && c->head_dim != 128)) {
     set_error("%s: bad cache (%d pages of %d tokens (a power of two, 16 to 128), %d heads of %d (64 or 128))", what,
               c->num_pages, c->page, c->n_kv_head, c->head_dim);
     return WG_ERR_INVALID;
@@ -351,6 +351,8 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_kernel(ReadArgs p) {
   }
 }
 
+constexpr int KV8_MAX_ROWS = 1 << 30;  // tokens of one call
+
 // Checks of a [n, heads, dim] tensor with rows of ld elements; *vec: whether
 // every head of every row starts on 16 bytes.
 int rows_check(const char* what, const char* name, const void* p, int dt, int64_t ld, int64_t width, bool* vec) {
@@ -395,7 +397,7 @@ extern "C" int wg_kv8_append(const wg_kv8* cache, const void* k, const void* v, 
   using namespace wg;
   const char* what = "wg_kv8_append";
   WG_CHECK(kv8_check(what, cache));
-  if (!dt_ok(dtype) || n < 0 || (n > 0 && !slots)) {
+  if (!dt_ok(dtype) || n < 0 || n > KV8_MAX_ROWS || (n > 0 && !slots)) {
     set_error("%s: bad argument (dtype %d, n %d)", what, dtype, n);
     return WG_ERR_INVALID;
   }
@@ -404,10 +406,6 @@ extern "C" int wg_kv8_append(const wg_kv8* cache, const void* k, const void* v, 
   const int64_t width = (int64_t)cache->n_kv_head * cache->head_dim;
   WG_CHECK(rows_check(what, "k", k, dtype, ldk, width, &vk));
   WG_CHECK(rows_check(what, "v", v, dtype, ldv, width, &vv));
-  if (2 * cache->n_kv_head > 65535 * 8) {
-    set_error("%s: too many heads", what);
-    return WG_ERR_INVALID;
-  }
   OpDevice dev;
   WG_CHECK(dev.enter(what, device));
   const Kv8Rows rows{k, v, ldk, ldv, cache->head_dim, 0, n, dtype, vk, vv};
@@ -419,7 +417,7 @@ extern "C" int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, voi
   using namespace wg;
   const char* what = "wg_kv8_read";
   WG_CHECK(kv8_check(what, cache));
-  if (!dt_ok(dtype) || n < 0 || (n > 0 && !slots)) {
+  if (!dt_ok(dtype) || n < 0 || n > KV8_MAX_ROWS || (n > 0 && !slots)) {
     set_error("%s: bad argument (dtype %d, n %d)", what, dtype, n);
     return WG_ERR_INVALID;
   }

@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p) {
         const int pos = base_sh[lo] + (i - beg), col = pos >> p.shift;
         const int id = col < held_sh[lo] ? p.table[(int64_t)(r0 + lo) * p.ldt + col]
                                          : p.free_pages[off_sh[lo] + col - held_sh[lo]];
-        out[k] = id < 0 ? -1 : (int)(((unsigned)id << p.shift) | (unsigned)(pos & (page - 1)));
+        // a page number that is none, or whose slots are past 32 bits, has none
+        out[k] = id < 0 || id > (0x7fffffff >> p.shift) ? -1 : (id << p.shift) | (pos & (page - 1));
       }
       if (vec && i0 >= first && i0 + 4 <= last) {
         *reinterpret_cast<int4*>(p.slots + i0) = make_int4(out[0], out[1], out[2], out[3]);
