@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
   constexpr int NT = D / 8;      // n-tiles of P.V
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-  const int tile = unit % p.tiles, h = (unit / p.tiles) % p.H, r = unit / p.tiles / p.H;
+  const int tile = 0, h = unit / p.R, r = unit % p.R;
   const int page = 1 << p.shift;
   int q0 = __ldg(p.cu_q + r);
   int nq = __ldg(p.cu_q + r + 1) - q0;
@@ -682,7 +682,7 @@ int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cuda
   at[1].val.clusterDim.y = 1;
   at[1].val.clusterDim.z = 1;
   cfg.attrs = pdl_enabled() ? at : at + 1;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (a.splits > 1 ? 1 : 0);
   return launch_check(cudaLaunchKernelEx(&cfg, k, a), "kv8_attention");
 }
 

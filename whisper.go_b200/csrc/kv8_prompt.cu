@@ -411,7 +411,7 @@ int launch_kv8_prompt(Kv8AttnArgs a, int head_dim, int64_t max_kv, cudaStream_t 
   at[1].val.clusterDim.y = 1;
   at[1].val.clusterDim.z = 1;
   cfg.attrs = pdl_enabled() ? at : at + 1;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (a.splits > 1 ? 1 : 0);
   return launch_check(cudaLaunchKernelEx(&cfg, pick(head_dim, 1 << a.shift), a), "kv8_prompt");
 }
 

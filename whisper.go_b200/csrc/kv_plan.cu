@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PlanArgs p) {
   __syncthreads();
   code = code_sh;
   if (p.barrier) cluster_sync();  // every CTA has read the cursor: it may be advanced in place
+  else __syncthreads();           // (one CTA: every thread has)
   if (rank == 0 && tid == 0) {
     p.status[0] = code;
     p.status[1] = code ? 0 : (int)total.b;
@@ -222,7 +223,7 @@ extern "C" int wg_kv_plan(const int32_t* lens, const int32_t* new_tokens, int R,
   const int64_t work = (int64_t)n_slots + R;
   int C = 1;
   while (C < PLAN_CTAS && (int64_t)C * PLAN_THREADS * 4 < work) C *= 2;
-  const bool cluster = C <= PLAN_CLUSTER, apart = cursor_out != cursor;
+  const bool cluster = C > 1 && C <= PLAN_CLUSTER, apart = C == 1 || cursor_out != cursor;
   PlanArgs a{lens, new_tokens, R, log2_of(page), free_pages, n_free, cursor, cursor_out, block_table, ld_table,
              max_pages, slots, n_slots, cu_new, status, cluster, cluster || apart};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -232,13 +233,13 @@ extern "C" int wg_kv_plan(const int32_t* lens, const int32_t* new_tokens, int R,
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster ? C : 1;
+  at[0].val.clusterDim.x = C;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.attrs = cluster ? at : at + 1;
+  cfg.numAttrs = (cluster ? 1 : 0) + (pdl_enabled() ? 1 : 0);
   WG_CHECK(launch_check(cudaLaunchKernelEx(&cfg, plan_kernel, a), "kv_plan"));
   if (a.advance) return WG_OK;
   return launch_check(launch_k(plan_cursor_kernel, dim3(1), dim3(1), 0, st, cursor, cursor_out, (const int*)status),

@@ -61,11 +61,6 @@ constexpr double SR_STEP = -0.69314718055994530942 / SR_TABLE;  // ln of a table
 constexpr float SR_OCTAVES = 46.5f;       // weights below 2^-46.5 are 0 in those units
 constexpr int SR_MAX_V = 1 << 18;
 constexpr int SR_PAD = 8;                 // a slice may start up to 7 elements into its 16 bytes
-// Bound on the relative error of a row's fp32 sum: ex2.approx 2^-22, three
-// roundings of its argument (3 * 2^-24 ln 2 of it, whose mean over the mass is
-// at most log2 V = 18: 2^-18.8), partial sums of at most 32 weights and the
-// adds that join them (2^-18.5).
-constexpr double SR_SUM_ERR = 1.0 / 131072;
 enum { SR_DONE = 0, SR_EXACT = 1, SR_WHOLE = 2 };  // what rank 0 still needs: nothing, the exact mass, the whole row
 typedef unsigned long long u64;
 
@@ -604,10 +599,17 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
               for (int q = 0; q < C; q++) all += sh.all[q];
               lo = hi = share(all);
             } else {
-              double z = 0.0;
-              for (int q = 0; q < C; q++) z += (double)sh.sum[q];
-              lo = share((u64)(z * (1.0 - SR_SUM_ERR) * 35184372088832.0));  // 2^45
-              hi = share((u64)(z * (1.0 + SR_SUM_ERR) * 35184372088832.0) + 1);
+              // the fp32 sum z of the weights 2^-y is within this of the real one,
+              // relatively: ex2.approx 2^-22; three roundings of y, each 2^-24 of it,
+              // and the mean of y over the mass is at most log2 V - log2 z (an
+              // entropy); per / 4 adds to a partial sum and at most 16 that join them
+              float z = 0.f;
+              for (int q = 0; q < C; q++) z += sh.sum[q];
+              const float ulp = 1.f / 16777216.f;
+              const double err = 4.f * ulp + 2.1f * ulp * fmaxf(0.f, log2f((float)s.V) + 0.01f - log2f(z)) +
+                                 (float)(per / 4 + 16) * ulp;
+              lo = share((u64)((double)z * (1.0 - err) * 35184372088832.0));  // 2^45
+              hi = share((u64)((double)z * (1.0 + err) * 35184372088832.0) + 1);
             }
           }
           // kept masses in index order; two ends of the top-p mass must keep the same ones,
@@ -980,7 +982,7 @@ int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
   at[1].val.clusterDim.y = 1;
   at[1].val.clusterDim.z = 1;
   cfg.attrs = pdl_enabled() ? at : at + 1;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (C > 1 ? 1 : 0);
   return launch_check(cudaLaunchKernelEx(&cfg, sample_rows_kernel, p, C, per), "sample_rows");
 }
 
