@@ -11,7 +11,11 @@
 // every new maximum. The price is a step of at most twice the finest one.
 //
 // Both are streams bounded by memory: K and V come in once (2 or 4 bytes a
-// value) and go out as one byte, or the reverse.
+// value) and go out as one byte, or the reverse. Measured on 96000 tokens of 20
+// heads of 64 in f16 (737 MB each way): append 161 us = 4.6 TB/s, 70 % of the
+// measured copy rate (16 warps an SM, each holding 8 KB while it looks for the
+// largest magnitude); read 137 us = 5.4 TB/s, 82 %. Small calls (64 tokens)
+// are launches: 6.5 us each with the host's part.
 #include "kernels.cuh"
 #include "ops.cuh"
 

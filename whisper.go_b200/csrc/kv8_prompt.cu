@@ -9,9 +9,13 @@
 // last visible token of the tile are never read. Few tiles over many tokens
 // are split over a cluster and joined through distributed shared memory.
 //
-// What bounds it is the MMA itself (one m16n8k16 per ~8.5 cycles and SM
-// quarter, measured), then shared-memory reads: 32 ldmatrix.x4 feed 64 MMAs
-// per chunk and warp at 64-wide heads.
+// The bound would be the MMA (one m16n8k16 per ~9 cycles and SM quarter,
+// measured) and the shared-memory reads that feed it (32 ldmatrix.x4 for 64
+// MMAs per chunk and warp at 64-wide heads). At prompts of a text context it is
+// latency: a tile has 1 to 7 chunks, and as much again goes into its start (the
+// request, its pages, the codes, Q) and its end. Measured: 16 ragged prompts of
+// up to 448 tokens, 20 heads, bf16: 37.5 us (61 us on 16-row tiles), 83 TFLOP/s
+// with the tensor pipe 24 % busy; 4 CTAs an SM against 3: 38 / 42 us.
 #include <cooperative_groups.h>
 
 #include "kv8_attn.cuh"
