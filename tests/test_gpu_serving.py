@@ -487,6 +487,22 @@ def test_sample_masked_rows():
                  [0, 0, 0, 0, 0.1, 0, 0.5, 0, 0, 0])
 
 
+@pytest.mark.parametrize("gap", [4.0, 9.0, 15.0, 19.0])
+def test_sample_logprob_of_a_nearly_certain_token(gap):
+    """log-prob = -log(1 + rest): the rest of the row is summed apart from the
+    maximum, so its digits stay: every weight exp(-gap - d) is within
+    2^-22 + 3 * 2^-24 * (its octaves, at most 60) and the sum's adds within 2^-18."""
+    V = 30000
+    rng = np.random.default_rng(int(gap))
+    x = (rng.standard_normal((2, V)) - gap - np.log(V)).astype(np.float32)
+    x[:, 77] = 0.0
+    x[1, 78] = 0.0
+    tok, lp = wgdec.sample_rows(torch.tensor(x, device=DEV), torch.tensor([0.5, 0.25], device=DEV))
+    for r in range(2):
+        _, want = ref.sample(x[r].astype(np.float64), 0.5 if r == 0 else 0.25)
+        assert int(tok[r]) == 77 and abs(float(lp[r]) - want) <= abs(want) * (2.0 ** -22 + 180 * 2.0 ** -24 + 2.0 ** -18)
+
+
 def test_sample_distribution():
     """Drawn frequencies follow the kept weights: 40,000 stratified draws of
     one row, so each token's count is within 1 of its share."""

@@ -36,8 +36,8 @@
 // whole row would cost as much again, so top-p asks for them only where bounds
 // on the fp32 sum do not settle the cut (3 % of such rows), and with eleven
 // operations each. Measured (a pass): one row of 51865 fp32 15 us (24 where
-// descents are needed), 48 of 51864 f16 30 us, 320 of 51866 fp32 90 us =
-// 0.74 TB/s. One CTA a row, streaming the row from L2 in every pass, was no
+// descents are needed), 48 of 51864 f16 32 us, 320 of 51866 fp32 95 us =
+// 0.70 TB/s. One CTA a row, streaming the row from L2 in every pass, was no
 // faster at 320 rows (top-k 81 us against 80) and 53 us at one.
 #include <cooperative_groups.h>
 
@@ -89,7 +89,8 @@ struct Shared {
   // per rank, pushed by every rank to every rank before a cluster barrier (a
   // remote store costs its sender nothing, a remote load is ~0.3 us of waiting)
   float mx[SR_MAX_CLUSTER], mn[SR_MAX_CLUSTER];
-  float sum[SR_MAX_CLUSTER];                       // fp32 sum of the slice's weights
+  float sum[SR_MAX_CLUSTER];                       // fp32 sum of the slice's weights below 1
+  unsigned ones[SR_MAX_CLUSTER];                   // and how many are 1 (the maxima)
   int first[SR_MAX_CLUSTER];                       // lowest index of the slice that holds the maximum
   u64 all[SR_MAX_CLUSTER], over[SR_MAX_CLUSTER];   // exact sums of the slice: whole, and above the likely bins
   u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
@@ -347,13 +348,24 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   // ---- fp32 sum of the weights, first maximum, histogram of counts
   const float t1 = fminf(fmaxf(T > 0.f ? T : 1.f, 1e-30f), 1e30f);
   const float c2 = 1.4426950408889634f / t1;
+  // log 2 of a weight: the product with 1 / (T ln 2) in two floats, so that its
+  // rounding does not lean every weight the same way
+  const float c2_lo = (float)(1.4426950408889634 / (double)t1 - (double)c2);
+  const float deep = -200.f / c2;  // 2^-200 is 0 as well, and the products stay finite
+  auto octaves = [&](float x) {
+    const float d = fmaxf(x - mx, deep);
+    return fmaf(d, c2, d * c2_lo);
+  };
   const float span = fminf(fmaxf(mx - mn, 1e-30f), SR_SPAN);
   const float bin_scale = (float)(SR_BINS - 1) / span;
   // nearest bin, the last one for everything further down (2^23 + b holds b in its low bits)
   auto bin_bits = [&](float x) { return fminf((mx - x) * bin_scale, (float)(SR_BINS - 1)) + 8388608.f; };
   auto bin_of = [&](float x) { return __float_as_int(bin_bits(x)) & (SR_BINS - 1); };
   {
+    // the maxima are counted, not summed: a row that is nearly certain keeps the
+    // digits of what the other tokens share
     float part[4] = {0.f, 0.f, 0.f, 0.f};
+    unsigned ones = 0;
     int first = 0x7fffffff;
     if (need_bins) {
       each([&](const float (&x)[4], int) {
@@ -361,9 +373,10 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
         int b[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          e[j] = ex2f((x[j] - mx) * c2);
+          e[j] = ex2f(octaves(x[j]));
           b[j] = bin_of(x[j]);
-          part[j] += e[j];
+          if (e[j] < 1.f) part[j] += e[j];
+          else ones++;
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -375,20 +388,25 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
       each([&](const float (&x)[4], int i) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          part[j] += ex2f((x[j] - mx) * c2);
+          const float e = ex2f(octaves(x[j]));
+          if (e < 1.f) part[j] += e;
+          else ones++;
           if (top1 && x[j] == mx) first = min(first, first_i + i + j);
         }
       });
     }
     float sum = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
     first = __reduce_min_sync(0xffffffffu, first);
-    if (lane == 0) { sh.red_f[0][warp] = sum; sh.red_c[warp] = (unsigned)first; }
+    ones = __reduce_add_sync(0xffffffffu, ones);
+    if (lane == 0) { sh.red_f[0][warp] = sum; sh.red_c[warp] = (unsigned)first; sh.red_m[warp] = ones; }
     __syncthreads();
     if (warp == 0) {
       sum = warp_sum(lane < SR_WARPS ? sh.red_f[0][lane] : 0.f);
       first = __reduce_min_sync(0xffffffffu, (int)sh.red_c[lane % SR_WARPS]);
+      ones = __reduce_add_sync(0xffffffffu, lane < SR_WARPS ? (unsigned)sh.red_m[lane] : 0u);
       if (lane < C) {
         peer(sh.sum, lane, C)[rank] = sum;
+        peer(sh.ones, lane, C)[rank] = ones;
         peer(sh.first, lane, C)[rank] = first;
       }
     }
@@ -402,8 +420,12 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
     s.tokens[r] = token;
     if (s.logprobs) {
       float z = 0.f;
-      for (int q = 0; q < C; q++) z += sh.sum[q];
-      s.logprobs[r] = (x - mx) / t1 - logf(z);
+      unsigned n1 = 0;
+      for (int q = 0; q < C; q++) {
+        z += sh.sum[q];
+        n1 += sh.ones[q];
+      }
+      s.logprobs[r] = (x - mx) / t1 - (logf((float)n1) + log1pf(z / (float)n1));
     }
   };
   // first running mass above u * mass
@@ -609,12 +631,12 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
               // the fp32 sum z of the weights 2^-y is within this of the real one,
               // relatively: ex2.approx 2^-22; three roundings of y, each 2^-24 of it,
               // and the mean of y over the mass is at most log2 V - log2 z (an
-              // entropy); per / 4 adds to a partial sum and at most 16 that join them
+              // entropy); per / 4 adds to a partial sum and at most 20 that join them
               float z = 0.f;
-              for (int q = 0; q < C; q++) z += sh.sum[q];
+              for (int q = 0; q < C; q++) z += sh.sum[q] + (float)sh.ones[q];
               const float ulp = 1.f / 16777216.f;
               const double err = 4.f * ulp + 2.1f * ulp * fmaxf(0.f, log2f((float)s.V) + 0.01f - log2f(z)) +
-                                 (float)(per / 4 + 16) * ulp;
+                                 (float)(per / 4 + 20) * ulp;
               lo = share((u64)((double)z * (1.0 - err) * 35184372088832.0));  // 2^45
               hi = share((u64)((double)z * (1.0 + err) * 35184372088832.0) + 1);
             }
