@@ -200,6 +200,33 @@ def test_append_token_by_token_grows_the_scale():
     assert (np.abs(host(vo) + host(k)) <= step[1][None, :, None]).all()
 
 
+@pytest.mark.parametrize("H,n_seq,page", [(9, 420, 32), (20, 280, 128)])
+def test_append_large_equals_its_parts(H, n_seq, page):
+    """A long call gives each CTA more tokens and more heads than a short one:
+    the same sequences appended a few at a time give the same bits."""
+    rng = np.random.default_rng(H + page)
+    lens = rng.integers(1, 200, n_seq)
+    first = np.concatenate([[0], np.cumsum(-(-lens // page))])
+    order = rng.permutation(first[-1])  # pages anywhere
+    slots, starts = [], []
+    for r, n in enumerate(lens):
+        starts.append(len(slots))
+        t = np.arange(n)
+        slots += list(order[first[r] + t // page] * page + t % page) + [-1] * (r % 3)
+    starts.append(len(slots))
+    n, D = len(slots), 64
+    k, v = (torch.tensor(rng.standard_normal((n, H, D), dtype=np.float32), device=DEV).half() for _ in range(2))
+    codes, scales = torch.zeros(len(order), 2, H, page, D, dtype=torch.int8, device=DEV), torch.zeros(len(order), 2, H, device=DEV)
+    whole, parts = wgdec.Kv8Cache(codes, scales), wgdec.Kv8Cache(codes.clone(), scales.clone())
+    at = i32(slots)
+    whole.append(k, v, at)
+    for r in range(0, n_seq, 5):
+        a, b = starts[r], starts[min(r + 5, n_seq)]
+        parts.append(k[a:b], v[a:b], at[a:b])
+    assert torch.equal(whole.scales, parts.scales) and torch.equal(whole.codes, parts.codes)
+    assert (whole.scales != 0).all()
+
+
 # ---- wg_kv8_attention -------------------------------------------------------------
 EPS = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 

@@ -12,7 +12,7 @@
 //
 // Both are streams bounded by memory: K and V come in once (2 or 4 bytes a
 // value) and go out as one byte, or the reverse. Measured on 96000 tokens of 20
-// heads of 64 in f16 (737 MB each way): append 161 us = 4.6 TB/s, 70 % of the
+// heads of 64 in f16 (737 MB each way): append 150 us = 4.9 TB/s, 75 % of the
 // measured copy rate (16 warps an SM, each holding 8 KB while it looks for the
 // largest magnitude); read 137 us = 5.4 TB/s, 82 %. Small calls (64 tokens)
 // are launches: 6.5 us each with the host's part.
@@ -122,7 +122,7 @@ struct AppendArgs {
   int dt;
   bool veck, vecv;
   const int* slots;
-  int n, chunk, units;  // tokens, tokens per CTA, (K|V, head) pairs
+  int n, chunk, units, group;  // tokens, tokens per CTA, (K|V, head) pairs, pairs per CTA
 };
 
 constexpr int APPEND_WARPS = 8;
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(AppendArgs p)
   }
   __syncthreads();
   const int runs = runs_sh;
-  const int u0 = blockIdx.y * APPEND_WARPS, nu = min(APPEND_WARPS, p.units - u0);
+  const int u0 = blockIdx.y * p.group, nu = min(p.group, p.units - u0);
   const int per_tok = p.D / EPL;         // lanes that a token takes
   const int tok_step = 32 / per_tok;     // tokens a warp takes at once
   const int sub = lane / per_tok, d = (lane % per_tok) * EPL;
@@ -382,12 +382,18 @@ int rows_check(const char* what, const char* name, const void* p, int dt, int64_
 int launch_kv8_append(const wg_kv8& c, const Kv8Rows& r, const int32_t* slots, int n, cudaStream_t st) {
   const int dt = r.dtype;
   AppendArgs a{c.codes, c.scales, c.num_pages * c.page, log2_of(c.page), c.n_kv_head, c.head_dim, r.k, r.v, r.ldk, r.ldv,
-               r.head_step, r.batch_step, r.batch, dt, r.veck, r.vecv, slots, n, 1, 2 * c.n_kv_head};
+               r.head_step, r.batch_step, r.batch, dt, r.veck, r.vecv, slots, n, 1, 2 * c.n_kv_head, APPEND_WARPS};
   // tokens a CTA looks through: few, so that short calls spread over the SMs
   // (every token may begin a run of its own), up to 64 where that leaves
   // enough CTAs
-  const int gy = (a.units + APPEND_WARPS - 1) / APPEND_WARPS;
-  while (a.chunk < APPEND_CHUNK && (int64_t)(n / (2 * a.chunk)) * gy >= 148 * 4) a.chunk *= 2;
+  const int per8 = (a.units + APPEND_WARPS - 1) / APPEND_WARPS;
+  while (a.chunk < APPEND_CHUNK && (int64_t)(n / (2 * a.chunk)) * per8 >= 148 * 4) a.chunk *= 2;
+  // two pairs a warp where that still leaves waves of CTAs: the search for the
+  // runs is shared (96000 tokens 162 -> 150 us; 3800 tokens 11.4 -> 12.3 us,
+  // so not there)
+  const int per16 = (a.units + 2 * APPEND_WARPS - 1) / (2 * APPEND_WARPS);
+  if (a.chunk == APPEND_CHUNK && (int64_t)(n / a.chunk) * per16 >= 148 * 8) a.group = 2 * APPEND_WARPS;
+  const int gy = (a.units + a.group - 1) / a.group;
   const dim3 grid((n + a.chunk - 1) / a.chunk, gy), block(APPEND_WARPS * 32);
   return launch_check(dt == WG_DT_F32 ? launch_k(append_kernel<4>, grid, block, 0, st, a)
                                       : launch_k(append_kernel<2>, grid, block, 0, st, a),
