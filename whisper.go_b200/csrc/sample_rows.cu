@@ -59,7 +59,6 @@ constexpr int SR_BINS = SR_BPT * SR_THREADS;  // of the first histogram
 constexpr int SR_SUB = SR_BPT * SR_THREADS;   // of a descent (9 bits)
 constexpr int SR_EPT = 4;                 // candidates a thread
 constexpr int SR_LIST = SR_EPT * SR_THREADS;  // that rank 0 can finish alone
-constexpr int SR_COUNT = 256;             // so many or fewer are ordered by counting instead of sorting
 constexpr int SR_MAX_CLUSTER = 8;
 constexpr int SR_TABLE = 256;
 constexpr float SR_SPAN = 40.f;           // logits that far below the maximum share the last bin
@@ -95,16 +94,14 @@ struct Shared {
   u64 all[SR_MAX_CLUSTER], over[SR_MAX_CLUSTER];   // exact sums of the slice: whole, and above the likely bins
   u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
   unsigned ties[SR_MAX_CLUSTER];                   // elements equal to the cut
-  unsigned listed[SR_MAX_CLUSTER];                 // candidates of the slice
   int again;                                       // from rank 0: SR_DONE, SR_EXACT or SR_WHOLE
   // read by peers after a cluster barrier
   alignas(16) uint2 hist[SR_BINS];                 // count, mass of the heavy ones (2^-16 units)
   union alignas(16) {
     uint4 sub[2][SR_SUB];  // descents: count, mass in three 15-bit digits (summed in 32 bits: for < 2^17 elements)
     struct {
-      float x[SR_LIST];    // candidates of the slice in index order
-      int i[SR_LIST];
-      u64 order[SR_LIST];  // rank 0: all candidates to order, then their kept masses in index order
+      int2 xi[SR_LIST];    // rank 0: the row's candidates in index order, pushed by every rank (logit, index)
+      u64 order[SR_LIST];  // the same to order, then their kept masses in index order
     } list;
     struct {
       u64 mass[SR_THREADS];       // kept mass of each thread's elements
@@ -121,9 +118,10 @@ struct Shared {
   unsigned found_c;
 };
 static_assert(SR_BPT == 2 && offsetof(Shared, hist) % 16 == 0, "a thread's bins are one uint4");
-static_assert(SR_COUNT <= SR_THREADS, "one candidate a thread");
 static_assert(offsetof(Shared, sub) % 16 == 0, "descent bins are read as uint4");
 constexpr int SR_HEAD = (int)((sizeof(Shared) + 15) / 16 * 16);  // the slice begins here
+constexpr int SR_SMEM_MAX = 227 * 1024;
+static_assert(SR_SMEM_MAX / (16 * SR_THREADS) <= 64, "a thread's groups of four are bits of one word");
 
 // The weight of a logit: the definition's 64-bit value by argument reduction.
 // With y = 256 (max - x) / (T ln 2) = n + r, n the nearest integer,
@@ -210,28 +208,6 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ void cluster_barrier(int C) {
   if (C > 1) cg::this_cluster().sync();
   else __syncthreads();
-}
-
-// Descending bitonic sort of n2 (a power of two, at most SR_LIST) values.
-// Strides up to 32 stay inside the 64 values of a warp's pairs.
-__device__ void sort_desc(u64* v, int n2) {
-  const int t = threadIdx.x;
-  __syncthreads();  // the values are in place
-  for (int size = 2; size <= n2; size <<= 1) {
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      if (stride >= 32) __syncthreads();
-      else __syncwarp();
-      for (int p = t; p < n2 / 2; p += SR_THREADS) {
-        const int i = 2 * p - (p & (stride - 1)), j = i + stride;
-        const u64 a = v[i], b = v[j];
-        if ((a < b) == ((i & size) == 0)) {
-          v[i] = b;
-          v[j] = a;
-        }
-      }
-    }
-  }
-  __syncthreads();
 }
 
 // grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the
@@ -459,12 +435,16 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
     // ---- the first histogram over the cluster: a thread has SR_BPT neighbours.
     // Masses are a guess, checked below: sums of 2^-16 units where the bin's
     // weights are heavy, count * weight at the middle of the bin where they are light
-    unsigned c1[SR_BPT] = {}, ct, c_in = 0;
+    unsigned c1[SR_BPT] = {}, lower[SR_BPT] = {}, ct, c_in = 0;  // lower: of the ranks before this one
     u64 m1[SR_BPT] = {}, mt, m_in = 0;
 #pragma unroll
     for (int q = 0; q < SR_MAX_CLUSTER; q++)
       if (q < C) {
         const uint4 v = *reinterpret_cast<const uint4*>(peer(sh.hist, q, C) + SR_BPT * tid);
+        if (q == rank) {
+          lower[0] = c1[0];
+          lower[1] = c1[1];
+        }
         c1[0] += v.x;
         m1[0] += v.y;
         c1[1] += v.z;
@@ -526,90 +506,86 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
     if (tid == last / SR_BPT) sh.found_c = last == SR_BINS - 1 ? (unsigned)s.V : c_in + c1[0] + (last % SR_BPT ? c1[1] : 0u);
     __syncthreads();
     if (sh.found_c <= SR_LIST) {
-      // ---- candidates in index order
+      // ---- candidates in index order, to rank 0: behind those of the ranks
+      // before, whose number the histograms tell (the last bin is not counted
+      // there, but rows so short have one rank)
       const float edge = 8388608.f + (float)last;
       auto candidate = [&](float x) { return bin_bits(x) <= edge && x > -INFINITY; };
       unsigned hits = 0, hits_t;
-      u64 none = 0, none_t;
-      each([&](const float (&x)[4], int) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) hits += candidate(x[j]);
-      });
-      const unsigned own = hits;
-      block_scan(sh, none, hits, &none_t, &hits_t);
-      unsigned at = hits - own;
-      if (own) each([&](const float (&x)[4], int i) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (candidate(x[j])) {
-            sh.list.x[at] = x[j];
-            sh.list.i[at++] = first_i + i + j;
-          }
-      });
-      if (tid == 0) peer(sh.listed, 0, C)[rank] = hits_t;
-      cluster_barrier(C);
-      // ---- rank 0 orders them: a thread gets up to SR_EPT, with their place in
-      // the order and the exact mass before them
-      u64 f[SR_EPT] = {}, o[SR_EPT] = {}, before[SR_EPT] = {}, inside = 0;
-      int place[SR_EPT], total = 0;
-#pragma unroll
-      for (int j = 0; j < SR_EPT; j++) place[j] = SR_LIST;
-      if (rank == 0) {
-        for (int q = 0; q < C; q++) {
-          const int cnt = (int)sh.listed[q];
-          const float* from = peer(sh.list.x, q, C);
-          for (int i = tid; i < cnt; i += SR_THREADS)
-            sh.list.order[total + i] = ((u64)key_of(from[i]) << 32) | (0xffffffffu - (unsigned)(total + i));
-          total += cnt;
-        }
-        if (total <= SR_COUNT) {
-          __syncthreads();
-          ulonglong2* both = reinterpret_cast<ulonglong2*>(sh.list.order);  // (order, mass)
-          u64 v = 0, fv = 0;
-          if (tid < total) {
-            v = sh.list.order[tid];
-            fv = weight(of_key((uint32_t)(v >> 32)));
-          }
-          __syncthreads();
-          if (tid < total) both[tid] = make_ulonglong2(v, fv);
-          __syncthreads();
-          if (tid < total) {
-            int ahead = 0;
-            u64 mass = 0;
-#pragma unroll 4
-            for (int j = 0; j < total; j++) {
-              const ulonglong2 w = both[j];
-              if (w.x > v) { ahead++; mass += w.y; }
-            }
-            o[0] = v;
-            f[0] = fv;
-            before[0] = mass;
-            place[0] = ahead;
-          }
-        } else {
-          int n2 = 2 * SR_COUNT;
-          while (n2 < total) n2 <<= 1;
-          for (int i = total + tid; i < n2; i += SR_THREADS) sh.list.order[i] = 0;
-          sort_desc(sh.list.order, n2);
-          u64 m = 0;
-#pragma unroll
-          for (int j = 0; j < SR_EPT; j++) {
-            const int e = SR_EPT * tid + j;
-            if (e < total) {
-              place[j] = e;
-              o[j] = sh.list.order[e];
-              f[j] = weight(of_key((uint32_t)(o[j] >> 32)));
-            }
-            before[j] = m;
-            m += f[j];
-          }
-          const u64 own_mass = m;
-          unsigned zero = 0, zero_t;
-          block_scan(sh, m, zero, &inside, &zero_t);
-#pragma unroll
-          for (int j = 0; j < SR_EPT; j++) before[j] += m - own_mass;
+      u64 base = (SR_BPT * tid <= last ? lower[0] : 0) + (SR_BPT * tid + 1 <= last ? lower[1] : 0), base_t;
+      u64 fours = 0;  // the groups of four that hold any: the bins fall with the logit, so the largest tells
+      for (int i = 0; i < per / 4; i++) {
+        const float4 v = mine[i];
+        if (candidate(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)))) {
+          fours |= 1ull << i;
+          hits += candidate(v.x) + candidate(v.y) + candidate(v.z) + candidate(v.w);
         }
       }
+      const unsigned own = hits;
+      block_scan(sh, base, hits, &base_t, &hits_t);
+      const int total = last == SR_BINS - 1 ? (int)hits_t : (int)sh.found_c;
+      int2* to = peer(sh.list.xi, 0, C) + (int)base_t + hits - own;
+      for (; fours; fours &= fours - 1) {
+        const int i = __ffsll((long long)fours) - 1;
+        const float4 v = mine[i];
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (candidate(x[j])) *to++ = make_int2(__float_as_int(x[j]), first_i + 4 * i + j);
+      }
+      cluster_barrier(C);
+      const bool alone = !by_p || by_k;  // rank 0 needs nothing more of its peers
+      if (alone && rank) return;
+      // ---- rank 0 orders them: into their bins, whose beginnings the histogram
+      // tells, then by counting inside a bin (a few elements; all of them when
+      // they are equal). Thread t gets places each * t and on, with the exact mass before them
+      u64 f[SR_EPT] = {}, o[SR_EPT] = {}, before[SR_EPT] = {};
+      const int each_t = (total + SR_THREADS - 1) / SR_THREADS;
+      if (rank == 0) {
+        unsigned* begin = reinterpret_cast<unsigned*>(sh.hist);  // read last before the barrier above
+        begin[SR_BPT * tid] = c_in;
+        begin[SR_BPT * tid + 1] = c_in + c1[0];
+        __syncthreads();
+        for (int i = tid; i < total; i += SR_THREADS) {
+          const float x = __int_as_float(sh.list.xi[i].x);
+          sh.list.order[atomicAdd(&begin[bin_of(x)], 1u)] = ((u64)key_of(x) << 32) | (0xffffffffu - (unsigned)i);
+        }
+        __syncthreads();  // a bin begins where the one before it ended
+        int at[SR_EPT];
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++) {
+          const int e = tid + j * SR_THREADS;
+          if (e >= total) continue;
+          o[j] = sh.list.order[e];
+          const int b = bin_of(of_key((uint32_t)(o[j] >> 32)));
+          const int from = b ? (int)begin[b - 1] : 0, end = (int)begin[b];
+          at[j] = from;
+          for (int i = from; i < end; i++) at[j] += sh.list.order[i] > o[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++)
+          if (tid + j * SR_THREADS < total) sh.list.order[at[j]] = o[j];
+        __syncthreads();
+        u64 m = 0, mt;
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++) {
+          const int e = each_t * tid + j;
+          o[j] = 0;
+          if (j < each_t && e < total) {
+            o[j] = sh.list.order[e];
+            f[j] = weight(of_key((uint32_t)(o[j] >> 32)));
+          }
+          before[j] = m;
+          m += f[j];
+        }
+        const u64 own_mass = m;
+        unsigned zero = 0, zero_t;
+        block_scan(sh, m, zero, &mt, &zero_t);
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++) before[j] += m - own_mass;
+      }
+      auto place = [&](int j) { return j < each_t ? min(each_t * tid + j, SR_LIST) : SR_LIST; };
       const int nk = by_k ? min(k, total) : total;
       for (int pass = 0;; pass++) {  // at most two: the second with the row's exact mass
         if (rank == 0) {
@@ -620,7 +596,7 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
               __syncthreads();
 #pragma unroll
               for (int j = 0; j < SR_EPT; j++)
-                if (place[j] == nk - 1) sh.found_m = before[j] + f[j];
+                if (place(j) == nk - 1) sh.found_m = before[j] + f[j];
               __syncthreads();
               lo = hi = share(sh.found_m);
             } else if (pass) {
@@ -647,9 +623,9 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
           u64 kept[SR_EPT] = {};
 #pragma unroll
           for (int j = 0; j < SR_EPT; j++) {
-            if (place[j] < nk && (!by_p || before[j] < lo)) kept[j] = by_m ? weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
-            unsure |= by_p && place[j] < nk && before[j] >= lo && before[j] < hi;
-            if (by_p && !covers && place[j] == total - 1) {
+            if (place(j) < nk && (!by_p || before[j] < lo)) kept[j] = by_m ? weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
+            unsure |= by_p && place(j) < nk && before[j] >= lo && before[j] < hi;
+            if (by_p && !covers && place(j) == total - 1) {
               ended = before[j] + f[j] < hi;
               past = before[j] + f[j] < lo;
             }
@@ -659,13 +635,12 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
           if (todo == SR_DONE) {
 #pragma unroll
             for (int j = 0; j < SR_EPT; j++)
-              if (place[j] < total) sh.list.order[0xffffffffu - (uint32_t)o[j]] = kept[j];
+              if (place(j) < total) sh.list.order[0xffffffffu - (uint32_t)o[j]] = kept[j];
             __syncthreads();
             u64 m = 0, mass, fk[SR_EPT];
 #pragma unroll
             for (int j = 0; j < SR_EPT; j++) {
-              const int e = SR_EPT * tid + j;
-              fk[j] = e < total ? sh.list.order[e] : 0;
+              fk[j] = place(j) < total ? sh.list.order[place(j)] : 0;
               m += fk[j];
             }
             const u64 own_mass = m;
@@ -676,19 +651,16 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
             int win = -1;
 #pragma unroll
             for (int j = 0; j < SR_EPT; j++) {
-              if (fk[j] && run < to && to <= run + fk[j]) win = SR_EPT * tid + j;
+              if (fk[j] && run < to && to <= run + fk[j]) win = place(j);
               run += fk[j];
             }
-            if (win >= 0) {
-              int q = 0;
-              while (win >= (int)sh.listed[q]) win -= (int)sh.listed[q++];
-              finish(peer(sh.list.i, q, C)[win], peer(sh.list.x, q, C)[win]);
-            }
+            if (win >= 0) finish(sh.list.xi[win].y, __int_as_float(sh.list.xi[win].x));
           } else if (tid < C) {
             peer(&sh, tid, C)->again = todo;
           }
         }
-        cluster_barrier(C);  // rank 0 has read its peers, and told them what it needs
+        if (alone) return;
+        cluster_barrier(C);  // rank 0 has told its peers what it needs
         const int todo = sh.again;
         if (todo == SR_DONE) return;
         if (todo == SR_WHOLE) break;
@@ -963,8 +935,6 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
 
 std::mutex g_attr_mu;
 bool g_attr_done[OPS_MAX_DEV];
-constexpr int SR_SMEM_MAX = 227 * 1024;
-
 int set_attributes(int device) {
   if (device < 0 || device >= OPS_MAX_DEV) {
     set_error("wg_sample_rows: device %d out of range", device);
