@@ -530,6 +530,44 @@ def test_sample_logprob_of_a_nearly_certain_token(gap):
         assert int(tok[r]) == 77 and abs(float(lp[r]) - want) <= abs(want) * (2.0 ** -22 + 180 * 2.0 ** -24 + 2.0 ** -18)
 
 
+@pytest.mark.parametrize("V,C", [(300, 1.5), (3001, 2.5), (51865, 2.5), (51865, 0.1)])
+def test_sample_at_the_edges_of_elements(V, C):
+    """Rows without filters, numbers as near to a running mass as fp32 has
+    them: beside every edge the 64-bit sums decide. The exact units (2^-45 of
+    the largest weight) are off by less than V 2^-46 <= 2^-30 of a row's mass;
+    numbers nearer than 2^-29 to an edge are not used."""
+    R = 96
+    rng = np.random.default_rng(V)
+    x = (rng.standard_normal(V) * C).astype(np.float32)
+    cum = np.cumsum(np.exp(x.astype(np.float64) - x.max()))
+    edge = cum / cum[-1]
+    u, want = [], []
+    for j in rng.integers(0, V - 1, 4 * R):
+        for step in (-1, 0, 1, 20, -20):  # ulps off the edge's fp32 value
+            v = np.float32(edge[j]) * np.float32(1 + step * 2.0 ** -23)
+            i = int(np.searchsorted(edge, float(v), side="right"))
+            near = min(abs(edge[q] - float(v)) for q in (max(0, i - 1), min(i, V - 1)))
+            if v < 1 and near > 2.0 ** -29:
+                u.append(v)
+                want.append(i)
+    u, want = u[:R], want[:R]
+    assert len(u) == R
+    lg = torch.tensor(x, device=DEV).expand(R, V).contiguous()
+    tok, _ = wgdec.sample_rows(lg, torch.tensor(np.array(u), device=DEV))
+    np.testing.assert_array_equal(host(tok), want)
+
+
+@pytest.mark.parametrize("n", [300, 1000])
+def test_sample_list_in_one_bin(n):
+    """Candidates that share a histogram bin, equal or an ulp apart."""
+    V = 9000
+    rng = np.random.default_rng(n)
+    x = np.full((4, V), -60.0)
+    for r in range(4):
+        x[r, rng.permutation(V)[:n]] = 5.0 + (np.arange(n) % (r + 1)) * 2.0 ** -10
+    check_sample(x, rng.random(4), [1.0] * 4, [n // 2, 0, 0, n // 3], [1.0, 0.6, 0.9, 0.5], [0, 0, 0, 0])
+
+
 def test_sample_distribution():
     """Drawn frequencies follow the kept weights: 40,000 stratified draws of
     one row, so each token's count is within 1 of its share."""

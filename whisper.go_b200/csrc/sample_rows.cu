@@ -13,31 +13,36 @@
 //
 // A cluster of C CTAs takes a row; each holds its slice in shared memory as
 // fp32, so the row is read from memory once and every later pass is over
-// shared memory. Nothing is sorted but a short list:
+// shared memory. Nothing is ordered but a short list:
 //  1. a histogram of counts over SR_BINS equal steps of the logit below the
 //     maximum (one shared atomic an element) gives the bin of the top-k cut,
 //     and with the masses of the heavy elements and count * exp(middle) for
 //     the light bins the likely bin of the top-p cut;
 //  2. where the bins that can be kept hold at most SR_LIST elements (as a
 //     rule: a nucleus, a top-k, a min-p set), those go to rank 0 in index
-//     order, which sorts them and finishes alone. Of the rest of the row only
-//     the exact mass is needed, and only by top-p without top-k;
+//     order, which puts them into their bins, orders each bin by counting
+//     (320 rows: nucleus 111 -> 102 us against a sort of the list, k 200 80 ->
+//     70) and finishes alone. Its peers leave then, except under top-p without
+//     top-k, which may need the exact mass of the rest of the row (k 50 84 ->
+//     66 us, with the lists pushed rather than fetched);
 //  3. else the cut is pinned by descents over the order-preserving bit
 //     patterns of the logits, 9 bits a pass, with exact counts and masses, and
 //     the draw walks cluster rank -> thread -> element over the kept masses of
-//     each thread's consecutive elements. Rows without filters go straight to
-//     that walk. Where the likely bin of a top-p cut was wrong the exact sums
-//     say so and the descent covers the whole row.
+//     each thread's consecutive elements. Where the likely bin of a top-p cut
+//     was wrong the exact sums say so and the descent covers the whole row;
+//  4. rows without filters are walked over their fp32 weights first, and over
+//     exact ones only where the number falls too near an element's edge for
+//     the bounds on those.
 //
 // What bounds it: latency. Of a row's ~15 us the load is 1.5, the exchanges of
 // the cluster (maxima, histogram, list) ~4, rank 0's ordering and draw ~3; the
-// SMs hold 111 rows of 51866 at once (three CTAs of 75 KB each), and rank 0's
-// end leaves its peers waiting (most stalls are barriers). 64-bit weights of a
+// SMs hold 111 rows of 51866 at once (three CTAs of 75 KB each), and most
+// stalls are barriers. 64-bit weights of a
 // whole row would cost as much again, so top-p asks for them only where bounds
 // on the fp32 sum do not settle the cut (3 % of such rows), and with eleven
 // operations each. Measured (a pass): one row of 51865 fp32 15 us (24 where
-// descents are needed), 48 of 51864 f16 32 us, 320 of 51866 fp32 95 us =
-// 0.70 TB/s. One CTA a row, streaming the row from L2 in every pass, was no
+// descents are needed), 48 of 51864 f16 24 us, 320 of 51866 fp32 84 us =
+// 0.79 TB/s. One CTA a row, streaming the row from L2 in every pass, was no
 // faster at 320 rows (top-k 81 us against 80) and 53 us at one.
 #include <cooperative_groups.h>
 
@@ -94,6 +99,8 @@ struct Shared {
   u64 all[SR_MAX_CLUSTER], over[SR_MAX_CLUSTER];   // exact sums of the slice: whole, and above the likely bins
   u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
   unsigned ties[SR_MAX_CLUSTER];                   // elements equal to the cut
+  double total[SR_MAX_CLUSTER];                    // the slice's fp32 weights, threads' sums added in 64 bits
+  int drawn;                                       // a rank has drawn the row's token
   int again;                                       // from rank 0: SR_DONE, SR_EXACT or SR_WHOLE
   // read by peers after a cluster barrier
   alignas(16) uint2 hist[SR_BINS];                 // count, mass of the heavy ones (2^-16 units)
@@ -232,7 +239,7 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
   const bool need_bins = !top1 && (by_k || by_p || by_m);
   for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.hist[i] = make_uint2(0u, 0u);
-  if (tid == 0) sh.again = 0;
+  if (tid == 0) sh.again = sh.drawn = 0;
 
   // ---- the slice into shared memory, 16-byte loads between its ragged ends;
   // it starts at the address's place in 16 bytes, so both sides are aligned
@@ -337,6 +344,7 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   // nearest bin, the last one for everything further down (2^23 + b holds b in its low bits)
   auto bin_bits = [&](float x) { return fminf((mx - x) * bin_scale, (float)(SR_BINS - 1)) + 8388608.f; };
   auto bin_of = [&](float x) { return __float_as_int(bin_bits(x)) & (SR_BINS - 1); };
+  double own = 0;  // this thread's weights
   {
     // the maxima are counted, not summed: a row that is nearly certain keeps the
     // digits of what the other tokens share
@@ -371,6 +379,7 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
         }
       });
     }
+    own = ((double)part[0] + part[1]) + ((double)part[2] + part[3]) + ones;
     float sum = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
     first = __reduce_min_sync(0xffffffffu, first);
     ones = __reduce_add_sync(0xffffffffu, ones);
@@ -404,10 +413,10 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
       s.logprobs[r] = (x - mx) / t1 - (logf((float)n1) + log1pf(z / (float)n1));
     }
   };
+  float u = s.u[r];
+  if (!(u >= 0.f)) u = 0.f;
   // first running mass above u * mass
   auto draw = [&](u64 mass) {
-    float u = s.u[r];
-    if (!(u >= 0.f)) u = 0.f;
     const double at = (double)u * (double)mass;
     const u64 goal = at < (double)mass ? (u64)at + 1 : mass;
     return goal > mass ? mass : goal;
@@ -418,7 +427,34 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
     const u64 goal = want >= 1.0 ? (u64)want : 1;
     return goal > mass ? mass : goal;
   };
-  if (top1 || need_bins) cluster_barrier(C);
+  // The fp32 weights 2^-y, and any sum of them, are off by at most this share of
+  // their whole sum z: ex2.approx 2^-22; three roundings of y, each 2^-24 of it,
+  // and the mean of y over the mass is at most log2 V - log2 z (an entropy);
+  // `adds` additions in fp32; 2^-24 for what the exact units round off (V * 2^-46)
+  auto off_by = [&](float z, int adds) {
+    return (5.f + 2.1f * fmaxf(0.f, log2f((float)s.V) + 0.01f - log2f(z)) + (float)adds) * (1.f / 16777216.f);
+  };
+  double pre = own;  // this thread's place in the slice's mass
+  if (!top1 && !need_bins) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, pre, d);
+      if (lane >= d) pre += v;
+    }
+    __syncthreads();  // red_m has been read
+    if (lane == 31) sh.red_m[warp] = (u64)__double_as_longlong(pre);
+    __syncthreads();
+    pre -= own;
+    double tot = 0;
+#pragma unroll
+    for (int w = 0; w < SR_WARPS; w++) {
+      const double v = __longlong_as_double((long long)sh.red_m[w]);
+      if (w < warp) pre += v;
+      tot += v;
+    }
+    if (tid < C) peer(sh.total, tid, C)[rank] = tot;
+  }
+  cluster_barrier(C);
   if (top1) {
     if (rank == 0 && tid == 0) {
       int f = 0x7fffffff;
@@ -426,6 +462,44 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
       finish(f, mx);
     }
     return;
+  }
+
+  if (!need_bins) {
+    // ---- the whole row is kept: the element that the number falls into by the
+    // fp32 weights is the right one where it lies further inside than these can
+    // be off, the sum before it and its place in the sum both
+    double z = 0, base = 0;
+    for (int q = 0; q < C; q++) {
+      if (q == rank) base = z;
+      z += sh.total[q];
+    }
+    const double at = (double)u * z, margin = 2.0 * (double)off_by((float)z, per / 4 + 2) * z;
+    const double b = base + pre;
+    const unsigned claim = __ballot_sync(0xffffffffu, at >= b && at < b + own);
+    if (claim) {
+      const int owner = __ffs(claim) - 1;
+      double run = __shfl_sync(0xffffffffu, b, owner);
+      const float* ox = xs + (warp * 32 + owner) * per;
+      for (int i0 = 0; i0 < per; i0 += 32) {
+        const int i = i0 + lane;
+        const float x = i < per ? ox[i] : -INFINITY;
+        const double e = ex2f(octaves(x));
+        double upto = e;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += v;
+        }
+        upto += run;
+        if (at - (upto - e) > margin && upto - at > margin) {
+          finish(c0 - lead + (warp * 32 + owner) * per + i, x);
+          for (int q = 0; q < C; q++) peer(&sh, q, C)->drawn = 1;
+        }
+        run = __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    cluster_barrier(C);
+    if (sh.drawn) return;
   }
 
   int kbin = SR_BINS - 1, pbin = 0;
@@ -604,15 +678,9 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
               for (int q = 0; q < C; q++) all += sh.all[q];
               lo = hi = share(all);
             } else {
-              // the fp32 sum z of the weights 2^-y is within this of the real one,
-              // relatively: ex2.approx 2^-22; three roundings of y, each 2^-24 of it,
-              // and the mean of y over the mass is at most log2 V - log2 z (an
-              // entropy); per / 4 adds to a partial sum and at most 20 that join them
               float z = 0.f;
               for (int q = 0; q < C; q++) z += sh.sum[q] + (float)sh.ones[q];
-              const float ulp = 1.f / 16777216.f;
-              const double err = 4.f * ulp + 2.1f * ulp * fmaxf(0.f, log2f((float)s.V) + 0.01f - log2f(z)) +
-                                 (float)(per / 4 + 20) * ulp;
+              const double err = off_by(z, per / 4 + 20);  // 20 join the partial sums
               lo = share((u64)((double)z * (1.0 - err) * 35184372088832.0));  // 2^45
               hi = share((u64)((double)z * (1.0 + err) * 35184372088832.0) + 1);
             }
