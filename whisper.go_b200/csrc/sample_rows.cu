@@ -93,13 +93,12 @@ struct Shared {
   // per rank, pushed by every rank to every rank before a cluster barrier (a
   // remote store costs its sender nothing, a remote load is ~0.3 us of waiting)
   float mx[SR_MAX_CLUSTER], mn[SR_MAX_CLUSTER];
-  float sum[SR_MAX_CLUSTER];                       // fp32 sum of the slice's weights below 1
+  double sum[SR_MAX_CLUSTER];                      // the slice's fp32 weights below 1, threads' sums added in 64 bits
   unsigned ones[SR_MAX_CLUSTER];                   // and how many are 1 (the maxima)
   int first[SR_MAX_CLUSTER];                       // lowest index of the slice that holds the maximum
   u64 all[SR_MAX_CLUSTER], over[SR_MAX_CLUSTER];   // exact sums of the slice: whole, and above the likely bins
   u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
   unsigned ties[SR_MAX_CLUSTER];                   // elements equal to the cut
-  double total[SR_MAX_CLUSTER];                    // the slice's fp32 weights, threads' sums added in 64 bits
   int drawn;                                       // a rank has drawn the row's token
   int again;                                       // from rank 0: SR_DONE, SR_EXACT or SR_WHOLE
   // read by peers after a cluster barrier
@@ -379,14 +378,18 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
         }
       });
     }
-    own = ((double)part[0] + part[1]) + ((double)part[2] + part[3]) + ones;
-    float sum = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
+    double sum = ((double)part[0] + part[1]) + ((double)part[2] + part[3]);
+    own = sum + ones;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     first = __reduce_min_sync(0xffffffffu, first);
     ones = __reduce_add_sync(0xffffffffu, ones);
-    if (lane == 0) { sh.red_f[0][warp] = sum; sh.red_c[warp] = (unsigned)first; sh.red_m[warp] = ones; }
+    if (lane == 0) { sh.red_o[warp] = (u64)__double_as_longlong(sum); sh.red_c[warp] = (unsigned)first; sh.red_m[warp] = ones; }
     __syncthreads();
     if (warp == 0) {
-      sum = warp_sum(lane < SR_WARPS ? sh.red_f[0][lane] : 0.f);
+      sum = __longlong_as_double((long long)sh.red_o[lane % SR_WARPS]);
+#pragma unroll
+      for (int d = SR_WARPS / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       first = __reduce_min_sync(0xffffffffu, (int)sh.red_c[lane % SR_WARPS]);
       ones = __reduce_add_sync(0xffffffffu, lane < SR_WARPS ? (unsigned)sh.red_m[lane] : 0u);
       if (lane < C) {
@@ -404,13 +407,13 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   auto finish = [&](int token, float x) {
     s.tokens[r] = token;
     if (s.logprobs) {
-      float z = 0.f;
+      double z = 0;
       unsigned n1 = 0;
       for (int q = 0; q < C; q++) {
         z += sh.sum[q];
         n1 += sh.ones[q];
       }
-      s.logprobs[r] = (x - mx) / t1 - (logf((float)n1) + log1pf(z / (float)n1));
+      s.logprobs[r] = (x - mx) / t1 - (logf((float)n1) + log1pf((float)z / (float)n1));
     }
   };
   float u = s.u[r];
@@ -430,9 +433,9 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   // The fp32 weights 2^-y, and any sum of them, are off by at most this share of
   // their whole sum z: ex2.approx 2^-22; three roundings of y, each 2^-24 of it,
   // and the mean of y over the mass is at most log2 V - log2 z (an entropy);
-  // `adds` additions in fp32; 2^-24 for what the exact units round off (V * 2^-46)
-  auto off_by = [&](float z, int adds) {
-    return (5.f + 2.1f * fmaxf(0.f, log2f((float)s.V) + 0.01f - log2f(z)) + (float)adds) * (1.f / 16777216.f);
+  // per / 4 additions in fp32; 2^-24 for what the exact units round off (V * 2^-46)
+  auto off_by = [&](float z) {
+    return (6.f + 2.1f * fmaxf(0.f, log2f((float)s.V) + 0.01f - log2f(z)) + (float)(per / 4)) * (1.f / 16777216.f);
   };
   double pre = own;  // this thread's place in the slice's mass
   if (!top1 && !need_bins) {
@@ -445,14 +448,9 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
     if (lane == 31) sh.red_m[warp] = (u64)__double_as_longlong(pre);
     __syncthreads();
     pre -= own;
-    double tot = 0;
 #pragma unroll
-    for (int w = 0; w < SR_WARPS; w++) {
-      const double v = __longlong_as_double((long long)sh.red_m[w]);
-      if (w < warp) pre += v;
-      tot += v;
-    }
-    if (tid < C) peer(sh.total, tid, C)[rank] = tot;
+    for (int w = 0; w < SR_WARPS; w++)
+      if (w < warp) pre += __longlong_as_double((long long)sh.red_m[w]);
   }
   cluster_barrier(C);
   if (top1) {
@@ -471,9 +469,9 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
     double z = 0, base = 0;
     for (int q = 0; q < C; q++) {
       if (q == rank) base = z;
-      z += sh.total[q];
+      z += sh.sum[q] + sh.ones[q];
     }
-    const double at = (double)u * z, margin = 2.0 * (double)off_by((float)z, per / 4 + 2) * z;
+    const double at = (double)u * z, margin = 2.0 * (double)off_by((float)z) * z;
     const double b = base + pre;
     const unsigned claim = __ballot_sync(0xffffffffu, at >= b && at < b + own);
     if (claim) {
@@ -678,11 +676,11 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
               for (int q = 0; q < C; q++) all += sh.all[q];
               lo = hi = share(all);
             } else {
-              float z = 0.f;
-              for (int q = 0; q < C; q++) z += sh.sum[q] + (float)sh.ones[q];
-              const double err = off_by(z, per / 4 + 20);  // 20 join the partial sums
-              lo = share((u64)((double)z * (1.0 - err) * 35184372088832.0));  // 2^45
-              hi = share((u64)((double)z * (1.0 + err) * 35184372088832.0) + 1);
+              double z = 0;
+              for (int q = 0; q < C; q++) z += sh.sum[q] + sh.ones[q];
+              const double err = off_by((float)z);
+              lo = share((u64)(z * (1.0 - err) * 35184372088832.0));  // 2^45
+              hi = share((u64)(z * (1.0 + err) * 35184372088832.0) + 1);
             }
           }
           // kept masses in index order; two ends of the top-p mass must keep the same ones,
