@@ -100,6 +100,9 @@ struct Shared {
   u64 kept[SR_MAX_CLUSTER];                        // kept mass without ties
   unsigned ties[SR_MAX_CLUSTER];                   // elements equal to the cut
   int drawn;                                       // a rank has drawn the row's token
+  unsigned listed;                                 // at rank 0: elements of the cut's bins
+  uint32_t cut_key;                                // from rank 0: the cut that their order gives, where cut_ties > 0
+  unsigned cut_ties;
   int again;                                       // from rank 0: SR_DONE, SR_EXACT or SR_WHOLE
   // read by peers after a cluster barrier
   alignas(16) uint2 hist[SR_BINS];                 // count, mass of the heavy ones (2^-16 units)
@@ -238,7 +241,10 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
   const bool need_bins = !top1 && (by_k || by_p || by_m);
   for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.hist[i] = make_uint2(0u, 0u);
-  if (tid == 0) sh.again = sh.drawn = 0;
+  if (tid == 0) {
+    sh.again = sh.drawn = 0;
+    sh.listed = sh.cut_ties = 0;
+  }
 
   // ---- the slice into shared memory, 16-byte loads between its ragged ends;
   // it starts at the address's place in 16 bytes, so both sides are aligned
@@ -751,11 +757,106 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   }
 
   // ---- the cut by descents
-  int level = 0;  // descents so far: their buffers alternate
-  if (need_bins) {
-    for (int i = tid; i < SR_SUB; i += SR_THREADS) sh.sub[0][i] = make_uint4(0u, 0u, 0u, 0u);
+  // By a list, once a row: the elements of bins ba..bb go to rank 0 in any order.
+  auto inside = [&](float x, int ba, int bb) {
+    const int b = bin_of(x);
+    return b >= ba && b <= bb && x > -INFINITY;
+  };
+  auto push_bins = [&](int ba, int bb, u64 fours, unsigned hits) {
+    const unsigned own_hits = hits;
+    unsigned hits_t;
+    u64 none = 0, none_t;
+    block_scan(sh, none, hits, &none_t, &hits_t);
+    if (tid == 0) sh.found[0] = (int)atomicAdd(peer(&sh.listed, 0, C), hits_t);
     __syncthreads();
-  }
+    unsigned at = (unsigned)sh.found[0] + hits - own_hits;
+    u64* to = peer(sh.list.order, 0, C);
+    for (; fours; fours &= fours - 1) {
+      const int i = __ffsll((long long)fours) - 1;
+      const float4 v = mine[i];
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (inside(x[j], ba, bb)) {
+          if (at < SR_LIST) to[at] = ((u64)key_of(x[j]) << 32) | (0xffffffffu - (unsigned)(first_i + 4 * i + j));
+          at++;
+        }
+    }
+  };
+  // Rank 0 orders them (SR_BINS parts of their bins, then by counting inside a
+  // part) and tells the element where the running count (or mass) reaches
+  // `target`. False where it does not, or where there are more than SR_LIST.
+  // A cluster barrier lies between the pushes and this.
+  auto cut_of_list = [&](bool mass, u64 target, int ba, int bb, u64 above, Cut* out) -> bool {
+    const int total = (int)sh.listed;
+    if (rank == 0 && total <= SR_LIST) {
+      const float fine = (float)SR_BINS / (float)(bb - ba + 1);
+      auto part_of = [&](u64 v) {  // falls with the logit
+        const float at = ((mx - of_key((uint32_t)(v >> 32))) * bin_scale - ((float)ba - 0.5f)) * fine;
+        return (int)fminf(fmaxf(at, 0.f), (float)(SR_BINS - 1));
+      };
+      unsigned* begin = reinterpret_cast<unsigned*>(sh.hist);  // read last before the barrier above
+      u64* by_part = reinterpret_cast<u64*>(sh.list.xi);
+      begin[SR_BPT * tid] = begin[SR_BPT * tid + 1] = 0;
+      __syncthreads();
+      for (int i = tid; i < total; i += SR_THREADS) atomicAdd(&begin[part_of(sh.list.order[i])], 1u);
+      __syncthreads();
+      const unsigned n0 = begin[SR_BPT * tid], n1 = begin[SR_BPT * tid + 1];
+      unsigned c = n0 + n1, tc;
+      u64 m = 0, tm;
+      block_scan(sh, m, c, &tm, &tc);
+      begin[SR_BPT * tid] = c - n0 - n1;
+      begin[SR_BPT * tid + 1] = c - n1;
+      __syncthreads();
+      for (int i = tid; i < total; i += SR_THREADS) {
+        const u64 v = sh.list.order[i];
+        by_part[atomicAdd(&begin[part_of(v)], 1u)] = v;
+      }
+      __syncthreads();  // a part begins where the one before it ended
+      for (int e = tid; e < total; e += SR_THREADS) {
+        const u64 v = by_part[e];
+        const int b = part_of(v), from = b ? (int)begin[b - 1] : 0, end = (int)begin[b];
+        int at = from;
+        for (int i = from; i < end; i++) at += by_part[i] > v;
+        sh.list.order[at] = v;
+      }
+      __syncthreads();
+      const int each_t = (total + SR_THREADS - 1) / SR_THREADS, e0 = each_t * tid;
+      u64 f[SR_EPT] = {};
+#pragma unroll
+      for (int j = 0; j < SR_EPT; j++) {
+        if (j < each_t && e0 + j < total) f[j] = mass ? weight(of_key((uint32_t)(sh.list.order[e0 + j] >> 32))) : 1;
+        m += f[j];
+      }
+      const u64 own_mass = m;
+      block_scan(sh, m, c, &tm, &tc);
+      u64 run = above + m - own_mass;
+#pragma unroll
+      for (int j = 0; j < SR_EPT; j++) {
+        if (f[j] && run < target && target <= run + f[j]) {
+          const int e = e0 + j;
+          const uint32_t key = (uint32_t)(sh.list.order[e] >> 32);
+          unsigned ties = 1;
+          while ((int)ties <= e && (uint32_t)(sh.list.order[e - ties] >> 32) == key) ties++;
+          for (int q = 0; q < C; q++) {
+            peer(&sh, q, C)->cut_key = key;
+            peer(&sh, q, C)->cut_ties = ties;
+          }
+        }
+        run += f[j];
+      }
+    }
+    cluster_barrier(C);
+    if (!sh.cut_ties) return false;
+    out->key = sh.cut_key;
+    out->ties = sh.cut_ties;
+    return true;
+  };
+  int level = 0;  // descents so far: their buffers alternate
+  auto clear = [&]() {
+    for (int i = tid; i < SR_SUB; i += SR_THREADS) sh.sub[level & 1][i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+  };
   // The cut where the running count (or mass) in descending order reaches
   // `target`, known to lie in bins ba..bb, above which there are `above`;
   // among the elements inside `in`. False where it does not lie there.
@@ -849,22 +950,41 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   Cut cut{0u, 0u};
   if (by_k) {
     const Cut every{0u, 0u};
-    if (!descend(every, false, (u64)k, kbin, kbin, kabove, &cut))
-      descend(every, false, (u64)k, 0, SR_BINS - 1, 0, &cut);
+    u64 fours = 0;
+    unsigned hits = 0;
+    for (int i = 0; i < per / 4; i++) {
+      const float4 v = mine[i];
+      const int h = inside(v.x, kbin, kbin) + inside(v.y, kbin, kbin) + inside(v.z, kbin, kbin) + inside(v.w, kbin, kbin);
+      if (h) fours |= 1ull << i;
+      hits += h;
+    }
+    push_bins(kbin, kbin, fours, hits);
+    cluster_barrier(C);
+    if (!cut_of_list(false, (u64)k, kbin, kbin, kabove, &cut)) {
+      clear();
+      if (!descend(every, false, (u64)k, kbin, kbin, kabove, &cut))
+        descend(every, false, (u64)k, 0, SR_BINS - 1, 0, &cut);
+    }
   }
   if (by_p) {
-    // exact masses: of the top-k, and of what lies above the likely bins
+    // exact masses: of the top-k, and of what lies above the likely bins; the list in the same pass
     const int ba = max(0, pbin - 1), bb = min(SR_BINS - 1, pbin + 1);
-    u64 over = 0;
+    u64 over = 0, fours = 0;
+    unsigned hits = 0;
     all = 0;
-    each([&](const float (&x)[4], int) {
+    each([&](const float (&x)[4], int i) {
+      int h = 0;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const u64 f = key_of(x[j]) > cut.key ? weight(x[j]) : 0;
         all += f;
         over += bin_of(x[j]) < ba ? f : 0;
+        h += inside(x[j], ba, bb);
       }
+      if (h) fours |= 1ull << (i / 4);
+      hits += h;
     });
+    if (!by_k) push_bins(ba, bb, fours, hits);
     all = warp_sum64(all);
     over = warp_sum64(over);
     __syncthreads();  // red_m has been read
@@ -892,8 +1012,11 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
     }
     const u64 goal = share(all);
     const Cut in = cut;
-    if (over >= goal || !descend(in, true, goal, ba, bb, over, &cut))
-      descend(in, true, goal, 0, SR_BINS - 1, 0, &cut);  // the guess was wrong: over the whole row
+    if (by_k || !cut_of_list(true, goal, ba, bb, over, &cut)) {
+      clear();
+      if (over >= goal || !descend(in, true, goal, ba, bb, over, &cut))
+        descend(in, true, goal, 0, SR_BINS - 1, 0, &cut);  // the guess was wrong: over the whole row
+    }
   }
 
   // ---- the kept mass of every thread's elements
