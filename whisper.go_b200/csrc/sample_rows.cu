@@ -25,25 +25,29 @@
 //     70) and finishes alone. Its peers leave then, except under top-p without
 //     top-k, which may need the exact mass of the rest of the row (k 50 84 ->
 //     66 us, with the lists pushed rather than fetched);
-//  3. else the cut is pinned by descents over the order-preserving bit
-//     patterns of the logits, 9 bits a pass, with exact counts and masses, and
-//     the draw walks cluster rank -> thread -> element over the kept masses of
-//     each thread's consecutive elements. Where the likely bin of a top-p cut
-//     was wrong the exact sums say so and the descent covers the whole row;
+//  3. else the few bins that hold the cut go to rank 0, which orders them and
+//     reads the cut off their running counts or exact masses (such rows 27 us
+//     alone, 38 to 47 with descents); where those bins hold too many, under
+//     both top-k and top-p, or where the likely bin was wrong, it is pinned by
+//     descents over the order-preserving bit patterns of the logits, 9 bits a
+//     pass, with exact counts and masses. The draw then walks cluster rank ->
+//     thread -> element over the kept masses of each thread's consecutive
+//     elements;
 //  4. rows without filters are walked over their fp32 weights first, and over
 //     exact ones only where the number falls too near an element's edge for
-//     the bounds on those.
+//     the bounds on those (320 such rows 81 -> 58 us).
 //
 // What bounds it: latency. Of a row's ~15 us the load is 1.5, the exchanges of
 // the cluster (maxima, histogram, list) ~4, rank 0's ordering and draw ~3; the
 // SMs hold 111 rows of 51866 at once (three CTAs of 75 KB each), and most
-// stalls are barriers. 64-bit weights of a
-// whole row would cost as much again, so top-p asks for them only where bounds
-// on the fp32 sum do not settle the cut (3 % of such rows), and with eleven
-// operations each. Measured (a pass): one row of 51865 fp32 15 us (24 where
-// descents are needed), 48 of 51864 f16 24 us, 320 of 51866 fp32 84 us =
-// 0.79 TB/s. One CTA a row, streaming the row from L2 in every pass, was no
-// faster at 320 rows (top-k 81 us against 80) and 53 us at one.
+// stalls are barriers. 64-bit weights of a whole row would cost as much again,
+// so top-p asks for them only where bounds on the fp32 sum do not settle the cut
+// (3 % of such rows), and with eleven operations each. Measured (a pass): one
+// row of 51865 fp32 15 us (24 where no short list holds the kept set), 48 of
+// 51864 f16 24 us, 320 of 51866 fp32 75 us = 0.88 TB/s; 61 us with a top-k in
+// the place of the nucleus rows, of which two in 54 have no short list and may
+// come last. One CTA a row, streaming the row from L2 in every pass: top-k 81 us
+// at 320 rows against 67, 53 at one row against 14.
 #include <cooperative_groups.h>
 
 #include <cstddef>
@@ -130,6 +134,17 @@ static_assert(SR_BPT == 2 && offsetof(Shared, hist) % 16 == 0, "a thread's bins 
 static_assert(offsetof(Shared, sub) % 16 == 0, "descent bins are read as uint4");
 constexpr int SR_HEAD = (int)((sizeof(Shared) + 15) / 16 * 16);  // the slice begins here
 constexpr int SR_SMEM_MAX = 227 * 1024;
+
+// Asked for anew where they are used: a pointer that went through memory would
+// be a generic one, and its accesses too.
+__device__ __forceinline__ Shared& shared_part() {
+  extern __shared__ __align__(16) uint8_t dyn[];
+  return *reinterpret_cast<Shared*>(dyn);
+}
+__device__ __forceinline__ float* shared_slice() {
+  extern __shared__ __align__(16) uint8_t dyn[];
+  return reinterpret_cast<float*>(dyn + SR_HEAD);
+}
 static_assert(SR_SMEM_MAX / (16 * SR_THREADS) <= 64, "a thread's groups of four are bits of one word");
 
 // The weight of a logit: the definition's 64-bit value by argument reduction.
@@ -138,7 +153,6 @@ static_assert(SR_SMEM_MAX / (16 * SR_THREADS) <= 64, "a thread's groups of four 
 // table, and a Taylor series (|r ln 2 / 256| <= 0.00136: four terms leave 4e-17).
 struct Weigh {
   double mx, c;  // c = 256 / (T ln 2)
-  const double* pow2;
   // w = v * 2^-oct
   __device__ __forceinline__ double value(float x, int* oct) const {
     const double magic = 6755399441055744.0;  // 2^52 + 2^51: a sum's low word is the nearest integer
@@ -151,7 +165,7 @@ struct Weigh {
     p = fma(p, r, a1);
     p = fma(p, r, 1.0);
     *oct = n >> 8;
-    return pow2[n & (SR_TABLE - 1)] * p;
+    return shared_part().pow2[n & (SR_TABLE - 1)] * p;
   }
   // w in units of 2^-45: v * 2^(45 - oct) + 2^52 leaves the rounded integer in the low 52 bits
   static __device__ __forceinline__ u64 fixed(double v, int oct) {
@@ -219,200 +233,49 @@ __device__ __forceinline__ void cluster_barrier(int C) {
   else __syncthreads();
 }
 
-// grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the
-// slice: `per` (4 times an odd number: no bank conflicts) consecutive elements
-// for each thread, padded with -inf
-__global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sample s, int C, int per) {
-  extern __shared__ __align__(16) uint8_t dyn[];
-  Shared& sh = *reinterpret_cast<Shared*>(dyn);
-  float* xs = reinterpret_cast<float*>(dyn + SR_HEAD);
-  pdl_trigger();
-  if (C > 1) cluster_arrive();
-  pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = blockIdx.x % C, r = blockIdx.x / C;
-  const int slice = per * SR_THREADS - SR_PAD;
-  const int c0 = min(s.V, rank * slice), n = min(s.V, c0 + slice) - c0;
-  const float T = s.temperature ? s.temperature[r] : 1.f;
-  const int k = s.top_k ? s.top_k[r] : 0;
-  const float top_p = s.top_p ? s.top_p[r] : 1.f, min_p = s.min_p ? s.min_p[r] : 0.f;
-  const bool by_k = k > 0 && k < s.V, by_p = !(top_p >= 1.f), by_m = min_p > 0.f;
-  // rows where only the first maximum can stay
-  const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
-  const bool need_bins = !top1 && (by_k || by_p || by_m);
-  for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.hist[i] = make_uint2(0u, 0u);
-  if (tid == 0) {
-    sh.again = sh.drawn = 0;
-    sh.listed = sh.cut_ties = 0;
-  }
+// What a row's passes share: kept in registers by the kernel, handed over in
+// memory to the passes that few rows need (in one body they cost the others
+// registers: one row 15.1 us, 15.9 in one body; 320 with a top-k 67 and 71).
+struct Row {
+  wg_sample s;
+  int C, rank, r, per, c0, lead;
+  int first_i;  // index of the thread's first element
+  int slice;
+  float mx, span, bin_scale, t1, c2, c2_lo, deep, u;
+  Weigh wt;
+  int k;
+  float top_p;
+  double least;  // min-p
+  bool by_k, by_p, by_m, need_bins;
 
-  // ---- the slice into shared memory, 16-byte loads between its ragged ends;
-  // it starts at the address's place in 16 bytes, so both sides are aligned
-  const int es = dt_bytes(s.dtype), vec = 16 / es;
-  const uint8_t* src = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + c0) * es;
-  const int lead = (int)((reinterpret_cast<uintptr_t>(src) / es) % vec);
-  float mx = -INFINITY, mn = INFINITY;
-  {
-    auto clean = [&](float x) {
-      x = x != x ? -INFINITY : x;
-      mx = fmaxf(mx, x);
-      mn = fminf(mn, x == -INFINITY ? INFINITY : x);  // the least finite one
-      return x;
-    };
-    const int head = min(n, (vec - lead) % vec), body = (n - head) / vec, tail = n - head - body * vec;
-    if (tid < lead) xs[tid] = -INFINITY;
-    for (int i = lead + n + tid; i < per * SR_THREADS; i += SR_THREADS) xs[i] = -INFINITY;
-    if (tid < head) xs[lead + tid] = clean(dt_load(src, tid, s.dtype));
-    if (tid < tail) xs[lead + n - tail + tid] = clean(dt_load(src, n - tail + tid, s.dtype));
-    const uint4* v = reinterpret_cast<const uint4*>(src + head * es);
-    float4* d = reinterpret_cast<float4*>(xs + lead + head);
-    constexpr int U = 4;  // loads in flight per thread
-    for (int i0 = tid; i0 < body; i0 += U * SR_THREADS) {
-      uint4 w[U];
-#pragma unroll
-      for (int j = 0; j < U; j++) w[j] = i0 + j * SR_THREADS < body ? __ldg(v + i0 + j * SR_THREADS) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < U; j++) {
-        const int i = i0 + j * SR_THREADS;
-        if (i >= body) break;
-        if (s.dtype == WG_DT_F32) {
-          d[i] = make_float4(clean(__uint_as_float(w[j].x)), clean(__uint_as_float(w[j].y)),
-                             clean(__uint_as_float(w[j].z)), clean(__uint_as_float(w[j].w)));
-        } else {
-          const float2 a = dt_unpack2(s.dtype, w[j].x), b = dt_unpack2(s.dtype, w[j].y);
-          const float2 e = dt_unpack2(s.dtype, w[j].z), f = dt_unpack2(s.dtype, w[j].w);
-          d[2 * i] = make_float4(clean(a.x), clean(a.y), clean(b.x), clean(b.y));
-          d[2 * i + 1] = make_float4(clean(e.x), clean(e.y), clean(f.x), clean(f.y));
-        }
-      }
-    }
-  }
-  for (int i = tid; i < SR_TABLE; i += SR_THREADS) sh.pow2[i] = exp2(-(double)i / SR_TABLE);
-  mx = warp_max(mx);
-  mn = -warp_max(-mn);
-  if (lane == 0) { sh.red_f[0][warp] = mx; sh.red_f[1][warp] = mn; }
-  __syncthreads();
-  if (C > 1) cluster_wait();  // every rank runs: its shared memory may be written
-  if (warp == 0) {
-    mx = warp_max(sh.red_f[0][lane % SR_WARPS]);
-    mn = -warp_max(-sh.red_f[1][lane % SR_WARPS]);
-    if (lane < C) {
-      peer(sh.mx, lane, C)[rank] = mx;
-      peer(sh.mn, lane, C)[rank] = mn;
-    }
-  }
-  cluster_barrier(C);
-  mx = sh.mx[0];
-  mn = sh.mn[0];
-  for (int q = 1; q < C; q++) {
-    mx = fmaxf(mx, sh.mx[q]);
-    mn = fminf(mn, sh.mn[q]);
-  }
-  if (mx == -INFINITY) {  // nothing to draw from (the same for every rank)
-    if (rank == 0 && tid == 0) {
-      s.tokens[r] = -1;
-      if (s.logprobs) s.logprobs[r] = -INFINITY;
-    }
-    return;
-  }
-  float4* mine = reinterpret_cast<float4*>(xs + tid * per);  // this thread's consecutive elements
-  const int first_i = c0 - lead + tid * per;                 // index of the first (below 0 only in padding)
-  if (mx == INFINITY) {  // the infinite ones share the mass: a row of 0 and -inf
-    auto flat = [](float x) { return x == INFINITY ? 0.f : -INFINITY; };
-    for (int i = 0; i < per / 4; i++) mine[i] = make_float4(flat(mine[i].x), flat(mine[i].y), flat(mine[i].z), flat(mine[i].w));
-    mx = mn = 0.f;
-    __syncthreads();
+  // this thread's consecutive elements
+  __device__ __forceinline__ const float4* mine() const {
+    return reinterpret_cast<const float4*>(shared_slice() + threadIdx.x * per);
   }
   // f(x[4], i) over the thread's elements, i the place of the first of the four
-  auto each = [&](auto&& f) {
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll 1
     for (int i = 0; i < per; i += 4) {
-      const float4 v = mine[i / 4];
+      const float4 v = mine()[i / 4];
       const float x[4] = {v.x, v.y, v.z, v.w};
       f(x, i);
     }
-  };
-
-  // ---- fp32 sum of the weights, first maximum, histogram of counts
-  const float t1 = fminf(fmaxf(T > 0.f ? T : 1.f, 1e-30f), 1e30f);
-  const float c2 = 1.4426950408889634f / t1;
-  // log 2 of a weight: the product with 1 / (T ln 2) in two floats, so that its
-  // rounding does not lean every weight the same way
-  const float c2_lo = (float)(1.4426950408889634 / (double)t1 - (double)c2);
-  const float deep = -200.f / c2;  // 2^-200 is 0 as well, and the products stay finite
-  auto octaves = [&](float x) {
+  }
+  __device__ __forceinline__ float octaves(float x) const {
     const float d = fmaxf(x - mx, deep);
     return fmaf(d, c2, d * c2_lo);
-  };
-  const float span = fminf(fmaxf(mx - mn, 1e-30f), SR_SPAN);
-  const float bin_scale = (float)(SR_BINS - 1) / span;
-  // nearest bin, the last one for everything further down (2^23 + b holds b in its low bits)
-  auto bin_bits = [&](float x) { return fminf((mx - x) * bin_scale, (float)(SR_BINS - 1)) + 8388608.f; };
-  auto bin_of = [&](float x) { return __float_as_int(bin_bits(x)) & (SR_BINS - 1); };
-  double own = 0;  // this thread's weights
-  {
-    // the maxima are counted, not summed: a row that is nearly certain keeps the
-    // digits of what the other tokens share
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-    unsigned ones = 0;
-    int first = 0x7fffffff;
-    if (need_bins) {
-      each([&](const float (&x)[4], int) {
-        float e[4];
-        int b[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          e[j] = ex2f(octaves(x[j]));
-          b[j] = bin_of(x[j]);
-          if (e[j] < 1.f) part[j] += e[j];
-          else ones++;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (b[j] < SR_BINS - 1) atomicAdd(&sh.hist[b[j]].x, 1u);  // the last bin is the rest
-          if (e[j] > SR_HEAVY) atomicAdd(&sh.hist[b[j]].y, (unsigned)(__float_as_int(e[j] + 128.f) - 0x43000000));
-        }
-      });
-    } else {
-      each([&](const float (&x)[4], int i) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float e = ex2f(octaves(x[j]));
-          if (e < 1.f) part[j] += e;
-          else ones++;
-          if (top1 && x[j] == mx) first = min(first, first_i + i + j);
-        }
-      });
-    }
-    double sum = ((double)part[0] + part[1]) + ((double)part[2] + part[3]);
-    own = sum + ones;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    first = __reduce_min_sync(0xffffffffu, first);
-    ones = __reduce_add_sync(0xffffffffu, ones);
-    if (lane == 0) { sh.red_o[warp] = (u64)__double_as_longlong(sum); sh.red_c[warp] = (unsigned)first; sh.red_m[warp] = ones; }
-    __syncthreads();
-    if (warp == 0) {
-      sum = __longlong_as_double((long long)sh.red_o[lane % SR_WARPS]);
-#pragma unroll
-      for (int d = SR_WARPS / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      first = __reduce_min_sync(0xffffffffu, (int)sh.red_c[lane % SR_WARPS]);
-      ones = __reduce_add_sync(0xffffffffu, lane < SR_WARPS ? (unsigned)sh.red_m[lane] : 0u);
-      if (lane < C) {
-        peer(sh.sum, lane, C)[rank] = sum;
-        peer(sh.ones, lane, C)[rank] = ones;
-        peer(sh.first, lane, C)[rank] = first;
-      }
-    }
   }
-  const Weigh wt{(double)mx, -1.0 / (SR_STEP * (double)t1), sh.pow2};
-  auto light = [&](float x) { return !((mx - x) * c2 < SR_OCTAVES); };
-  auto weight = [&](float x) { return light(x) ? (u64)0 : wt.fixed_of(x); };
-  const double least = (double)min_p;
-  auto weight_kept = [&](float x) { return light(x) ? (u64)0 : by_m ? wt.fixed_from(x, least) : wt.fixed_of(x); };
-  auto finish = [&](int token, float x) {
+  // nearest bin, the last one for everything further down (2^23 + b holds b in its low bits)
+  __device__ __forceinline__ float bin_bits(float x) const { return fminf((mx - x) * bin_scale, (float)(SR_BINS - 1)) + 8388608.f; }
+  __device__ __forceinline__ int bin_of(float x) const { return __float_as_int(bin_bits(x)) & (SR_BINS - 1); }
+  __device__ __forceinline__ bool light(float x) const { return !((mx - x) * c2 < SR_OCTAVES); }
+  __device__ __forceinline__ u64 weight(float x) const { return light(x) ? (u64)0 : wt.fixed_of(x); }
+  __device__ __forceinline__ u64 weight_kept(float x) const { return light(x) ? (u64)0 : by_m ? wt.fixed_from(x, least) : wt.fixed_of(x); }
+  __device__ __forceinline__ void finish(int token, float x) const {
     s.tokens[r] = token;
     if (s.logprobs) {
+      const Shared& sh = shared_part();
       double z = 0;
       unsigned n1 = 0;
       for (int q = 0; q < C; q++) {
@@ -421,342 +284,39 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
       }
       s.logprobs[r] = (x - mx) / t1 - (logf((float)n1) + log1pf((float)z / (float)n1));
     }
-  };
-  float u = s.u[r];
-  if (!(u >= 0.f)) u = 0.f;
+  }
   // first running mass above u * mass
-  auto draw = [&](u64 mass) {
+  __device__ __forceinline__ u64 draw(u64 mass) const {
     const double at = (double)u * (double)mass;
     const u64 goal = at < (double)mass ? (u64)at + 1 : mass;
     return goal > mass ? mass : goal;
-  };
+  }
   // the running mass that top-p asks for
-  auto share = [&](u64 mass) {
+  __device__ __forceinline__ u64 share(u64 mass) const {
     const double want = ceil((double)top_p * (double)mass);
     const u64 goal = want >= 1.0 ? (u64)want : 1;
     return goal > mass ? mass : goal;
-  };
+  }
   // The fp32 weights 2^-y, and any sum of them, are off by at most this share of
   // their whole sum z: ex2.approx 2^-22; three roundings of y, each 2^-24 of it,
   // and the mean of y over the mass is at most log2 V - log2 z (an entropy);
   // per / 4 additions in fp32; 2^-24 for what the exact units round off (V * 2^-46)
-  auto off_by = [&](float z) {
+  __device__ __forceinline__ float off_by(float z) const {
     return (6.f + 2.1f * fmaxf(0.f, log2f((float)s.V) + 0.01f - log2f(z)) + (float)(per / 4)) * (1.f / 16777216.f);
-  };
-  double pre = own;  // this thread's place in the slice's mass
-  if (!top1 && !need_bins) {
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double v = __shfl_up_sync(0xffffffffu, pre, d);
-      if (lane >= d) pre += v;
-    }
-    __syncthreads();  // red_m has been read
-    if (lane == 31) sh.red_m[warp] = (u64)__double_as_longlong(pre);
-    __syncthreads();
-    pre -= own;
-#pragma unroll
-    for (int w = 0; w < SR_WARPS; w++)
-      if (w < warp) pre += __longlong_as_double((long long)sh.red_m[w]);
-  }
-  cluster_barrier(C);
-  if (top1) {
-    if (rank == 0 && tid == 0) {
-      int f = 0x7fffffff;
-      for (int q = 0; q < C; q++) f = min(f, sh.first[q]);
-      finish(f, mx);
-    }
-    return;
   }
 
-  if (!need_bins) {
-    // ---- the whole row is kept: the element that the number falls into by the
-    // fp32 weights is the right one where it lies further inside than these can
-    // be off, the sum before it and its place in the sum both
-    double z = 0, base = 0;
-    for (int q = 0; q < C; q++) {
-      if (q == rank) base = z;
-      z += sh.sum[q] + sh.ones[q];
-    }
-    const double at = (double)u * z, margin = 2.0 * (double)off_by((float)z) * z;
-    const double b = base + pre;
-    const unsigned claim = __ballot_sync(0xffffffffu, at >= b && at < b + own);
-    if (claim) {
-      const int owner = __ffs(claim) - 1;
-      double run = __shfl_sync(0xffffffffu, b, owner);
-      const float* ox = xs + (warp * 32 + owner) * per;
-      for (int i0 = 0; i0 < per; i0 += 32) {
-        const int i = i0 + lane;
-        const float x = i < per ? ox[i] : -INFINITY;
-        const double e = ex2f(octaves(x));
-        double upto = e;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const double v = __shfl_up_sync(0xffffffffu, upto, d);
-          if (lane >= d) upto += v;
-        }
-        upto += run;
-        if (at - (upto - e) > margin && upto - at > margin) {
-          finish(c0 - lead + (warp * 32 + owner) * per + i, x);
-          for (int q = 0; q < C; q++) peer(&sh, q, C)->drawn = 1;
-        }
-        run = __shfl_sync(0xffffffffu, upto, 31);
-      }
-    }
-    cluster_barrier(C);
-    if (sh.drawn) return;
-  }
+  __device__ void long_passes(int kbin, int pbin, unsigned kabove) const;
+};
 
-  int kbin = SR_BINS - 1, pbin = 0;
-  unsigned kabove = 0;
-  u64 all = 0;
-  if (need_bins) {
-    // ---- the first histogram over the cluster: a thread has SR_BPT neighbours.
-    // Masses are a guess, checked below: sums of 2^-16 units where the bin's
-    // weights are heavy, count * weight at the middle of the bin where they are light
-    unsigned c1[SR_BPT] = {}, lower[SR_BPT] = {}, ct, c_in = 0;  // lower: of the ranks before this one
-    u64 m1[SR_BPT] = {}, mt, m_in = 0;
-#pragma unroll
-    for (int q = 0; q < SR_MAX_CLUSTER; q++)
-      if (q < C) {
-        const uint4 v = *reinterpret_cast<const uint4*>(peer(sh.hist, q, C) + SR_BPT * tid);
-        if (q == rank) {
-          lower[0] = c1[0];
-          lower[1] = c1[1];
-        }
-        c1[0] += v.x;
-        m1[0] += v.y;
-        c1[1] += v.z;
-        m1[1] += v.w;
-      }
-#pragma unroll
-    for (int b = 0; b < SR_BPT; b++) {
-      const float mid = ex2f(-(float)(SR_BPT * tid + b) * (span / (float)(SR_BINS - 1)) * c2);
-      m1[b] = mid > SR_HEAVY ? m1[b] << 16 : (u64)((float)c1[b] * mid * 4294967296.f);
-      c_in += c1[b];
-      m_in += m1[b];
-    }
-    block_scan(sh, m_in, c_in, &mt, &ct);
-    c_in -= c1[0] + c1[1];  // what is above this thread's bins
-    m_in -= m1[0] + m1[1];
-    if (tid == 0) { sh.found[0] = sh.found[1] = SR_BINS - 1; sh.found_c = ct; sh.found_m = mt; }
-    __syncthreads();
-    if (by_k) {
-      unsigned c = c_in;
-      u64 m = m_in;
-#pragma unroll
-      for (int b = 0; b < SR_BPT; b++) {
-        if (c < (unsigned)k && (unsigned)k <= c + c1[b]) {
-          sh.found[0] = SR_BPT * tid + b;
-          sh.found_c = c;
-          sh.found_m = m + (u64)((float)m1[b] * ((float)(k - (int)c) / (float)c1[b]));
-        }
-        c += c1[b];
-        m += m1[b];
-      }
-    }
-    __syncthreads();
-    kbin = sh.found[0];
-    kabove = sh.found_c;
-    if (by_p) {
-      const u64 goal = max((u64)1, (u64)((double)sh.found_m * (double)top_p));
-      u64 m = m_in;
-#pragma unroll
-      for (int b = 0; b < SR_BPT; b++) {
-        if (m < goal && goal <= m + m1[b]) sh.found[1] = SR_BPT * tid + b;
-        m += m1[b];
-      }
-      __syncthreads();
-      pbin = min(kbin, sh.found[1]);
-    }
-    // ---- the bins that can be kept, and how many elements they hold
-    int last = kbin;
-    bool covers = by_k;  // the bins hold all that can stay, whatever the guess is worth
-    if (!by_k) {
-      if (by_p) last = min(SR_BINS - 1, pbin + 1);
-      if (by_m) {  // min-p keeps max - x <= T ln(1 / min_p); two bins on the safe side
-        const float reach = -log2f(min_p) / c2 * bin_scale;
-        const int down = reach < (float)(SR_BINS - 4) ? (int)reach + 3 : SR_BINS - 1;
-        covers = down <= last;
-        last = min(last, down);
-      }
-    }
-    __syncthreads();
-    if (tid == last / SR_BPT) sh.found_c = last == SR_BINS - 1 ? (unsigned)s.V : c_in + c1[0] + (last % SR_BPT ? c1[1] : 0u);
-    __syncthreads();
-    if (sh.found_c <= SR_LIST) {
-      // ---- candidates in index order, to rank 0: behind those of the ranks
-      // before, whose number the histograms tell (the last bin is not counted
-      // there, but rows so short have one rank)
-      const float edge = 8388608.f + (float)last;
-      auto candidate = [&](float x) { return bin_bits(x) <= edge && x > -INFINITY; };
-      unsigned hits = 0, hits_t;
-      u64 base = (SR_BPT * tid <= last ? lower[0] : 0) + (SR_BPT * tid + 1 <= last ? lower[1] : 0), base_t;
-      u64 fours = 0;  // the groups of four that hold any: the bins fall with the logit, so the largest tells
-      for (int i = 0; i < per / 4; i++) {
-        const float4 v = mine[i];
-        if (candidate(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)))) {
-          fours |= 1ull << i;
-          hits += candidate(v.x) + candidate(v.y) + candidate(v.z) + candidate(v.w);
-        }
-      }
-      const unsigned own = hits;
-      block_scan(sh, base, hits, &base_t, &hits_t);
-      const int total = last == SR_BINS - 1 ? (int)hits_t : (int)sh.found_c;
-      int2* to = peer(sh.list.xi, 0, C) + (int)base_t + hits - own;
-      for (; fours; fours &= fours - 1) {
-        const int i = __ffsll((long long)fours) - 1;
-        const float4 v = mine[i];
-        const float x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (candidate(x[j])) *to++ = make_int2(__float_as_int(x[j]), first_i + 4 * i + j);
-      }
-      cluster_barrier(C);
-      const bool alone = !by_p || by_k;  // rank 0 needs nothing more of its peers
-      if (alone && rank) return;
-      // ---- rank 0 orders them: into their bins, whose beginnings the histogram
-      // tells, then by counting inside a bin (a few elements; all of them when
-      // they are equal). Thread t gets places each * t and on, with the exact mass before them
-      u64 f[SR_EPT] = {}, o[SR_EPT] = {}, before[SR_EPT] = {};
-      const int each_t = (total + SR_THREADS - 1) / SR_THREADS;
-      if (rank == 0) {
-        unsigned* begin = reinterpret_cast<unsigned*>(sh.hist);  // read last before the barrier above
-        begin[SR_BPT * tid] = c_in;
-        begin[SR_BPT * tid + 1] = c_in + c1[0];
-        __syncthreads();
-        for (int i = tid; i < total; i += SR_THREADS) {
-          const float x = __int_as_float(sh.list.xi[i].x);
-          sh.list.order[atomicAdd(&begin[bin_of(x)], 1u)] = ((u64)key_of(x) << 32) | (0xffffffffu - (unsigned)i);
-        }
-        __syncthreads();  // a bin begins where the one before it ended
-        int at[SR_EPT];
-#pragma unroll
-        for (int j = 0; j < SR_EPT; j++) {
-          const int e = tid + j * SR_THREADS;
-          if (e >= total) continue;
-          o[j] = sh.list.order[e];
-          const int b = bin_of(of_key((uint32_t)(o[j] >> 32)));
-          const int from = b ? (int)begin[b - 1] : 0, end = (int)begin[b];
-          at[j] = from;
-          for (int i = from; i < end; i++) at[j] += sh.list.order[i] > o[j];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < SR_EPT; j++)
-          if (tid + j * SR_THREADS < total) sh.list.order[at[j]] = o[j];
-        __syncthreads();
-        u64 m = 0, mt;
-#pragma unroll
-        for (int j = 0; j < SR_EPT; j++) {
-          const int e = each_t * tid + j;
-          o[j] = 0;
-          if (j < each_t && e < total) {
-            o[j] = sh.list.order[e];
-            f[j] = weight(of_key((uint32_t)(o[j] >> 32)));
-          }
-          before[j] = m;
-          m += f[j];
-        }
-        const u64 own_mass = m;
-        unsigned zero = 0, zero_t;
-        block_scan(sh, m, zero, &mt, &zero_t);
-#pragma unroll
-        for (int j = 0; j < SR_EPT; j++) before[j] += m - own_mass;
-      }
-      auto place = [&](int j) { return j < each_t ? min(each_t * tid + j, SR_LIST) : SR_LIST; };
-      const int nk = by_k ? min(k, total) : total;
-      for (int pass = 0;; pass++) {  // at most two: the second with the row's exact mass
-        if (rank == 0) {
-          u64 lo = 0, hi = 0;  // the running mass that top-p asks for, as far as it is known
-          if (by_p) {
-            if (by_k) {
-              if (tid == 0) sh.found_m = 0;
-              __syncthreads();
-#pragma unroll
-              for (int j = 0; j < SR_EPT; j++)
-                if (place(j) == nk - 1) sh.found_m = before[j] + f[j];
-              __syncthreads();
-              lo = hi = share(sh.found_m);
-            } else if (pass) {
-              all = 0;
-              for (int q = 0; q < C; q++) all += sh.all[q];
-              lo = hi = share(all);
-            } else {
-              double z = 0;
-              for (int q = 0; q < C; q++) z += sh.sum[q] + sh.ones[q];
-              const double err = off_by((float)z);
-              lo = share((u64)(z * (1.0 - err) * 35184372088832.0));  // 2^45
-              hi = share((u64)(z * (1.0 + err) * 35184372088832.0) + 1);
-            }
-          }
-          // kept masses in index order; two ends of the top-p mass must keep the same ones,
-          // and a list that ends before them decides nothing
-          bool unsure = false, past = false, ended = false;
-          u64 kept[SR_EPT] = {};
-#pragma unroll
-          for (int j = 0; j < SR_EPT; j++) {
-            if (place(j) < nk && (!by_p || before[j] < lo)) kept[j] = by_m ? weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
-            unsure |= by_p && place(j) < nk && before[j] >= lo && before[j] < hi;
-            if (by_p && !covers && place(j) == total - 1) {
-              ended = before[j] + f[j] < hi;
-              past = before[j] + f[j] < lo;
-            }
-          }
-          const int doubt = __syncthreads_or(unsure || ended), whole = __syncthreads_or(past);
-          const int todo = whole ? SR_WHOLE : doubt ? SR_EXACT : SR_DONE;
-          if (todo == SR_DONE) {
-#pragma unroll
-            for (int j = 0; j < SR_EPT; j++)
-              if (place(j) < total) sh.list.order[0xffffffffu - (uint32_t)o[j]] = kept[j];
-            __syncthreads();
-            u64 m = 0, mass, fk[SR_EPT];
-#pragma unroll
-            for (int j = 0; j < SR_EPT; j++) {
-              fk[j] = place(j) < total ? sh.list.order[place(j)] : 0;
-              m += fk[j];
-            }
-            const u64 own_mass = m;
-            unsigned zero = 0, zero_t;
-            block_scan(sh, m, zero, &mass, &zero_t);
-            const u64 to = draw(mass);
-            u64 run = m - own_mass;
-            int win = -1;
-#pragma unroll
-            for (int j = 0; j < SR_EPT; j++) {
-              if (fk[j] && run < to && to <= run + fk[j]) win = place(j);
-              run += fk[j];
-            }
-            if (win >= 0) finish(sh.list.xi[win].y, __int_as_float(sh.list.xi[win].x));
-          } else if (tid < C) {
-            peer(&sh, tid, C)->again = todo;
-          }
-        }
-        if (alone) return;
-        cluster_barrier(C);  // rank 0 has told its peers what it needs
-        const int todo = sh.again;
-        if (todo == SR_DONE) return;
-        if (todo == SR_WHOLE) break;
-        // the exact mass of the row
-        all = 0;
-        each([&](const float (&x)[4], int) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) all += weight(x[j]);
-        });
-        all = warp_sum64(all);
-        __syncthreads();  // `again` and red_m have been read
-        if (lane == 0) sh.red_m[warp] = all;
-        if (tid == 0) sh.again = SR_DONE;
-        __syncthreads();
-        if (warp == 0) {
-          all = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
-          if (lane == 0) peer(sh.all, 0, C)[rank] = all;
-        }
-        cluster_barrier(C);
-      }
-    }
-  }
-
-  // ---- the cut by descents
+// Rows whose kept set no short list holds, and rows without filters that the
+// fp32 weights do not decide.
+__device__ __forceinline__ void Row::long_passes(int kbin, int pbin, unsigned kabove) const {
+  Shared& sh = shared_part();
+  const float* xs = shared_slice();
+  const float4* mine = this->mine();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  u64 all;
+  // ---- the cut
   // By a list, once a row: the elements of bins ba..bb go to rank 0 in any order.
   auto inside = [&](float x, int ba, int bb) {
     const int b = bin_of(x);
@@ -1092,7 +652,7 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
       goal = sh.found_m;
       left = sh.found_c;
       // element: the owner's consecutive ones, 32 at a time
-      const int qc0 = min(s.V, q * slice);
+      const int es = dt_bytes(s.dtype), vec = 16 / es, qc0 = min(s.V, q * slice);
       const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + qc0) * es;
       const int qi = qc0 - (int)((reinterpret_cast<uintptr_t>(qsrc) / es) % vec) + owner * per;
       const float* qx = peer(xs, q, C) + owner * per;
@@ -1122,6 +682,500 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   cluster_barrier(C);  // rank 0 has read its peers
 }
 
+__device__ __noinline__ void finish_long(const Row& given, int kbin, int pbin, unsigned kabove) {
+  const Row row = given;  // into registers
+  row.long_passes(kbin, pbin, kabove);
+}
+
+// grid (C * R), cluster (C, 1, 1); dynamic shared memory: Shared, then the
+// slice: `per` (4 times an odd number: no bank conflicts) consecutive elements
+// for each thread, padded with -inf
+__global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sample s, int C, int per) {
+  Shared& sh = shared_part();
+  float* xs = shared_slice();
+  pdl_trigger();
+  if (C > 1) cluster_arrive();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x % C, r = blockIdx.x / C;
+  const int slice = per * SR_THREADS - SR_PAD;
+  const int c0 = min(s.V, rank * slice), n = min(s.V, c0 + slice) - c0;
+  const float T = s.temperature ? s.temperature[r] : 1.f;
+  const int k = s.top_k ? s.top_k[r] : 0;
+  const float top_p = s.top_p ? s.top_p[r] : 1.f, min_p = s.min_p ? s.min_p[r] : 0.f;
+  const bool by_k = k > 0 && k < s.V, by_p = !(top_p >= 1.f), by_m = min_p > 0.f;
+  // rows where only the first maximum can stay
+  const bool top1 = !(T > 0.f) || k == 1 || !(top_p > 0.f) || !(min_p <= 1.f);
+  const bool need_bins = !top1 && (by_k || by_p || by_m);
+  for (int i = tid; i < SR_BINS; i += SR_THREADS) sh.hist[i] = make_uint2(0u, 0u);
+  if (tid == 0) {
+    sh.again = sh.drawn = 0;
+    sh.listed = sh.cut_ties = 0;
+  }
+
+  // ---- the slice into shared memory, 16-byte loads between its ragged ends;
+  // it starts at the address's place in 16 bytes, so both sides are aligned
+  const int es = dt_bytes(s.dtype), vec = 16 / es;
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(s.logits) + ((int64_t)r * s.ld + c0) * es;
+  const int lead = (int)((reinterpret_cast<uintptr_t>(src) / es) % vec);
+  float mx = -INFINITY, mn = INFINITY;
+  {
+    auto clean = [&](float x) {
+      x = x != x ? -INFINITY : x;
+      mx = fmaxf(mx, x);
+      mn = fminf(mn, x == -INFINITY ? INFINITY : x);  // the least finite one
+      return x;
+    };
+    const int head = min(n, (vec - lead) % vec), body = (n - head) / vec, tail = n - head - body * vec;
+    if (tid < lead) xs[tid] = -INFINITY;
+    for (int i = lead + n + tid; i < per * SR_THREADS; i += SR_THREADS) xs[i] = -INFINITY;
+    if (tid < head) xs[lead + tid] = clean(dt_load(src, tid, s.dtype));
+    if (tid < tail) xs[lead + n - tail + tid] = clean(dt_load(src, n - tail + tid, s.dtype));
+    const uint4* v = reinterpret_cast<const uint4*>(src + head * es);
+    float4* d = reinterpret_cast<float4*>(xs + lead + head);
+    constexpr int U = 4;  // loads in flight per thread
+    for (int i0 = tid; i0 < body; i0 += U * SR_THREADS) {
+      uint4 w[U];
+#pragma unroll
+      for (int j = 0; j < U; j++) w[j] = i0 + j * SR_THREADS < body ? __ldg(v + i0 + j * SR_THREADS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < U; j++) {
+        const int i = i0 + j * SR_THREADS;
+        if (i >= body) break;
+        if (s.dtype == WG_DT_F32) {
+          d[i] = make_float4(clean(__uint_as_float(w[j].x)), clean(__uint_as_float(w[j].y)),
+                             clean(__uint_as_float(w[j].z)), clean(__uint_as_float(w[j].w)));
+        } else {
+          const float2 a = dt_unpack2(s.dtype, w[j].x), b = dt_unpack2(s.dtype, w[j].y);
+          const float2 e = dt_unpack2(s.dtype, w[j].z), f = dt_unpack2(s.dtype, w[j].w);
+          d[2 * i] = make_float4(clean(a.x), clean(a.y), clean(b.x), clean(b.y));
+          d[2 * i + 1] = make_float4(clean(e.x), clean(e.y), clean(f.x), clean(f.y));
+        }
+      }
+    }
+  }
+  for (int i = tid; i < SR_TABLE; i += SR_THREADS) sh.pow2[i] = exp2(-(double)i / SR_TABLE);
+  mx = warp_max(mx);
+  mn = -warp_max(-mn);
+  if (lane == 0) { sh.red_f[0][warp] = mx; sh.red_f[1][warp] = mn; }
+  __syncthreads();
+  if (C > 1) cluster_wait();  // every rank runs: its shared memory may be written
+  if (warp == 0) {
+    mx = warp_max(sh.red_f[0][lane % SR_WARPS]);
+    mn = -warp_max(-sh.red_f[1][lane % SR_WARPS]);
+    if (lane < C) {
+      peer(sh.mx, lane, C)[rank] = mx;
+      peer(sh.mn, lane, C)[rank] = mn;
+    }
+  }
+  cluster_barrier(C);
+  mx = sh.mx[0];
+  mn = sh.mn[0];
+  for (int q = 1; q < C; q++) {
+    mx = fmaxf(mx, sh.mx[q]);
+    mn = fminf(mn, sh.mn[q]);
+  }
+  if (mx == -INFINITY) {  // nothing to draw from (the same for every rank)
+    if (rank == 0 && tid == 0) {
+      s.tokens[r] = -1;
+      if (s.logprobs) s.logprobs[r] = -INFINITY;
+    }
+    return;
+  }
+  float4* mine = reinterpret_cast<float4*>(xs + tid * per);  // this thread's consecutive elements
+  const int first_i = c0 - lead + tid * per;                 // index of the first (below 0 only in padding)
+  if (mx == INFINITY) {  // the infinite ones share the mass: a row of 0 and -inf
+    auto flat = [](float x) { return x == INFINITY ? 0.f : -INFINITY; };
+    for (int i = 0; i < per / 4; i++) mine[i] = make_float4(flat(mine[i].x), flat(mine[i].y), flat(mine[i].z), flat(mine[i].w));
+    mx = mn = 0.f;
+    __syncthreads();
+  }
+  // ---- fp32 sum of the weights, first maximum, histogram of counts
+  const float t1 = fminf(fmaxf(T > 0.f ? T : 1.f, 1e-30f), 1e30f);
+  const float c2 = 1.4426950408889634f / t1;
+  // log 2 of a weight: the product with 1 / (T ln 2) in two floats, so that its
+  // rounding does not lean every weight the same way
+  const float c2_lo = (float)(1.4426950408889634 / (double)t1 - (double)c2);
+  const float deep = -200.f / c2;  // 2^-200 is 0 as well, and the products stay finite
+  const float span = fminf(fmaxf(mx - mn, 1e-30f), SR_SPAN);
+  const float bin_scale = (float)(SR_BINS - 1) / span;
+  float u = s.u[r];
+  if (!(u >= 0.f)) u = 0.f;
+  const Row row{s, C, rank, r, per, c0, lead, first_i, slice, mx, span, bin_scale, t1, c2, c2_lo, deep, u,
+                Weigh{(double)mx, -1.0 / (SR_STEP * (double)t1)}, k, top_p, (double)min_p, by_k, by_p, by_m, need_bins};
+  double own = 0;  // this thread's weights
+  {
+    // the maxima are counted, not summed: a row that is nearly certain keeps the
+    // digits of what the other tokens share
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    unsigned ones = 0;
+    int first = 0x7fffffff;
+    if (need_bins) {
+      row.each([&](const float (&x)[4], int) {
+        float e[4];
+        int b[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          e[j] = ex2f(row.octaves(x[j]));
+          b[j] = row.bin_of(x[j]);
+          if (e[j] < 1.f) part[j] += e[j];
+          else ones++;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (b[j] < SR_BINS - 1) atomicAdd(&sh.hist[b[j]].x, 1u);  // the last bin is the rest
+          if (e[j] > SR_HEAVY) atomicAdd(&sh.hist[b[j]].y, (unsigned)(__float_as_int(e[j] + 128.f) - 0x43000000));
+        }
+      });
+    } else {
+      row.each([&](const float (&x)[4], int i) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float e = ex2f(row.octaves(x[j]));
+          if (e < 1.f) part[j] += e;
+          else ones++;
+          if (top1 && x[j] == mx) first = min(first, first_i + i + j);
+        }
+      });
+    }
+    double sum = ((double)part[0] + part[1]) + ((double)part[2] + part[3]);
+    own = sum + ones;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    first = __reduce_min_sync(0xffffffffu, first);
+    ones = __reduce_add_sync(0xffffffffu, ones);
+    if (lane == 0) { sh.red_o[warp] = (u64)__double_as_longlong(sum); sh.red_c[warp] = (unsigned)first; sh.red_m[warp] = ones; }
+    __syncthreads();
+    if (warp == 0) {
+      sum = __longlong_as_double((long long)sh.red_o[lane % SR_WARPS]);
+#pragma unroll
+      for (int d = SR_WARPS / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      first = __reduce_min_sync(0xffffffffu, (int)sh.red_c[lane % SR_WARPS]);
+      ones = __reduce_add_sync(0xffffffffu, lane < SR_WARPS ? (unsigned)sh.red_m[lane] : 0u);
+      if (lane < C) {
+        peer(sh.sum, lane, C)[rank] = sum;
+        peer(sh.ones, lane, C)[rank] = ones;
+        peer(sh.first, lane, C)[rank] = first;
+      }
+    }
+  }
+  double pre = own;  // this thread's place in the slice's mass
+  if (!top1 && !need_bins) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, pre, d);
+      if (lane >= d) pre += v;
+    }
+    __syncthreads();  // red_m has been read
+    if (lane == 31) sh.red_m[warp] = (u64)__double_as_longlong(pre);
+    __syncthreads();
+    pre -= own;
+#pragma unroll
+    for (int w = 0; w < SR_WARPS; w++)
+      if (w < warp) pre += __longlong_as_double((long long)sh.red_m[w]);
+  }
+  cluster_barrier(C);
+  if (top1) {
+    if (rank == 0 && tid == 0) {
+      int f = 0x7fffffff;
+      for (int q = 0; q < C; q++) f = min(f, sh.first[q]);
+      row.finish(f, mx);
+    }
+    return;
+  }
+
+  if (!need_bins) {
+    // ---- the whole row is kept: the element that the number falls into by the
+    // fp32 weights is the right one where it lies further inside than these can
+    // be off, the sum before it and its place in the sum both
+    double z = 0, base = 0;
+    for (int q = 0; q < C; q++) {
+      if (q == rank) base = z;
+      z += sh.sum[q] + sh.ones[q];
+    }
+    const double at = (double)u * z, margin = 2.0 * (double)row.off_by((float)z) * z;
+    const double b = base + pre;
+    const unsigned claim = __ballot_sync(0xffffffffu, at >= b && at < b + own);
+    if (claim) {
+      const int owner = __ffs(claim) - 1;
+      double run = __shfl_sync(0xffffffffu, b, owner);
+      const float* ox = xs + (warp * 32 + owner) * per;
+      for (int i0 = 0; i0 < per; i0 += 32) {
+        const int i = i0 + lane;
+        const float x = i < per ? ox[i] : -INFINITY;
+        const double e = ex2f(row.octaves(x));
+        double upto = e;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += v;
+        }
+        upto += run;
+        if (at - (upto - e) > margin && upto - at > margin) {
+          row.finish(c0 - lead + (warp * 32 + owner) * per + i, x);
+          for (int q = 0; q < C; q++) peer(&sh, q, C)->drawn = 1;
+        }
+        run = __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    cluster_barrier(C);
+    if (sh.drawn) return;
+  }
+
+  int kbin = SR_BINS - 1, pbin = 0;
+  unsigned kabove = 0;
+  u64 all = 0;
+  if (need_bins) {
+    // ---- the first histogram over the cluster: a thread has SR_BPT neighbours.
+    // Masses are a guess, checked below: sums of 2^-16 units where the bin's
+    // weights are heavy, count * weight at the middle of the bin where they are light
+    unsigned c1[SR_BPT] = {}, lower[SR_BPT] = {}, ct, c_in = 0;  // lower: of the ranks before this one
+    u64 m1[SR_BPT] = {}, mt, m_in = 0;
+#pragma unroll
+    for (int q = 0; q < SR_MAX_CLUSTER; q++)
+      if (q < C) {
+        const uint4 v = *reinterpret_cast<const uint4*>(peer(sh.hist, q, C) + SR_BPT * tid);
+        if (q == rank) {
+          lower[0] = c1[0];
+          lower[1] = c1[1];
+        }
+        c1[0] += v.x;
+        m1[0] += v.y;
+        c1[1] += v.z;
+        m1[1] += v.w;
+      }
+#pragma unroll
+    for (int b = 0; b < SR_BPT; b++) {
+      const float mid = ex2f(-(float)(SR_BPT * tid + b) * (span / (float)(SR_BINS - 1)) * c2);
+      m1[b] = mid > SR_HEAVY ? m1[b] << 16 : (u64)((float)c1[b] * mid * 4294967296.f);
+      c_in += c1[b];
+      m_in += m1[b];
+    }
+    block_scan(sh, m_in, c_in, &mt, &ct);
+    c_in -= c1[0] + c1[1];  // what is above this thread's bins
+    m_in -= m1[0] + m1[1];
+    if (tid == 0) { sh.found[0] = sh.found[1] = SR_BINS - 1; sh.found_c = ct; sh.found_m = mt; }
+    __syncthreads();
+    if (by_k) {
+      unsigned c = c_in;
+      u64 m = m_in;
+#pragma unroll
+      for (int b = 0; b < SR_BPT; b++) {
+        if (c < (unsigned)k && (unsigned)k <= c + c1[b]) {
+          sh.found[0] = SR_BPT * tid + b;
+          sh.found_c = c;
+          sh.found_m = m + (u64)((float)m1[b] * ((float)(k - (int)c) / (float)c1[b]));
+        }
+        c += c1[b];
+        m += m1[b];
+      }
+    }
+    __syncthreads();
+    kbin = sh.found[0];
+    kabove = sh.found_c;
+    if (by_p) {
+      const u64 goal = max((u64)1, (u64)((double)sh.found_m * (double)top_p));
+      u64 m = m_in;
+#pragma unroll
+      for (int b = 0; b < SR_BPT; b++) {
+        if (m < goal && goal <= m + m1[b]) sh.found[1] = SR_BPT * tid + b;
+        m += m1[b];
+      }
+      __syncthreads();
+      pbin = min(kbin, sh.found[1]);
+    }
+    // ---- the bins that can be kept, and how many elements they hold
+    int last = kbin;
+    bool covers = by_k;  // the bins hold all that can stay, whatever the guess is worth
+    if (!by_k) {
+      if (by_p) last = min(SR_BINS - 1, pbin + 1);
+      if (by_m) {  // min-p keeps max - x <= T ln(1 / min_p); two bins on the safe side
+        const float reach = -log2f(min_p) / c2 * bin_scale;
+        const int down = reach < (float)(SR_BINS - 4) ? (int)reach + 3 : SR_BINS - 1;
+        covers = down <= last;
+        last = min(last, down);
+      }
+    }
+    __syncthreads();
+    if (tid == last / SR_BPT) sh.found_c = last == SR_BINS - 1 ? (unsigned)s.V : c_in + c1[0] + (last % SR_BPT ? c1[1] : 0u);
+    __syncthreads();
+    if (sh.found_c <= SR_LIST) {
+      // ---- candidates in index order, to rank 0: behind those of the ranks
+      // before, whose number the histograms tell (the last bin is not counted
+      // there, but rows so short have one rank)
+      const float edge = 8388608.f + (float)last;
+      auto candidate = [&](float x) { return row.bin_bits(x) <= edge && x > -INFINITY; };
+      unsigned hits = 0, hits_t;
+      u64 base = (SR_BPT * tid <= last ? lower[0] : 0) + (SR_BPT * tid + 1 <= last ? lower[1] : 0), base_t;
+      u64 fours = 0;  // the groups of four that hold any: the bins fall with the logit, so the largest tells
+      for (int i = 0; i < per / 4; i++) {
+        const float4 v = mine[i];
+        if (candidate(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)))) {
+          fours |= 1ull << i;
+          hits += candidate(v.x) + candidate(v.y) + candidate(v.z) + candidate(v.w);
+        }
+      }
+      const unsigned own = hits;
+      block_scan(sh, base, hits, &base_t, &hits_t);
+      const int total = last == SR_BINS - 1 ? (int)hits_t : (int)sh.found_c;
+      int2* to = peer(sh.list.xi, 0, C) + (int)base_t + hits - own;
+      for (; fours; fours &= fours - 1) {
+        const int i = __ffsll((long long)fours) - 1;
+        const float4 v = mine[i];
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (candidate(x[j])) *to++ = make_int2(__float_as_int(x[j]), first_i + 4 * i + j);
+      }
+      cluster_barrier(C);
+      const bool alone = !by_p || by_k;  // rank 0 needs nothing more of its peers
+      if (alone && rank) return;
+      // ---- rank 0 orders them: into their bins, whose beginnings the histogram
+      // tells, then by counting inside a bin (a few elements; all of them when
+      // they are equal). Thread t gets places each * t and on, with the exact mass before them
+      u64 f[SR_EPT] = {}, o[SR_EPT] = {}, before[SR_EPT] = {};
+      const int each_t = (total + SR_THREADS - 1) / SR_THREADS;
+      if (rank == 0) {
+        unsigned* begin = reinterpret_cast<unsigned*>(sh.hist);  // read last before the barrier above
+        begin[SR_BPT * tid] = c_in;
+        begin[SR_BPT * tid + 1] = c_in + c1[0];
+        __syncthreads();
+        for (int i = tid; i < total; i += SR_THREADS) {
+          const float x = __int_as_float(sh.list.xi[i].x);
+          sh.list.order[atomicAdd(&begin[row.bin_of(x)], 1u)] = ((u64)key_of(x) << 32) | (0xffffffffu - (unsigned)i);
+        }
+        __syncthreads();  // a bin begins where the one before it ended
+        int at[SR_EPT];
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++) {
+          const int e = tid + j * SR_THREADS;
+          if (e >= total) continue;
+          o[j] = sh.list.order[e];
+          const int b = row.bin_of(of_key((uint32_t)(o[j] >> 32)));
+          const int from = b ? (int)begin[b - 1] : 0, end = (int)begin[b];
+          at[j] = from;
+          for (int i = from; i < end; i++) at[j] += sh.list.order[i] > o[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++)
+          if (tid + j * SR_THREADS < total) sh.list.order[at[j]] = o[j];
+        __syncthreads();
+        u64 m = 0, mt;
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++) {
+          const int e = each_t * tid + j;
+          o[j] = 0;
+          if (j < each_t && e < total) {
+            o[j] = sh.list.order[e];
+            f[j] = row.weight(of_key((uint32_t)(o[j] >> 32)));
+          }
+          before[j] = m;
+          m += f[j];
+        }
+        const u64 own_mass = m;
+        unsigned zero = 0, zero_t;
+        block_scan(sh, m, zero, &mt, &zero_t);
+#pragma unroll
+        for (int j = 0; j < SR_EPT; j++) before[j] += m - own_mass;
+      }
+      auto place = [&](int j) { return j < each_t ? min(each_t * tid + j, SR_LIST) : SR_LIST; };
+      const int nk = by_k ? min(k, total) : total;
+      for (int pass = 0;; pass++) {  // at most two: the second with the row's exact mass
+        if (rank == 0) {
+          u64 lo = 0, hi = 0;  // the running mass that top-p asks for, as far as it is known
+          if (by_p) {
+            if (by_k) {
+              if (tid == 0) sh.found_m = 0;
+              __syncthreads();
+#pragma unroll
+              for (int j = 0; j < SR_EPT; j++)
+                if (place(j) == nk - 1) sh.found_m = before[j] + f[j];
+              __syncthreads();
+              lo = hi = row.share(sh.found_m);
+            } else if (pass) {
+              all = 0;
+              for (int q = 0; q < C; q++) all += sh.all[q];
+              lo = hi = row.share(all);
+            } else {
+              double z = 0;
+              for (int q = 0; q < C; q++) z += sh.sum[q] + sh.ones[q];
+              const double err = row.off_by((float)z);
+              lo = row.share((u64)(z * (1.0 - err) * 35184372088832.0));  // 2^45
+              hi = row.share((u64)(z * (1.0 + err) * 35184372088832.0) + 1);
+            }
+          }
+          // kept masses in index order; two ends of the top-p mass must keep the same ones,
+          // and a list that ends before them decides nothing
+          bool unsure = false, past = false, ended = false;
+          u64 kept[SR_EPT] = {};
+#pragma unroll
+          for (int j = 0; j < SR_EPT; j++) {
+            if (place(j) < nk && (!by_p || before[j] < lo)) kept[j] = by_m ? row.weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
+            unsure |= by_p && place(j) < nk && before[j] >= lo && before[j] < hi;
+            if (by_p && !covers && place(j) == total - 1) {
+              ended = before[j] + f[j] < hi;
+              past = before[j] + f[j] < lo;
+            }
+          }
+          const int doubt = __syncthreads_or(unsure || ended), whole = __syncthreads_or(past);
+          const int todo = whole ? SR_WHOLE : doubt ? SR_EXACT : SR_DONE;
+          if (todo == SR_DONE) {
+#pragma unroll
+            for (int j = 0; j < SR_EPT; j++)
+              if (place(j) < total) sh.list.order[0xffffffffu - (uint32_t)o[j]] = kept[j];
+            __syncthreads();
+            u64 m = 0, mass, fk[SR_EPT];
+#pragma unroll
+            for (int j = 0; j < SR_EPT; j++) {
+              fk[j] = place(j) < total ? sh.list.order[place(j)] : 0;
+              m += fk[j];
+            }
+            const u64 own_mass = m;
+            unsigned zero = 0, zero_t;
+            block_scan(sh, m, zero, &mass, &zero_t);
+            const u64 to = row.draw(mass);
+            u64 run = m - own_mass;
+            int win = -1;
+#pragma unroll
+            for (int j = 0; j < SR_EPT; j++) {
+              if (fk[j] && run < to && to <= run + fk[j]) win = place(j);
+              run += fk[j];
+            }
+            if (win >= 0) row.finish(sh.list.xi[win].y, __int_as_float(sh.list.xi[win].x));
+          } else if (tid < C) {
+            peer(&sh, tid, C)->again = todo;
+          }
+        }
+        if (alone) return;
+        cluster_barrier(C);  // rank 0 has told its peers what it needs
+        const int todo = sh.again;
+        if (todo == SR_DONE) return;
+        if (todo == SR_WHOLE) break;
+        // the exact mass of the row
+        all = 0;
+        row.each([&](const float (&x)[4], int) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) all += row.weight(x[j]);
+        });
+        all = warp_sum64(all);
+        __syncthreads();  // `again` and red_m have been read
+        if (lane == 0) sh.red_m[warp] = all;
+        if (tid == 0) sh.again = SR_DONE;
+        __syncthreads();
+        if (warp == 0) {
+          all = warp_sum64(lane < SR_WARPS ? sh.red_m[lane] : 0);
+          if (lane == 0) peer(sh.all, 0, C)[rank] = all;
+        }
+        cluster_barrier(C);
+      }
+    }
+  }
+
+  const Row apart = row;  // in memory for this call only
+  finish_long(apart, kbin, pbin, kabove);
+}
+
 std::mutex g_attr_mu;
 bool g_attr_done[OPS_MAX_DEV];
 int set_attributes(int device) {
@@ -1144,8 +1198,9 @@ int launch_sample_rows(const wg_sample& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));
   // CTAs a row: 8 while they all fit the SMs, else 4 (two halves of a row of
   // 51866 fp32 leave one CTA to an SM), none with less than 2048 elements
-  // (their exchanges cost more than such slices). Measured at 51866 fp32: one
-  // row 21 / 16 / 13 us with 2 / 4 / 8 CTAs; 320 rows with a top-k 108 / 74 / 91.
+  // (their exchanges cost more than such slices). Measured with 2 / 4 / 8 CTAs
+  // at a top-k: one row of 51865 fp32 21 / 16 / 14 us, 48 of 51864 f16 22 / 21 /
+  // 24, 320 of 51866 fp32 102 / 67 / 104.
   int C = p.R * 8 <= 148 ? 8 : 4;
   while (C > 1 && p.V <= 2048 * (C / 2)) C /= 2;
   // elements a thread: 4 times an odd number that covers the slice and its padding
