@@ -19,16 +19,10 @@ DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 ITEM = {"f32": 4, "f16": 2, "bf16": 2}
 
 
-wgdec = None
-
-
 def _wgdec():
-    """The framework's module, imported once (its folder's name is no module name)."""
-    global wgdec
-    if wgdec is None:
+    if str(ROOT / "whisper.go_b200") not in sys.path:
         sys.path.insert(0, str(ROOT / "whisper.go_b200"))
-        import wgdec as module
-        wgdec = module
+    import wgdec
     return wgdec
 
 
@@ -351,9 +345,9 @@ def run(s):
         _append(s)
         _read(s)
         return {"k": s["k_out"], "v": s["v_out"], "scales": s["scales"]}
-    lib = _wgdec()
+    wgdec = _wgdec()
     if op == "plan":
-        lib.kv_plan(s["lens"], s["new"], case["page"], s["free"], s["cursor"], s["table"], s["slots"], s["cu"],
+        wgdec.kv_plan(s["lens"], s["new"], case["page"], s["free"], s["cursor"], s["table"], s["slots"], s["cu"],
                       s["status"], cursor_out=s["cursor_out"])
         return {"table": s["table"], "slots": s["slots"], "cu": s["cu"], "cursor": s["cursor_out"],
                 "status": s["status"]}
@@ -362,7 +356,7 @@ def run(s):
                              causal=case["causal"], scale=s["scale"], out=s["out"])
         return s["out"]
     if op == "sample":
-        lib.sample_rows(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"],
+        wgdec.sample_rows(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"],
                           min_p=s["min_p"], tokens=s["tokens"], logprobs=s["logprobs"])
         return {"tokens": s["tokens"], "logprobs": s["logprobs"]}
     s["cache"].append(s["k"], s["v"], s["slots"])
