@@ -431,7 +431,8 @@ int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, void* k, void*
  * Rows of `out` that belong to no request are left as they were; a request
  * whose cu_q pair is out of range or descending has no rows. No row may
  * belong to two requests.
- * max_q: no request has more query rows (rows past it are not computed);
+ * max_q: no request has more query rows (rows past it are not computed; what
+ * lies above n_q counts as n_q; times n_head / n_kv_head at most 2^30);
  * max_kv: the longest kv_lens, a hint for how to split the work (any value
  * gives the same sums up to rounding).
  * q: WG_DT_*; its rows enter the product in f16 after an exact scaling by a power of

@@ -368,6 +368,31 @@ def test_attention_nan_and_infinite_queries_stay_in_their_rows():
         assert torch.equal(out[r], clean[r])
 
 
+@pytest.mark.parametrize("nq", [[30, 9], [3, 2]], ids=str)
+def test_attention_bounds_far_above_the_queries(nq):
+    """max_q is a bound: "no limit" computes the same rows as n_q does, bit for
+    bit (and as the tight value, where that chooses the same kernel), and
+    nothing around them is touched."""
+    rng = np.random.default_rng(sum(nq))
+    page, H, G, D, lens = 16, 1, 2, 64, [37, 20]
+    codes, scales, cache = make_cache(rng, 8, page, H, D)
+    table = i32(rng.permutation(8)[:6].reshape(2, 3))
+    cu = np.concatenate([[0], np.cumsum(nq)])
+    q = rows(rng, int(cu[-1]), H * G, D, "f16", spread=False)
+    outs = []
+    for max_q in (max(nq), 2 ** 31 - 1, int(cu[-1])):
+        buf = torch.full((256 + int(cu[-1]) + 256, H * G, D), 77.0, dtype=torch.float16, device=DEV)
+        cache.attention(q, i32(cu), i32(lens), table, max_q=max_q, max_kv=37, out=buf[256:-256])
+        assert (buf[:256] == 77.0).all() and (buf[-256:] == 77.0).all()
+        outs.append(host(buf[256:-256]))
+    want, most = ref.attention(codes, scales, host(q), cu, lens, host(table), H * G, True, D ** -0.5)
+    for out in outs:
+        check_attn(out, want, most, "f16", "f16", host(q), codes, scales, D ** -0.5, 37)
+    np.testing.assert_array_equal(outs[1], outs[2])
+    if max(nq) * G > 16:
+        np.testing.assert_array_equal(outs[0], outs[2])
+
+
 def test_offsets_past_32_bits():
     """A cache of 4.6 GB: pages whose codes lie beyond 2^32 bytes are written, read and attended to."""
     page, H, D = 64, 20, 64

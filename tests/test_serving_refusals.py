@@ -134,3 +134,16 @@ def test_mirror_refuses_host_tensors_and_wrong_shapes():
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(wgdec.DecodeError):
         wgdec.kv_plan(i, i, 16, i, i[:1], torch.zeros(2, 2, dtype=torch.int32), i, torch.zeros(3, dtype=torch.int32), i)
+
+
+@pytest.mark.parametrize("n_q,max_q,n_head,refused", [(1 << 29, 1 << 30, 6, True), (1 << 30, (1 << 30) - 1, 4, True),
+                                                      (1 << 29, 2 ** 31 - 1, 4, False), (1, 2 ** 31 - 1, 64, False),
+                                                      (2 ** 31 - 1, 1 << 29, 4, False)])
+def test_attention_rows_are_counted_in_32_bits(n_q, max_q, n_head, refused):
+    """(query, grouped head) rows of one K/V head: the lesser of max_q and n_q counts, and at most 2^30 of them pass."""
+    p = attn(n_q=n_q, max_q=max_q, n_head=n_head, ldq=64 * n_head, ldo=64 * n_head, n_requests=0)
+    assert wgdec.lib().wg_kv8_attention(ctypes.byref(cache()), ctypes.byref(p), 0, None) == 0  # no request: no work
+    if refused or wgdec.device_count() == 0:  # what passes would run
+        p.n_requests = 2
+        status = wgdec.lib().wg_kv8_attention(ctypes.byref(cache()), ctypes.byref(p), 0, None)
+        assert status == (INVALID if refused else NO_DEVICE) and (not refused or "too many" in last())

@@ -654,14 +654,15 @@ int init_kv8_attention(int device) { return set_attributes(device); }
 int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cudaStream_t st) {
   WG_CHECK(set_attributes(device));
   const int G = p.n_head / c.n_kv_head;
+  const int max_q = p.max_q < p.n_q ? p.max_q : p.n_q;  // no request has more: a loose bound makes no empty tiles
   Kv8AttnArgs a{};
   a.codes = c.codes; a.scales = c.scales; a.num_pages = c.num_pages; a.shift = log2_of(c.page);
   a.H = c.n_kv_head; a.G = G; a.q = p.q; a.ldq = p.ldq; a.qdt = p.q_dtype; a.cu_q = p.cu_q; a.n_q = p.n_q;
   a.kv_lens = p.kv_lens; a.table = p.block_table; a.ldt = p.ld_table; a.max_pages = p.max_pages; a.R = p.n_requests;
-  a.causal = p.causal; a.max_q = p.max_q; a.scale = p.scale; a.out = p.out; a.ldo = p.ldo; a.odt = p.out_dtype;
+  a.causal = p.causal; a.max_q = max_q; a.scale = p.scale; a.out = p.out; a.ldo = p.ldo; a.odt = p.out_dtype;
   a.q_vec = p.q_dtype != WG_DT_F32 && aligned16(p.q) && p.ldq % 8 == 0;
   a.o_vec = aligned16(p.out) && p.ldo % 8 == 0;
-  const int64_t rows = (int64_t)p.max_q * G;
+  const int64_t rows = (int64_t)max_q * G;
   const int64_t kv = p.max_kv < ((int64_t)p.max_pages << a.shift) ? p.max_kv : (int64_t)p.max_pages << a.shift;
   if (rows > 16) return launch_kv8_prompt(a, c.head_dim, kv, st);  // more than one MMA's rows
   const int64_t tiles = 1, units = (int64_t)c.n_kv_head * p.n_requests;
@@ -722,6 +723,11 @@ extern "C" int wg_kv8_attention(const wg_kv8* cache, const wg_kv8_attn* p, int d
     return WG_ERR_INVALID;
   }
   if (p->n_requests == 0 || p->n_q == 0 || p->max_q == 0) return WG_OK;
+  // the kernels count a head's (query, grouped head) rows, rounded up to a tile, in 32 bits
+  if ((int64_t)(p->max_q < p->n_q ? p->max_q : p->n_q) * (p->n_head / cache->n_kv_head) > KV8_MAX_ATTN_ROWS) {
+    set_error("%s: %d query rows of %d grouped heads are too many", what, p->n_q, p->n_head / cache->n_kv_head);
+    return WG_ERR_INVALID;
+  }
   const int64_t width = (int64_t)p->n_head * cache->head_dim;
   if (!p->q || !p->out || !p->cu_q || !p->kv_lens || (p->max_pages > 0 && !p->block_table) || p->ldq < width ||
       p->ldo < width || reinterpret_cast<uintptr_t>(p->q) % dt_bytes(p->q_dtype) ||

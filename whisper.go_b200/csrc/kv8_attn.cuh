@@ -32,6 +32,7 @@ struct Kv8AttnArgs {
 };
 
 
+constexpr int KV8_MAX_ATTN_ROWS = 1 << 30;  // (query, grouped head) rows of one request and K/V head
 constexpr int KV8_MAX_SPLIT = 16;  // CTAs that share a tile's tokens (a cluster)
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
