@@ -388,6 +388,7 @@ typedef struct wg_kv8 {
  *   cu_new[0..R]           : where each request's new tokens begin in `slots`
  *   *cursor_out            : the advanced cursor (may be `cursor` itself)
  *   status[0], status[1]   : WG_PLAN_*, and the pages taken
+ * R from 1 to 2^30, n_slots at most 2^30.
  * A step that cannot be planned takes no page: status holds the largest code
  * that applies, slots are all -1, cu_new all 0, the cursor and the table stay. */
 enum {

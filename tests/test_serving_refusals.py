@@ -147,3 +147,10 @@ def test_attention_rows_are_counted_in_32_bits(n_q, max_q, n_head, refused):
         p.n_requests = 2
         status = wgdec.lib().wg_kv8_attention(ctypes.byref(cache()), ctypes.byref(p), 0, None)
         assert status == (INVALID if refused else NO_DEVICE) and (not refused or "too many" in last())
+
+
+@pytest.mark.parametrize("R,n_slots", [((1 << 30) + 1, 8), (2 ** 31 - 1, 8), (3, (1 << 30) + 1), (3, 2 ** 31 - 1)])
+def test_plan_refuses_what_its_indices_cannot_step_over(R, n_slots):
+    """The kernel steps 32-bit indices by up to 2^18 past R and n_slots, so both end at 2^30."""
+    assert wgdec.lib().wg_kv_plan(PTR, PTR, R, 16, PTR, 10, PTR, PTR, PTR, 4, 4, PTR, n_slots, PTR, PTR, 0, None) == INVALID
+    assert last().startswith("wg_kv_plan")

@@ -23,6 +23,7 @@ namespace {
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_CLUSTER = 8;
 constexpr int PLAN_CTAS = 64;
+constexpr int PLAN_MAX = 1 << 30;  // requests, and slots: the kernel steps 32-bit indices past them
 
 struct PlanArgs {
   const int* lens;
@@ -212,9 +213,10 @@ extern "C" int wg_kv_plan(const int32_t* lens, const int32_t* new_tokens, int R,
     set_error("wg_kv_plan: null argument");
     return WG_ERR_INVALID;
   }
-  if (R <= 0 || !kv_page_ok(page) || n_free < 0 || n_slots < 0 || max_pages <= 0 || ld_table < max_pages) {
-    set_error("wg_kv_plan: bad argument (R %d, page %d (a power of two, 16 to 128), n_free %d, n_slots %d, "
-              "max_pages %d, ld_table %lld)", R, page, n_free, n_slots, max_pages, (long long)ld_table);
+  if (R <= 0 || R > PLAN_MAX || !kv_page_ok(page) || n_free < 0 || n_slots < 0 || n_slots > PLAN_MAX || max_pages <= 0 ||
+      ld_table < max_pages) {
+    set_error("wg_kv_plan: bad argument (R %d and n_slots %d (at most %d), page %d (a power of two, 16 to 128), n_free %d, "
+              "max_pages %d, ld_table %lld)", R, n_slots, PLAN_MAX, page, n_free, max_pages, (long long)ld_table);
     return WG_ERR_INVALID;
   }
   OpDevice dev;
