@@ -393,6 +393,50 @@ def test_attention_bounds_far_above_the_queries(nq):
         np.testing.assert_array_equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("nq,G,page", [(1, 1, 64), (5, 1, 16), (1, 4, 32), (3, 4, 16), (16, 1, 64), (30, 1, 32)])
+def test_attention_queries_of_one_sign(nq, G, page):
+    """Queries far from zero on one side, keys whose sums nearly cancel: every
+    product and partial sum of codes and these queries fits 24 bits, so scores
+    carry no rounding of the sum of the queries."""
+    rng = np.random.default_rng(nq * G + page)
+    H, D, n = 2, 128, 100
+    codes, scales, cache = make_cache(rng, 8, page, H, D)
+    codes[:, 0, :, :, 1::2] = -codes[:, 0, :, :, 0::2]
+    scales[:, 0] = 1.0
+    cache.codes.copy_(torch.tensor(codes))
+    cache.scales.copy_(torch.tensor(scales))
+    table = rng.permutation(8)[None]
+    q = rows(rng, nq, H * G, D, "f16", spread=False)
+    q.copy_(q.float().clamp(-3, 3) * 0.05 + 8.0)  # steps of 2^-7 below 8, 2^-8 above
+    out = torch.full_like(q, 77.0)
+    cache.attention(q, i32([0, nq]), i32([n]), i32(table), max_q=nq, max_kv=n, causal=False, out=out)
+    want, most = ref.attention(codes, scales, host(q), [0, nq], [n], table, H * G, False, D ** -0.5)
+    check_attn(host(out), want, most, "f16", "f16", host(q), codes, scales, D ** -0.5, n)
+
+
+@pytest.mark.parametrize("nq,G,D,page", [(1, 1, 64, 64), (1, 8, 64, 16), (1, 2, 128, 32), (12, 1, 64, 64), (4, 4, 128, 16),
+                                         (40, 1, 64, 32)])
+def test_attention_small_values_beside_a_strong_zero(nq, G, D, page):
+    """A token 9.6 nats above 63 others, its value 0 and theirs one step: the
+    output is their weights alone (each an f16 of 11 bits, all alike, 2^-11),
+    with the scores and fp32 sums within 2^-13 and the output rounded by
+    2^-11. No rounding of the strong token's weight times an offset is in it."""
+    pages = 64 // page
+    codes = np.zeros((pages, 2, 1, page, D), np.int8)
+    codes[:, 1] = 1
+    codes[0, 0, 0, 7, 0], codes[0, 1, 0, 7] = 127, 0
+    scales = np.ones((pages, 2, 1), np.float32)
+    scales[:, 1] = 16.0
+    cache = wgdec.Kv8Cache(torch.tensor(codes, device=DEV), torch.tensor(scales, device=DEV))
+    q = torch.zeros(nq, G, D, dtype=torch.float16, device=DEV)
+    q[:, :, 0] = 9.6 / (127 * D ** -0.5)
+    top = 127 * D ** -0.5 * float(q[0, 0, 0])
+    out = torch.empty_like(q)
+    cache.attention(q, i32([0, nq]), i32([64]), i32(np.arange(pages)[None]), max_q=nq, max_kv=64, causal=False, out=out)
+    want = 16.0 * 63 * np.exp(-top) / (1 + 63 * np.exp(-top))
+    assert np.abs(host(out) / want - 1).max() <= 2.0 ** -11 + 2.0 ** -13 + 2.0 ** -11
+
+
 def test_offsets_past_32_bits():
     """A cache of 4.6 GB: pages whose codes lie beyond 2^32 bytes are written, read and attended to."""
     page, H, D = 64, 20, 64

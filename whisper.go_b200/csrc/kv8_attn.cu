@@ -16,9 +16,11 @@
 //    tokens, beams and grouped heads take one read. Up to 8 of them are the
 //    columns of the MMA and tokens (then dims) its 16 rows, which halves the
 //    MMAs and accumulators; 9 to 16 are its rows;
-//  - a byte becomes 1152 + code by one byte permute for two; the 1152 comes out
-//    through the accumulator (K: 1152 * sum q; V: 1152 * the row's weights, which
-//    an MMA over ones sums);
+//  - two bytes become 1152 + code by one byte permute, and codes by one packed
+//    subtraction. (Left in and taken out through the accumulators the 1152 saves
+//    that subtraction, 50.4 us against 51.8 in the cross case below, but 1152 *
+//    sum q and 1152 * sum p leave their rounding behind: an output of small
+//    values beside a strong zero was 10 % off.)
 //  - every warp streams its own 32-token chunks through its own ring of
 //    cp.async stages (no CTA barrier in the loop, no bounded wait needed: a
 //    cp.async group always completes);
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
   // are scaled by a power of two so that they fit f16: bf16 stays exact down
   // to 2^-23 of the row's largest value, fp32 is rounded to f16's 11 bits.
   uint32_t qa_f[D / 16][4];
-  float mul_a, mul_b, q_sum = 0.f;
+  float mul_a, mul_b;
   {
     float e[2];
     const float sign = p.scale < 0.f ? -1.f : 1.f;
@@ -242,7 +244,6 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
         const int o = (j / 4) * 16 + (j % 4) * 4;
         qa_f[j][half] = pack_f16(x[o] * up, x[o + 1] * up);
         qa_f[j][2 + half] = pack_f16(x[o + 2] * up, x[o + 3] * up);
-        if (HALF) q_sum += sum_f16(qa_f[j][0]) + sum_f16(qa_f[j][2]);  // of the row's f16 values
       }
     }
     mul_a = e[0] * fabsf(p.scale) * KV8_LOG2E;  // scores in units of log 2
@@ -255,15 +256,11 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
   for (int j = 0; j < OT; j++) o_acc[j][0] = o_acc[j][1] = o_acc[j][2] = o_acc[j][3] = 0.f;
   // of rows g and g + 8, or with few rows of queries 2t and 2t + 1
   float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
-  float mul0 = 0.f, mul1 = 0.f, bias0 = 0.f, bias1 = 0.f;
+  float mul0 = 0.f, mul1 = 0.f;
   int lim0 = 0, lim1 = 0;
   if (HALF) {  // lane 4r + t holds row r's factors
-    q_sum += __shfl_xor_sync(0xffffffffu, q_sum, 1);
-    q_sum += __shfl_xor_sync(0xffffffffu, q_sum, 2);
     mul0 = __shfl_sync(0xffffffffu, mul_a, 8 * t);
     mul1 = __shfl_sync(0xffffffffu, mul_a, 8 * t + 4);
-    bias0 = -1152.f * __shfl_sync(0xffffffffu, q_sum, 8 * t);
-    bias1 = -1152.f * __shfl_sync(0xffffffffu, q_sum, 8 * t + 4);
     lim0 = __shfl_sync(0xffffffffu, lim_a, 8 * t);
     lim1 = __shfl_sync(0xffffffffu, lim_a, 8 * t + 4);
   }
@@ -278,7 +275,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
 
     if constexpr (HALF) {
       // ---- at most 8 rows: tokens (then dims) are the MMA's 16 rows, queries
-      // its 8 columns. q . (codes + 1152), the 1152 taken out through C
+      // its 8 columns
       float s[2][4];
 #pragma unroll
       for (int i = 0; i < 2; i++) {
@@ -291,9 +288,9 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const int ks = b * 4 + j;
-            const uint32_t a0 = codes_up<0x4140>(u[j]), a1 = codes_up<0x4140>(v[j]);
-            const uint32_t a2 = codes_up<0x4342>(u[j]), a3 = codes_up<0x4342>(v[j]);
-            if (ks == 0) mma16816_cols(s[i], a0, a1, a2, a3, qa_f[0][0], qa_f[0][2], bias0, bias1);
+            const uint32_t a0 = codes_f16<0x4140>(u[j]), a1 = codes_f16<0x4140>(v[j]);
+            const uint32_t a2 = codes_f16<0x4342>(u[j]), a3 = codes_f16<0x4342>(v[j]);
+            if (ks == 0) mma16816_zero(s[i], a0, a1, a2, a3, qa_f[0][0], qa_f[0][2]);
             else mma16816(s[i], a0, a1, a2, a3, qa_f[ks][0], qa_f[ks][2]);
           }
         }
@@ -344,12 +341,12 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
         pb[i][0] = transpose8(pack_f16(ex2(fmaf(s[i][0], step0, -ref0)), ex2(fmaf(s[i][1], step1, -ref1))));
         pb[i][1] = transpose8(pack_f16(ex2(fmaf(s[i][2], step0, -ref0)), ex2(fmaf(s[i][3], step1, -ref1))));
       }
-      // their sums, by the same MMA over a matrix of ones: they go into l (so
-      // that the rounded weights sum to one) and take the 1152 out of V's codes
+      // their sums, by the same MMA over a matrix of ones, go into l (so that the
+      // rounded weights sum to one)
       constexpr uint32_t ONES = 0x3c003c00u;
       float rs[2][4];
-      mma16816_cols(rs[0], ONES, ONES, ONES, ONES, pb[0][0], pb[0][1], 0.f, 0.f);
-      if (SMALL) mma16816_cols(rs[1], ONES, ONES, ONES, ONES, pb[1][0], pb[1][1], 0.f, 0.f);
+      mma16816_zero(rs[0], ONES, ONES, ONES, ONES, pb[0][0], pb[0][1]);
+      if (SMALL) mma16816_zero(rs[1], ONES, ONES, ONES, ONES, pb[1][0], pb[1][1]);
       else mma16816(rs[0], ONES, ONES, ONES, ONES, pb[1][0], pb[1][1]);
       l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
       l_b += SMALL ? rs[0][1] + rs[1][1] : rs[0][1];
@@ -368,10 +365,9 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
           for (int hf = 0; hf < 2; hf++) {
             const uint32_t z0 = __byte_perm(w[hf][0][k], w[hf][1][k], e ? 0x7362 : 0x5140);
             const uint32_t z1 = __byte_perm(w[hf][2][k], w[hf][3][k], e ? 0x7362 : 0x5140);
-            const uint32_t a0 = codes_up<0x4140>(z0), a1 = codes_up<0x4342>(z0);
-            const uint32_t a2 = codes_up<0x4140>(z1), a3 = codes_up<0x4342>(z1);
-            if (SMALL || hf == 0)
-              mma16816_cols(acc[hf], a0, a1, a2, a3, pb[hf][0], pb[hf][1], -1152.f * rs[hf][0], -1152.f * rs[hf][1]);
+            const uint32_t a0 = codes_f16<0x4140>(z0), a1 = codes_f16<0x4342>(z0);
+            const uint32_t a2 = codes_f16<0x4140>(z1), a3 = codes_f16<0x4342>(z1);
+            if (SMALL || hf == 0) mma16816_zero(acc[hf], a0, a1, a2, a3, pb[hf][0], pb[hf][1]);
             else mma16816(acc[0], a0, a1, a2, a3, pb[1][0], pb[1][1]);
           }
 #pragma unroll
@@ -394,7 +390,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             if (b == 0 && j == 0)
-              mma16816_c(s[n], qa_f[0], codes_f16<0x4140>(w[0]), codes_f16<0x4342>(w[0]), 0.f, 0.f);
+              mma16816_zero(s[n], qa_f[0], codes_f16<0x4140>(w[0]), codes_f16<0x4342>(w[0]));
             else
               mma16816(s[n], qa_f[b * 4 + j], codes_f16<0x4140>(w[j]), codes_f16<0x4342>(w[j]));
           }
@@ -457,13 +453,13 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
         pf[n >> 1][(n & 1) * 2 + 1] =
             pack_f16(ex2(fmaf(s[n][2], step_b, -ref_b)), ex2(fmaf(s[n][3], step_b, -ref_b)));
       }
-      // their row sums, by the same MMA over a matrix of ones: they go into l (so
-      // that the rounded weights sum to one) and take the 1152 out of the codes
+      // their row sums, by the same MMA over a matrix of ones, go into l (so that
+      // the rounded weights sum to one)
       float rs[2][4];
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
         if (hf == 1 && !SMALL) mma16816(rs[0], pf[1], 0x3c003c00u, 0x3c003c00u);
-        else mma16816_c(rs[hf], pf[hf], 0x3c003c00u, 0x3c003c00u, 0.f, 0.f);
+        else mma16816_zero(rs[hf], pf[hf], 0x3c003c00u, 0x3c003c00u);
       }
       l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
       l_b += SMALL ? rs[0][2] + rs[1][2] : rs[0][2];
@@ -488,9 +484,9 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
           float acc[2][4];
 #pragma unroll
           for (int hf = 0; hf < 2; hf++) {
-            const uint32_t b0 = (dd & 1) ? codes_up<0x4342>(z[hf][dd >> 1]) : codes_up<0x4140>(z[hf][dd >> 1]);
-            const uint32_t b1 = (dd & 1) ? codes_up<0x4342>(z[hf][2 + (dd >> 1)]) : codes_up<0x4140>(z[hf][2 + (dd >> 1)]);
-            if (SMALL || hf == 0) mma16816_c(acc[hf], pf[hf], b0, b1, -1152.f * rs[hf][0], -1152.f * rs[hf][2]);
+            const uint32_t b0 = (dd & 1) ? codes_f16<0x4342>(z[hf][dd >> 1]) : codes_f16<0x4140>(z[hf][dd >> 1]);
+            const uint32_t b1 = (dd & 1) ? codes_f16<0x4342>(z[hf][2 + (dd >> 1)]) : codes_f16<0x4140>(z[hf][2 + (dd >> 1)]);
+            if (SMALL || hf == 0) mma16816_zero(acc[hf], pf[hf], b0, b1);
             else mma16816(acc[0], pf[1], b0, b1);
           }
 #pragma unroll

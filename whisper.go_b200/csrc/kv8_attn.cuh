@@ -41,21 +41,16 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// d = a * b + c for a C that is the same for a row's columns (c0: row g, c1: row g + 8)
-__device__ __forceinline__ void mma16816_c(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
-                                           float c1) {
+// d = a * b
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-// d = a * b + c for a C that is the same for a column's rows (c0: column 2t, c1: column 2t + 1)
-__device__ __forceinline__ void mma16816_cols(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1, float c0, float c1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  mma16816_zero(d, a[0], a[1], a[2], a[3], b0, b1);
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -68,24 +63,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// Bytes (already offset by 128: code + 128) LO / HI of w as an f16 pair:
-// 0x6400 | u is 1024 + u, exact: code + 1152.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes_up(uint32_t w) { return __byte_perm(w, 0x64646464u, SEL); }
-// The codes themselves.
+// Two bytes of w (already offset by 128: code + 128) as an f16 pair of codes:
+// 0x6400 | u is 1024 + u, exact, and so is its difference from 1152.
 template <int SEL>
 __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-  const uint32_t h = codes_up<SEL>(w);
+  const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ float sum_f16(uint32_t w) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return f.x + f.y;
 }
 // 2^x, x <= 0 (hardware approximation, 2^-22 relative; 0 for -inf)
 __device__ __forceinline__ float ex2(float x) {

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(PW * 32, D == 64 ? 4 : 2) prompt_attn_kernel(c
       for (int kk = 0; kk < KS / 2; kk++) {
         uint32_t b[4];
         ldm4(b, ku + f_off<D>(n * 8 + (lane & 7), kk * 4 + (lane >> 3)));
-        if (kk == 0) mma16816_c(s[n], qf[0], b[0], b[1], 0.f, 0.f);
+        if (kk == 0) mma16816_zero(s[n], qf[0], b[0], b[1]);
         else mma16816(s[n], qf[2 * kk], b[0], b[1]);
         mma16816(s[n], qf[2 * kk + 1], b[2], b[3]);
       }
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(PW * 32, D == 64 ? 4 : 2) prompt_attn_kernel(c
       pf[n >> 1][(n & 1) * 2 + 1] = pack_f16(ex2(s[n][2] - ref_b), ex2(s[n][3] - ref_b));
     }
     float rs[4];
-    mma16816_c(rs, pf[0], 0x3c003c00u, 0x3c003c00u, 0.f, 0.f);
+    mma16816_zero(rs, pf[0], 0x3c003c00u, 0x3c003c00u);
 #pragma unroll
     for (int q = 1; q < 4; q++) mma16816(rs, pf[q], 0x3c003c00u, 0x3c003c00u);
     l_a += rs[0];
@@ -293,8 +293,8 @@ __global__ void __launch_bounds__(PW * 32, D == 64 ? 4 : 2) prompt_attn_kernel(c
           uint32_t b[4];
           ldm4t(b, vu + f_off<D>(step * 16 + (lane & 15), j + (lane >> 4)));
           if (k == 0) {
-            mma16816_c(a0, pf[step], b[0], b[1], 0.f, 0.f);
-            mma16816_c(a1, pf[step], b[2], b[3], 0.f, 0.f);
+            mma16816_zero(a0, pf[step], b[0], b[1]);
+            mma16816_zero(a1, pf[step], b[2], b[3]);
           } else {
             mma16816(a0, pf[step], b[0], b[1]);
             mma16816(a1, pf[step], b[2], b[3]);
