@@ -437,6 +437,36 @@ def test_attention_small_values_beside_a_strong_zero(nq, G, D, page):
     assert np.abs(host(out) / want - 1).max() <= 2.0 ** -11 + 2.0 ** -13 + 2.0 ** -11
 
 
+@pytest.mark.parametrize("gap", [9.0, 17.5, 19.0, 23.0])
+@pytest.mark.parametrize("nq,G,D,page", [(1, 1, 64, 64), (1, 4, 128, 16), (1, 12, 64, 16), (1, 16, 128, 32), (5, 1, 64, 16),
+                                         (33, 1, 64, 16), (20, 1, 128, 64)])
+def test_attention_many_weak_tokens_under_a_strong_one(nq, G, D, page, gap):
+    """One token `gap` nats above n others that share what is left of the mass,
+    and all of the output: its own value is 0. The weak weights are all alike,
+    so their rounding to f16 shows as it is: by 2^-11 where they are normal
+    numbers (2^-28 of the largest and up), else by 2^-39 of the largest. The
+    scores (25 to 33 octaves in fp32, products and sums of one term) and the
+    fp32 sums stay within 2^-13, the output is rounded by 2^-11."""
+    n = 60000
+    pages = -(-n // page)
+    strong = 31 * page + 7
+    codes = np.zeros((pages, 2, 1, page, D), np.int8)
+    codes[:, 1] = 100
+    codes[31, 0, 0, 7, 0], codes[31, 1, 0, 7] = 127, 0
+    scales = np.ones((pages, 2, 1), np.float32)
+    scales[:, 1] = 2.0 ** 6
+    cache = wgdec.Kv8Cache(torch.tensor(codes, device=DEV), torch.tensor(scales, device=DEV))
+    q = torch.zeros(nq, G, D, dtype=torch.float16, device=DEV)
+    q[:, :, 0] = gap / (127 * D ** -0.5)
+    top = 127 * D ** -0.5 * float(q[0, 0, 0])
+    out = torch.empty_like(q)
+    cache.attention(q, i32([0, nq]), i32([n]), i32(np.arange(pages)[None]), max_q=nq, max_kv=n, causal=False, out=out)
+    weak = np.exp(-top) * (n - 1)
+    want = 6400.0 * weak / (1 + weak)
+    tol = 2.0 ** -11 if np.exp(-top) >= 2.0 ** -28 else 2.0 ** -39 / np.exp(-top)
+    assert strong < n and np.abs(host(out) / want - 1).max() <= tol + 2.0 ** -13 + 2.0 ** -11
+
+
 def test_offsets_past_32_bits():
     """A cache of 4.6 GB: pages whose codes lie beyond 2^32 bytes are written, read and attended to."""
     page, H, D = 64, 20, 64

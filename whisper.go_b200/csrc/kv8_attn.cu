@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
     __syncwarp();
     uint8_t* st = ring + stage * stage_bytes<D>();
     const float* sc = reinterpret_cast<const float*>(st + 2 * CH * D);
-    const float sk0 = sc[0], sk1 = sc[1], sv0 = sc[2], sv1 = sc[3];
+    const float sk0 = sc[0], sk1 = sc[1], sv0 = sc[2] * KV8_UNLIFT, sv1 = sc[3] * KV8_UNLIFT;
     const bool ok0 = reinterpret_cast<const int*>(sc)[4] != 0, ok1 = reinterpret_cast<const int*>(sc)[5] != 0;
 
     if constexpr (HALF) {
@@ -333,13 +333,13 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
         m_a = x0;
         m_b = x1;
       }
-      // weights rounded to f16 (2^-12 of a weight that is at most 1), queries in
-      // rows: the other operand of P.V
+      // lifted weights rounded to f16, queries in rows: the other operand of P.V
+      const float lift0 = KV8_LIFT - ref0, lift1 = KV8_LIFT - ref1;
       uint32_t pb[2][2];
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        pb[i][0] = transpose8(pack_f16(ex2(fmaf(s[i][0], step0, -ref0)), ex2(fmaf(s[i][1], step1, -ref1))));
-        pb[i][1] = transpose8(pack_f16(ex2(fmaf(s[i][2], step0, -ref0)), ex2(fmaf(s[i][3], step1, -ref1))));
+        pb[i][0] = transpose8(pack_weights(ex2(fmaf(s[i][0], step0, lift0)), ex2(fmaf(s[i][1], step1, lift1))));
+        pb[i][1] = transpose8(pack_weights(ex2(fmaf(s[i][2], step0, lift0)), ex2(fmaf(s[i][3], step1, lift1))));
       }
       // their sums, by the same MMA over a matrix of ones, go into l (so that the
       // rounded weights sum to one)
@@ -348,8 +348,8 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
       mma16816_zero(rs[0], ONES, ONES, ONES, ONES, pb[0][0], pb[0][1]);
       if (SMALL) mma16816_zero(rs[1], ONES, ONES, ONES, ONES, pb[1][0], pb[1][1]);
       else mma16816(rs[0], ONES, ONES, ONES, ONES, pb[1][0], pb[1][1]);
-      l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
-      l_b += SMALL ? rs[0][1] + rs[1][1] : rs[0][1];
+      l_a = fmaf(SMALL ? rs[0][0] + rs[1][0] : rs[0][0], KV8_UNLIFT, l_a);
+      l_b = fmaf(SMALL ? rs[0][1] + rs[1][1] : rs[0][1], KV8_UNLIFT, l_b);
       // ---- V^T.P^T: rows g and g + 8 of m-tile j are dims 2j and 2j + 1 of lane g's D/8
       const uint8_t* vs = st + CH * D;
       constexpr int VW = D / 32;  // words of a lane's dims per token
@@ -445,13 +445,14 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
         m_a = x_a;
         m_b = x_b;
       }
-      // weights rounded to f16 for the MMA (2^-12 of a weight that is at most 1)
+      // lifted weights rounded to f16 for the MMA
+      const float lift_a = KV8_LIFT - ref_a, lift_b = KV8_LIFT - ref_b;
       uint32_t pf[2][4];
 #pragma unroll
       for (int n = 0; n < 4; n++) {
-        pf[n >> 1][(n & 1) * 2] = pack_f16(ex2(fmaf(s[n][0], step_a, -ref_a)), ex2(fmaf(s[n][1], step_a, -ref_a)));
+        pf[n >> 1][(n & 1) * 2] = pack_weights(ex2(fmaf(s[n][0], step_a, lift_a)), ex2(fmaf(s[n][1], step_a, lift_a)));
         pf[n >> 1][(n & 1) * 2 + 1] =
-            pack_f16(ex2(fmaf(s[n][2], step_b, -ref_b)), ex2(fmaf(s[n][3], step_b, -ref_b)));
+            pack_weights(ex2(fmaf(s[n][2], step_b, lift_b)), ex2(fmaf(s[n][3], step_b, lift_b)));
       }
       // their row sums, by the same MMA over a matrix of ones, go into l (so that
       // the rounded weights sum to one)
@@ -461,8 +462,8 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
         if (hf == 1 && !SMALL) mma16816(rs[0], pf[1], 0x3c003c00u, 0x3c003c00u);
         else mma16816_zero(rs[hf], pf[hf], 0x3c003c00u, 0x3c003c00u);
       }
-      l_a += SMALL ? rs[0][0] + rs[1][0] : rs[0][0];
-      l_b += SMALL ? rs[0][2] + rs[1][2] : rs[0][2];
+      l_a = fmaf(SMALL ? rs[0][0] + rs[1][0] : rs[0][0], KV8_UNLIFT, l_a);
+      l_b = fmaf(SMALL ? rs[0][2] + rs[1][2] : rs[0][2], KV8_UNLIFT, l_b);
       // ---- P.V: n-tile j of lane g is dim g * (D/8) + j; tokens 2t, 2t+1, 2t+8, 2t+9 of each 16
       const uint8_t* vs = st + CH * D;
       constexpr int VW = D / 32;  // words of a lane's dims per token

@@ -75,7 +75,20 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
 }
-// 2^x, x <= 0 (hardware approximation, 2^-22 relative; 0 for -inf)
+// A pair of softmax weights, at most 2^KV8_LIFT for the row's largest, as f16.
+// Lifted, a weight is rounded by at most 2^-11 of itself down to 2^-28 of the
+// largest, and by at most 2^-39 of the largest below that; unlifted, weights
+// under 2^-25 would vanish, which under one strong token costs 60000 weak ones
+// 1e-3 of the row's mass. An exponent above the lift (the rounding of scores of
+// 2^25 and more) saturates.
+constexpr float KV8_LIFT = 14.f;
+constexpr float KV8_UNLIFT = 1.f / 16384.f;
+__device__ __forceinline__ uint32_t pack_weights(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+// 2^x, x <= KV8_LIFT (hardware approximation, 2^-22 relative; 0 for -inf)
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -266,24 +266,25 @@ __global__ void __launch_bounds__(PW * 32, D == 64 ? 4 : 2) prompt_attn_kernel(c
       m_a = x_a;
       m_b = x_b;
     }
-    // weights rounded to f16 (2^-12 of a weight that is at most 1); their sum, by
-    // the same MMA over a matrix of ones, is that of the rounded ones
+    // lifted weights rounded to f16; their sum, by the same MMA over a matrix of
+    // ones, is that of the rounded ones
+    const float lift_a = KV8_LIFT - ref_a, lift_b = KV8_LIFT - ref_b;
     uint32_t pf[4][4];
 #pragma unroll
     for (int n = 0; n < 8; n++) {
-      pf[n >> 1][(n & 1) * 2] = pack_f16(ex2(s[n][0] - ref_a), ex2(s[n][1] - ref_a));
-      pf[n >> 1][(n & 1) * 2 + 1] = pack_f16(ex2(s[n][2] - ref_b), ex2(s[n][3] - ref_b));
+      pf[n >> 1][(n & 1) * 2] = pack_weights(ex2(s[n][0] + lift_a), ex2(s[n][1] + lift_a));
+      pf[n >> 1][(n & 1) * 2 + 1] = pack_weights(ex2(s[n][2] + lift_b), ex2(s[n][3] + lift_b));
     }
     float rs[4];
     mma16816_zero(rs, pf[0], 0x3c003c00u, 0x3c003c00u);
 #pragma unroll
     for (int q = 1; q < 4; q++) mma16816(rs, pf[q], 0x3c003c00u, 0x3c003c00u);
-    l_a += rs[0];
-    l_b += rs[2];
+    l_a = fmaf(rs[0], KV8_UNLIFT, l_a);
+    l_b = fmaf(rs[2], KV8_UNLIFT, l_b);
     // ---- P.V: the tokens of a page into fresh accumulators, which its scale joins to the sum
 #pragma unroll
     for (int q = 0; q < PT / GT; q++) {
-      const float f = mt[q * (GT / 16)].y;
+      const float f = mt[q * (GT / 16)].y * KV8_UNLIFT;
 #pragma unroll
       for (int j = 0; j < NT; j += 2) {
         float a0[4], a1[4];
