@@ -436,9 +436,11 @@ int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, void* k, void*
  * lies above n_q counts as n_q; times n_head / n_kv_head at most 2^30);
  * max_kv: the longest kv_lens, a hint for how to split the work (any value
  * gives the same sums up to rounding).
- * q: WG_DT_*; its rows enter the product in f16 after an exact scaling by a power of
- * two (fp32 is rounded to 11 bits). Weights are rounded to 11 bits (to 2^-39 of the largest
- * below 2^-28 of it); sums and the softmax are fp32. out: WG_DT_F16 or WG_DT_BF16. */
+ * q: WG_DT_*; its rows enter the product in f16 after an exact scaling by a
+ * power of two: f16 as it is, bf16 exact down to 2^-31 of a head's largest
+ * magnitude, fp32 rounded to 11 bits (to 2^-39 of the largest below 2^-28 of
+ * it). Weights are rounded to 11 bits (to 2^-39 of the largest below 2^-28 of
+ * it); sums and the softmax are fp32. out: WG_DT_F16 or WG_DT_BF16. */
 typedef struct wg_kv8_attn {
   const void* q;
   int64_t ldq;

@@ -467,6 +467,50 @@ def test_attention_many_weak_tokens_under_a_strong_one(nq, G, D, page, gap):
     assert strong < n and np.abs(host(out) / want - 1).max() <= tol + 2.0 ** -13 + 2.0 ** -11
 
 
+@pytest.mark.parametrize("qdt", ["bf16", "f32"])
+@pytest.mark.parametrize("nq,G,D,page", [(1, 1, 64, 16), (2, 3, 128, 64), (11, 1, 64, 32), (24, 1, 128, 16), (24, 1, 64, 64)])
+def test_attention_queries_of_a_wide_range(nq, G, D, page, qdt):
+    """A query's largest value meets codes of 0; the rest, 2^-22 of it, make the
+    scores. 8 bits (bf16) or 11 bits (fp32) of every value reach the product."""
+    rng = np.random.default_rng(nq + D)
+    H, n = 1, 90
+    codes, scales, cache = make_cache(rng, 8, page, H, D)
+    codes[:, 0, ..., 3] = 0
+    scales[:, 0] = 2.0 ** -5
+    cache.codes.copy_(torch.tensor(codes))
+    cache.scales.copy_(torch.tensor(scales))
+    table = rng.permutation(8)[None]
+    steps = 128 if qdt == "bf16" else 1024
+    x = (1 + rng.integers(0, steps, (nq, H * G, D)) / steps) * rng.choice([-1, 1], (nq, H * G, D)) * 2.0 ** -22
+    x[..., 3] = 1.0
+    q = torch.tensor(x, dtype=DT[qdt], device=DEV)
+    np.testing.assert_array_equal(host(q), x)
+    scale = 2.0 ** 22 * D ** -0.5
+    out = torch.full((nq, H * G, D), 77.0, dtype=torch.float16, device=DEV)
+    cache.attention(q, i32([0, nq]), i32([n]), i32(table), max_q=nq, max_kv=n, causal=False, scale=scale, out=out)
+    want, most = ref.attention(codes, scales, x, [0, nq], [n], table, H * G, False, scale)
+    check_attn(host(out), want, most, "f16", "exact", x, codes, scales, scale, n)
+
+
+@pytest.mark.parametrize("mul", [2.0 ** 126, 2.0 ** -100, 2.0 ** -120])
+@pytest.mark.parametrize("nq", [1, 10, 20])
+def test_attention_queries_at_the_ends_of_bf16(nq, mul):
+    rng = np.random.default_rng(nq)
+    H, D, n, page = 1, 64, 60, 16
+    codes, scales, cache = make_cache(rng, 4, page, H, D)
+    table = rng.permutation(4)[None]
+    x = np.clip(rng.standard_normal((nq, H, D)), -1.9, 1.9)
+    q = (torch.tensor(x, dtype=torch.bfloat16, device=DEV).double() * mul).to(torch.bfloat16)
+    # scores of order 1: the scale takes back what it can, the page's steps the rest
+    scale = min(max(1.0 / mul, 2.0 ** -120), 2.0 ** 100) / 8
+    scales[:, 0] = 1.0 / (mul * scale * 64 * 8)
+    cache.scales.copy_(torch.tensor(scales))
+    out = torch.full((nq, H, D), 77.0, dtype=torch.bfloat16, device=DEV)
+    cache.attention(q, i32([0, nq]), i32([n]), i32(table), max_q=nq, max_kv=n, causal=False, scale=scale, out=out)
+    want, most = ref.attention(codes, scales, host(q), [0, nq], [n], table, H, False, float(np.float32(scale)))
+    check_attn(host(out), want, most, "bf16", "bf16", host(q), codes, scales, scale, n)
+
+
 def test_offsets_past_32_bits():
     """A cache of 4.6 GB: pages whose codes lie beyond 2^32 bytes are written, read and attended to."""
     page, H, D = 64, 20, 64

@@ -197,8 +197,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
 
   // ---- Q as A fragments: thread t of row g takes dims 16t..16t+15 of each
   // 64 (the 16 consecutive codes it reads of a token). Rows of bf16 or fp32
-  // are scaled by a power of two so that they fit f16: bf16 stays exact down
-  // to 2^-23 of the row's largest value, fp32 is rounded to f16's 11 bits.
+  // are scaled by a power of two so that they fit f16 (query_range).
   uint32_t qa_f[D / 16][4];
   float mul_a, mul_b;
   {
@@ -234,10 +233,8 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
       float up = sign;
       e[half] = 1.f;
       if (p.qdt != WG_DT_F16 && mx > 0.f && mx <= 3.402823466e38f) {
-        // 2^-k and 2^k with 2^k <= mx < 2^(k+1)
-        const int k = min(max((int)(__float_as_uint(mx) >> 23) - 127, -120), 120);
-        up = sign * __uint_as_float((uint32_t)(127 - k) << 23);
-        e[half] = __uint_as_float((uint32_t)(127 + k) << 23);
+        query_range(mx, &up, &e[half]);
+        up *= sign;
       }
 #pragma unroll
       for (int j = 0; j < D / 16; j++) {  // MMA k step j: dims 16t + 4(j%4) .. +3 of 64-block j/4

@@ -133,8 +133,7 @@ __global__ void __launch_bounds__(PW * 32, D == 64 ? 4 : 2) prompt_attn_kernel(c
   if (c < c_end) fetch(c);
 
   // ---- Q through the second buffer: rows of bf16 or fp32 are scaled by a power
-  // of two to fit f16 (bf16 exact down to 2^-23 of the row's largest, fp32
-  // rounded to 11 bits); D/8 lanes take a row, 8 dims each
+  // of two to fit f16 (query_range); D/8 lanes take a row, 8 dims each
   uint32_t qf[KS][4];
   float mul[2];
   {
@@ -170,9 +169,8 @@ __global__ void __launch_bounds__(PW * 32, D == 64 ? 4 : 2) prompt_attn_kernel(c
 #pragma unroll
         for (int o = 1; o < RL; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         if (mx > 0.f && mx <= 3.402823466e38f) {
-          const int k = min(max((int)(__float_as_uint(mx) >> 23) - 127, -120), 120);
-          up = sign * __uint_as_float((uint32_t)(127 - k) << 23);
-          e = __uint_as_float((uint32_t)(127 + k) << 23);
+          query_range(mx, &up, &e);
+          up *= sign;
         }
       }
       *reinterpret_cast<uint4*>(qs + f_off<D>(row, c8)) =
