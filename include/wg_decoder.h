@@ -473,8 +473,10 @@ int wg_kv8_attention(const wg_kv8* cache, const wg_kv8_attn* p, int device, void
  * temperature, top_k, top_p, min_p: [R], or NULL for 1, 0, 1 and 0.
  * tokens [R]; logprobs [R] or NULL: log softmax(z) of the token over the whole
  * row (z = logit where temperature <= 0). Decisions are made on masses held
- * in 64 bits (fixed point), so a result does not depend on how a
- * row was split. */
+ * in 64 bits (fixed point, units of 2^-45 of the largest weight, so weights
+ * below 2^-46 of it have no mass), and a result does not depend on how a row
+ * was split. u = 0 (or no number, or negative) gives the first kept token
+ * whatever its weight. */
 typedef struct wg_sample {
   const void* logits;
   int64_t ld;

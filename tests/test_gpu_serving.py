@@ -700,6 +700,25 @@ def test_sample_at_the_edges_of_elements(V, C):
     np.testing.assert_array_equal(host(tok), want)
 
 
+@pytest.mark.parametrize("V", [300, 1000, 3001, 4099, 51865])
+@pytest.mark.parametrize("depth", [25.0, 31.9, 33.0, 40.0, 300.0])
+def test_sample_the_number_zero(V, depth):
+    """u = 0 is the first kept token in index order, also where its weight is
+    far below the units in which masses are held; with and without filters,
+    beside rows whose number is not 0."""
+    sets = [dict(), dict(k=40), dict(k=V - 7), dict(p=0.9), dict(m=1e-20), dict(m=1e-12), dict(k=200, m=1e-16), dict(T=0.5),
+            dict(k=30, p=0.5), dict(k=V // 2, p=0.999999), dict(m=1e-44), dict(T=0.0), dict(k=V // 2, T=3.0, m=1e-17)]
+    R = 2 * len(sets)
+    rng = np.random.default_rng(V + int(depth))
+    x = rng.standard_normal((R, V)) * 2 - depth
+    x[:, V // 2] = 0.0
+    x[3, :5] = -np.inf
+    x[4, 0] = np.nan
+    get = lambda n, d: np.array([s.get(n, d) for s in sets + sets])  # noqa: E731
+    u = np.where(np.arange(R) < len(sets), 0.0, rng.random(R))
+    check_sample(x, u, get("T", 1.0), get("k", 0), get("p", 1.0), get("m", 0.0))
+
+
 @pytest.mark.parametrize("n", [300, 1000])
 def test_sample_list_in_one_bin(n):
     """Candidates that share a histogram bin, equal or an ulp apart."""

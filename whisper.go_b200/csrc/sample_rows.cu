@@ -177,7 +177,13 @@ struct Weigh {
     const double v = value(x, &oct);
     return fixed(v, oct);
   }
-  // the same, 0 where w < least
+  // for octaves below 1022
+  __device__ __forceinline__ bool at_least(float x, double least) const {
+    int oct;
+    const double v = value(x, &oct);
+    return v * __hiloint2double((1023 - oct) << 20, 0) >= least;
+  }
+  // in those units, 0 where w < least
   __device__ __forceinline__ u64 fixed_from(float x, double least) const {
     int oct;
     const double v = value(x, &oct);
@@ -271,7 +277,15 @@ struct Row {
   __device__ __forceinline__ int bin_of(float x) const { return __float_as_int(bin_bits(x)) & (SR_BINS - 1); }
   __device__ __forceinline__ bool light(float x) const { return !((mx - x) * c2 < SR_OCTAVES); }
   __device__ __forceinline__ u64 weight(float x) const { return light(x) ? (u64)0 : wt.fixed_of(x); }
-  __device__ __forceinline__ u64 weight_kept(float x) const { return light(x) ? (u64)0 : by_m ? wt.fixed_from(x, least) : wt.fixed_of(x); }
+  __device__ __forceinline__ u64 weight_kept(float x) const {
+    if (u == 0.f) return first_kept(x);
+    return light(x) ? (u64)0 : by_m ? wt.fixed_from(x, least) : wt.fixed_of(x);
+  }
+  // The number 0 falls on the first token that stays, however small its weight:
+  // all count alike. (min_p, an fp32 number, is at least 2^-149.)
+  __device__ __forceinline__ u64 first_kept(float x) const {
+    return x > -INFINITY && (!by_m || ((mx - x) * c2 < 160.f && wt.at_least(x, least)));
+  }
   __device__ __forceinline__ void finish(int token, float x) const {
     s.tokens[r] = token;
     if (s.logprobs) {
@@ -1111,7 +1125,7 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
           u64 kept[SR_EPT] = {};
 #pragma unroll
           for (int j = 0; j < SR_EPT; j++) {
-            if (place(j) < nk && (!by_p || before[j] < lo)) kept[j] = by_m ? row.weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
+            if (place(j) < nk && (!by_p || before[j] < lo)) kept[j] = by_m || u == 0.f ? row.weight_kept(of_key((uint32_t)(o[j] >> 32))) : f[j];
             unsure |= by_p && place(j) < nk && before[j] >= lo && before[j] < hi;
             if (by_p && !covers && place(j) == total - 1) {
               ended = before[j] + f[j] < hi;
