@@ -44,8 +44,7 @@
 namespace wg {
 namespace {
 
-template <int D>
-constexpr int warps_of() { return 4; }  // warps per CTA (6 and 8 were slower at 128-wide heads: 52 -> 56, 67 us)
+constexpr int AW = 4;        // warps per CTA (6 and 8 were slower at 128-wide heads: 52 -> 56, 67 us)
 constexpr int CH = 32;       // tokens per chunk
 constexpr int STAGES = 2;    // more hide no more: 3 and 4 stages left 64 x 1500 tokens at 52 us
 template <int D>
@@ -53,7 +52,7 @@ constexpr int stage_bytes() { return 2 * CH * D + 32; }  // K, V, {sk[2], sv[2],
 template <int D>
 constexpr int warp_bytes() { return STAGES * stage_bytes<D>(); }
 template <int D>
-constexpr int smem_bytes() { return warps_of<D>() * warp_bytes<D>(); }
+constexpr int smem_bytes() { return AW * warp_bytes<D>(); }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -115,31 +114,29 @@ __device__ __forceinline__ void load_v(const uint8_t* vs, int g, int t, uint32_t
 // HALF: at most 8 rows are live, so the MMA's rows 8..15 are not processed
 // past the products. SMALL: 16-token pages (two pages, and scales, per chunk).
 template <int D, bool HALF, bool SMALL>
-__global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_attn_kernel(const Kv8AttnArgs p) {
+__global__ void __launch_bounds__(AW * 32, D == 64 ? 5 : 2) decode_attn_kernel(const Kv8AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
-  constexpr int AW = warps_of<D>();
   constexpr int PARTS = D / 16;  // 16-byte pieces of a token
   constexpr int NT = D / 8;      // n-tiles of P.V
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-  const int tile = 0, h = unit / p.R, r = unit % p.R;
+  const int h = unit / p.R, r = unit % p.R;
   const int page = 1 << p.shift;
   int q0 = __ldg(p.cu_q + r);
   int nq = __ldg(p.cu_q + r + 1) - q0;
   if (q0 < 0 || nq < 0 || q0 > p.n_q || nq > p.n_q - q0) nq = 0;
-  const int rows = min(16, min(nq, p.max_q) * p.G - tile * 16);
-  if (rows <= 0) return;  // the whole cluster: no row of this tile exists
+  const int rows = min(16, min(nq, p.max_q) * p.G);
+  if (rows <= 0) return;  // the whole cluster: the request has no row
   const int len = min(max(__ldg(p.kv_lens + r), 0), (int)min((int64_t)p.max_pages << p.shift, (int64_t)0x7fffff00));
   const int* table = p.table + (int64_t)r * p.ldt;
-  const int row0 = tile * 16;
   // tokens [0, lim) are visible to a row
-  const int qa = (row0 + g) / p.G, qb = (row0 + g + 8) / p.G, qlast = (row0 + rows - 1) / p.G;
+  const int qa = g / p.G, qb = (g + 8) / p.G, qlast = (rows - 1) / p.G;
   const int lim_a = p.causal ? max(0, len - nq + qa + 1) : len;
   const int lim_b = p.causal ? max(0, len - nq + qb + 1) : len;
   const int hi = p.causal ? max(0, len - nq + qlast + 1) : len;
-  const int lo_lim = p.causal ? max(0, len - nq + row0 / p.G + 1) : len;  // every row sees [0, lo_lim)
+  const int lo_lim = p.causal ? max(0, len - nq + 1) : len;  // every row sees [0, lo_lim)
   const int nch = (hi + CH - 1) / CH, per = (nch + p.splits - 1) / p.splits;
   const int c_end = min(nch, (rank + 1) * per);
   int c = rank * per + warp;
@@ -207,7 +204,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
     for (int half = 0; half < (HALF ? 1 : 2); half++) {
       const int row = g + half * 8;
       const bool live = row < rows;
-      const int qi = (row0 + row) / p.G, hg = (row0 + row) % p.G;
+      const int qi = row / p.G, hg = row % p.G;
       const int64_t base = (int64_t)(q0 + qi) * p.ldq + ((int64_t)h * p.G + hg) * D + 16 * t;
       float x[D / 4];
       float mx = 0.f;
@@ -596,7 +593,7 @@ __global__ void __launch_bounds__(warps_of<D>() * 32, D == 64 ? 5 : 2) decode_at
       m = nm;
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // nothing visible: zeros; NaN stays
-    const int qi = (row0 + row) / p.G, hg = (row0 + row) % p.G;
+    const int qi = row / p.G, hg = row % p.G;
     const int64_t at = (int64_t)(q0 + qi) * p.ldo + ((int64_t)h * p.G + hg) * D + d;
     if (p.o_vec) {
       *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) =
@@ -659,17 +656,15 @@ int launch_kv8_attention(const wg_kv8& c, const wg_kv8_attn& p, int device, cuda
   const int64_t rows = (int64_t)max_q * G;
   const int64_t kv = p.max_kv < ((int64_t)p.max_pages << a.shift) ? p.max_kv : (int64_t)p.max_pages << a.shift;
   if (rows > 16) return launch_kv8_prompt(a, c.head_dim, kv, st);  // more than one MMA's rows
-  const int64_t tiles = 1, units = (int64_t)c.n_kv_head * p.n_requests;
+  const int64_t units = (int64_t)c.n_kv_head * p.n_requests;
   const int64_t chunks = (kv + CH - 1) / CH;
-  // CTAs per tile: enough for two rounds of the SMs' resident CTAs, no less
+  // CTAs per (request, K/V head): enough for two rounds of the SMs' resident CTAs, no less
   // than two chunks for each warp, and no CTA with more than 64 chunks
   // (2048 tokens), so that one long request among short ones is spread too
-  const int AW = c.head_dim == 64 ? warps_of<64>() : warps_of<128>();
   int64_t s = (148 * 6 + units - 1) / units;
   if (s > chunks / (2 * AW)) s = chunks / (2 * AW);
   if (s < (chunks + 63) / 64) s = (chunks + 63) / 64;
   a.splits = (int)(s < 1 ? 1 : s > KV8_MAX_SPLIT ? KV8_MAX_SPLIT : s);
-  a.tiles = (int)tiles;
   if (units * a.splits > 0x7fffffffLL) {
     set_error("wg_kv8_attention: %lld CTAs are more than a grid holds", (long long)(units * a.splits));
     return WG_ERR_INVALID;

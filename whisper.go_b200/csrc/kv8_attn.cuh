@@ -23,7 +23,7 @@ struct Kv8AttnArgs {
   const int* table;
   int64_t ldt;
   int max_pages, R;
-  int tiles, splits, causal, max_q;
+  int tiles, splits, causal, max_q;  // tiles: of kv8_prompt.cu
   float scale;
   void* out;
   int64_t ldo;
@@ -33,7 +33,7 @@ struct Kv8AttnArgs {
 
 
 constexpr int KV8_MAX_ATTN_ROWS = 1 << 30;  // (query, grouped head) rows of one request and K/V head
-constexpr int KV8_MAX_SPLIT = 16;  // CTAs that share a tile's tokens (a cluster)
+constexpr int KV8_MAX_SPLIT = 16;  // CTAs that share the tokens of a tile, or of a few rows (a cluster)
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(

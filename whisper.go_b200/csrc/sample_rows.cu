@@ -244,7 +244,7 @@ __device__ __forceinline__ void cluster_barrier(int C) {
 // registers: one row 15.1 us, 15.9 in one body; 320 with a top-k 67 and 71).
 struct Row {
   wg_sample s;
-  int C, rank, r, per, c0, lead;
+  int C, rank, r, per;
   int first_i;  // index of the thread's first element
   int slice;
   float mx, span, bin_scale, t1, c2, c2_lo, deep, u;
@@ -252,7 +252,7 @@ struct Row {
   int k;
   float top_p;
   double least;  // min-p
-  bool by_k, by_p, by_m, need_bins;
+  bool by_k, by_p, by_m;
 
   // this thread's consecutive elements
   __device__ __forceinline__ const float4* mine() const {
@@ -815,8 +815,8 @@ __global__ void __launch_bounds__(SR_THREADS, 3) sample_rows_kernel(const wg_sam
   const float bin_scale = (float)(SR_BINS - 1) / span;
   float u = s.u[r];
   if (!(u >= 0.f)) u = 0.f;
-  const Row row{s, C, rank, r, per, c0, lead, first_i, slice, mx, span, bin_scale, t1, c2, c2_lo, deep, u,
-                Weigh{(double)mx, -1.0 / (SR_STEP * (double)t1)}, k, top_p, (double)min_p, by_k, by_p, by_m, need_bins};
+  const Row row{s, C, rank, r, per, first_i, slice, mx, span, bin_scale, t1, c2, c2_lo, deep, u,
+                Weigh{(double)mx, -1.0 / (SR_STEP * (double)t1)}, k, top_p, (double)min_p, by_k, by_p, by_m};
   double own = 0;  // this thread's weights
   {
     // the maxima are counted, not summed: a row that is nearly certain keeps the
