@@ -122,6 +122,126 @@ def test_cross_cache8_decodes(beam):
     m.close()
 
 
+def coarse_encoders(m, n, T):
+    """Encoder outputs with a frame eight times as large in every page of 64: the
+    page's steps are coarse, so logits with the 8-bit cache lie an order of
+    magnitude further from those without it than the gates are wide."""
+    encs = []
+    for u in range(n):
+        e = m.encoder_output(u, T).copy()
+        e[5::64] *= 8
+        encs.append(e)
+    return encs
+
+
+def gate_of(want):
+    return min(ATOL, RTOL * float(np.abs(want).max()))
+
+
+class Quantised:
+    """The numpy decoder's penalised logits by token prefix, and how far a device logit may be off."""
+
+    def __init__(self, m, dec, encs):
+        self.m, self.dec, self.encs, self.seen = m, dec, encs, {}
+
+    def __call__(self, u, tokens):
+        key = (u, tuple(int(t) for t in tokens))
+        if key not in self.seen:
+            raw = forward(self.m, self.encs[u], list(key[1]))
+            x = oracle.apply_penalty(raw.astype(np.float32), np.asarray(key[1], np.int32)).astype(np.float64)
+            x[self.dec.eot] = -np.inf
+            self.seen[key] = x, gate_of(raw)
+        return self.seen[key]
+
+
+def test_cross_cache8_logits_are_not_the_f16_cache_s(monkeypatch):
+    """Where the two caches' logits differ by many gates, the device's with the option are the quantised ones."""
+    m = wgdec.SyntheticModel(51864, 384, 6, 2, 448, "Q8_0", seed=33)
+    dec = wgdec.WhisperDecoder(m)
+    encs = coarse_encoders(m, 2, 130)
+    forced = np.random.default_rng(4).integers(0, 50257, size=(2, 2))
+    got8 = dec.teacher_forced_logits(encs, PROMPT, forced, cross_cache8=True)
+    got16 = dec.teacher_forced_logits(encs, PROMPT, forced)
+    for u in range(2):
+        tokens = PROMPT + [int(forced[u, 0])]
+        want8 = forward(m, encs[u], tokens)
+        with monkeypatch.context() as mp:
+            mp.setitem(globals(), "quantised", lambda x: x)
+            want16 = forward(m, encs[u], tokens)
+        g = gate_of(want8)
+        assert np.abs(want8 - want16).max() > 8 * g
+        assert np.abs(got8[1, u] - want8).max() <= g and np.abs(got16[1, u] - want16).max() <= g
+    dec.close()
+    m.close()
+
+
+def test_cross_cache8_greedy_tokens():
+    """Each token of three utterances decoded at once is the numpy decoder's
+    maximum (to twice the logits' gate), and each utterance alone gives the
+    same tokens up to such a tie."""
+    m = wgdec.SyntheticModel(51864, 384, 6, 2, 448, "Q8_0", seed=33)
+    dec = wgdec.WhisperDecoder(m)
+    encs = coarse_encoders(m, 3, 130)
+    logits = Quantised(m, dec, encs)
+    p8 = wgdec.DecoderParams(prompt=PROMPT, max_tokens=6, cross_cache8=True, suppress_eot=True, no_fallback=True)
+    toks, lens, _ = dec.decode_tokens(encs, p8)
+    assert (lens == 10).all() and len({tuple(t) for t in toks.tolist()}) == 3
+    for u in range(3):
+        for s in range(4, 10):
+            x, g = logits(u, toks[u, :s])
+            assert x[toks[u, s]] >= x.max() - 2 * g, (u, s)
+        alone = dec.decode_tokens([encs[u]], p8)[0][0]
+        off = np.flatnonzero(alone[:10] != toks[u, :10])
+        if off.size:
+            x, g = logits(u, toks[u, :off[0]])
+            assert abs(x[alone[off[0]]] - x[toks[u, off[0]]]) <= 4 * g, u
+    dec.close()
+    m.close()
+
+
+def test_cross_cache8_beams():
+    """Five beams of three utterances, step by step: every hypothesis' score is
+    the sum of its tokens' log-probs in the numpy decoder (each off by at most
+    twice the logits' gate), the first token of all of them its maximum (the five
+    equal prompts of the start each offer it, and it ranks first), and each
+    utterance alone finds hypotheses of the same scores."""
+    B, M, U = 5, 3, 3
+    m = wgdec.SyntheticModel(51864, 384, 6, 2, 448, "Q8_0", seed=33)
+    dec = wgdec.WhisperDecoder(m)
+    encs = coarse_encoders(m, U, 130)
+    logits = Quantised(m, dec, encs)
+    params = wgdec.DecoderParams(prompt=PROMPT, beam_size=B, max_tokens=M, cross_cache8=True, suppress_eot=True)
+
+    def steps_of(which):
+        job, out = wgdec.Job(dec, len(which), 130, params), []
+        job.upload([encs[u] for u in which])
+        job.start()
+        for _ in range(M):
+            job.step(1)
+            out.append([a.copy() for a in job.beams()])
+        job.close()
+        return out
+
+    together, alone = steps_of(range(U)), [steps_of([u]) for u in range(U)]
+    for st in range(M):
+        toks, lens, scores = together[st]
+        for u in range(U):
+            for b in range(B):
+                assert lens[u, b] == len(PROMPT) + st + 1
+                seq, want, slack = toks[u, b, :lens[u, b]], 0.0, 0.0
+                for s in range(len(PROMPT), len(seq)):
+                    x, g = logits(u, seq[:s])
+                    want += x[seq[s]] - x.max() - np.log(np.exp(x - x.max()).sum())
+                    slack += 2 * g
+                assert abs(scores[u, b] - want) <= slack + 1e-5 * abs(want), (st, u, b)
+            x, g = logits(u, PROMPT)
+            assert x[toks[u, :, 4]].min() >= x.max() - 2 * g
+            # sorted by score and length alike, near-ties may swap tokens but not move a rank's score
+            assert np.abs(alone[u][st][2][0] - scores[u]).max() <= 2 * slack
+    dec.close()
+    m.close()
+
+
 @pytest.mark.parametrize("settings", [dict(top_k=5), dict(top_p=0.8, temperature=0.7), dict(min_p=0.1),
                                       dict(top_k=40, top_p=0.95, min_p=0.01, temperature=1.5), dict(cross_cache8=True)],
                          ids=str)
