@@ -616,6 +616,22 @@ def test_sample_defaults_and_many_rows():
     check_sample(x, rng.random(400), None, None, None, None)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [2049, 3001, 4095, 4096])
+def test_sample_vocabularies_of_two_slices(V, dt):
+    """Short and long kept sets, exact masses, ties and edges of rows that two CTAs share."""
+    sets = SETTINGS + [dict(k=1025), dict(k=V - 3), dict(k=1500, p=0.999, T=2.0), dict(p=0.99, T=4.0), dict(p=0.5, T=9.0, m=1e-3),
+                       dict(m=1e-6), dict(m=1e-3, T=5.0), dict(k=1024, m=0.2, T=3.0), dict(p=0.9999999)]
+    get = lambda n, d: np.array([s.get(n, d) for s in sets])  # noqa: E731
+    rng = np.random.default_rng(V)
+    R = len(sets)
+    for shape in range(3):
+        x = rng.standard_normal((R, V)) * (2.5, 0.05, 2.0)[shape]
+        if shape == 2:
+            x = np.round(x)  # ties by the hundred, at every cut
+        check_sample(x, rng.random(R), get("T", 1.0), get("k", 0), get("p", 1.0), get("m", 0.0), dt, ld_pad=shape)
+
+
 @pytest.mark.parametrize("V", [130001, 262144])
 def test_sample_wide_vocabularies(V):
     rng = np.random.default_rng(V)
