@@ -360,8 +360,9 @@ int wg_model_matmul_noalloc(wg_model* m, int replica, int layer, int which,
  *    writes what another one reads or writes. Make the first call of each
  *    operator on a device before a capture.
  *  - Rows are `ld` ELEMENTS apart, the heads and dims of a row contiguous.
- *    Any stride and any address that fits the type is accepted; rows that
- *    start on 16 bytes are moved with wide loads.
+ *    Any stride and any address that fits the type is accepted (what does not,
+ *    of any tensor, is refused); rows that start on 16 bytes are moved with
+ *    wide loads.
  *  - Lengths, slots and page numbers are checked on the device: what is out
  *    of range is not read or written (see each call). */
 enum { WG_DT_F32 = 0, WG_DT_F16 = 1, WG_DT_BF16 = 30 }; /* GGUF ids of these types */

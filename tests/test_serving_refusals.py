@@ -154,3 +154,19 @@ def test_plan_refuses_what_its_indices_cannot_step_over(R, n_slots):
     """The kernel steps 32-bit indices by up to 2^18 past R and n_slots, so both end at 2^30."""
     assert wgdec.lib().wg_kv_plan(PTR, PTR, R, 16, PTR, 10, PTR, PTR, PTR, 4, 4, PTR, n_slots, PTR, PTR, 0, None) == INVALID
     assert last().startswith("wg_kv_plan")
+
+
+def test_tensors_off_their_types_alignment():
+    """Every int32 and fp32 tensor is checked: a kernel that met one of these would fault."""
+    L, off = wgdec.lib(), PTR + 2
+    good = [PTR, PTR, 3, 16, PTR, 10, PTR, PTR, PTR, 4, 4, PTR, 8, PTR, PTR, 0, None]
+    for at in (0, 1, 4, 6, 7, 8, 11, 13, 14):
+        args = list(good)
+        args[at] = off
+        assert L.wg_kv_plan(*args) == INVALID and "aligned" in last(), at
+    assert L.wg_kv8_append(ctypes.byref(cache()), PTR, PTR, 1, 128, 128, off, 4, 0, None) == INVALID
+    assert L.wg_kv8_read(ctypes.byref(cache()), off, 4, PTR, PTR, 1, 128, 128, 0, None) == INVALID
+    for name in ("cu_q", "kv_lens", "block_table"):
+        assert L.wg_kv8_attention(ctypes.byref(cache()), ctypes.byref(attn(**{name: off})), 0, None) == INVALID, name
+    for name in ("u", "temperature", "top_k", "top_p", "min_p", "tokens", "logprobs"):
+        assert L.wg_sample_rows(ctypes.byref(smp(**{name: off})), 0, None) == INVALID, name

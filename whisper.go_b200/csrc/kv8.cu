@@ -407,8 +407,8 @@ extern "C" int wg_kv8_append(const wg_kv8* cache, const void* k, const void* v, 
   using namespace wg;
   const char* what = "wg_kv8_append";
   WG_CHECK(kv8_check(what, cache));
-  if (!dt_ok(dtype) || n < 0 || n > KV8_MAX_ROWS || (n > 0 && !slots)) {
-    set_error("%s: bad argument (dtype %d, n %d)", what, dtype, n);
+  if (!dt_ok(dtype) || n < 0 || n > KV8_MAX_ROWS || (n > 0 && !slots) || !aligned4(slots)) {
+    set_error("%s: bad argument (dtype %d, n %d, slots null or misaligned)", what, dtype, n);
     return WG_ERR_INVALID;
   }
   if (n == 0) return WG_OK;
@@ -427,8 +427,8 @@ extern "C" int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, voi
   using namespace wg;
   const char* what = "wg_kv8_read";
   WG_CHECK(kv8_check(what, cache));
-  if (!dt_ok(dtype) || n < 0 || n > KV8_MAX_ROWS || (n > 0 && !slots)) {
-    set_error("%s: bad argument (dtype %d, n %d)", what, dtype, n);
+  if (!dt_ok(dtype) || n < 0 || n > KV8_MAX_ROWS || (n > 0 && !slots) || !aligned4(slots)) {
+    set_error("%s: bad argument (dtype %d, n %d, slots null or misaligned)", what, dtype, n);
     return WG_ERR_INVALID;
   }
   if (n == 0) return WG_OK;

@@ -720,7 +720,7 @@ extern "C" int wg_kv8_attention(const wg_kv8* cache, const wg_kv8_attn* p, int d
   const int64_t width = (int64_t)p->n_head * cache->head_dim;
   if (!p->q || !p->out || !p->cu_q || !p->kv_lens || (p->max_pages > 0 && !p->block_table) || p->ldq < width ||
       p->ldo < width || reinterpret_cast<uintptr_t>(p->q) % dt_bytes(p->q_dtype) ||
-      reinterpret_cast<uintptr_t>(p->out) % 2) {
+      reinterpret_cast<uintptr_t>(p->out) % 2 || !aligned4(p->cu_q, p->kv_lens, p->block_table)) {
     set_error("%s: null or misaligned tensor, or rows closer than %lld elements", what, (long long)width);
     return WG_ERR_INVALID;
   }

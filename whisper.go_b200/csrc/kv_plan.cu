@@ -213,6 +213,10 @@ extern "C" int wg_kv_plan(const int32_t* lens, const int32_t* new_tokens, int R,
     set_error("wg_kv_plan: null argument");
     return WG_ERR_INVALID;
   }
+  if (!aligned4(lens, new_tokens, free_pages, cursor, cursor_out, block_table, slots, cu_new, status)) {
+    set_error("wg_kv_plan: a tensor is not aligned to its type");
+    return WG_ERR_INVALID;
+  }
   if (R <= 0 || R > PLAN_MAX || !kv_page_ok(page) || n_free < 0 || n_slots < 0 || n_slots > PLAN_MAX || max_pages <= 0 ||
       ld_table < max_pages) {
     set_error("wg_kv_plan: bad argument (R %d and n_slots %d (at most %d), page %d (a power of two, 16 to 128), n_free %d, "

@@ -84,6 +84,9 @@ inline int log2_of(int pow2) {
   while ((1 << s) < pow2) s++;
   return s;
 }
+// int32 and fp32 tensors: what starts elsewhere would fault the GPU
+template <typename... P>
+inline bool aligned4(const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) == 0; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace wg

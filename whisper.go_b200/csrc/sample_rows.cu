@@ -1257,7 +1257,8 @@ extern "C" int wg_sample_rows(const wg_sample* p, int device, void* stream) {
     return WG_ERR_UNSUPPORTED;
   }
   if (p->R == 0) return WG_OK;
-  if (!p->logits || !p->u || !p->tokens || reinterpret_cast<uintptr_t>(p->logits) % dt_bytes(p->dtype)) {
+  if (!p->logits || !p->u || !p->tokens || reinterpret_cast<uintptr_t>(p->logits) % dt_bytes(p->dtype) ||
+      !aligned4(p->u, p->temperature, p->top_k, p->top_p, p->min_p, p->tokens, p->logprobs)) {
     set_error("%s: null or misaligned tensor", what);
     return WG_ERR_INVALID;
   }
