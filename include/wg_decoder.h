@@ -425,7 +425,8 @@ int wg_kv8_read(const wg_kv8* cache, const int32_t* slots, int n, void* k, void*
 /* Attention of the query rows of n_requests requests over their cached tokens:
  *   softmax(scale * q K^T) V, query head j on K/V head j / (n_head / n_kv_head).
  * Request r's queries are rows cu_q[r] .. cu_q[r+1]-1 of q; they see the
- * first kv_lens[r] tokens of the pages in row r of block_table; with `causal`
+ * first kv_lens[r] tokens (first cut to 0 .. max_pages * page) of the pages in
+ * row r of block_table; with `causal`
  * the queries are the last tokens of those: query i of nq sees the first
  * kv_lens[r] - nq + i + 1. Without it every query sees all of them (cross-
  * attention: the beams of an utterance are its queries). A query that sees

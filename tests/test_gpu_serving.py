@@ -368,6 +368,27 @@ def test_attention_nan_and_infinite_queries_stay_in_their_rows():
         assert torch.equal(out[r], clean[r])
 
 
+@pytest.mark.parametrize("nq,page", [(6, 32), (13, 16), (13, 64), (40, 16), (40, 64)])
+@pytest.mark.parametrize("qdt", ["f16", "f32"])
+def test_attention_nan_and_infinite_queries_in_every_kernel(nq, page, qdt):
+    """Rows with a NaN or an infinity give no number, the rows around them their own."""
+    rng = np.random.default_rng(nq + page)
+    H, D = 1, 64
+    codes, scales, cache = make_cache(rng, 8, page, H, D)
+    table = i32(rng.permutation(8)[:6][None])
+    q = rows(rng, nq, H, D, qdt, spread=False)
+    clean = torch.empty(nq, H, D, dtype=torch.bfloat16, device=DEV)
+    cache.attention(q, i32([0, nq]), i32([90]), table, max_q=nq, max_kv=90, out=clean)
+    q[1, 0, 3], q[4, 0, 9], q[nq - 1, 0, 0] = float("nan"), float("inf"), -float("inf")
+    out = torch.empty_like(clean)
+    cache.attention(q, i32([0, nq]), i32([90]), table, max_q=nq, max_kv=90, out=out)
+    bad = [1, 4, nq - 1]
+    assert torch.isnan(out[1]).all() and not torch.isfinite(out[bad]).any()
+    for r in range(nq):
+        if r not in bad:
+            assert torch.equal(out[r], clean[r]), r
+
+
 @pytest.mark.parametrize("nq", [[30, 9], [3, 2]], ids=str)
 def test_attention_bounds_far_above_the_queries(nq):
     """max_q is a bound: "no limit" computes the same rows as n_q does, bit for

@@ -10,12 +10,14 @@
 // magnitude passes an octave, where amax / 127 would be rounded again with
 // every new maximum. The price is a step of at most twice the finest one.
 //
-// Both are streams bounded by memory: K and V come in once (2 or 4 bytes a
-// value) and go out as one byte, or the reverse. Measured on 96000 tokens of 20
-// heads of 64 in f16 (737 MB each way): append 150 us = 4.9 TB/s, 75 % of the
-// measured copy rate (16 warps an SM, each holding 8 KB while it looks for the
-// largest magnitude); read 137 us = 5.4 TB/s, 82 %. Small calls (64 tokens)
-// are launches: 6.5 us each with the host's part.
+// Both are streams bounded by memory: K and V come in (2 or 4 bytes a value;
+// once where a run of tokens in a page holds up to 8 KB a head, which a warp
+// keeps while it looks for the largest magnitude: 64 tokens of 64 16-bit values;
+// of longer runs all but the last 8 KB are read a second time) and go out as one
+// byte, or the reverse. Measured on 96000 tokens of 20 heads of 64 in f16 in
+// pages of 64 (737 MB each way): append 150 us = 4.9 TB/s, 75 % of the measured
+// copy rate (16 warps an SM); read 137 us = 5.4 TB/s, 82 %. Small calls (64
+// tokens) are launches and the host's part, 6.5 to 9 us each.
 #include "kernels.cuh"
 #include "ops.cuh"
 
@@ -134,8 +136,8 @@ constexpr int PAGE_MAX = 128;
 // finds the runs that begin among its `chunk` tokens (grid x) and its warps
 // deal the (run, unit) pairs of its 8 units (grid y). The run's values stay in
 // registers between finding the largest magnitude and coding (8 KB a warp: a
-// page of 64 tokens of 64 16-bit values), so they are read once; what is
-// longer is read again from its second block on.
+// page of 64 tokens of 64 16-bit values), so they are read once; of what is
+// longer the last block is held and the ones before it are read again.
 template <int ES>
 __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(AppendArgs p) {
   pdl_trigger();

@@ -10,7 +10,7 @@
 // The codes are exact in f16, so both products run on mma.m16n8k16 (f16 in,
 // fp32 accumulators); scales multiply the fp32 results. What bounds it is the
 // cache's bytes (2 * D bytes per token and head), and next to them the
-// instructions that turn a byte into an f16: 112 of the ~440 that a warp spends
+// instructions that turn a byte into an f16: 176 of the ~497 that a warp spends
 // on 32 tokens of 64-wide heads. So:
 //  - (query, grouped head) pairs that share a K/V head are one tile: single
 //    tokens, beams and grouped heads take one read. Up to 8 of them are the
@@ -21,6 +21,10 @@
 //    that subtraction, 50.4 us against 51.8 in the cross case below, but 1152 *
 //    sum q and 1152 * sum p leave their rounding behind: an output of small
 //    values beside a strong zero was 10 % off.)
+//  - what meets the codes in an MMA is f16 too: the softmax weights are lifted
+//    and rounded (pack_weights), fp32 queries rounded to 11 bits (query_range)
+//    as the f16 cache's cross-attention rounds them; their low parts would cost
+//    as many MMAs again;
 //  - every warp streams its own 32-token chunks through its own ring of
 //    cp.async stages (no CTA barrier in the loop, no bounded wait needed: a
 //    cp.async group always completes);
@@ -30,11 +34,11 @@
 //  - tokens are split over the CTAs of a cluster and joined through
 //    distributed shared memory: one launch, no workspace in global memory.
 // Measured: 64 utterances x 1500 tokens x 20 heads, 5 queries each (248 MB)
-// 48 us = 5.15 TB/s, 79 % of the measured copy rate (the ALU pipe is 56 % busy,
-// issue slots 57 %); two requests of 60001 and ~29000 tokens, 8 heads of 128,
-// 4 grouped queries (183 MB) 52 us = 3.5 TB/s (at most 16 CTAs a head: ~7 warps
-// an SM, bound by each warp's own latency); 229 tokens of 6 heads 7.6 us a call,
-// most of it the launch.
+// 50 us = 4.95 TB/s, 75 % of the measured copy rate (issue slots 63 % busy);
+// two requests of 60001 and ~29000 tokens, 8 heads of 128, 4 grouped queries
+// (183 MB) 56 us = 3.3 TB/s (at most 16 CTAs a head: ~7 warps an SM, bound by
+// each warp's own latency); 229 tokens of 6 heads 8 to 13 us a call, most of it
+// the host's part and the launch.
 #include <cooperative_groups.h>
 
 #include <mutex>

@@ -73,7 +73,8 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
 }
 // Powers of two that take a row of bf16 or fp32 queries into f16 and back, from
 // its largest magnitude: that goes to [2^14, 2^15), so bf16 values stay exact
-// down to 2^-31 of it and fp32 values keep 11 bits down to 2^-28 of it.
+// down to 2^-31 of it and fp32 values keep 11 bits down to 2^-28 of it (as long
+// as it is 2^-112 or more).
 __device__ __forceinline__ void query_range(float largest, float* up, float* down) {
   const int k = max((int)(__float_as_uint(largest) >> 23) - 127, -112);
   *up = __uint_as_float((uint32_t)(127 + 14 - k) << 23);

@@ -14,7 +14,7 @@
 // advanced in place must not be written before every CTA has read it: up to
 // PLAN_CLUSTER CTAs are a cluster with a barrier for that, more leave the
 // cursor to a second launch of one thread (1500 prompts of up to 448 tokens:
-// 31 us with 8 CTAs, 17 with 64).
+// 31 us with 8 CTAs, 13 to 17 with 64).
 #include "ops.cuh"
 
 namespace wg {

@@ -44,7 +44,7 @@
 // so top-p asks for them only where bounds on the fp32 sum do not settle the cut
 // (3 % of such rows), and with eleven operations each. Measured (a pass): one
 // row of 51865 fp32 15 us (24 where no short list holds the kept set), 48 of
-// 51864 f16 24 us, 320 of 51866 fp32 75 us = 0.88 TB/s; 61 us with a top-k in
+// 51864 f16 25 us, 320 of 51866 fp32 76 us = 0.87 TB/s; 61 us with a top-k in
 // the place of the nucleus rows, of which two in 54 have no short list and may
 // come last. One CTA a row, streaming the row from L2 in every pass: top-k 81 us
 // at 320 rows against 67, 53 at one row against 14.
