@@ -389,6 +389,35 @@ def test_attention_nan_and_infinite_queries_in_every_kernel(nq, page, qdt):
             assert torch.equal(out[r], clean[r]), r
 
 
+@pytest.mark.parametrize("log2", [5, 20, 24, 27, 30, 34, 50, 90])
+@pytest.mark.parametrize("nq,G,D,page", [(1, 1, 64, 64), (3, 2, 64, 16), (2, 2, 128, 32), (12, 1, 64, 32), (3, 4, 128, 16),
+                                         (40, 1, 64, 64), (24, 1, 128, 16)])
+def test_attention_of_any_size_of_scores(nq, G, D, page, log2):
+    """Scores so far apart that one token takes all, up to sizes where fp32 has
+    no digits left behind the point: the output is that token's value."""
+    rng = np.random.default_rng(nq + G + log2)
+    H, n = 1, 150
+    codes, scales, cache = make_cache(rng, -(-n // page), page, H, D)
+    # queries along dim 0 alone: the best token's code there leads the others' by 47
+    codes[:, 0] = rng.integers(-3, 4, codes[:, 0].shape)
+    codes[:, 0, :, :, 0] = 8 * rng.integers(-10, 11, codes.shape[0] * page).reshape(-1, 1, page)
+    best = int(rng.integers(0, n))
+    codes[best // page, 0, :, best % page, 0] = 127
+    scales[:, 0] = 1.0
+    cache.codes.copy_(torch.tensor(codes))
+    cache.scales.copy_(torch.tensor(scales))
+    x = np.zeros((nq, H * G, D))
+    x[..., 0] = 2.0 ** log2 * (1 + rng.integers(0, 128, (nq, H * G)) / 128)
+    q = torch.tensor(x, dtype=torch.bfloat16, device=DEV)
+    table = np.arange(codes.shape[0])[None]
+    out = torch.full((nq, H * G, D), 77.0, dtype=torch.float16, device=DEV)
+    cache.attention(q, i32([0, nq]), i32([n]), i32(table), max_q=nq, max_kv=n, causal=False, scale=0.25, out=out)
+    want, most = ref.attention(codes, scales, x, [0, nq], [n], table, H * G, False, 0.25)
+    v = codes[best // page, 1, 0, best % page].astype(np.float64) * scales[best // page, 1, 0]
+    assert np.abs(want[0][0] - v).max() <= 1e-9  # 2^5 * 0.25 * 47 steps above the next: all others under e^-376
+    check_attn(host(out), want, most, "f16", "bf16", x, codes, scales, 0.25, n)
+
+
 @pytest.mark.parametrize("nq", [[30, 9], [3, 2]], ids=str)
 def test_attention_bounds_far_above_the_queries(nq):
     """max_q is a bound: "no limit" computes the same rows as n_q does, bit for

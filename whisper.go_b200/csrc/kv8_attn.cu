@@ -331,13 +331,15 @@ __global__ void __launch_bounds__(AW * 32, D == 64 ? 5 : 2) decode_attn_kernel(c
         m_a = x0;
         m_b = x1;
       }
-      // lifted weights rounded to f16, queries in rows: the other operand of P.V
+      // lifted weights rounded to f16, queries in rows: the other operand of P.V.
+      // The products are rounded as the maximum's was: fused with the sum, a
+      // maximum of 2^25 and more would miss itself by octaves
       const float lift0 = KV8_LIFT - ref0, lift1 = KV8_LIFT - ref1;
       uint32_t pb[2][2];
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        pb[i][0] = transpose8(pack_weights(ex2(fmaf(s[i][0], step0, lift0)), ex2(fmaf(s[i][1], step1, lift1))));
-        pb[i][1] = transpose8(pack_weights(ex2(fmaf(s[i][2], step0, lift0)), ex2(fmaf(s[i][3], step1, lift1))));
+        pb[i][0] = transpose8(pack_weights(ex2(__fmul_rn(s[i][0], step0) + lift0), ex2(__fmul_rn(s[i][1], step1) + lift1)));
+        pb[i][1] = transpose8(pack_weights(ex2(__fmul_rn(s[i][2], step0) + lift0), ex2(__fmul_rn(s[i][3], step1) + lift1)));
       }
       // their sums, by the same MMA over a matrix of ones, go into l (so that the
       // rounded weights sum to one)
@@ -443,14 +445,14 @@ __global__ void __launch_bounds__(AW * 32, D == 64 ? 5 : 2) decode_attn_kernel(c
         m_a = x_a;
         m_b = x_b;
       }
-      // lifted weights rounded to f16 for the MMA
+      // lifted weights rounded to f16 for the MMA (products rounded as the maximum's)
       const float lift_a = KV8_LIFT - ref_a, lift_b = KV8_LIFT - ref_b;
       uint32_t pf[2][4];
 #pragma unroll
       for (int n = 0; n < 4; n++) {
-        pf[n >> 1][(n & 1) * 2] = pack_weights(ex2(fmaf(s[n][0], step_a, lift_a)), ex2(fmaf(s[n][1], step_a, lift_a)));
+        pf[n >> 1][(n & 1) * 2] = pack_weights(ex2(__fmul_rn(s[n][0], step_a) + lift_a), ex2(__fmul_rn(s[n][1], step_a) + lift_a));
         pf[n >> 1][(n & 1) * 2 + 1] =
-            pack_weights(ex2(fmaf(s[n][2], step_b, lift_b)), ex2(fmaf(s[n][3], step_b, lift_b)));
+            pack_weights(ex2(__fmul_rn(s[n][2], step_b) + lift_b), ex2(__fmul_rn(s[n][3], step_b) + lift_b));
       }
       // their row sums, by the same MMA over a matrix of ones, go into l (so that
       // the rounded weights sum to one)
