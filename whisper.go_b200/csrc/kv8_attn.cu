@@ -34,7 +34,8 @@
 //  - tokens are split over the CTAs of a cluster and joined through
 //    distributed shared memory: one launch, no workspace in global memory.
 // Measured: 64 utterances x 1500 tokens x 20 heads, 5 queries each (248 MB)
-// 50 us = 4.95 TB/s, 75 % of the measured copy rate (issue slots 63 % busy);
+// 50 to 53 us = 4.7 to 4.95 TB/s, 71 to 75 % of the measured copy rate (issue
+// slots 63 % busy);
 // two requests of 60001 and ~29000 tokens, 8 heads of 128, 4 grouped queries
 // (183 MB) 56 us = 3.3 TB/s (at most 16 CTAs a head: ~7 warps an SM, bound by
 // each warp's own latency); 229 tokens of 6 heads 8 to 13 us a call, most of it
